@@ -27,7 +27,8 @@ EXPORTS = ("msd_packed_weight_elems", "msd_workspace_bytes", "msd_default_workgr
            "msd_sample_token_noalloc", "msd_verify_workspace_bytes", "msd_verify",
            "msd_decode_steps", "msd_tiles_bytes", "msd_pack_tiles", "msd_set_launch_graphs",
            "msd_config_support", "msd_xent_workspace_bytes", "msd_xent_plan",
-           "msd_xent_targets", "msd_xent_forward", "msd_xent_backward")
+           "msd_xent_targets", "msd_xent_forward", "msd_xent_backward",
+           "msd_attn_workspace_bytes", "msd_attn_forward", "msd_attn_backward")
 
 # Paths of the library (bits of msd_config_support)
 PATHS = {"decode": 1, "prefill": 2, "verify": 4, "batched": 8, "sample": 16, "batched_step": 32}
@@ -41,6 +42,14 @@ class MsdConfig(ctypes.Structure):
     def from_dict(cls, c):
         return cls(c["vocab_size"], c["d_model"], c["n_heads"], c["n_kv_heads"], c["n_layers"],
                    c.get("d_head", c["d_model"] // c["n_heads"]), c["d_ff"], c["context_len"])
+
+
+class MsdAttn(ctypes.Structure):
+    """One attention call (include/mslayers.h): strides are (sequence, row, head), in elements."""
+    _fields_ = [(k, ctypes.c_int32) for k in ("n_seqs", "q_len", "k_len", "n_heads", "n_kv_heads", "d_head", "causal")]
+    _fields_ += [("scale", ctypes.c_float), ("q_rows", ctypes.c_int64), ("k_rows", ctypes.c_int64)]
+    _fields_ += [(k, ctypes.c_int64 * 3) for k in ("q_stride", "k_stride", "v_stride", "dout_stride")]
+    _fields_ += [("seqs", ctypes.c_void_p)]
 
 
 class MsdError(RuntimeError):
@@ -132,8 +141,24 @@ def lib():
     L.msd_xent_forward.restype = I32
     L.msd_xent_backward.argtypes = [P, P, P, P, P, I32, I32, I32, I32, P, P, P, P, P]
     L.msd_xent_backward.restype = I32
+    AP = ctypes.POINTER(MsdAttn)
+    L.msd_attn_workspace_bytes.argtypes = [AP, I32]
+    L.msd_attn_workspace_bytes.restype = I64
+    L.msd_attn_forward.argtypes = [AP, P, P, P, P, P, P, P]
+    L.msd_attn_forward.restype = I32
+    L.msd_attn_backward.argtypes = [AP, P, P, P, P, P, P, P, P, P, P, P]
+    L.msd_attn_backward.restype = I32
     _lib = L
     return L
+
+
+def launch(fn, what, device, *args):
+    """fn(*args, stream) on the device's current torch stream, with that device current; raises for its error code."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        return check(fn(*args, stream), what)
+    with torch.cuda.device(device):
+        return check(fn(*args, stream), what)
 
 
 def check(code, what):

@@ -1,0 +1,201 @@
+"""Attention for training and scoring: grouped heads, forward and a backward that recomputes the probabilities.
+
+The reference's causal_attention (model.py:122-147) between its projections: q (T, n_heads, d_head), k and v
+(T, n_kv, d_head), over torch tensors on the GPU in bf16, with autograd:
+
+  attention(q, k, v, causal=True, scale=None, sequences=None)
+
+What runs (``msd_attn_forward`` / ``msd_attn_backward``, ``csrc/attn.hip``): one pass over the keys with the running
+maximum and sum of the softmax, so no score matrix is stored; the forward keeps each row's logsumexp, from which the
+backward forms the probabilities again.  Scores, softmax statistics and every sum are f32; the probabilities and the
+scores' gradients are rounded to bf16 as operands of the matrix cores, the results once to bf16.  Deterministic.
+"""
+import ctypes
+import functools
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+
+class Sequences:
+    """Which rows of flat q (Nq, n_heads, d_head) and k, v (Nk, n_kv, d_head) tensors belong to which sequence.
+
+    Sequence s has ``q_lens[s]`` query rows from ``q_starts[s]`` and ``k_lens[s]`` key rows from ``k_starts[s]``; the
+    starts default to the sequences packed one behind the other, the keys to the queries' (self-attention).  A padded
+    batch is its flat view with ``q_starts=range(0, B * T, T)`` and each sequence's own length.  Rows of no sequence are
+    neither read nor attended to; their outputs and gradients are zeros.  Built once per batch from host integers
+    (checked here) and used by every layer; the device copy is made on the current stream."""
+
+    def __init__(self, q_lens, k_lens=None, q_starts=None, k_starts=None, device="cuda"):
+        q_lens = [int(n) for n in q_lens]
+        if k_lens is None and k_starts is None and q_starts is not None:
+            k_starts = q_starts
+        k_lens = q_lens if k_lens is None else [int(n) for n in k_lens]
+        q_starts, self.q_end, self.q_count = _ranges(q_lens, q_starts, "q")
+        k_starts, self.k_end, self.k_count = _ranges(k_lens, k_starts, "k")
+        if len(q_lens) != len(k_lens):
+            raise ValueError(f"{len(q_lens)} query and {len(k_lens)} key sequences")
+        self.n = len(q_lens)
+        self.q_longest, self.k_longest = max(q_lens, default=0), max(k_lens, default=0)
+        rows = [x for s in zip(q_starts, q_lens, k_starts, k_lens) for x in s]
+        self.table = torch.tensor(rows, dtype=torch.int32).reshape(-1, 4).to(device)
+
+
+def _ranges(lens, starts, what):
+    """(starts, one past the last row, rows in all) of checked, disjoint ranges."""
+    if any(n < 0 for n in lens):
+        raise ValueError(f"negative {what} length")
+    if starts is None:
+        starts, at = [], 0
+        for n in lens:
+            starts.append(at)
+            at += n
+    starts = [int(x) for x in starts]
+    if len(starts) != len(lens):
+        raise ValueError(f"{len(starts)} {what} starts for {len(lens)} lengths")
+    end = 0
+    for at, n in sorted((a, n) for a, n in zip(starts, lens) if n):
+        if at < end:
+            raise ValueError(f"{what} ranges overlap or start below 0")
+        end = at + n
+    if end >= 2 ** 31 or any(not 0 <= a < 2 ** 31 for a in starts):
+        raise ValueError(f"{what} ranges outside [0, 2**31)")
+    return starts, end, sum(lens)
+
+
+def _operand(x):
+    """x with contiguous heads on 16-byte boundaries, as the kernels' loads take it (copied only where it is not)."""
+    rows, heads = x.shape[-3], x.shape[-2]
+    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(n <= 1 or k % 8 == 0 for n, k in zip(x.shape, x.stride()[:-1])):
+        if 64 * x.stride(-3) * (rows > 1) + heads * x.stride(-2) * (heads > 1) < 2 ** 30:
+            return x
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def _strides(x):
+    """(sequence, row, head) strides; 0 along an axis of one (or none)."""
+    s = tuple(0 if n <= 1 else k for n, k in zip(x.shape[:-1], x.stride()))
+    return s if len(s) == 3 else (0, *s)
+
+
+@functools.lru_cache(maxsize=256)
+def _call(q_shape, k_shape, q_stride, k_stride, v_stride, dout_stride, causal, scale, sequences):
+    """(arguments, bytes of the forward's and of the backward's workspace) of one shape; sequences: None or the
+    (count, longest q, longest k) of a table that the caller puts in."""
+    *_, H, D = q_shape
+    a = _lib.MsdAttn()
+    if sequences is None:
+        a.n_seqs = q_shape[0] if len(q_shape) == 4 else 1
+        a.q_len, a.k_len = q_shape[-3], k_shape[-3]
+    else:
+        a.n_seqs, a.q_len, a.k_len = sequences
+        a.seqs = 16   # any aligned address: only looked at for its presence here
+    a.q_rows, a.k_rows = math.prod(q_shape[:-2]), math.prod(k_shape[:-2])
+    a.n_heads, a.n_kv_heads, a.d_head, a.causal, a.scale = H, k_shape[-2], D, causal, scale
+    for name, s in (("q_stride", q_stride), ("k_stride", k_stride), ("v_stride", v_stride), ("dout_stride", dout_stride)):
+        getattr(a, name)[:] = s
+    sizes = [_lib.check(_lib.lib().msd_attn_workspace_bytes(ctypes.byref(a), i), "msd_attn_workspace_bytes") for i in (0, 1)]
+    return a, *sizes
+
+
+def _arguments(q, k, v, dout_stride, causal, scale, sequences):
+    table = None if sequences is None else (sequences.n, sequences.q_longest, sequences.k_longest)
+    a, fwd, bwd = _call(q.shape, k.shape, _strides(q), _strides(k), _strides(v), dout_stride, causal, scale, table)
+    if sequences is not None:
+        a = _lib.MsdAttn.from_buffer_copy(a)   # (the cached one is shared by threads)
+        a.seqs = sequences.table.data_ptr()
+    return ctypes.byref(a), fwd, bwd
+
+
+def _check(q, k, v, scale, sequences):
+    if q.dim() not in (3, 4) or k.dim() != q.dim() or v.shape != k.shape:
+        raise ValueError(f"q (batch, rows, heads, d_head) or (rows, heads, d_head) and k, v alike expected, got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    if not q.dtype == k.dtype == v.dtype == torch.bfloat16:
+        raise ValueError("q, k and v must be bfloat16")
+    if not (q.is_cuda and k.is_cuda and v.is_cuda) or not q.device == k.device == v.device:
+        raise ValueError("q, k and v must be on one GPU")
+    D, H, KV = q.shape[-1], q.shape[-2], k.shape[-2]
+    if k.shape[-1] != D or D % 8 or not 0 < D <= 128:
+        raise ValueError(f"d_head must be a multiple of 8 up to 128, the same for q, k and v (got {D} and {k.shape[-1]})")
+    if KV == 0 or H == 0 or H % KV:
+        raise ValueError(f"n_heads ({H}) must be a multiple of n_kv_heads ({KV})")
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"scale must be positive (got {scale})")
+    if q.dim() == 4 and q.shape[0] != k.shape[0]:
+        raise ValueError(f"q holds {q.shape[0]} sequences, k and v {k.shape[0]}")
+    if sequences is not None:
+        if q.dim() != 3:
+            raise ValueError("sequences go with flat q (rows, heads, d_head)")
+        if sequences.q_end > q.shape[0] or sequences.k_end > k.shape[0]:
+            raise ValueError(f"sequences reach row {sequences.q_end} of {q.shape[0]} query rows and row "
+                             f"{sequences.k_end} of {k.shape[0]} key rows")
+        if sequences.table.device != q.device:
+            raise ValueError(f"sequences were made for {sequences.table.device}, q is on {q.device}")
+
+
+def _empty(like, rows):
+    """A contiguous output of like's shape; zeros where the sequences leave rows out."""
+    whole = rows is None or rows == like.shape[0]
+    return (torch.empty if whole else torch.zeros)(like.shape, dtype=like.dtype, device=like.device)
+
+
+def _workspace(like, n):
+    return like.new_empty(n, dtype=torch.uint8) if n else None
+
+
+def _forward(q, k, v, causal, scale, sequences, keep):
+    q, k, v = _operand(q), _operand(k), _operand(v)
+    a, n, _ = _arguments(q, k, v, (0, 0, 0), causal, scale, sequences)
+    out = _empty(q, sequences and sequences.q_count)
+    lse = q.new_empty(out.shape[:-1], dtype=torch.float32) if keep else None
+    ws = _workspace(q, n)
+    _lib.launch(_lib.lib().msd_attn_forward, "msd_attn_forward", q.device, a, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                out.data_ptr(), lse.data_ptr() if keep else None, ws.data_ptr() if n else None)
+    return q, k, v, out, lse
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, causal, scale, sequences):
+        q, k, v, out, lse = _forward(q, k, v, causal, scale, sequences, True)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.how = causal, scale, sequences
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        causal, scale, sequences = ctx.how
+        dout = _operand(dout)
+        a, _, n = _arguments(q, k, v, _strides(dout), causal, scale, sequences)
+        dq = _empty(q, sequences and sequences.q_count)
+        dk, dv = (_empty(x, sequences and sequences.k_count) for x in (k, v))
+        ws = _workspace(q, n)
+        _lib.launch(_lib.lib().msd_attn_backward, "msd_attn_backward", q.device, a, q.data_ptr(), k.data_ptr(),
+                    v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                    dv.data_ptr(), ws.data_ptr() if n else None)
+        return dq, dk, dv, None, None, None
+
+
+def attention(q, k, v, causal=True, scale=None, sequences=None):
+    """softmax(scale q k^T) v for every head, q head h with k/v head h // (n_heads // n_kv_heads).
+
+    q (batch, Tq, n_heads, d_head), k and v (batch, Tk, n_kv_heads, d_head), or without the batch axis one sequence, or
+    with ``sequences`` (a ``Sequences``) several in flat tensors; bf16 on one GPU, any strides, d_head a multiple of 8 up
+    to 128.  ``causal``: query i sees keys 0 .. Tk - Tq + i (the last query the last key, as one token sees its cache).
+    A query that sees nothing has output 0.  ``scale`` defaults to d_head ** -0.5.  Returns q's shape, contiguous.
+
+    What lies behind a sequence's own rows is not read.  Within a sequence, a key or value row that is not finite
+    reaches every query that sees it, and may reach those that do not."""
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    _check(q, k, v, scale, sequences)
+    causal = bool(causal)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Attention.apply(q, k, v, causal, scale, sequences)
+    return _forward(q, k, v, causal, scale, sequences, False)[3]
