@@ -5,7 +5,7 @@
  *   msd_attn_forward, msd_attn_backward
  *                      <- model.py:122-147 causal_attention's dot_product_attention (q (T, n_heads, d_head), k and v
  *                         (T, n_kv, d_head)) and its gradient
- *   msd_rotary         <- model.py:110-119 apply_rope on q and k, and (sign -1) its gradient
+ *   msd_rope_apply     <- model.py:110-119 apply_rope on q and k, and (sign -1) its gradient
  *   msd_rms_forward, msd_rms_backward
  *                      <- model.py:94-98 rms_norm and :157 the residual's addition, and their gradients
  *   msd_swiglu_forward, msd_swiglu_backward
@@ -65,6 +65,64 @@ int32_t msd_attn_forward(const msd_attn* a, const void* q, const void* k, const 
 int32_t msd_attn_backward(const msd_attn* a, const void* q, const void* k, const void* v, const void* out,
                           const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
                           void* stream);
+
+/* Value types of the calls below. */
+enum { MSD_BF16 = 0, MSD_F32 = 1 };
+
+/* Rotary positions applied to q and k: batch x tokens rows of n_heads (n_kv_heads) heads of d_head contiguous values,
+ * by (batch, token, head) strides in elements; outputs contiguous, of the same type (MSD_BF16 or MSD_F32).  The first
+ * d_rot (even) values of a head are pairs, (i, i + d_rot / 2) or, interleaved, (2 i, 2 i + 1), i < d_rot / 2; pair i at
+ * position p becomes amplitude times itself turned by 2 pi p turns[i] (sign -1: back, which is the gradient).  The
+ * others are copied.  p: positions (device, 4- or 8-byte integers by position_bytes, (batch, token) strides), or, with
+ * position_bytes 0, start + token. */
+typedef struct msd_rope {
+  int32_t batch, tokens, n_heads, n_kv_heads, d_head, d_rot;
+  int32_t interleaved, type, sign, position_bytes;
+  float amplitude;
+  int64_t start;
+  int64_t q_stride[3], k_stride[3], position_stride[2];
+} msd_rope;
+
+/* turns: device f64 (d_rot / 2); the angle is formed in f64 and reduced to less than a turn before it is rounded.
+ * k and k_out may be NULL with n_kv_heads 0.  batch * tokens * (n_heads + n_kv_heads) * d_head < 2^40, d_head <= 4096,
+ * n_heads + n_kv_heads <= 4096. */
+int32_t msd_rope_apply(const msd_rope* r, const void* q, const void* k, const void* positions, const double* turns,
+                       void* q_out, void* k_out, void* stream);
+
+/* Bytes of an 8-bit checkpoint of rows x d values (16-byte aligned device memory): int8 rows padded to 128 columns,
+ * then one f32 scale per row and 128 columns.  For the block's largest magnitude m, a value x is kept as
+ * rint(x * (127 / m)) and stands for that times (m / 127), all in f32; a block below 2^-100 is kept as zeros; a block
+ * that holds a NaN or an infinity stands for NaN. */
+int64_t msd_checkpoint_bytes(int64_t rows, int32_t d);
+
+/* y = s / sqrt(mean(s^2) + eps) * scale per row of d values, s = x + residual rounded to their type (x itself without a
+ * residual).  x, residual: rows of d contiguous values, `*_stride` elements apart, of `type`; y and sum (= s; NULL
+ * without a residual) contiguous, of the same type; scale (d) of scale_type.  rstd: f32 (rows), or NULL when no backward
+ * follows; checkpoint: NULL, or msd_checkpoint_bytes(rows, d) for s * rstd in 8 bits.  1 <= d <= 16384, rows < 2^31. */
+int32_t msd_rms_forward(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                        const void* scale, int32_t scale_type, int64_t rows, int32_t d, int32_t type, float eps, void* y,
+                        void* sum, float* rstd, void* checkpoint, void* stream);
+
+/* Bytes of msd_rms_backward's workspace (needs no initialisation; belongs to one call at a time). */
+int64_t msd_rms_workspace_bytes(int64_t rows, int32_t d);
+
+/* dx (contiguous): the gradient of x, and of the residual: rstd (dy scale - n mean(dy scale n)) + dsum with n = s rstd;
+ * dsum NULL or the gradient of `sum`.  dscale (of scale_type; NULL: not wanted): sum over the rows of dy n, the rows'
+ * f32 partial sums added in a fixed order.  From s (the forward's sum, or x) or, when checkpoint is not NULL, from the
+ * forward's checkpoint in place of n. */
+int32_t msd_rms_backward(const void* s, int64_t s_stride, const float* rstd, const void* checkpoint, const void* scale,
+                         int32_t scale_type, const void* dy, int64_t dy_stride, const void* dsum, int64_t dsum_stride,
+                         int64_t rows, int32_t d, int32_t type, void* dx, void* dscale, void* workspace, void* stream);
+
+/* y = gate / (1 + exp(-gate)) * up, rows of d contiguous values `*_stride` elements apart, y contiguous.  checkpoint:
+ * NULL, or 2 msd_checkpoint_bytes(rows, d): gate's, then up's.  d >= 1, rows * d < 2^40, d < 2^24. */
+int32_t msd_swiglu_forward(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, int64_t rows,
+                           int32_t d, int32_t type, void* y, void* checkpoint, void* stream);
+
+/* dgate, dup (contiguous) from gate and up or, when checkpoint is not NULL, from the forward's checkpoint. */
+int32_t msd_swiglu_backward(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride,
+                            const void* checkpoint, const void* dy, int64_t dy_stride, int64_t rows, int32_t d,
+                            int32_t type, void* dgate, void* dup, void* stream);
 
 #ifdef __cplusplus
 }

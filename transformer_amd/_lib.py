@@ -28,7 +28,9 @@ EXPORTS = ("msd_packed_weight_elems", "msd_workspace_bytes", "msd_default_workgr
            "msd_decode_steps", "msd_tiles_bytes", "msd_pack_tiles", "msd_set_launch_graphs",
            "msd_config_support", "msd_xent_workspace_bytes", "msd_xent_plan",
            "msd_xent_targets", "msd_xent_forward", "msd_xent_backward",
-           "msd_attn_workspace_bytes", "msd_attn_forward", "msd_attn_backward")
+           "msd_attn_workspace_bytes", "msd_attn_forward", "msd_attn_backward", "msd_rope_apply",
+           "msd_checkpoint_bytes", "msd_rms_forward", "msd_rms_workspace_bytes", "msd_rms_backward",
+           "msd_swiglu_forward", "msd_swiglu_backward")
 
 # Paths of the library (bits of msd_config_support)
 PATHS = {"decode": 1, "prefill": 2, "verify": 4, "batched": 8, "sample": 16, "batched_step": 32}
@@ -50,6 +52,14 @@ class MsdAttn(ctypes.Structure):
     _fields_ += [("scale", ctypes.c_float), ("q_rows", ctypes.c_int64), ("k_rows", ctypes.c_int64)]
     _fields_ += [(k, ctypes.c_int64 * 3) for k in ("q_stride", "k_stride", "v_stride", "dout_stride")]
     _fields_ += [("seqs", ctypes.c_void_p)]
+
+
+class MsdRope(ctypes.Structure):
+    """Rotary positions of one call (include/mslayers.h): strides are (batch, token, head), in elements."""
+    _fields_ = [(k, ctypes.c_int32) for k in ("batch", "tokens", "n_heads", "n_kv_heads", "d_head", "d_rot", "interleaved",
+                                              "type", "sign", "position_bytes")]
+    _fields_ += [("amplitude", ctypes.c_float), ("start", ctypes.c_int64), ("q_stride", ctypes.c_int64 * 3),
+                 ("k_stride", ctypes.c_int64 * 3), ("position_stride", ctypes.c_int64 * 2)]
 
 
 class MsdError(RuntimeError):
@@ -148,8 +158,44 @@ def lib():
     L.msd_attn_forward.restype = I32
     L.msd_attn_backward.argtypes = [AP, P, P, P, P, P, P, P, P, P, P, P]
     L.msd_attn_backward.restype = I32
+    F = ctypes.c_float
+    L.msd_rope_apply.argtypes = [ctypes.POINTER(MsdRope), P, P, P, P, P, P, P]
+    L.msd_rope_apply.restype = I32
+    L.msd_checkpoint_bytes.argtypes = [I64, I32]
+    L.msd_checkpoint_bytes.restype = I64
+    L.msd_rms_forward.argtypes = [P, I64, P, I64, P, I32, I64, I32, I32, F, P, P, P, P, P]
+    L.msd_rms_forward.restype = I32
+    L.msd_rms_workspace_bytes.argtypes = [I64, I32]
+    L.msd_rms_workspace_bytes.restype = I64
+    L.msd_rms_backward.argtypes = [P, I64, P, P, P, I32, P, I64, P, I64, I64, I32, I32, P, P, P, P]
+    L.msd_rms_backward.restype = I32
+    L.msd_swiglu_forward.argtypes = [P, I64, P, I64, I64, I32, I32, P, P, P]
+    L.msd_swiglu_forward.restype = I32
+    L.msd_swiglu_backward.argtypes = [P, I64, P, I64, P, P, I64, I64, I32, I32, P, P, P]
+    L.msd_swiglu_backward.restype = I32
     _lib = L
     return L
+
+
+# Value types of the layer operators (include/mslayers.h)
+TYPES = {torch.bfloat16: 0, torch.float32: 1}
+
+
+def rows_of(x):
+    """(x as rows of contiguous values, the stride between them): a view wherever x's strides allow one."""
+    x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+    if x.shape[1] > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    return x, x.stride(0) if x.shape[0] > 1 else 0
+
+
+def keep_bytes(rows, d, checkpoint):
+    """Bytes of one tensor's checkpoint (msd_checkpoint_bytes); 0 where it is kept as it is."""
+    if checkpoint is None:
+        return 0
+    if checkpoint != "int8":
+        raise ValueError(f'checkpoint must be None or "int8" (got {checkpoint!r})')
+    return check(lib().msd_checkpoint_bytes(rows, d), "msd_checkpoint_bytes")
 
 
 def launch(fn, what, device, *args):

@@ -18,7 +18,7 @@ HIPCC_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-shared", f"--offload-arch={ARCH}"
 
 LIBS = {
     "libmsdecode.so": ["csrc/msdecode.hip", "csrc/sample.hip", "csrc/prefill.hip", "csrc/batched.hip",
-                       "csrc/xent.hip", "csrc/attn.hip"],
+                       "csrc/xent.hip", "csrc/attn.hip", "csrc/layers.hip"],
 }
 
 
