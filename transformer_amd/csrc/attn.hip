@@ -50,7 +50,10 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kKeys = 64;        // rows of an LDS tile
+constexpr int kKeys = 64;        // keys of an LDS tile
+// Rows of an LDS tile of q and dout
+template <int DP>
+constexpr int tile_rows() { return DP <= 64 ? 64 : 32; }
 constexpr uint32_t kOutside = 0x80000000u;   // a buffer offset past every descriptor: the load gives zeros
 
 struct View {
@@ -64,14 +67,16 @@ struct Args {
   const int32_t* seqs;
   int n_seqs, q_len, k_len;
   int H, KV, g, D, causal;
-  uint32_t g_magic;         // r / g = umulhi(r, g_magic) for g > 1, r < 2^31 (see magic())
+  uint32_t g_magic;         // r / g = umulhi(2 r, g_magic) >> g_shift for r < 2^30 (see magic())
   int g_shift;
   float c, scale;
   int tiles;                // row (or key) tiles of the longest sequence
-  int splits;
+  int splits;               // forward: of the keys
+  int tile_rows, head_parts, row_parts, chunk;   // dK and dV: see KeyPart
   int64_t q_rows, k_rows;
   uint16_t *out, *dq, *dk, *dv;
-  float *lse, *delta;
+  float* lse;
+  float* stats;             // backward: (-lse / c, -D) of every row, in the order of lse
   float* part;              // forward: [splits][q_rows * H][D + 1]; backward: [2][splits][k_rows * KV][D]
 };
 
@@ -92,7 +97,7 @@ __device__ __forceinline__ const uint16_t* origin(const Args& p, const View& v, 
 }
 
 __device__ __forceinline__ int div_g(const Args& p, int r) {
-  return p.g_magic ? int(__umulhi(uint32_t(r), p.g_magic) >> p.g_shift) : r >> p.g_shift;
+  return int(__umulhi(2 * uint32_t(r), p.g_magic) >> p.g_shift);
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -123,13 +128,37 @@ __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
 #endif
 }
 
-// 16 bytes at byte offset `off` of the tensor part at `base` (wave-uniform), zeros for kOutside
-__device__ __forceinline__ u32x4 load16(const uint16_t* base, uint32_t off) {
+// 64 lanes' 16 bytes at byte offsets `off` from `base` (wave-uniform) straight to the 1 KB of LDS at byte address `to`
+// (lane after lane); kOutside gives zeros.  In assembly, because the compiler would wait for it before
+// every LDS read that follows; dma_wait() is the wait, and what the workgroup's other waves fetched needs its barrier too.
+// (m0, the LDS base, is set in the same statement: the compiler has no use of its own for it in these kernels.)
+__device__ __forceinline__ void dma(const uint16_t* base, uint32_t off, uint32_t to) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, 0x7fffffff, 0x00020000);
-  return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(r));
+#endif
+}
+// 64 lanes' 4 bytes to the 256 bytes of LDS at `to`
+__device__ __forceinline__ void dma4(const float* base, uint32_t off, uint32_t to) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, 0x7fffffff, 0x00020000);
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(r));
+#endif
+}
+// Until at most N of this wave's loads are outstanding (they return in order).  The compiler counts it, so that its own
+// loads before the last N need no further wait.
+template <int N = 0>
+__device__ __forceinline__ void dma_wait() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+#endif
+}
+__device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef __attribute__((address_space(3))) const uint8_t lds_u8;
+  return uint32_t(__builtin_amdgcn_readfirstlane(int(reinterpret_cast<uintptr_t>((lds_u8*)p))));
 #else
-  return u32x4{};
+  return 0;
 #endif
 }
 
@@ -170,51 +199,26 @@ __device__ __forceinline__ bf16x8 cols_operand(const uint8_t* tile, int row0, in
 #endif
 }
 
-// A 64-row tile of K or V on its way to LDS
-template <int DP, int NT>
-struct KeyTile {
-  static constexpr int P = pitch<DP>(), C = P / 16, N = kKeys * C / NT;
-  u32x4 x[N];
-  __device__ __forceinline__ void load(const uint16_t* base, int64_t row_stride, int row0, int n_rows, int D, int tid) {
-    const uint16_t* at = base + int64_t(row0) * row_stride;
+// A tile of R rows on its way to LDS: wave w of NW fetches its instructions w, w + NW, ..
+template <int DP, int NW, int R = kKeys>
+struct Tile {
+  static constexpr int P = pitch<DP>(), C = P / 16, N = R * P / 1024 / NW;
+  static_assert(64 * NW % C == 0, "an instruction's rows are a fixed number apart");
+  int row;            // of the first instruction
+  uint32_t off[N];
+  __device__ __forceinline__ void init(int64_t row_stride, int D, int lane, int wv) {
+    row = (64 * wv + lane) / C;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int i = tid + NT * u, r = i / C, c = i % C;
-      x[u] = load16(at, row0 + r < n_rows && 8 * c < D ? uint32_t(r) * uint32_t(row_stride) * 2 + 16 * c : kOutside);
+      const int r = row + 64 * NW / C * u, c = (64 * wv + lane) % C ^ swizzle<P>(r);
+      off[u] = 8 * c < D ? uint32_t(r) * uint32_t(row_stride) * 2 + 16 * c : kOutside;
     }
   }
-  __device__ __forceinline__ void store(uint8_t* tile, int tid) const {
+  // rows from `base` on, `left` of which exist: the others are zeros
+  __device__ __forceinline__ void load(uint8_t* tile, const uint16_t* base, int left, int wv) const {
+    const uint32_t to = lds_address(tile) + 1024 * wv;
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int i = tid + NT * u, r = i / C, c = i % C;
-      *reinterpret_cast<u32x4*>(tile + piece_at<P>(r, c)) = x[u];
-    }
-  }
-};
-
-// A 64-row tile of q or dout rows (position r / g, head r % g)
-template <int DP, int NT>
-struct RowTile {
-  static constexpr int P = pitch<DP>(), C = P / 16, N = kKeys * C / NT;
-  u32x4 x[N];
-  __device__ __forceinline__ void load(const Args& p, const uint16_t* base, const View& v, int row0, int n_rows,
-                                       int tid) {
-    const int pos0 = div_g(p, row0);
-    const uint16_t* at = base + int64_t(pos0) * v.row;
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int i = tid + NT * u, r = row0 + i / C, c = i % C, pos = div_g(p, r);
-      x[u] = load16(at, r < n_rows && 8 * c < p.D ? (uint32_t(pos - pos0) * uint32_t(v.row) +
-                                                     uint32_t(r - pos * p.g) * uint32_t(v.head)) * 2 + 16 * c
-                                                  : kOutside);
-    }
-  }
-  __device__ __forceinline__ void store(uint8_t* tile, int tid) const {
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int i = tid + NT * u, r = i / C, c = i % C;
-      *reinterpret_cast<u32x4*>(tile + piece_at<P>(r, c)) = x[u];
-    }
+    for (int u = 0; u < N; ++u) dma(base, row + 64 * NW / C * u < left ? off[u] : kOutside, to + 1024 * NW * u);
   }
 };
 
@@ -237,6 +241,13 @@ __device__ __forceinline__ void wave_lds_order() {
 #if defined(__HIP_DEVICE_COMPILE__)
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
+#endif
+}
+
+// LDS reads and matrix products keep their order across; other arithmetic may move
+__device__ __forceinline__ void order_reads() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_sched_barrier(0x406);
 #endif
 }
 
@@ -300,15 +311,18 @@ __device__ __forceinline__ bool row_job(const Args& p, RowJob& j, int lane, int 
   return true;
 }
 
+// Where a row's statistics lie: sequence by sequence, head by head
 __device__ __forceinline__ int64_t stat_index(const Args& p, const RowJob& j) {
-  return int64_t(j.s.qs) * p.H + int64_t(j.kvh) * j.rows + j.r;
+  return int64_t(j.s.qs) * p.H + int64_t(j.head) * j.s.qn + j.pos;
 }
 
 // ---- forward ----
+// Per 32 keys: the scores' maximum; the probabilities, while the matrix cores form the next 32 keys' scores; then their
+// product with V.  So the scores run 32 keys ahead, K one tile ahead of V: three K buffers and two of V, one barrier a tile.
 template <int DP, int NW>
 __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attn_fwd(Args p) {
-  constexpr int P = pitch<DP>(), TILE = kKeys * P, NT = 64 * NW;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TILE];
+  constexpr int P = pitch<DP>(), TILE = kKeys * P;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[5 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   RowJob j;
   if (!row_job<NW>(p, j, lane, wv)) return;
@@ -321,73 +335,81 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attn_fwd(Args p) {
   f32x16 o[DP / 32] = {};
   float m = -INFINITY, l = 0;   // running maximum of c s, up to 2^8 too small; sum of 2^(c s - m) over this lane's keys
 
-  KeyTile<DP, NT> kt, vt;
+  auto scores = [&](const uint8_t* K, int row0) {
+    f32x16 s = {};
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) s = mfma(rows_operand<P>(K, row0, ks, lane), q[ks], s);
+    return s;
+  };
+  // s: the scores of 32 keys from key0, which lie from row0 of V; next: where the next 32 keys' K rows lie
+  auto step = [&](f32x16& s, f32x16& ahead, const uint8_t* V, int row0, int key0, const uint8_t* next, int next_row0) {
+    if (key0 + 32 > j.wave_full) {   // the diagonal or the end
+      const int left = j.seen - key0 - 4 * (lane >> 5);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i >> 2) + (i & 3) >= left) s[i] = -INFINITY;
+    }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+    top = fmaxf(top, swap_halves(top)) * p.c;
+    if (__any(top > m + 8.0f)) {   // rescaling by less than 2^8 can wait: f32 sums and bf16 P keep their precision
+      const float mn = fmaxf(m, top), by = mn == -INFINITY ? 1.0f : exp2_hw(m - mn);
+      m = mn;
+      l *= by;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) o[d] *= by;
+    }
+    const float sub = m == -INFINITY ? 0.0f : m;
+    ahead = scores(next, next_row0);
+    float sum = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = exp2_hw(fmaf(s[i], p.c, -sub));
+      sum += s[i];
+    }
+    l += sum;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bf16x8 pr = pack8(s, 8 * h);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) o[d] = mfma(cols_operand<P>(V, row0 + 16 * h, d, lane), pr, o[d]);
+    }
+  };
+
+  Tile<DP, NW> kt, vt;
+  kt.init(p.k.row, p.D, lane, wv);
+  vt.init(p.v.row, p.D, lane, wv);
+  auto load_k = [&](uint8_t* to, int t) { kt.load(to, kb + int64_t(t) * kKeys * p.k.row, j.s.kn - t * kKeys, wv); };
+  auto load_v = [&](uint8_t* to, int t) { vt.load(to, vb + int64_t(t) * kKeys * p.v.row, j.s.kn - t * kKeys, wv); };
+  uint8_t *k0 = lds, *k1 = lds + TILE, *k2 = lds + 2 * TILE, *v0 = lds + 3 * TILE, *v1 = lds + 4 * TILE;
+  f32x16 s0, s1;
   if (j.t0 < j.t1) {
-    kt.load(kb, p.k.row, j.t0 * kKeys, j.s.kn, p.D, tid);
-    vt.load(vb, p.v.row, j.t0 * kKeys, j.s.kn, p.D, tid);
-    kt.store(lds, tid);
-    vt.store(lds + TILE, tid);
+    load_k(k0, j.t0);
+    load_v(v0, j.t0);
+    load_k(k1, j.t0 + 1);
   }
+  dma_wait();
   __syncthreads();
+  if (j.t0 < j.t1) s0 = scores(k0, 0);
   for (int t = j.t0; t < j.t1; ++t) {
-    const uint8_t* K = lds + ((t - j.t0) & 1) * 2 * TILE;
-    const uint8_t* V = K + TILE;
-    uint8_t* next = lds + ((t - j.t0 + 1) & 1) * 2 * TILE;
     if (t + 1 < j.t1) {
-      kt.load(kb, p.k.row, (t + 1) * kKeys, j.s.kn, p.D, tid);
-      vt.load(vb, p.v.row, (t + 1) * kKeys, j.s.kn, p.D, tid);
+      load_k(k2, t + 2);
+      load_v(v1, t + 1);
     }
     const int key0 = t * kKeys;
     if (key0 < j.wave_end) {
-      f32x16 s[2] = {};
-#pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) s[b] = mfma(rows_operand<P>(K, 32 * b, ks, lane), q[ks], s[b]);
-      if (key0 + kKeys > j.wave_full) {   // the diagonal or the end
-        const int left = j.seen - key0 - 4 * (lane >> 5);
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * b + 8 * (i >> 2) + (i & 3) >= left) s[b][i] = -INFINITY;
-      }
-      float top = s[0][0];
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-      top = fmaxf(top, swap_halves(top)) * p.c;
-      if (__any(top > m + 8.0f)) {   // rescaling by less than 2^8 can wait: f32 sums and bf16 P keep their precision
-        const float mn = fmaxf(m, top), by = mn == -INFINITY ? 1.0f : exp2_hw(m - mn);
-        m = mn;
-        l *= by;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) o[d] *= by;
-      }
-      const float sub = m == -INFINITY ? 0.0f : m;
-      float sum = 0;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[b][i] = exp2_hw(fmaf(s[b][i], p.c, -sub));
-          sum += s[b][i];
-        }
-      l += sum;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const bf16x8 pr = pack8(s[b], 8 * h);
-#pragma unroll
-          for (int d = 0; d < DP / 32; ++d) o[d] = mfma(cols_operand<P>(V, 32 * b + 16 * h, d, lane), pr, o[d]);
-        }
+      step(s0, s1, v0, 0, key0, k0, 32);
+      step(s1, s0, v0, 32, key0 + 32, k1, 0);
     }
-    if (t + 1 < j.t1) {
-      kt.store(next, tid);
-      vt.store(next + TILE, tid);
-    }
+    uint8_t* k = k0;
+    k0 = k1;
+    k1 = k2;
+    k2 = k;
+    uint8_t* v = v0;
+    v0 = v1;
+    v1 = v;
+    dma_wait();
     __syncthreads();
   }
   l += swap_halves(l);
@@ -427,7 +449,7 @@ __global__ void attn_join(Args p) {
   const int64_t rows = int64_t(s.qn) * p.H, row = id / per;
   if (row >= rows) return;
   const int c = int(id - row * per) * 8;
-  const int64_t at = int64_t(s.qs) * p.H + row;   // statistics order: kv head, position, head of the group
+  const int64_t at = int64_t(s.qs) * p.H + row;   // in the statistics' order
   const float* w = p.part + int64_t(p.splits) * n * p.D;
   float m = -INFINITY;
   for (int z = 0; z < p.splits; ++z) {
@@ -445,19 +467,19 @@ __global__ void attn_join(Args p) {
     for (int i = 0; i < 8; ++i) acc[i] = fmaf(e, from[i], acc[i]);
   }
   const float by = l == 0 ? 0.0f : 1.0f / l;
-  const int kvh = int(row / (int64_t(s.qn) * p.g)), r = int(row - int64_t(kvh) * s.qn * p.g), pos = r / p.g;
+  const int head = int(row) / s.qn, pos = int(row) - head * s.qn;
   u32x4 x;
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = pack2(acc[2 * i] * by, acc[2 * i + 1] * by);
-  *reinterpret_cast<u32x4*>(p.out + (int64_t(s.qs + pos) * p.H + kvh * p.g + (r - pos * p.g)) * p.D + c) = x;
+  *reinterpret_cast<u32x4*>(p.out + (int64_t(s.qs + pos) * p.H + head) * p.D + c) = x;
   if (p.lse && c == 0) p.lse[at] = l == 0 ? INFINITY : m + __log2f(l);
 }
 
 // ---- backward ----
-// dQ of 32 rows a wave; also D_i = dO_i.O_i, which attn_dkv reads
+// dQ of 32 rows a wave; also D_i = dO_i.O_i, which attn_dkv reads beside lse
 template <int DP, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p) {
-  constexpr int P = pitch<DP>(), TILE = kKeys * P, NT = 64 * NW;
+  constexpr int P = pitch<DP>(), TILE = kKeys * P;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   RowJob j;
@@ -480,25 +502,24 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p) {
   }
   delta += swap_halves(delta);
   const float lse = j.ok ? p.lse[stat_index(p, j)] : INFINITY;
-  if (j.ok && lane < 32) p.delta[stat_index(p, j)] = delta;
+  if (j.ok && lane < 32) *reinterpret_cast<f32x2*>(p.stats + 2 * stat_index(p, j)) = f32x2{-lse / p.c, -delta};
 
   f32x16 dq[DP / 32] = {};
-  KeyTile<DP, NT> kt, vt;
-  if (j.t0 < j.t1) {
-    kt.load(kb, p.k.row, j.t0 * kKeys, j.s.kn, p.D, tid);
-    vt.load(vb, p.v.row, j.t0 * kKeys, j.s.kn, p.D, tid);
-    kt.store(lds, tid);
-    vt.store(lds + TILE, tid);
-  }
+  Tile<DP, NW> kt, vt;
+  kt.init(p.k.row, p.D, lane, wv);
+  vt.init(p.v.row, p.D, lane, wv);
+  auto load = [&](uint8_t* to, int t) {
+    kt.load(to, kb + int64_t(t) * kKeys * p.k.row, j.s.kn - t * kKeys, wv);
+    vt.load(to + TILE, vb + int64_t(t) * kKeys * p.v.row, j.s.kn - t * kKeys, wv);
+  };
+  if (j.t0 < j.t1) load(lds, j.t0);
+  dma_wait();
   __syncthreads();
   for (int t = j.t0; t < j.t1; ++t) {
-    const uint8_t* K = lds + ((t - j.t0) & 1) * 2 * TILE;
+    uint8_t* K = lds + ((t - j.t0) & 1) * 2 * TILE;
     const uint8_t* V = K + TILE;
     uint8_t* next = lds + ((t - j.t0 + 1) & 1) * 2 * TILE;
-    if (t + 1 < j.t1) {
-      kt.load(kb, p.k.row, (t + 1) * kKeys, j.s.kn, p.D, tid);
-      vt.load(vb, p.v.row, (t + 1) * kKeys, j.s.kn, p.D, tid);
-    }
+    if (t + 1 < j.t1) load(next, t + 1);
     const int key0 = t * kKeys;
     if (key0 < j.wave_end) {
       const bool edge = key0 + kKeys > j.wave_full;
@@ -511,12 +532,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p) {
           s = mfma(rows_operand<P>(K, 32 * b, ks, lane), q[ks], s);
           dp = mfma(rows_operand<P>(V, 32 * b, ks, lane), dO[ks], dp);
         }
+        if (edge)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float x = exp2_hw(fmaf(s[i], p.c, -lse)) * (dp[i] - delta);
-          if (edge && 32 * b + 8 * (i >> 2) + (i & 3) >= left) x = 0;
-          s[i] = x;
-        }
+          for (int i = 0; i < 16; ++i)
+            if (32 * b + 8 * (i >> 2) + (i & 3) >= left) s[i] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = exp2_hw(fmaf(s[i], p.c, -lse)) * (dp[i] - delta);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const bf16x8 ds = pack8(s, 8 * h);
@@ -525,10 +546,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p) {
         }
       }
     }
-    if (t + 1 < j.t1) {
-      kt.store(next, tid);
-      vt.store(next + TILE, tid);
-    }
+    dma_wait();
     __syncthreads();
   }
   const int r0 = j.r - (lane & 31);
@@ -539,135 +557,268 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p) {
   });
 }
 
-// dK and dV of 128 keys, 32 a wave; the rows of all heads of the group, 64 at a time
+// Row tiles of R rows (of one head) that see a key of the 128 of block kb: [first, first + n)
+__device__ __forceinline__ int row_tiles(const Args& p, const Seq& s, int kb, int& first) {
+  first = p.causal ? min(max(128 * kb - (s.kn - s.qn), 0), s.qn) / p.tile_rows : 0;
+  return (s.qn + p.tile_rows - 1) / p.tile_rows - first;
+}
+
+// The work on 128 keys: the row tiles of the group's heads, head by head.  The heads are shared out to p.head_parts parts,
+// each part's list of tiles to p.row_parts parts of p.chunk tiles for one head, of which the block's first `parts` are not
+// empty.
+struct KeyPart {
+  int n, first;   // row tiles a head
+  int t0, t1, parts;
+};
+__device__ __forceinline__ KeyPart key_part(const Args& p, const Seq& s, int kb, int z, int n_heads) {
+  KeyPart k;
+  k.n = row_tiles(p, s, kb, k.first);
+  const int n = k.n * n_heads, chunk = p.chunk * n_heads;
+  k.parts = max((k.n + p.chunk - 1) / p.chunk, 1);
+  k.t0 = min(z * chunk, n);
+  k.t1 = min(k.t0 + chunk, n);
+  return k;
+}
+
+// The way through the row tiles of a part, from the last rows to the first, head by head: where the next tile
+// lies.  Workgroups of one K/V head start on the same rows and so share them in L2.
 template <int DP>
-__global__ __launch_bounds__(256, 2) void attn_dkv(Args p) {
-  constexpr int P = pitch<DP>(), TILE = kKeys * P, NT = 256;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TILE];
-  __shared__ __attribute__((aligned(16))) float stats[2][3][64];   // lse, D and the keys seen, of a tile's rows
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int heads = p.n_seqs * p.KV, id = blockIdx.x % heads, b = id / p.KV, kvh = id % p.KV;
-  const Seq s = sequence(p, b);
-  const int kb0 = int(blockIdx.x / heads) * 128;   // (the first keys are seen by the most rows)
-  if (kb0 >= s.kn) return;
-  const int k0 = kb0 + 32 * wv, key = k0 + (lane & 31);
-  const bool ok = key < s.kn;
-  const int rows = s.qn * p.g, last = s.kn - s.qn + 1;
-  const uint16_t* qb = origin(p, p.q, b, s.qs, kvh * p.g);
-  const uint16_t* db = origin(p, p.dout, b, s.qs, kvh * p.g);
-
-  bf16x8 k[DP / 16], v[DP / 16];
-  row_operands<DP>(k, origin(p, p.k, b, s.ks, kvh), int64_t(key) * p.k.row, ok, p.D, lane);
-  row_operands<DP>(v, origin(p, p.v, b, s.ks, kvh), int64_t(key) * p.v.row, ok, p.D, lane);
-
-  // row tiles that see a key of this workgroup, and this split's part of them
-  const int first = p.causal ? min(max(kb0 - last + 1, 0), s.qn) * p.g / 64 : 0;
-  const int n = (rows + 63) / 64 - first;
-  const int t0 = first + int(int64_t(n) * blockIdx.y / p.splits), t1 = first + int(int64_t(n) * (blockIdx.y + 1) / p.splits);
-  const int64_t stat0 = int64_t(s.qs) * p.H + int64_t(kvh) * rows;
-
-  f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
-  RowTile<DP, NT> qt, dt;
-  float st = 0;
-  auto load = [&](int t) {
-    qt.load(p, qb, p.q, 64 * t, rows, tid);
-    dt.load(p, db, p.dout, 64 * t, rows, tid);
-    const int r = 64 * t + lane;
-    if (wv == 0) st = r < rows ? p.lse[stat0 + r] : INFINITY;
-    if (wv == 1) st = r < rows ? p.delta[stat0 + r] : 0.0f;
-    if (wv == 2) st = __int_as_float(r >= rows ? 0 : p.causal ? min(max(last + div_g(p, r), 0), s.kn) : s.kn);
-  };
-  auto store = [&](int buf) {
-    qt.store(lds + buf * 2 * TILE, tid);
-    dt.store(lds + buf * 2 * TILE + TILE, tid);
-    if (wv < 3) stats[buf][wv][lane] = st;
-  };
-  if (t0 < t1) {
-    load(t0);
-    store(0);
+struct RowStream {
+  static constexpr int R = tile_rows<DP>();
+  const uint16_t *q, *dout;
+  const float* stats;
+  int row0, left, before;   // its first row; tiles still to come, it included; tiles of its head before it
+  __device__ __forceinline__ void start(const Args& p, const KeyPart& w, const Seq& s, const uint16_t* q0, const uint16_t* d0,
+                                        const float* stats0) {
+    const int t = w.t0, n = max(w.n, 1), head = t / n;
+    left = w.t1 - t;
+    before = n - 1 - t % n;
+    row0 = (w.first + before) * R;
+    q = q0 + int64_t(head) * p.q.head + int64_t(row0) * p.q.row;
+    dout = d0 + int64_t(head) * p.dout.head + int64_t(row0) * p.dout.row;
+    stats = stats0 + 2 * (int64_t(head) * s.qn + row0);
   }
-  __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    const uint8_t* Q = lds + buf * 2 * TILE;
+  __device__ __forceinline__ void advance(const Args& p, const KeyPart& w, const Seq& s) {
+    --left;
+    row0 -= R;
+    q -= R * p.q.row;
+    dout -= R * p.dout.row;
+    stats -= 2 * R;
+    if (--before < 0) {   // to the next head's last rows
+      const int n = w.n;
+      before += n;
+      row0 += n * R;
+      q += int64_t(n * R) * p.q.row + p.q.head;
+      dout += int64_t(n * R) * p.dout.row + p.dout.head;
+      stats += 2 * (n * R + s.qn);
+    }
+  }
+};
+
+// dK and dV of 128 keys, 32 a wave.  Two workgroups a CU, so that one's first loads and last stores (8 us together) are
+// behind the other's products.
+template <int DP>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_dkv(Args p) {
+  constexpr int P = pitch<DP>(), R = tile_rows<DP>(), TILE = R * P, STAGE = 2 * TILE + 8 * R, S = DP <= 64 ? 3 : 2, SUB = R / 32;
+  constexpr int DB = DP / 32, LOADS = 2 * TILE / 1024 / 4 + 1;   // of a wave and stage
+  __shared__ __attribute__((aligned(16))) uint8_t lds[S * STAGE + 128 * P];
+  static_assert(sizeof(lds) <= 80 * 1024 && S * STAGE >= 4 * 32 * P, "two workgroups a CU; the results' staging");
+  uint8_t* vs = lds + S * STAGE;   // the workgroup's V rows: in registers they would spill
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // the first keys, which the most rows see, first; workgroups of the same rows are `jobs` apart: with 8 jobs, or a
+  // multiple, on one XCD
+  const int parts = p.head_parts * p.row_parts, jobs = p.n_seqs * p.KV * parts, id = blockIdx.x % jobs, kb = blockIdx.x / jobs;
+  const int z = id / (p.n_seqs * p.KV), zh = z / p.row_parts, zr = z % p.row_parts;
+  const int b = id / p.KV % p.n_seqs, kvh = id % p.KV;
+  const int h0 = zh * p.g / p.head_parts, n_heads = (zh + 1) * p.g / p.head_parts - h0;
+  const Seq s = sequence(p, b);
+  if (128 * kb >= s.kn) return;
+  const KeyPart w = key_part(p, s, kb, zr, n_heads);
+  if (zr >= w.parts) return;   // (a block that no row sees has one, which writes its zeros)
+  const int last = s.kn - s.qn + 1;
+  const uint16_t* qb = origin(p, p.q, b, s.qs, kvh * p.g + h0);
+  const uint16_t* db = origin(p, p.dout, b, s.qs, kvh * p.g + h0);
+  const float* sb = p.stats + 2 * (int64_t(s.qs) * p.H + int64_t(kvh * p.g + h0) * s.qn);
+  const int k0 = 128 * kb + 32 * wv, key = k0 + (lane & 31);
+  const bool ok = key < s.kn;
+  bf16x8 k[DP / 16];
+  row_operands<DP>(k, origin(p, p.k, b, s.ks, kvh), int64_t(key) * p.k.row, ok, p.D, lane);
+  Tile<DP, 4, 128> vt;
+  vt.init(p.v.row, p.D, lane, wv);
+  vt.load(vs, origin(p, p.v, b, s.ks, kvh) + int64_t(128 * kb) * p.v.row, s.kn - 128 * kb, wv);
+  Tile<DP, 4, R> qt, dt;
+  qt.init(p.q.row, p.D, lane, wv);
+  dt.init(p.dout.row, p.D, lane, wv);
+  // the (-lse / c, -D) pairs of a tile's rows as two rows of R: 64 lanes fetch one of them, or both of 32
+  const int stat_row = lane & (R - 1), stat_plane = R == 64 ? wv & 1 : lane >> 5;
+
+  f32x16 dk[DB] = {}, dv[DB] = {};
+  RowStream<DP> rs;
+  rs.start(p, w, s, qb, db, sb);
+  int slot_next = 0, slot = 0;
+  auto load = [&]() {   // (past the last tile too, of zeros: every stage is the same number of loads)
+    uint8_t* to = lds + slot_next * STAGE;
+    const int n = rs.left > 0 ? s.qn - rs.row0 : 0;
+    qt.load(to, rs.q, n, wv);
+    dt.load(to + TILE, rs.dout, n, wv);
+    dma4(rs.stats, stat_row < n ? 8 * stat_row + 4 * stat_plane : kOutside, lds_address(to + 2 * TILE) + (R == 64 ? 256 * (wv & 1) : 0));
+    rs.advance(p, w, s);
+    slot_next = slot_next + 1 == S ? 0 : slot_next + 1;
+  };
+  int rows[S - 1];   // the first rows of the tiles on their way
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) {
+    rows[i] = rs.row0;
+    load();
+  }
+  dma_wait();   // (for k, so that the compiler does not wait for all loads in the loop)
+  for (int t = w.t0; t < w.t1; ++t) {
+    // this wave's loads of the tile have landed; behind the barrier everyone's have, and the tile before is done with
+    dma_wait<(S - 2) * LOADS>();
+    __syncthreads();
+    const uint8_t* Q = lds + slot * STAGE;
     const uint8_t* dO = Q + TILE;
-    if (t + 1 < t1) load(t + 1);
-    // (uniform) whether every row of the tile sees all 32 keys of the wave
-    const int r_lo = 64 * t;
-    const bool edge = r_lo + 64 > rows || (p.causal && last + div_g(p, r_lo) < k0 + 32) || k0 + 32 > s.kn;
+    const float* stats = reinterpret_cast<const float*>(Q + 2 * TILE);
+    const int row0 = rows[0];
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      f32x16 sc = {}, dp = {};
+    for (int i = 0; i + 1 < S - 1; ++i) rows[i] = rows[i + 1];
+    rows[S - 2] = rs.row0;
+    load();
+    slot = slot + 1 == S ? 0 : slot + 1;
+
+    // The tile's products as a list of steps of W LDS operands; the operands of step n + 1 are on their way while step n
+    // multiplies (left to itself the compiler waits for each operand in turn).
+    constexpr int W = DP <= 64 ? 4 : 2, KS = DP / 16, SG = KS % W ? 2 : W, PG = W / 2, DG = DB % (W / 2) ? 1 : W / 2;
+    constexpr int M1 = KS / SG, M2 = KS / PG, M3 = 2 * DB / DG, N1 = SUB * M1, N2 = N1 + SUB * M2, N3 = N2 + SUB * M3;
+    bf16x8 f[2][W], pr[SUB][2], ds[SUB][2];
+    f32x16 sc[SUB], dp[SUB];   // they start as -lse / c and -D, row by row
+    auto read = [&](int n) {
+      bf16x8(&to)[W] = f[n & 1];
+      if (n < N1) {
+        const int a = n / M1, i0 = n % M1 * SG;
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
-        sc = mfma(rows_operand<P>(Q, 32 * a, ks, lane), k[ks], sc);
-        dp = mfma(rows_operand<P>(dO, 32 * a, ks, lane), v[ks], dp);
+        for (int i = 0; i < SG; ++i) to[i] = rows_operand<P>(Q, 32 * a, i0 + i, lane);
+      } else if (n < N2) {
+        const int a = (n - N1) / M2, i0 = (n - N1) % M2 * PG;
+#pragma unroll
+        for (int i = 0; i < PG; ++i) {
+          to[2 * i] = rows_operand<P>(dO, 32 * a, i0 + i, lane);
+          to[2 * i + 1] = rows_operand<P>(vs, 32 * wv, i0 + i, lane);
+        }
+      } else if (n < N3) {
+        const int a = (n - N2) / M3, h = (n - N2) % M3 / (DB / DG), d = (n - N2) % (DB / DG) * DG;
+#pragma unroll
+        for (int i = 0; i < DG; ++i) {
+          to[2 * i] = cols_operand<P>(dO, 32 * a + 16 * h, d + i, lane);
+          to[2 * i + 1] = cols_operand<P>(Q, 32 * a + 16 * h, d + i, lane);
+        }
       }
+    };
+    auto begin = [&](f32x16& x, const float* from) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int r = 32 * a + 8 * u + 4 * (lane >> 5);
-        const f32x4 lse = *reinterpret_cast<const f32x4*>(&stats[buf][0][r]);
-        const f32x4 del = *reinterpret_cast<const f32x4*>(&stats[buf][1][r]);
+        const f32x4 y = *reinterpret_cast<const f32x4*>(from + 8 * u + 4 * (lane >> 5));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = exp2_hw(fmaf(sc[4 * u + i], p.c, -lse[i]));
-          float y = x * (dp[4 * u + i] - del[i]);
-          if (edge && key >= __float_as_int(stats[buf][2][r + i])) x = y = 0;
-          sc[4 * u + i] = x;
-          dp[4 * u + i] = y;
+        for (int i = 0; i < 4; ++i) x[4 * u + i] = y[i];
+      }
+    };
+    begin(sc[0], stats);
+    read(0);
+#pragma unroll
+    for (int n = 0; n < N3; ++n) {
+      if (n < N2 && n + 1 < N1 && (n + 1) % M1 == 0) begin(sc[(n + 1) / M1], stats + 32 * ((n + 1) / M1));
+      if (n + 1 >= N1 && n + 1 < N2 && (n + 1 - N1) % M2 == 0) begin(dp[(n + 1 - N1) / M2], stats + R + 32 * ((n + 1 - N1) / M2));
+      read(n + 1);
+      order_reads();
+      bf16x8(&x)[W] = f[n & 1];
+      if (n < N1) {
+        const int a = n / M1, i0 = n % M1 * SG;
+#pragma unroll
+        for (int i = 0; i < SG; ++i) sc[a] = mfma(x[i], k[i0 + i], sc[a]);
+      } else if (n < N2) {
+        const int a = (n - N1) / M2;
+#pragma unroll
+        for (int i = 0; i < PG; ++i) dp[a] = mfma(x[2 * i], x[2 * i + 1], dp[a]);
+      } else {
+        const int a = (n - N2) / M3, h = (n - N2) % M3 / (DB / DG), d = (n - N2) % (DB / DG) * DG;
+#pragma unroll
+        for (int i = 0; i < DG; ++i) {
+          dv[d + i] = mfma(x[2 * i], pr[a][h], dv[d + i]);
+          dk[d + i] = mfma(x[2 * i + 1], ds[a][h], dk[d + i]);
         }
       }
+      if (n == N1 - 1) {
+        // the diagonal (rows that do not exist have q, dout, lse and D of 0 and add nothing; keys that do not exist are
+        // not stored)
+        if (p.causal && last + row0 < k0 + 32) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const bf16x8 pr = pack8(sc, 8 * h), ds = pack8(dp, 8 * h);
+          for (int a = 0; a < SUB; ++a) {
+            const int hidden = key - last - row0 - 32 * a - 4 * (lane >> 5);   // rows up to here do not see the key
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          dv[d] = mfma(cols_operand<P>(dO, 32 * a + 16 * h, d, lane), pr, dv[d]);
-          dk[d] = mfma(cols_operand<P>(Q, 32 * a + 16 * h, d, lane), ds, dk[d]);
+            for (int i = 0; i < 16; ++i)
+              if (8 * (i >> 2) + (i & 3) <= hidden) sc[a][i] = -INFINITY;
+          }
         }
+#pragma unroll
+        for (int a = 0; a < SUB; ++a) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[a][i] = exp2_hw(sc[a][i] * p.c);
+          pr[a][0] = pack8(sc[a], 0);
+          pr[a][1] = pack8(sc[a], 8);
+        }
+      }
+      if (n >= N1 && n < N2 && (n + 1 - N1) % M2 == 0) {
+        const int a = (n - N1) / M2;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dp[a][i] *= sc[a][i];
+        ds[a][0] = pack8(dp[a], 0);
+        ds[a][1] = pack8(dp[a], 8);
       }
     }
-    if (t + 1 < t1) store((t - t0 + 1) & 1);
-    __syncthreads();
   }
-  if (p.splits > 1) {
-    if (!ok) return;
-    const int64_t n = p.k_rows * p.KV * p.D;
-    float* to = p.part + int64_t(blockIdx.y) * n + (int64_t(s.ks + key) * p.KV + kvh) * p.D;
+  dma_wait();
+  __syncthreads();
+  if (parts > 1 && (p.head_parts > 1 || w.parts > 1)) {
+    float* to = p.part + ((int64_t(z) * p.k_rows + s.ks + key) * p.KV + kvh) * p.D;
+    const int64_t all = parts * p.k_rows * p.KV * p.D;
+    if (ok)
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+      for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int c = 32 * d + 8 * u + 4 * (lane >> 5);
-        if (c < p.D) {
-          *reinterpret_cast<f32x4*>(to + c) = f32x4{dk[d][4 * u], dk[d][4 * u + 1], dk[d][4 * u + 2], dk[d][4 * u + 3]};
-          *reinterpret_cast<f32x4*>(to + p.splits * n + c) =
-              f32x4{dv[d][4 * u], dv[d][4 * u + 1], dv[d][4 * u + 2], dv[d][4 * u + 3]};
+        for (int u = 0; u < 4; ++u) {
+          const int c = 32 * d + 8 * u + 4 * (lane >> 5);
+          if (c < p.D) {
+            *reinterpret_cast<f32x4*>(to + c) = f32x4{dk[d][4 * u], dk[d][4 * u + 1], dk[d][4 * u + 2], dk[d][4 * u + 3]};
+            *reinterpret_cast<f32x4*>(to + all + c) = f32x4{dv[d][4 * u], dv[d][4 * u + 1], dv[d][4 * u + 2], dv[d][4 * u + 3]};
+          }
         }
-      }
     return;
   }
   auto row = [&](uint16_t* base, int r) -> uint16_t* {
     return k0 + r < s.kn ? base + (int64_t(s.ks + k0 + r) * p.KV + kvh) * p.D : nullptr;
   };
-  uint8_t* stage = lds + wv * 32 * P;
-  store_rows<DP>(stage, dk, p.scale, p.D, lane, [&](int r) { return row(p.dk, r); });
-  store_rows<DP>(stage, dv, 1.0f, p.D, lane, [&](int r) { return row(p.dv, r); });
+  store_rows<DP>(lds + wv * 32 * P, dk, p.scale, p.D, lane, [&](int r) { return row(p.dk, r); });
+  store_rows<DP>(lds + wv * 32 * P, dv, 1.0f, p.D, lane, [&](int r) { return row(p.dv, r); });
 }
 
-// dK and dV as the sum of their parts, in the order of the splits: 8 values a thread, of the rows of a sequence
+// dK and dV as the sum of their parts, in order: 8 values a thread, of the rows of a sequence
 __global__ void attn_sum_parts(Args p) {
   const Seq s = sequence(p, blockIdx.y);
   const int64_t n = p.k_rows * p.KV * p.D, own = int64_t(s.kn) * p.KV * p.D;
   const int64_t i = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) * 8;
   if (i >= own) return;
-  const int64_t at = int64_t(s.ks) * p.KV * p.D + i;
   const bool v = blockIdx.z;
-  const float* from = p.part + (v ? p.splits * n : 0) + at;
+  const int64_t at = int64_t(s.ks) * p.KV * p.D + i;
+  const float* from = p.part + (v ? p.head_parts * p.row_parts * n : 0) + at;
+  const int kb = int(i / (p.KV * p.D)) / 128;
   f32x4 a = {}, b = {};
-  for (int z = 0; z < p.splits; ++z) {
-    a += *reinterpret_cast<const f32x4*>(from + z * n);
-    b += *reinterpret_cast<const f32x4*>(from + z * n + 4);
+  for (int zh = 0; zh < p.head_parts; ++zh) {
+    const KeyPart w = key_part(p, s, kb, 0, 1);
+    if (p.head_parts == 1 && w.parts == 1) return;   // written as they are
+    for (int z = 0; z < w.parts; ++z) {
+      a += *reinterpret_cast<const f32x4*>(from + (zh * p.row_parts + z) * n);
+      b += *reinterpret_cast<const f32x4*>(from + (zh * p.row_parts + z) * n + 4);
+    }
   }
   const float by = v ? 1.0f : p.scale;
   a *= by;
@@ -678,19 +829,19 @@ __global__ void attn_sum_parts(Args p) {
 // ---- host ----
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// r / g for 0 <= r < 2^31: a shift for powers of two, else umulhi by ceil(2^(32 + s) / g) with 2^s < g: the error g m -
-// 2^(32 + s) is below g <= 2^(s + 1), so r < 2^31 gives the exact quotient
+// m = ceil(2^(31 + s) / g) with 2^s <= g < 2^(s + 1): g m - 2^(31 + s) is below g < 2^(s + 1), so that floor(r m / 2^(31 +
+// s)) is r / g for r < 2^30
 void magic(uint32_t g, uint32_t& m, int& s) {
   s = 31 - __builtin_clz(g);
-  m = 0;
-  if ((g & (g - 1)) == 0) return;
-  m = uint32_t(((uint64_t(1) << (32 + s)) + g - 1) / g);
+  m = uint32_t(((uint64_t(1) << (31 + s)) + g - 1) / g);
 }
 
+constexpr int kLeast = 8;    // row tiles of a part at least
 struct Plan {
   int waves;          // of a forward or dQ workgroup
   int tiles, splits;  // forward: row tiles, splits of the keys
-  int dq_waves, dq_tiles, key_tiles, row_splits;
+  int dq_waves, dq_tiles, key_tiles;
+  int tile_rows, head_parts, row_parts, chunk;   // dK and dV: see KeyPart
 };
 
 constexpr int kCus = 256;
@@ -698,7 +849,7 @@ constexpr int64_t kMostGroups = (int64_t(1) << 32) / 256 - 1;   // a launch has 
 
 Plan plan(const msd_attn& a) {
   Plan p;
-  const int64_t heads = int64_t(a.n_seqs) * a.n_kv_heads, rows = int64_t(a.q_len) * (a.n_heads / a.n_kv_heads);
+  const int64_t heads = int64_t(a.n_seqs) * a.n_kv_heads, g = a.n_heads / a.n_kv_heads, rows = a.q_len * g;
   const int64_t key_tiles = std::max<int64_t>(cdiv(a.k_len, kKeys), 1);
   p.waves = heads * cdiv(rows, 128) >= kCus ? 4 : 1;
   p.tiles = int(cdiv(rows, 32 * p.waves));
@@ -707,8 +858,16 @@ Plan plan(const msd_attn& a) {
   p.dq_waves = p.waves;
   p.dq_tiles = p.tiles;
   p.key_tiles = int(cdiv(a.k_len, 128));
-  const int64_t wgs = heads * p.key_tiles;
-  p.row_splits = int(wgs >= 2 * kCus ? 1 : std::max<int64_t>(1, std::min(cdiv(2 * kCus, std::max<int64_t>(wgs, 1)), cdiv(rows, 128))));
+  // dK and dV: parts of a key block until every CU has two workgroups, four where the mask or the lengths make them uneven:
+  // the heads of a group first, then the rows, as long as a part's K, V and results are worth their traffic.  Sequences of
+  // different lengths are counted by their rows, so that the longest's workgroups do not outlast all others'.
+  const int64_t blocks = a.seqs ? a.n_kv_heads * cdiv(a.k_rows, 128) : heads * p.key_tiles;
+  const int64_t want = cdiv((a.causal || a.seqs ? 4 : 2) * kCus, std::max<int64_t>(blocks, 1));
+  p.head_parts = int(std::min<int64_t>(want, g));
+  p.tile_rows = a.d_head <= 64 ? tile_rows<64>() : tile_rows<128>();
+  const int64_t most = cdiv(a.q_len, p.tile_rows);
+  p.chunk = int(std::max<int64_t>(cdiv(most, cdiv(want, p.head_parts)), kLeast));
+  p.row_parts = int(std::max<int64_t>(1, cdiv(most, p.chunk)));
   return p;
 }
 
@@ -727,7 +886,7 @@ int32_t check(const msd_attn* a, bool backward) {
     return MSD_E_CONFIG;
   const int64_t most = int64_t(1) << 31;
   if (a->q_rows >= most || a->k_rows >= most || a->q_rows * a->n_heads >= most || a->k_rows * a->n_kv_heads >= most ||
-      int64_t(a->q_len) * a->n_heads >= most || int64_t(a->n_seqs) * a->n_kv_heads >= (1 << 20) || a->n_seqs > 65535)
+      int64_t(a->q_len) * (a->n_heads / a->n_kv_heads) >= (1 << 30) - 256 || int64_t(a->n_seqs) * a->n_kv_heads >= (1 << 20) || a->n_seqs > 65535)
     return MSD_E_CONFIG;
   if (!a->seqs && (a->q_rows != int64_t(a->n_seqs) * a->q_len || a->k_rows != int64_t(a->n_seqs) * a->k_len)) return MSD_E_CONFIG;
   if (a->q_len > a->q_rows || a->k_len > a->k_rows) return MSD_E_CONFIG;
@@ -788,8 +947,8 @@ extern "C" int64_t msd_attn_workspace_bytes(const msd_attn* a, int32_t backward)
   if (rc != MSD_OK) return rc;
   const Plan pl = plan(*a);
   if (!backward) return pl.splits > 1 ? 4 * pl.splits * a->q_rows * a->n_heads * (a->d_head + 1) : 0;
-  const int64_t parts = pl.row_splits > 1 ? 8 * pl.row_splits * a->k_rows * a->n_kv_heads * a->d_head : 0;
-  return up(4 * a->q_rows * a->n_heads) + parts;
+  const int64_t n = pl.head_parts * pl.row_parts, parts = n > 1 ? 8 * n * a->k_rows * a->n_kv_heads * a->d_head : 0;
+  return up(8 * a->q_rows * a->n_heads) + parts;
 }
 
 extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void* k, const void* v, void* out, float* lse,
@@ -830,14 +989,14 @@ extern "C" int32_t msd_attn_backward(const msd_attn* a, const void* q, const voi
       (a->k_len && (bad(k) || bad(v) || bad(dk) || bad(dv))))
     return MSD_E_ARG;
   const Plan pl = plan(*a);
-  if (bad(workspace) && (a->q_len || pl.row_splits > 1)) return MSD_E_ARG;
+  if (bad(workspace) && (a->q_len || pl.head_parts * pl.row_parts > 1)) return MSD_E_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
   Args p = args(*a, q, k, v);
   p.dout = view(dout, a->dout_stride);
   p.o = static_cast<const uint16_t*>(out);
   p.lse = const_cast<float*>(lse);
-  p.delta = static_cast<float*>(workspace);
-  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + up(4 * a->q_rows * a->n_heads));
+  p.stats = static_cast<float*>(workspace);
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + up(8 * a->q_rows * a->n_heads));
   p.dq = static_cast<uint16_t*>(dq);
   p.dk = static_cast<uint16_t*>(dk);
   p.dv = static_cast<uint16_t*>(dv);
@@ -853,11 +1012,14 @@ extern "C" int32_t msd_attn_backward(const msd_attn* a, const void* q, const voi
     }
     if (a->k_len) {
       p.tiles = pl.key_tiles;
-      p.splits = pl.row_splits;
-      hipLaunchKernelGGL((attn_dkv<DP>), dim3(unsigned(pl.key_tiles) * heads, pl.row_splits), dim3(256), 0, s, p);
+      p.tile_rows = pl.tile_rows;
+      p.head_parts = pl.head_parts;
+      p.row_parts = pl.row_parts;
+      p.chunk = pl.chunk;
+      hipLaunchKernelGGL((attn_dkv<DP>), dim3(unsigned(pl.key_tiles) * heads * (pl.head_parts * pl.row_parts)), dim3(256), 0, s, p);
     }
   });
-  if (a->k_len && pl.row_splits > 1) {
+  if (a->k_len && pl.head_parts * pl.row_parts > 1) {
     const int64_t n = int64_t(a->k_len) * a->n_kv_heads * (a->d_head / 8);
     hipLaunchKernelGGL(attn_sum_parts, dim3(unsigned(cdiv(n, 256)), a->n_seqs, 2), dim3(256), 0, s, p);
   }
