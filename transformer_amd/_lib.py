@@ -8,6 +8,7 @@ import ctypes
 import os
 
 import torch  # noqa: F401  (load torch's HIP runtime before the library)
+from torch.autograd.function import once_differentiable
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmsdecode.so")
@@ -177,16 +178,50 @@ def lib():
     return L
 
 
+# The raw handle of the current stream and the current device, without the objects around them: an operator's backward runs in
+# the autograd engine's thread, where every such call costs several times what it does elsewhere
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def launch(fn, what, index, *args):
+    """fn(*args, stream) on the current torch stream of GPU ``index``, with that GPU current; raises for its error code."""
+    if _device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc < 0:
+        raise MsdError(rc, what)
+
+
+def empty(x):
+    """A contiguous tensor of x's shape, type and device."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def first_order(backward):
+    """once_differentiable, without its cost where no second derivative is asked for (gradients are not recorded then)."""
+    slow = once_differentiable(backward)
+
+    def f(ctx, *grads):
+        return slow(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return f
+
+
 # Value types of the layer operators (include/mslayers.h)
 TYPES = {torch.bfloat16: 0, torch.float32: 1}
 
 
 def rows_of(x):
     """(x as rows of contiguous values, the stride between them): a view wherever x's strides allow one."""
-    x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
-    if x.shape[1] > 1 and x.stride(1) != 1:
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    row, col = x.stride()
+    if col != 1 and x.shape[1] > 1:
         x = x.contiguous()
-    return x, x.stride(0) if x.shape[0] > 1 else 0
+        row = x.stride(0)
+    return x, row   # (one row's stride is not used)
 
 
 def keep_bytes(rows, d, checkpoint):
@@ -196,15 +231,6 @@ def keep_bytes(rows, d, checkpoint):
     if checkpoint != "int8":
         raise ValueError(f'checkpoint must be None or "int8" (got {checkpoint!r})')
     return check(lib().msd_checkpoint_bytes(rows, d), "msd_checkpoint_bytes")
-
-
-def launch(fn, what, device, *args):
-    """fn(*args, stream) on the device's current torch stream, with that device current; raises for its error code."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        return check(fn(*args, stream), what)
-    with torch.cuda.device(device):
-        return check(fn(*args, stream), what)
 
 
 def check(code, what):

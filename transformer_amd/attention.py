@@ -15,7 +15,6 @@ import functools
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -140,8 +139,8 @@ def _check(q, k, v, scale, sequences):
 
 def _empty(like, rows):
     """A contiguous output of like's shape; zeros where the sequences leave rows out."""
-    whole = rows is None or rows == like.shape[0]
-    return (torch.empty if whole else torch.zeros)(like.shape, dtype=like.dtype, device=like.device)
+    x = _lib.empty(like)
+    return x if rows is None or rows == like.shape[0] else x.zero_()
 
 
 def _workspace(like, n):
@@ -150,34 +149,37 @@ def _workspace(like, n):
 
 def _forward(q, k, v, causal, scale, sequences, keep):
     q, k, v = _operand(q), _operand(k), _operand(v)
-    a, n, _ = _arguments(q, k, v, (0, 0, 0), causal, scale, sequences)
+    # dout's strides are the backward's own; a contiguous one's (out's) are put in here
     out = _empty(q, sequences and sequences.q_count)
-    lse = q.new_empty(out.shape[:-1], dtype=torch.float32) if keep else None
+    how = _arguments(q, k, v, _strides(out), causal, scale, sequences)
+    a, n, _ = how
+    lse = out.new_empty(out.shape[:-1], dtype=torch.float32) if keep else None
     ws = _workspace(q, n)
-    _lib.launch(_lib.lib().msd_attn_forward, "msd_attn_forward", q.device, a, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                out.data_ptr(), lse.data_ptr() if keep else None, ws.data_ptr() if n else None)
-    return q, k, v, out, lse
+    _lib.launch(_lib.lib().msd_attn_forward, "msd_attn_forward", out.get_device(), a, q.data_ptr(), k.data_ptr(),
+                v.data_ptr(), out.data_ptr(), lse.data_ptr() if keep else None, ws.data_ptr() if n else None)
+    return q, k, v, out, lse, how
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, causal, scale, sequences):
-        q, k, v, out, lse = _forward(q, k, v, causal, scale, sequences, True)
+        q, k, v, out, lse, how = _forward(q, k, v, causal, scale, sequences, True)
         ctx.save_for_backward(q, k, v, out, lse)
-        ctx.how = causal, scale, sequences
+        ctx.how = how, causal, scale, sequences
         return out
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
-        causal, scale, sequences = ctx.how
-        dout = _operand(dout)
-        a, _, n = _arguments(q, k, v, _strides(dout), causal, scale, sequences)
+        (a, _, n), causal, scale, sequences = ctx.how
+        if not dout.is_contiguous() or dout.data_ptr() % 16:
+            dout = _operand(dout)
+            a, _, n = _arguments(q, k, v, _strides(dout), causal, scale, sequences)
         dq = _empty(q, sequences and sequences.q_count)
         dk, dv = (_empty(x, sequences and sequences.k_count) for x in (k, v))
         ws = _workspace(q, n)
-        _lib.launch(_lib.lib().msd_attn_backward, "msd_attn_backward", q.device, a, q.data_ptr(), k.data_ptr(),
+        _lib.launch(_lib.lib().msd_attn_backward, "msd_attn_backward", dout.get_device(), a, q.data_ptr(), k.data_ptr(),
                     v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
                     dv.data_ptr(), ws.data_ptr() if n else None)
         return dq, dk, dv, None, None, None

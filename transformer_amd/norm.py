@@ -10,58 +10,55 @@ values) for the backward instead of holding on to x or h: half the memory of bf1
 values that the checkpoint stands for, off by up to 1/254 of a block's largest.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
 
 def _forward(x, scale, residual, eps, checkpoint, keep):
-    shape = x.shape
     rows, stride = _lib.rows_of(x)
     n, d = rows.shape
     res, res_stride = _lib.rows_of(residual) if residual is not None else (None, 0)
     scale = scale.contiguous()
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    total = torch.empty(shape, dtype=x.dtype, device=x.device) if res is not None else None
+    y = _lib.empty(x)
+    total = _lib.empty(x) if res is not None else None
     rstd = rows.new_empty(n, dtype=torch.float32) if keep else None
     held = rows.new_empty(_lib.keep_bytes(n, d, checkpoint), dtype=torch.uint8) if keep and checkpoint else None
-    _lib.launch(_lib.lib().msd_rms_forward, "msd_rms_forward", x.device, rows.data_ptr(), stride,
+    _lib.launch(_lib.lib().msd_rms_forward, "msd_rms_forward", y.get_device(), rows.data_ptr(), stride,
                 None if res is None else res.data_ptr(), res_stride, scale.data_ptr(), _lib.TYPES[scale.dtype], n, d,
-                _lib.TYPES[x.dtype], eps, y.data_ptr(), None if total is None else total.data_ptr(),
+                _lib.TYPES[y.dtype], eps, y.data_ptr(), None if total is None else total.data_ptr(),
                 None if rstd is None else rstd.data_ptr(), None if held is None else held.data_ptr())
-    return y, total, scale, rstd, held, rows
+    return y, total, scale, rstd, held, rows, stride
 
 
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, scale, residual, eps, checkpoint):
-        y, total, scale, rstd, held, rows = _forward(x, scale, residual, eps, checkpoint, True)
-        kept = held if held is not None else total if total is not None else rows
-        ctx.save_for_backward(kept, scale, rstd)
-        ctx.how = x.shape, x.dtype, held is not None, residual is not None
+        y, total, scale, rstd, held, rows, stride = _forward(x, scale, residual, eps, checkpoint, True)
+        ctx.save_for_backward(held if held is not None else total if total is not None else rows, scale, rstd)
+        n, d = rows.shape
+        parts = _lib.check(_lib.lib().msd_rms_workspace_bytes(n, d), "msd_rms_workspace_bytes") // 4
+        ctx.how = n, d, stride if total is None else d, held is not None, residual is not None, parts
         ctx.set_materialize_grads(False)
         return y if total is None else (y, total)
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dy, dtotal=None):
-        kept, scale, rstd = ctx.saved_tensors
-        shape, dtype, held, residual = ctx.how
+        n, d, stride, held, residual, parts = ctx.how
         if dy is None:   # only the sum was used: the norm adds nothing
             return dtotal, None, dtotal if residual else None, None, None
-        d, n = shape[-1], rstd.numel()
-        s, s_stride = (None, 0) if held else _lib.rows_of(kept)
-        dy, dy_stride = _lib.rows_of(dy)
+        kept, scale, rstd = ctx.saved_tensors
+        rows, dy_stride = _lib.rows_of(dy)
         ds, ds_stride = _lib.rows_of(dtotal) if dtotal is not None else (None, 0)
-        dx = torch.empty(shape, dtype=dtype, device=rstd.device)
+        dx = _lib.empty(dy)
         dscale = ws = None
         if ctx.needs_input_grad[1]:
-            dscale = torch.empty_like(scale)
-            ws = rstd.new_empty(_lib.check(_lib.lib().msd_rms_workspace_bytes(n, d), "msd_rms_workspace_bytes") // 4)
-        _lib.launch(_lib.lib().msd_rms_backward, "msd_rms_backward", rstd.device, None if held else s.data_ptr(), s_stride,
-                    rstd.data_ptr(), kept.data_ptr() if held else None, scale.data_ptr(), _lib.TYPES[scale.dtype],
-                    dy.data_ptr(), dy_stride, None if ds is None else ds.data_ptr(), ds_stride, n, d, _lib.TYPES[dtype],
-                    dx.data_ptr(), None if dscale is None else dscale.data_ptr(), None if ws is None else ws.data_ptr())
+            dscale, ws = torch.empty_like(scale), rstd.new_empty(parts)
+        at = kept.data_ptr()
+        _lib.launch(_lib.lib().msd_rms_backward, "msd_rms_backward", dy.get_device(), None if held else at, stride,
+                    rstd.data_ptr(), at if held else None, scale.data_ptr(), _lib.TYPES[scale.dtype], rows.data_ptr(),
+                    dy_stride, None if ds is None else ds.data_ptr(), ds_stride, n, d, _lib.TYPES[dy.dtype], dx.data_ptr(),
+                    None if dscale is None else dscale.data_ptr(), None if ws is None else ws.data_ptr())
         return dx, dscale, dx if residual else None, None, None
 
 

@@ -13,7 +13,6 @@ import functools
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -92,9 +91,9 @@ def _apply(q, k, turns, amplitude, positions, start, layout, sign):
         pos_stride = positions.stride() if positions.dim() == 2 else (0, *positions.stride())
     r = _call(q.shape, 0 if k is None else k.shape[-2], _strides(q), (0, 0, 0) if k is None else _strides(k), q.dtype,
               2 * turns.numel(), amplitude, LAYOUTS[layout], sign, pos_bytes, pos_stride, start)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    _lib.launch(_lib.lib().msd_rope_apply, "msd_rope_apply", q.device, ctypes.byref(r), q.data_ptr(),
+    q_out = _lib.empty(q)
+    k_out = None if k is None else _lib.empty(k)
+    _lib.launch(_lib.lib().msd_rope_apply, "msd_rope_apply", q.get_device(), ctypes.byref(r), q.data_ptr(),
                 None if k is None else k.data_ptr(), None if positions is None else positions.data_ptr(), turns.data_ptr(),
                 q_out.data_ptr(), None if k is None else k_out.data_ptr())
     return q_out, k_out
@@ -109,7 +108,7 @@ class _Rotary(torch.autograd.Function):
         return q if k is None else (q, k)
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dq, dk=None):
         turns, positions = ctx.saved_tensors
         amplitude, start, layout = ctx.how

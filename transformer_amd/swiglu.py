@@ -9,7 +9,6 @@ holding on to them: half the memory of bf16 for the widest activations of a laye
 values that the checkpoint stands for, off by up to 1/254 of a block's largest.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -18,38 +17,35 @@ def _forward(gate, up, checkpoint, keep):
     g, g_stride = _lib.rows_of(gate)
     u, u_stride = _lib.rows_of(up)
     n, d = g.shape
-    y = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    y = _lib.empty(gate)
     held = g.new_empty(2 * _lib.keep_bytes(n, d, checkpoint), dtype=torch.uint8) if keep and checkpoint else None
-    _lib.launch(_lib.lib().msd_swiglu_forward, "msd_swiglu_forward", gate.device, g.data_ptr(), g_stride, u.data_ptr(),
-                u_stride, n, d, _lib.TYPES[gate.dtype], y.data_ptr(), None if held is None else held.data_ptr())
-    return y, g, u, held
+    _lib.launch(_lib.lib().msd_swiglu_forward, "msd_swiglu_forward", y.get_device(), g.data_ptr(), g_stride, u.data_ptr(),
+                u_stride, n, d, _lib.TYPES[y.dtype], y.data_ptr(), None if held is None else held.data_ptr())
+    return y, g, u, held, (g_stride, u_stride)
 
 
 class _Swiglu(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, up, checkpoint):
-        y, g, u, held = _forward(gate, up, checkpoint, True)
-        ctx.save_for_backward(*((held,) if held is not None else (g, u)))
-        ctx.how = gate.shape, gate.dtype
+        y, g, u, held, ctx.strides = _forward(gate, up, checkpoint, True)
+        if held is None:
+            ctx.save_for_backward(g, u)
+        else:
+            ctx.save_for_backward(held)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_lib.first_order
     def backward(ctx, dy):
-        shape, dtype = ctx.how
-        held, g, u, strides = None, None, None, (0, 0)
-        if len(ctx.saved_tensors) == 1:
-            held, = ctx.saved_tensors
-        else:
-            g, u = ctx.saved_tensors
-            strides = tuple(x.stride(0) if x.shape[0] > 1 else 0 for x in (g, u))
-        dy, dy_stride = _lib.rows_of(dy)
-        n, d = dy.shape
-        dgate, dup = (torch.empty(shape, dtype=dtype, device=dy.device) for _ in range(2))
-        _lib.launch(_lib.lib().msd_swiglu_backward, "msd_swiglu_backward", dy.device, None if held is not None else g.data_ptr(),
-                    strides[0], None if held is not None else u.data_ptr(), strides[1],
-                    None if held is None else held.data_ptr(), dy.data_ptr(), dy_stride, n, d, _lib.TYPES[dtype],
-                    dgate.data_ptr(), dup.data_ptr())
+        saved = ctx.saved_tensors
+        rows, stride = _lib.rows_of(dy)
+        n, d = rows.shape
+        dgate, dup = _lib.empty(dy), _lib.empty(dy)
+        kept = len(saved) == 1
+        g, u, held = (None, None, saved[0].data_ptr()) if kept else (saved[0].data_ptr(), saved[1].data_ptr(), None)
+        _lib.launch(_lib.lib().msd_swiglu_backward, "msd_swiglu_backward", dy.get_device(), g, ctx.strides[0], u,
+                    ctx.strides[1], held, rows.data_ptr(), stride, n, d, _lib.TYPES[dy.dtype], dgate.data_ptr(),
+                    dup.data_ptr())
         return dgate, dup, None
 
 
