@@ -32,9 +32,9 @@ extern "C" {
  *
  * seqs == NULL: n_seqs sequences of q_len query rows and k_len key rows each; q_rows = n_seqs * q_len and k_rows =
  * n_seqs * k_len.  seqs != NULL: a device array of n_seqs (q_start, q_len, k_start, k_len), rows of one flat tensor of
- * q_rows (k_rows) rows (the sequence strides are not used), 16-byte aligned, with q_len and k_len here the longest.
- * The ranges must lie inside the rows and not overlap one another; rows outside every range are neither read nor
- * written.
+ * q_rows (k_rows) rows (the sequence strides are not used), 16-byte aligned, and seqs_host the same numbers on the host,
+ * read during the call; q_len and k_len here are the longest.  The ranges must lie inside the rows and not overlap one
+ * another; rows outside every range are neither read nor written.  The longest sequences first run fastest.
  *
  * causal: query i of a sequence sees keys 0 .. k_len - q_len + i (the last query sees the last key).  A query that
  * sees nothing has output 0 and contributes to no gradient.
@@ -49,7 +49,7 @@ typedef struct msd_attn {
   float scale;
   int64_t q_rows, k_rows;
   int64_t q_stride[3], k_stride[3], v_stride[3], dout_stride[3];   /* sequence, row, head */
-  const int32_t* seqs;
+  const int32_t *seqs, *seqs_host;
 } msd_attn;
 
 /* Bytes of device workspace of a forward (backward != 0: of a backward) call, 0 or more.  Needs no initialisation;

@@ -42,7 +42,7 @@ def test_sequences(args, match):
 
 def test_sequence_tables():
     s = Sequences([3, 0, 5], device="cpu")
-    assert s.table.tolist() == [[0, 3, 0, 3], [3, 0, 3, 0], [3, 5, 3, 5]] and s.table.dtype == torch.int32
+    assert s.table.tolist() == [[3, 5, 3, 5], [0, 3, 0, 3], [3, 0, 3, 0]] and s.table.dtype == torch.int32
     assert (s.n, s.q_longest, s.k_longest, s.q_end, s.k_end, s.q_count, s.k_count) == (3, 5, 5, 8, 8, 8, 8)
     s = Sequences([2, 1], q_starts=range(0, 10, 5), device="cpu")   # a padded batch: the keys lie where the queries do
     assert s.table.tolist() == [[0, 2, 0, 2], [5, 1, 5, 1]] and (s.q_end, s.q_count) == (6, 3)
@@ -51,8 +51,13 @@ def test_sequence_tables():
     assert Sequences([], device="cpu").table.shape == (0, 4)
 
 
+HOST = (ctypes.c_int32 * 8)(0, 10, 0, 20, 10, 9, 20, 20)
+
+
 def _args(**kw):
     a = _lib.MsdAttn()
+    if kw.get("seqs"):
+        kw = {"seqs_host": ctypes.addressof(HOST), **kw}
     base = dict(n_seqs=2, q_len=10, k_len=20, n_heads=4, n_kv_heads=2, d_head=64, causal=1, scale=0.125, q_rows=20, k_rows=40)
     base.update({k: v for k, v in kw.items() if "stride" not in k})
     for k, v in base.items():
@@ -70,7 +75,8 @@ BAD = [dict(n_seqs=-1), dict(q_len=-1), dict(k_len=-1), dict(n_heads=0), dict(n_
        dict(scale=float("inf")), dict(q_rows=21), dict(k_rows=39), dict(q_stride=(2560, 256, 60)),
        dict(k_stride=(2560, -128, 64)), dict(v_stride=(2560, 1 << 25, 64)), dict(q_rows=1 << 31, seqs=16),
        dict(q_rows=5, seqs=16), dict(n_seqs=70000, q_rows=700000, k_rows=1400000),
-       dict(q_rows=1 << 30, k_rows=40, seqs=16)]
+       dict(q_rows=1 << 30, k_rows=40, seqs=16), dict(q_rows=18, seqs=16), dict(k_rows=39, seqs=16), dict(q_len=9, seqs=16),
+       dict(k_len=19, seqs=16), dict(q_len=1 << 29, q_rows=1 << 29, n_seqs=1)]
 
 
 @pytest.mark.parametrize("kw", BAD)
@@ -96,7 +102,10 @@ def test_c_refuses_pointers():
             args = [p] * 10
             args[i] = bad
             assert L.msd_attn_backward(ctypes.byref(a), *args, None) == _lib.MSD_E_ARG
-    a = _args(seqs=4100)
+    for kw in (dict(seqs=4100), dict(seqs=16, seqs_host=None), dict(seqs=16, seqs_host=4098)):
+        a = _args(**kw)
+        assert L.msd_attn_workspace_bytes(ctypes.byref(a), 0) == _lib.MSD_E_ARG
+    assert L.msd_attn_workspace_bytes(ctypes.byref(_args(seqs=16)), 0) >= 0
     assert L.msd_attn_forward(ctypes.byref(a), p, p, p, p, p, p, None) == _lib.MSD_E_ARG
     a = _args(dout_stride=(1, 1, 1))
     assert L.msd_attn_backward(ctypes.byref(a), *[p] * 10, None) == _lib.MSD_E_CONFIG

@@ -52,7 +52,7 @@ class MsdAttn(ctypes.Structure):
     _fields_ = [(k, ctypes.c_int32) for k in ("n_seqs", "q_len", "k_len", "n_heads", "n_kv_heads", "d_head", "causal")]
     _fields_ += [("scale", ctypes.c_float), ("q_rows", ctypes.c_int64), ("k_rows", ctypes.c_int64)]
     _fields_ += [(k, ctypes.c_int64 * 3) for k in ("q_stride", "k_stride", "v_stride", "dout_stride")]
-    _fields_ += [("seqs", ctypes.c_void_p)]
+    _fields_ += [("seqs", ctypes.c_void_p), ("seqs_host", ctypes.c_void_p)]
 
 
 class MsdRope(ctypes.Structure):

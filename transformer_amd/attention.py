@@ -39,8 +39,10 @@ class Sequences:
             raise ValueError(f"{len(q_lens)} query and {len(k_lens)} key sequences")
         self.n = len(q_lens)
         self.q_longest, self.k_longest = max(q_lens, default=0), max(k_lens, default=0)
-        rows = [x for s in zip(q_starts, q_lens, k_starts, k_lens) for x in s]
-        self.table = torch.tensor(rows, dtype=torch.int32).reshape(-1, 4).to(device)
+        rows = sorted(zip(q_starts, q_lens, k_starts, k_lens), key=lambda r: -r[1] * r[3])   # the most work first
+        self.host = torch.tensor(rows, dtype=torch.int32).reshape(-1, 4)
+        self.table = self.host.to(device)
+        self._calls = {}
 
 
 def _ranges(lens, starts, what):
@@ -81,33 +83,37 @@ def _strides(x):
     return s if len(s) == 3 else (0, *s)
 
 
-@functools.lru_cache(maxsize=256)
-def _call(q_shape, k_shape, q_stride, k_stride, v_stride, dout_stride, causal, scale, sequences):
-    """(arguments, bytes of the forward's and of the backward's workspace) of one shape; sequences: None or the
-    (count, longest q, longest k) of a table that the caller puts in."""
+def _call(q_shape, k_shape, q_stride, k_stride, v_stride, dout_stride, causal, scale, sequences=None):
+    """(arguments, bytes of the forward's and of the backward's workspace) of one shape."""
     *_, H, D = q_shape
     a = _lib.MsdAttn()
     if sequences is None:
         a.n_seqs = q_shape[0] if len(q_shape) == 4 else 1
         a.q_len, a.k_len = q_shape[-3], k_shape[-3]
     else:
-        a.n_seqs, a.q_len, a.k_len = sequences
-        a.seqs = 16   # any aligned address: only looked at for its presence here
+        a.n_seqs, a.q_len, a.k_len = sequences.n, sequences.q_longest, sequences.k_longest
+        a.seqs, a.seqs_host = sequences.table.data_ptr() or 16, sequences.host.data_ptr() or 16   # (no sequence: not read)
     a.q_rows, a.k_rows = math.prod(q_shape[:-2]), math.prod(k_shape[:-2])
     a.n_heads, a.n_kv_heads, a.d_head, a.causal, a.scale = H, k_shape[-2], D, causal, scale
     for name, s in (("q_stride", q_stride), ("k_stride", k_stride), ("v_stride", v_stride), ("dout_stride", dout_stride)):
         getattr(a, name)[:] = s
     sizes = [_lib.check(_lib.lib().msd_attn_workspace_bytes(ctypes.byref(a), i), "msd_attn_workspace_bytes") for i in (0, 1)]
-    return a, *sizes
+    return ctypes.byref(a), *sizes
+
+
+_dense_call = functools.lru_cache(maxsize=256)(_call)
 
 
 def _arguments(q, k, v, dout_stride, causal, scale, sequences):
-    table = None if sequences is None else (sequences.n, sequences.q_longest, sequences.k_longest)
-    a, fwd, bwd = _call(q.shape, k.shape, _strides(q), _strides(k), _strides(v), dout_stride, causal, scale, table)
-    if sequences is not None:
-        a = _lib.MsdAttn.from_buffer_copy(a)   # (the cached one is shared by threads)
-        a.seqs = sequences.table.data_ptr()
-    return ctypes.byref(a), fwd, bwd
+    key = (q.shape, k.shape, _strides(q), _strides(k), _strides(v), dout_stride, causal, scale)
+    if sequences is None:
+        return _dense_call(*key)
+    found = sequences._calls.get(key)   # (kept with the sequences: the layers of a step make the same call)
+    if found is None:
+        if len(sequences._calls) >= 64:
+            sequences._calls.clear()
+        found = sequences._calls[key] = _call(*key, sequences)
+    return found
 
 
 def _check(q, k, v, scale, sequences):

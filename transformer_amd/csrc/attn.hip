@@ -70,7 +70,6 @@ struct Args {
   uint32_t g_magic;         // r / g = umulhi(2 r, g_magic) >> g_shift for r < 2^30 (see magic())
   int g_shift;
   float c, scale;
-  int tiles;                // row (or key) tiles of the longest sequence
   int splits;               // forward: of the keys
   int tile_rows, head_parts, row_parts, chunk;   // dK and dV: see KeyPart
   int64_t q_rows, k_rows;
@@ -82,6 +81,15 @@ struct Args {
 
 struct Seq {
   int qs, qn, ks, kn;
+};
+
+// Which sequence a workgroup works on.  Sequences of one shape: `each` jobs a sequence, a sequence's in a stride of `n_seqs`
+// (the jobs of all sequences with the most work come first).  Otherwise, for up to kMostSeqs of them, the first job of each,
+// as the host has counted them; beyond that the longest's number of jobs for each, of which the others' are empty.
+constexpr int kMostSeqs = 256;
+struct Jobs {
+  int counted;              // sequences in `first`, or 0
+  int32_t first[kMostSeqs];
 };
 
 __device__ __forceinline__ Seq sequence(const Args& p, int b) {
@@ -274,6 +282,31 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, const f32x16 (&acc)[D
   wave_lds_order();
 }
 
+// The priority of a wave with n of at most `most` pieces of work before it: the longest set how long a launch takes, and
+// otherwise share their SIMDs evenly with shorter ones that could wait
+__device__ __forceinline__ void prioritise(int n, int most) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  if (4 * n > 3 * most) __builtin_amdgcn_s_setprio(3);
+  else if (2 * n > most) __builtin_amdgcn_s_setprio(2);
+  else if (4 * n > most) __builtin_amdgcn_s_setprio(1);
+#endif
+}
+
+// The sequence that job i belongs to, and its number among that sequence's jobs
+__device__ __forceinline__ int job_sequence(const Args& p, const Jobs& jobs, int i, int& local, int lane) {
+  if (!jobs.counted) {
+    local = i / p.n_seqs;
+    return i % p.n_seqs;
+  }
+  int b = -1;   // one less than the number of sequences that begin at or before i
+#pragma unroll
+  for (int k = 0; k < kMostSeqs; k += 64)
+    if (k < jobs.counted) b += __popcll(__ballot(k + lane < jobs.counted && jobs.first[k + lane] <= i));
+  b = __builtin_amdgcn_readfirstlane(b);
+  local = i - jobs.first[b];
+  return b;
+}
+
 // What a workgroup of row tiles works on: 32 rows a wave, keys [k_lo, k_hi) in tiles of 64
 struct RowJob {
   Seq s;
@@ -286,15 +319,14 @@ struct RowJob {
 };
 
 template <int NW>
-__device__ __forceinline__ bool row_job(const Args& p, RowJob& j, int lane, int wv) {
-  const int heads = p.n_seqs * p.KV, id = blockIdx.x % heads;
-  const int tile = p.tiles - 1 - int(blockIdx.x / heads);   // the longest key ranges first
-  j.b = id / p.KV;
-  j.kvh = id % p.KV;
+__device__ __forceinline__ bool row_job(const Args& p, const Jobs& jobs, RowJob& j, int lane, int wv) {
+  j.kvh = blockIdx.x % p.KV;
+  int local;
+  j.b = job_sequence(p, jobs, blockIdx.x / p.KV, local, lane);
   j.s = sequence(p, j.b);
   j.rows = j.s.qn * p.g;
-  const int r0 = tile * 32 * NW;
-  if (r0 >= j.rows) return false;
+  const int r0 = ((j.rows + 32 * NW - 1) / (32 * NW) - 1 - local) * 32 * NW;   // the longest key ranges first
+  if (r0 < 0) return false;
   j.r = r0 + 32 * wv + (lane & 31);
   j.ok = j.r < j.rows;
   j.pos = div_g(p, min(j.r, j.rows - 1));
@@ -306,8 +338,10 @@ __device__ __forceinline__ bool row_job(const Args& p, RowJob& j, int lane, int 
   j.wave_full = seen_by(w0);
   j.wave_end = seen_by(w1);
   const int n = (seen_by(wg) + kKeys - 1) / kKeys;
-  j.t0 = int(int64_t(n) * blockIdx.y / p.splits);
-  j.t1 = int(int64_t(n) * (blockIdx.y + 1) / p.splits);
+  const int per = n / p.splits, more = n % p.splits, y = blockIdx.y;
+  j.t0 = per * y + min(y, more);
+  j.t1 = j.t0 + per + (y < more);
+  prioritise(j.t1 - j.t0, (p.k_len + kKeys - 1) / kKeys / p.splits);
   return true;
 }
 
@@ -320,12 +354,12 @@ __device__ __forceinline__ int64_t stat_index(const Args& p, const RowJob& j) {
 // Per 32 keys: the scores' maximum; the probabilities, while the matrix cores form the next 32 keys' scores; then their
 // product with V.  So the scores run 32 keys ahead, K one tile ahead of V: three K buffers and two of V, one barrier a tile.
 template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attn_fwd(Args p) {
+__global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attn_fwd(Args p, Jobs jobs) {
   constexpr int P = pitch<DP>(), TILE = kKeys * P;
   __shared__ __attribute__((aligned(16))) uint8_t lds[5 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   RowJob j;
-  if (!row_job<NW>(p, j, lane, wv)) return;
+  if (!row_job<NW>(p, jobs, j, lane, wv)) return;
   const uint16_t* kb = origin(p, p.k, j.b, j.s.ks, j.kvh);
   const uint16_t* vb = origin(p, p.v, j.b, j.s.ks, j.kvh);
 
@@ -440,50 +474,73 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attn_fwd(Args p) {
   });
 }
 
-// The parts of a row over the splits, weighted by 2^(lse_z - lse): one thread for 8 values
-__global__ void attn_join(Args p) {
-  const int per = p.D / 8;
-  const int64_t n = p.q_rows * p.H, id = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int b = blockIdx.y;
-  const Seq s = sequence(p, b);
-  const int64_t rows = int64_t(s.qn) * p.H, row = id / per;
-  if (row >= rows) return;
-  const int c = int(id - row * per) * 8;
+// A row from its parts over the splits, weighted by 2^(lse_z - lse).  16 lanes a row's 8-value pieces (as many as it has), G
+// of them in turn over the splits, joined through LDS in order; 16 / G rows a workgroup.
+constexpr int kJoinLanes = 256;
+template <int G>
+__global__ __launch_bounds__(kJoinLanes) void attn_join(Args p) {
+  __shared__ float lds[kJoinLanes][11];
+  const int tid = threadIdx.x, c = tid % 16, zg = tid / 16 % G;
+  const Seq s = sequence(p, blockIdx.y);
+  const int64_t n = p.q_rows * p.H, rows = int64_t(s.qn) * p.H, row = int64_t(blockIdx.x) * (kJoinLanes / 16 / G) + tid / 16 / G;
   const int64_t at = int64_t(s.qs) * p.H + row;   // in the statistics' order
+  const bool ok = row < rows && 8 * c < p.D;
   const float* w = p.part + int64_t(p.splits) * n * p.D;
-  float m = -INFINITY;
-  for (int z = 0; z < p.splits; ++z) {
-    const float x = w[z * n + at];
-    if (x != INFINITY) m = fmaxf(m, x);
-  }
-  float acc[8] = {}, l = 0;
-  for (int z = 0; z < p.splits; ++z) {
-    const float x = w[z * n + at];
-    if (x == INFINITY) continue;   // nothing seen in this part
-    const float e = exp2_hw(x - m);
-    const float* from = p.part + (z * n + at) * p.D + c;
-    l += e;
+  float m = -INFINITY, l = 0, acc[8] = {};
+  if (ok)
+#pragma unroll 2
+    for (int z = zg; z < p.splits; z += G) {
+      const float x = w[z * n + at];
+      const float* from = p.part + (z * n + at) * p.D + 8 * c;
+      const f32x4 a = *reinterpret_cast<const f32x4*>(from), b = *reinterpret_cast<const f32x4*>(from + 4);
+      if (x == INFINITY) continue;   // nothing seen in this part
+      const float mn = fmaxf(m, x), old = exp2_hw(m - mn), e = exp2_hw(x - mn);   // (a NaN stays one through e)
+      m = mn;
+      l = fmaf(l, old, e);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = fmaf(e, from[i], acc[i]);
+      for (int i = 0; i < 4; ++i) {
+        acc[i] = fmaf(acc[i], old, e * a[i]);
+        acc[4 + i] = fmaf(acc[4 + i], old, e * b[i]);
+      }
+    }
+  lds[tid][0] = m;
+  lds[tid][1] = l;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) lds[tid][2 + i] = acc[i];
+  __syncthreads();
+  if (zg || !ok) return;
+  m = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < G; ++g) m = fmaxf(m, lds[tid + 16 * g][0]);
+  l = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const float* x = lds[tid + 16 * g];
+    const float e = x[1] == 0 ? 0.0f : exp2_hw(x[0] - m);
+    l = fmaf(e, x[1], l);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = fmaf(e, x[2 + i], acc[i]);
   }
   const float by = l == 0 ? 0.0f : 1.0f / l;
   const int head = int(row) / s.qn, pos = int(row) - head * s.qn;
   u32x4 x;
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = pack2(acc[2 * i] * by, acc[2 * i + 1] * by);
-  *reinterpret_cast<u32x4*>(p.out + (int64_t(s.qs + pos) * p.H + head) * p.D + c) = x;
+  *reinterpret_cast<u32x4*>(p.out + (int64_t(s.qs + pos) * p.H + head) * p.D + 8 * c) = x;
   if (p.lse && c == 0) p.lse[at] = l == 0 ? INFINITY : m + __log2f(l);
 }
 
 // ---- backward ----
 // dQ of 32 rows a wave; also D_i = dO_i.O_i, which attn_dkv reads beside lse
 template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p) {
+__global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p, Jobs jobs) {
   constexpr int P = pitch<DP>(), TILE = kKeys * P;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   RowJob j;
-  if (!row_job<NW>(p, j, lane, wv)) return;
+  if (!row_job<NW>(p, jobs, j, lane, wv)) return;
   const uint16_t* kb = origin(p, p.k, j.b, j.s.ks, j.kvh);
   const uint16_t* vb = origin(p, p.v, j.b, j.s.ks, j.kvh);
 
@@ -564,8 +621,7 @@ __device__ __forceinline__ int row_tiles(const Args& p, const Seq& s, int kb, in
 }
 
 // The work on 128 keys: the row tiles of the group's heads, head by head.  The heads are shared out to p.head_parts parts,
-// each part's list of tiles to p.row_parts parts of p.chunk tiles for one head, of which the block's first `parts` are not
-// empty.
+// each part's list of tiles to parts of p.chunk of them: at most p.row_parts, here `parts`.
 struct KeyPart {
   int n, first;   // row tiles a head
   int t0, t1, parts;
@@ -573,11 +629,23 @@ struct KeyPart {
 __device__ __forceinline__ KeyPart key_part(const Args& p, const Seq& s, int kb, int z, int n_heads) {
   KeyPart k;
   k.n = row_tiles(p, s, kb, k.first);
-  const int n = k.n * n_heads, chunk = p.chunk * n_heads;
-  k.parts = max((k.n + p.chunk - 1) / p.chunk, 1);
-  k.t0 = min(z * chunk, n);
-  k.t1 = min(k.t0 + chunk, n);
+  const int n = k.n * n_heads;
+  k.parts = max((n + p.chunk - 1) / p.chunk, 1);
+  k.t0 = min(z * p.chunk, n);
+  k.t1 = min(k.t0 + p.chunk, n);
   return k;
+}
+
+// Blocks of 128 keys that have a part z (of all heads of a group): the first ones, and every block has part 0
+__host__ __device__ inline int blocks_with_part(const Seq& s, int z, int g, int tile_rows, int chunk, bool causal) {
+  const int blocks = (s.kn + 127) / 128, tiles = (s.qn + tile_rows - 1) / tile_rows;
+  if (z == 0) return blocks;
+  const int most = tiles - (int(int64_t(z) * chunk / g) + 1);   // row tiles that may lie before the block's first
+  if (most < 0) return 0;
+  const int64_t end = int64_t(most + 1) * tile_rows;            // the block's first row lies before it
+  if (!causal || end > s.qn) return blocks;
+  const int64_t keys = end + s.kn - s.qn;                       // 128 kb - (kn - qn) < end
+  return keys <= 0 ? 0 : int(keys + 127) / 128 < blocks ? int(keys + 127) / 128 : blocks;
 }
 
 // The way through the row tiles of a part, from the last rows to the first, head by head: where the next tile
@@ -618,23 +686,37 @@ struct RowStream {
 // dK and dV of 128 keys, 32 a wave.  Two workgroups a CU, so that one's first loads and last stores (8 us together) are
 // behind the other's products.
 template <int DP>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_dkv(Args p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_dkv(Args p, Jobs jobs) {
   constexpr int P = pitch<DP>(), R = tile_rows<DP>(), TILE = R * P, STAGE = 2 * TILE + 8 * R, S = DP <= 64 ? 3 : 2, SUB = R / 32;
   constexpr int DB = DP / 32, LOADS = 2 * TILE / 1024 / 4 + 1;   // of a wave and stage
   __shared__ __attribute__((aligned(16))) uint8_t lds[S * STAGE + 128 * P];
   static_assert(sizeof(lds) <= 80 * 1024 && S * STAGE >= 4 * 32 * P, "two workgroups a CU; the results' staging");
   uint8_t* vs = lds + S * STAGE;   // the workgroup's V rows: in registers they would spill
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // the first keys, which the most rows see, first; workgroups of the same rows are `jobs` apart: with 8 jobs, or a
-  // multiple, on one XCD
-  const int parts = p.head_parts * p.row_parts, jobs = p.n_seqs * p.KV * parts, id = blockIdx.x % jobs, kb = blockIdx.x / jobs;
-  const int z = id / (p.n_seqs * p.KV), zh = z / p.row_parts, zr = z % p.row_parts;
-  const int b = id / p.KV % p.n_seqs, kvh = id % p.KV;
-  const int h0 = zh * p.g / p.head_parts, n_heads = (zh + 1) * p.g / p.head_parts - h0;
+  // the first keys, which the most rows see, first
+  int b, kvh, kb, zh = 0, zr;
+  if (jobs.counted) {   // part by part, block by block
+    kvh = blockIdx.x % p.KV;
+    b = job_sequence(p, jobs, blockIdx.x / p.KV, kb, lane);
+  } else {   // workgroups of the same rows are all = n_seqs * KV * parts apart: with 8 of them, or a multiple, on one XCD
+    const int all = p.n_seqs * p.KV * p.head_parts * p.row_parts, id = blockIdx.x % all, z = id / (p.n_seqs * p.KV);
+    kb = blockIdx.x / all;
+    zh = z / p.row_parts;
+    zr = z % p.row_parts;
+    b = id / p.KV % p.n_seqs;
+    kvh = id % p.KV;
+  }
   const Seq s = sequence(p, b);
+  if (jobs.counted) {
+    zr = 0;
+    for (int n; kb >= (n = blocks_with_part(s, zr, p.g, p.tile_rows, p.chunk, p.causal)) && zr < p.row_parts; ++zr) kb -= n;
+  }
+  const int parts = p.head_parts * p.row_parts, z = zh * p.row_parts + zr;
+  const int h0 = zh * p.g / p.head_parts, n_heads = (zh + 1) * p.g / p.head_parts - h0;
   if (128 * kb >= s.kn) return;
   const KeyPart w = key_part(p, s, kb, zr, n_heads);
   if (zr >= w.parts) return;   // (a block that no row sees has one, which writes its zeros)
+  prioritise(w.t1 - w.t0, p.chunk);
   const int last = s.kn - s.qn + 1;
   const uint16_t* qb = origin(p, p.q, b, s.qs, kvh * p.g + h0);
   const uint16_t* db = origin(p, p.dout, b, s.qs, kvh * p.g + h0);
@@ -801,29 +883,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   store_rows<DP>(lds + wv * 32 * P, dv, 1.0f, p.D, lane, [&](int r) { return row(p.dv, r); });
 }
 
-// dK and dV as the sum of their parts, in order: 8 values a thread, of the rows of a sequence
-__global__ void attn_sum_parts(Args p) {
-  const Seq s = sequence(p, blockIdx.y);
-  const int64_t n = p.k_rows * p.KV * p.D, own = int64_t(s.kn) * p.KV * p.D;
-  const int64_t i = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) * 8;
-  if (i >= own) return;
+// dK (blockIdx.z 0) and dV of 128 keys as the sum of their parts, in order: 8 values a thread
+__global__ __launch_bounds__(256) void attn_sum_parts(Args p, Jobs jobs) {
+  int kb;
+  const int b = job_sequence(p, jobs, blockIdx.x, kb, threadIdx.x & 63);
+  const Seq s = sequence(p, b);
+  const int width = p.KV * p.D, i = (blockIdx.y * 256 + threadIdx.x) * 8, row = i / width;
+  if (row >= 128 || 128 * kb + row >= s.kn) return;
   const bool v = blockIdx.z;
-  const int64_t at = int64_t(s.ks) * p.KV * p.D + i;
+  const int64_t n = p.k_rows * width, at = int64_t(s.ks + 128 * kb) * width + i;
   const float* from = p.part + (v ? p.head_parts * p.row_parts * n : 0) + at;
-  const int kb = int(i / (p.KV * p.D)) / 128;
-  f32x4 a = {}, b = {};
+  f32x4 x = {}, y = {};
   for (int zh = 0; zh < p.head_parts; ++zh) {
-    const KeyPart w = key_part(p, s, kb, 0, 1);
+    const KeyPart w = key_part(p, s, kb, 0, (zh + 1) * p.g / p.head_parts - zh * p.g / p.head_parts);
     if (p.head_parts == 1 && w.parts == 1) return;   // written as they are
+#pragma unroll 4
     for (int z = 0; z < w.parts; ++z) {
-      a += *reinterpret_cast<const f32x4*>(from + (zh * p.row_parts + z) * n);
-      b += *reinterpret_cast<const f32x4*>(from + (zh * p.row_parts + z) * n + 4);
+      x += *reinterpret_cast<const f32x4*>(from + (zh * p.row_parts + z) * n);
+      y += *reinterpret_cast<const f32x4*>(from + (zh * p.row_parts + z) * n + 4);
     }
   }
   const float by = v ? 1.0f : p.scale;
-  a *= by;
-  b *= by;
-  *reinterpret_cast<u32x4*>((v ? p.dv : p.dk) + at) = u32x4{pack2(a[0], a[1]), pack2(a[2], a[3]), pack2(b[0], b[1]), pack2(b[2], b[3])};
+  x *= by;
+  y *= by;
+  *reinterpret_cast<u32x4*>((v ? p.dv : p.dk) + at) = u32x4{pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3])};
 }
 
 // ---- host ----
@@ -838,37 +921,81 @@ void magic(uint32_t g, uint32_t& m, int& s) {
 
 constexpr int kLeast = 8;    // row tiles of a part at least
 struct Plan {
-  int waves;          // of a forward or dQ workgroup
-  int tiles, splits;  // forward: row tiles, splits of the keys
-  int dq_waves, dq_tiles, key_tiles;
-  int tile_rows, head_parts, row_parts, chunk;   // dK and dV: see KeyPart
+  int waves, splits;         // of a forward or dQ workgroup; forward: splits of the keys
+  int64_t groups;            // row tiles of all sequences and K/V heads
+  int key_tiles;             // of the longest
+  int64_t key_groups;        // dK and dV: workgroups
+  int tile_rows, head_parts, row_parts, chunk;   // see KeyPart
+  int64_t blocks;            // of 128 keys, of all sequences
+  Jobs rows, keys, sums;
 };
 
 constexpr int kCus = 256;
 constexpr int64_t kMostGroups = (int64_t(1) << 32) / 256 - 1;   // a launch has fewer than 2^32 threads a dimension
 
-Plan plan(const msd_attn& a) {
-  Plan p;
-  const int64_t heads = int64_t(a.n_seqs) * a.n_kv_heads, g = a.n_heads / a.n_kv_heads, rows = a.q_len * g;
+Seq host_seq(const msd_attn& a, int b) {
+  if (!a.seqs) return {0, a.q_len, 0, a.k_len};
+  const int32_t* s = a.seqs_host + 4 * b;
+  return {s[0], s[1], s[2], s[3]};
+}
+
+void plan(const msd_attn& a, Plan& p) {
+  const int64_t g = a.n_heads / a.n_kv_heads, n = a.n_seqs;
+  const bool counted = a.seqs && n <= kMostSeqs;
+  // jobs of all sequences, f(sequence) each
+  auto count = [&](Jobs& jobs, auto f) {
+    jobs.counted = counted ? int(n) : 0;
+    if (!counted) return int64_t(n * f(Seq{0, a.q_len, 0, a.k_len}));
+    int64_t all = 0;
+    for (int b = 0; b < n; ++b) {
+      jobs.first[b] = int(std::min<int64_t>(all, INT32_MAX));
+      all += f(host_seq(a, b));
+    }
+    return all;
+  };
+  auto row_groups = [&](int waves) {
+    return count(p.rows, [&](Seq s) { return cdiv(s.qn * g, 32 * waves); }) * a.n_kv_heads;
+  };
+  p.waves = 4;
+  p.groups = row_groups(4);
+  if (p.groups < kCus) {   // 32-row workgroups fill more CUs
+    p.waves = 1;
+    p.groups = row_groups(1);
+  }
+  // few rows: the keys are split too, into at least two tiles each
   const int64_t key_tiles = std::max<int64_t>(cdiv(a.k_len, kKeys), 1);
-  p.waves = heads * cdiv(rows, 128) >= kCus ? 4 : 1;
-  p.tiles = int(cdiv(rows, 32 * p.waves));
-  const int64_t groups = heads * p.tiles;
-  p.splits = int(groups >= 2 * kCus ? 1 : std::max<int64_t>(1, std::min(cdiv(4 * kCus, std::max<int64_t>(groups, 1)), cdiv(key_tiles, 2))));
-  p.dq_waves = p.waves;
-  p.dq_tiles = p.tiles;
+  p.splits = int(p.groups >= 2 * kCus ? 1 : std::max<int64_t>(1, std::min(cdiv(4 * kCus, std::max<int64_t>(p.groups, 1)), cdiv(key_tiles, 2))));
   p.key_tiles = int(cdiv(a.k_len, 128));
-  // dK and dV: parts of a key block until every CU has two workgroups, four where the mask or the lengths make them uneven:
-  // the heads of a group first, then the rows, as long as a part's K, V and results are worth their traffic.  Sequences of
-  // different lengths are counted by their rows, so that the longest's workgroups do not outlast all others'.
-  const int64_t blocks = a.seqs ? a.n_kv_heads * cdiv(a.k_rows, 128) : heads * p.key_tiles;
-  const int64_t want = cdiv((a.causal || a.seqs ? 4 : 2) * kCus, std::max<int64_t>(blocks, 1));
-  p.head_parts = int(std::min<int64_t>(want, g));
+  // dK and dV: parts of a key block until every CU has two workgroups, four where the mask makes them uneven: the heads of a
+  // group first, whose parts are alike, then the rows, as long as a part's K, V and results are worth their traffic.
+  // Sequences of different lengths: parts of as many tiles as make that many of them.
   p.tile_rows = a.d_head <= 64 ? tile_rows<64>() : tile_rows<128>();
   const int64_t most = cdiv(a.q_len, p.tile_rows);
-  p.chunk = int(std::max<int64_t>(cdiv(most, cdiv(want, p.head_parts)), kLeast));
-  p.row_parts = int(std::max<int64_t>(1, cdiv(most, p.chunk)));
-  return p;
+  if (counted) {
+    int64_t all = 0;
+    for (int b = 0; b < n; ++b) {
+      const Seq s = host_seq(a, b);
+      all += cdiv(s.qn, p.tile_rows) * cdiv(s.kn, 128);
+    }
+    p.head_parts = 1;
+    p.chunk = int(std::max<int64_t>(cdiv(all * a.n_heads / (a.causal ? 2 : 1), 4 * kCus), kLeast));
+  } else {
+    const int64_t want = cdiv((a.causal ? 4 : 2) * kCus, std::max<int64_t>(n * a.n_kv_heads * p.key_tiles, 1));
+    p.head_parts = int(std::min<int64_t>(want, g));
+    p.chunk = int(std::max<int64_t>(cdiv(most, cdiv(want, p.head_parts)), kLeast) * cdiv(g, p.head_parts));
+  }
+  p.row_parts = int(std::max<int64_t>(1, cdiv(most * cdiv(g, p.head_parts), p.chunk)));
+  p.blocks = count(p.sums, [&](Seq s) { return cdiv(s.kn, 128); });
+  if (counted)
+    p.key_groups = a.n_kv_heads * count(p.keys, [&](Seq s) {
+      int64_t all = 0;
+      for (int z = 0; z < p.row_parts; ++z) all += blocks_with_part(s, z, int(g), p.tile_rows, p.chunk, a.causal != 0);
+      return all;
+    });
+  else {
+    p.keys.counted = 0;
+    p.key_groups = n * a.n_kv_heads * p.key_tiles * p.head_parts * p.row_parts;
+  }
 }
 
 bool fits(const int64_t (&s)[3], int64_t heads) {
@@ -878,7 +1005,8 @@ bool fits(const int64_t (&s)[3], int64_t heads) {
   return s[1] <= most / 64 && s[2] <= most / heads && 64 * s[1] + heads * s[2] < most;
 }
 
-int32_t check(const msd_attn* a, bool backward) {
+// whether the library takes the call, and how
+int32_t check(const msd_attn* a, bool backward, Plan& p) {
   if (!a) return MSD_E_ARG;
   if (a->n_seqs < 0 || a->q_len < 0 || a->k_len < 0 || a->n_heads <= 0 || a->n_kv_heads <= 0 || a->n_heads % a->n_kv_heads ||
       a->d_head <= 0 || a->d_head > 128 || a->d_head % 8 || !(a->scale > 0) || !isfinite(a->scale) || a->q_rows < 0 ||
@@ -886,17 +1014,24 @@ int32_t check(const msd_attn* a, bool backward) {
     return MSD_E_CONFIG;
   const int64_t most = int64_t(1) << 31;
   if (a->q_rows >= most || a->k_rows >= most || a->q_rows * a->n_heads >= most || a->k_rows * a->n_kv_heads >= most ||
-      int64_t(a->q_len) * (a->n_heads / a->n_kv_heads) >= (1 << 30) - 256 || int64_t(a->n_seqs) * a->n_kv_heads >= (1 << 20) || a->n_seqs > 65535)
+      int64_t(a->q_len) * (a->n_heads / a->n_kv_heads) >= (1 << 30) - 256 || int64_t(a->n_seqs) * a->n_kv_heads >= (1 << 20) || a->n_heads > 8192 || a->n_seqs > 65535)
     return MSD_E_CONFIG;
   if (!a->seqs && (a->q_rows != int64_t(a->n_seqs) * a->q_len || a->k_rows != int64_t(a->n_seqs) * a->k_len)) return MSD_E_CONFIG;
   if (a->q_len > a->q_rows || a->k_len > a->k_rows) return MSD_E_CONFIG;
   const int64_t g = a->n_heads / a->n_kv_heads;
   if (!fits(a->q_stride, g) || !fits(a->k_stride, 1) || !fits(a->v_stride, 1) || (backward && !fits(a->dout_stride, g)))
     return MSD_E_CONFIG;
-  if (int64_t(a->n_seqs) * a->n_kv_heads * std::max(cdiv(int64_t(a->q_len) * g, 128), cdiv(a->k_len, 128)) > kMostGroups)
-    return MSD_E_CONFIG;
-  if (a->seqs && reinterpret_cast<uintptr_t>(a->seqs) % 16) return MSD_E_ARG;
-  return MSD_OK;
+  if (a->seqs) {
+    if (reinterpret_cast<uintptr_t>(a->seqs) % 16 || !a->seqs_host || reinterpret_cast<uintptr_t>(a->seqs_host) % 4) return MSD_E_ARG;
+    for (int b = 0; b < a->n_seqs; ++b) {
+      const Seq s = host_seq(*a, b);
+      if (s.qs < 0 || s.qn < 0 || s.ks < 0 || s.kn < 0 || s.qn > a->q_len || s.kn > a->k_len || s.qs > a->q_rows - s.qn ||
+          s.ks > a->k_rows - s.kn)
+        return MSD_E_CONFIG;
+    }
+  }
+  plan(*a, p);
+  return std::max(p.groups, p.key_groups) > kMostGroups || p.splits > 65535 ? MSD_E_CONFIG : MSD_OK;
 }
 
 bool bad(const void* p) { return !p || reinterpret_cast<uintptr_t>(p) % 16; }
@@ -943,9 +1078,9 @@ int64_t up(int64_t x) { return cdiv(x, 256) * 256; }
 using namespace msa;
 
 extern "C" int64_t msd_attn_workspace_bytes(const msd_attn* a, int32_t backward) {
-  const int32_t rc = check(a, false);
+  Plan pl;
+  const int32_t rc = check(a, false, pl);
   if (rc != MSD_OK) return rc;
-  const Plan pl = plan(*a);
   if (!backward) return pl.splits > 1 ? 4 * pl.splits * a->q_rows * a->n_heads * (a->d_head + 1) : 0;
   const int64_t n = pl.head_parts * pl.row_parts, parts = n > 1 ? 8 * n * a->k_rows * a->n_kv_heads * a->d_head : 0;
   return up(8 * a->q_rows * a->n_heads) + parts;
@@ -953,28 +1088,28 @@ extern "C" int64_t msd_attn_workspace_bytes(const msd_attn* a, int32_t backward)
 
 extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void* k, const void* v, void* out, float* lse,
                                     void* workspace, void* stream) {
-  const int32_t rc = check(a, false);
+  Plan pl;
+  const int32_t rc = check(a, false, pl);
   if (rc != MSD_OK) return rc;
   if (a->n_seqs == 0 || a->q_len == 0) return MSD_OK;
   if (bad(q) || bad(out) || (a->k_len && (bad(k) || bad(v)))) return MSD_E_ARG;
-  const Plan pl = plan(*a);
   if (pl.splits > 1 && bad(workspace)) return MSD_E_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
   Args p = args(*a, q, k, v);
   p.out = static_cast<uint16_t*>(out);
   p.lse = lse;
   p.part = static_cast<float*>(workspace);
-  p.tiles = pl.tiles;
   p.splits = pl.splits;
-  const dim3 grid(unsigned(pl.tiles) * a->n_seqs * a->n_kv_heads, pl.splits);
+  const dim3 grid(unsigned(pl.groups), pl.splits);
   with_head(a->d_head, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
-    if (pl.waves == 4) hipLaunchKernelGGL((attn_fwd<DP, 4>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((attn_fwd<DP, 1>), grid, dim3(64), 0, s, p);
+    if (pl.waves == 4) hipLaunchKernelGGL((attn_fwd<DP, 4>), grid, dim3(256), 0, s, p, pl.rows);
+    else hipLaunchKernelGGL((attn_fwd<DP, 1>), grid, dim3(64), 0, s, p, pl.rows);
   });
   if (pl.splits > 1) {
-    const int64_t n = int64_t(a->q_len) * a->n_heads * (a->d_head / 8);
-    hipLaunchKernelGGL(attn_join, dim3(unsigned(cdiv(n, 128)), a->n_seqs), dim3(128), 0, s, p);
+    const int64_t rows = int64_t(a->q_len) * a->n_heads;
+    if (pl.splits > 4) hipLaunchKernelGGL(attn_join<16>, dim3(unsigned(rows), a->n_seqs), dim3(kJoinLanes), 0, s, p);
+    else hipLaunchKernelGGL(attn_join<4>, dim3(unsigned(cdiv(rows, 4)), a->n_seqs), dim3(kJoinLanes), 0, s, p);
   }
   return launched();
 }
@@ -982,13 +1117,13 @@ extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void
 extern "C" int32_t msd_attn_backward(const msd_attn* a, const void* q, const void* k, const void* v, const void* out,
                                      const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
                                      void* stream) {
-  const int32_t rc = check(a, true);
+  Plan pl;
+  const int32_t rc = check(a, true, pl);
   if (rc != MSD_OK) return rc;
   if (a->n_seqs == 0 || (a->q_len == 0 && a->k_len == 0)) return MSD_OK;
   if ((a->q_len && (bad(q) || bad(out) || bad(lse) || bad(dout) || bad(dq))) ||
       (a->k_len && (bad(k) || bad(v) || bad(dk) || bad(dv))))
     return MSD_E_ARG;
-  const Plan pl = plan(*a);
   if (bad(workspace) && (a->q_len || pl.head_parts * pl.row_parts > 1)) return MSD_E_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
   Args p = args(*a, q, k, v);
@@ -1000,28 +1135,25 @@ extern "C" int32_t msd_attn_backward(const msd_attn* a, const void* q, const voi
   p.dq = static_cast<uint16_t*>(dq);
   p.dk = static_cast<uint16_t*>(dk);
   p.dv = static_cast<uint16_t*>(dv);
-  const unsigned heads = unsigned(a->n_seqs) * a->n_kv_heads;
   with_head(a->d_head, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
-    if (a->q_len) {
-      p.tiles = pl.dq_tiles;
+    if (pl.groups) {
       p.splits = 1;
-      const dim3 grid(unsigned(pl.dq_tiles) * heads);
-      if (pl.dq_waves == 4) hipLaunchKernelGGL((attn_dq<DP, 4>), grid, dim3(256), 0, s, p);
-      else hipLaunchKernelGGL((attn_dq<DP, 1>), grid, dim3(64), 0, s, p);
+      const dim3 grid(unsigned(pl.groups));
+      if (pl.waves == 4) hipLaunchKernelGGL((attn_dq<DP, 4>), grid, dim3(256), 0, s, p, pl.rows);
+      else hipLaunchKernelGGL((attn_dq<DP, 1>), grid, dim3(64), 0, s, p, pl.rows);
     }
-    if (a->k_len) {
-      p.tiles = pl.key_tiles;
+    if (pl.key_groups) {
       p.tile_rows = pl.tile_rows;
       p.head_parts = pl.head_parts;
       p.row_parts = pl.row_parts;
       p.chunk = pl.chunk;
-      hipLaunchKernelGGL((attn_dkv<DP>), dim3(unsigned(pl.key_tiles) * heads * (pl.head_parts * pl.row_parts)), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((attn_dkv<DP>), dim3(unsigned(pl.key_groups)), dim3(256), 0, s, p, pl.keys);
     }
   });
-  if (a->k_len && pl.head_parts * pl.row_parts > 1) {
-    const int64_t n = int64_t(a->k_len) * a->n_kv_heads * (a->d_head / 8);
-    hipLaunchKernelGGL(attn_sum_parts, dim3(unsigned(cdiv(n, 256)), a->n_seqs, 2), dim3(256), 0, s, p);
+  if (pl.key_groups && pl.head_parts * pl.row_parts > 1) {
+    const int64_t slices = cdiv(128 * int64_t(a->n_kv_heads) * a->d_head, 2048);
+    hipLaunchKernelGGL(attn_sum_parts, dim3(unsigned(pl.blocks), unsigned(slices), 2), dim3(256), 0, s, p, pl.sums);
   }
   return launched();
 }
