@@ -978,7 +978,7 @@ void plan(const msd_attn& a, Plan& p) {
       all += cdiv(s.qn, p.tile_rows) * cdiv(s.kn, 128);
     }
     p.head_parts = 1;
-    p.chunk = int(std::max<int64_t>(cdiv(all * a.n_heads / (a.causal ? 2 : 1), 4 * kCus), kLeast));
+    p.chunk = int(std::max<int64_t>(cdiv(all * a.n_heads / (a.causal ? 2 : 1), 2 * kCus), kLeast));
   } else {
     const int64_t want = cdiv((a.causal ? 4 : 2) * kCus, std::max<int64_t>(n * a.n_kv_heads * p.key_tiles, 1));
     p.head_parts = int(std::min<int64_t>(want, g));

@@ -465,8 +465,9 @@ unsigned glu_setup(GluArgs& p, int64_t rows, int d, const void* checkpoint_) {
 
 // ---- rotary positions ----
 // A workgroup takes kTokens tokens: their cosines and sines once, to LDS, for all heads; then units of work, a unit being
-// W values of a head's copied part, W interleaved values, or W first and W second values of pairs.
-constexpr int kTokens = 8;
+// W values of a head's copied part, W interleaved values, or W first and W second values of pairs.  A lane keeps one unit
+// of the token (its head and place) over the tokens, kDeep of them in flight.
+constexpr int kTokens = 8, kDeep = 4;
 
 struct RopeArgs {
   const void *q, *k, *positions;
@@ -475,24 +476,25 @@ struct RopeArgs {
   int64_t q_stride[3], k_stride[3], pos_stride[2], start, rows;
   int tokens, H, KV, D, rot, position_bytes, interleaved;
   float amplitude, sign;
-  Div by_tokens, by_token_units, by_head_units;
-  int rot_units;   // units of a head that turn
+  Div by_head_units;
+  int token_units, groups;   // units of a token; tokens that the 256 lanes work on at a time
+  int rot_units;             // units of a head that turn
 };
 
-template <class T, int W>
-__device__ __forceinline__ void load_w(const T* p, float (&v)[8]) {
-  if constexpr (W == 8) load8(p, 8, v);
-  else load8(p, 1, v);
-}
-template <class T, int W>
-__device__ __forceinline__ void store_w(T* p, const float (&v)[8]) {
-  if constexpr (W == 8) store8(p, 8, v);
-  else store8(p, 1, v);
+template <int W>
+__device__ __forceinline__ void turn8(float (&a)[8], float (&c)[8], const float2* w) {   // pairs (a[j], c[j])
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+    const float x = a[j], y = c[j];
+    a[j] = x * w[j].x - y * w[j].y;
+    c[j] = x * w[j].y + y * w[j].x;
+  }
 }
 
 template <class T, int W>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs p) {
   extern __shared__ float2 turn[];   // (cos, sin) of kTokens tokens, rot / 2 pairs each
+  __shared__ int64_t q_at[kTokens], k_at[kTokens];
   const int half = p.rot / 2;
   const int64_t row0 = int64_t(blockIdx.x) * kTokens;
   const int n = int(min(int64_t(kTokens), p.rows - row0));
@@ -504,58 +506,72 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs p) {
       const int64_t at = b * p.pos_stride[0] + tok * p.pos_stride[1];
       pos = p.position_bytes == 8 ? static_cast<const int64_t*>(p.positions)[at] : int64_t(static_cast<const int32_t*>(p.positions)[at]);
     }
+    if (j == 0) {
+      q_at[t] = b * p.q_stride[0] + tok * p.q_stride[1];
+      k_at[t] = b * p.k_stride[0] + tok * p.k_stride[1];
+    }
     const double a = double(pos) * p.turns[j];
     float s, c;
     sincospif(2.0f * float(a - floor(a)), &s, &c);
     turn[i] = make_float2(c * p.amplitude, s * p.amplitude * p.sign);
   }
   __syncthreads();
-  const int heads = p.H + p.KV, units = int(p.by_head_units.n);
-  for (uint32_t i = threadIdx.x; i < uint32_t(n) * p.by_token_units.n; i += 256) {
-    const int t = p.by_token_units(i), in = i - t * p.by_token_units.n;
-    int h = p.by_head_units(in);
-    const int u = in - h * units;
-    const int64_t row = row0 + t, b = row / p.tokens, tok = row - b * p.tokens;
-    const bool isk = h >= p.H;
+  const int units = int(p.by_head_units.n), group = p.groups > 1 ? int(threadIdx.x) / p.token_units : 0;
+  if (group >= p.groups) return;
+  for (int i = p.groups > 1 ? int(threadIdx.x) - group * p.token_units : int(threadIdx.x); i < p.token_units; i += 256) {
+    int h = p.by_head_units(i);
+    const int u = i - h * units;
+    const bool isk = h >= p.H, copied = u >= p.rot_units;
     if (isk) h -= p.H;
-    const T* from = isk ? static_cast<const T*>(p.k) + b * p.k_stride[0] + tok * p.k_stride[1] + h * p.k_stride[2]
-                        : static_cast<const T*>(p.q) + b * p.q_stride[0] + tok * p.q_stride[1] + h * p.q_stride[2];
-    T* to = isk ? static_cast<T*>(p.k_out) + (row * p.KV + h) * p.D : static_cast<T*>(p.q_out) + (row * p.H + h) * p.D;
-    float a[8], c[8];
-    if (u >= p.rot_units) {   // the part that does not turn
-      const int at = p.rot + (u - p.rot_units) * W;
-      load_w<T, W>(from + at, a);
-      store_w<T, W>(to + at, a);
-    } else if (!p.interleaved) {
-      const int at = u * W;
-      load_w<T, W>(from + at, a);
-      load_w<T, W>(from + half + at, c);
+    // where the unit's values lie in the head, where its second ones (or, of eight interleaved values, the second four)
+    const int at = copied ? p.rot + (u - p.rot_units) * W : p.interleaved ? u * (W == 8 ? 8 : 2) : u * W;
+    const int pair = p.interleaved ? u * (W == 8 ? 4 : 1) : u * W;
+    const T* from = (isk ? static_cast<const T*>(p.k) + h * p.k_stride[2] : static_cast<const T*>(p.q) + h * p.q_stride[2]) + at;
+    const int heads = isk ? p.KV : p.H;
+    T* to = static_cast<T*>(isk ? p.k_out : p.q_out) + (row0 * heads + h) * p.D + at;
+    const int64_t* row_at = isk ? k_at : q_at;
+    const int64_t step = int64_t(heads) * p.D;
+    for (int t0 = group; t0 < n; t0 += kDeep * p.groups) {
+      float a[kDeep][8], c[kDeep][8];
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const float2 w = turn[t * half + at + j];
-        const float x = a[j], y = c[j];
-        a[j] = x * w.x - y * w.y;
-        c[j] = x * w.y + y * w.x;
+      for (int d = 0; d < kDeep; ++d) {
+        const int t = t0 + d * p.groups;
+        if (t >= n) break;
+        const T* x = from + row_at[t];
+        if constexpr (W == 8) {
+          load8(x, 8, a[d]);
+          if (!copied && !p.interleaved) load8(x + half, 8, c[d]);
+        } else {
+          load8(x, 1, a[d]);
+          if (!copied) load8(x + (p.interleaved ? 1 : half), 1, c[d]);
+        }
       }
-      store_w<T, W>(to + at, a);
-      store_w<T, W>(to + half + at, c);
-    } else if constexpr (W == 8) {
-      load_w<T, 8>(from + u * 8, a);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 w = turn[t * half + u * 4 + j];
-        const float x = a[2 * j], y = a[2 * j + 1];
-        a[2 * j] = x * w.x - y * w.y;
-        a[2 * j + 1] = x * w.y + y * w.x;
+      for (int d = 0; d < kDeep; ++d) {
+        const int t = t0 + d * p.groups;
+        if (t >= n) break;
+        T* y = to + t * step;
+        const float2* w = turn + t * half + pair;
+        if (copied) {
+          if constexpr (W == 8) store8(y, 8, a[d]);
+          else store8(y, 1, a[d]);
+        } else if constexpr (W == 8) {
+          if (p.interleaved) {
+            float e[8] = {a[d][0], a[d][2], a[d][4], a[d][6]}, f[8] = {a[d][1], a[d][3], a[d][5], a[d][7]};
+            turn8<4>(e, f, w);
+            const float r[8] = {e[0], f[0], e[1], f[1], e[2], f[2], e[3], f[3]};
+            store8(y, 8, r);
+          } else {
+            turn8<8>(a[d], c[d], w);
+            store8(y, 8, a[d]);
+            store8(y + half, 8, c[d]);
+          }
+        } else {
+          turn8<1>(a[d], c[d], w);
+          store8(y, 1, a[d]);
+          store8(y + (p.interleaved ? 1 : half), 1, c[d]);
+        }
       }
-      store_w<T, 8>(to + u * 8, a);
-    } else {
-      load8(from + 2 * u, 2, a);
-      const float2 w = turn[t * half + u];
-      const float x = a[0], y = a[1];
-      a[0] = x * w.x - y * w.y;
-      a[1] = x * w.y + y * w.x;
-      store8(to + 2 * u, 2, a);
     }
   }
 }
@@ -749,7 +765,8 @@ extern "C" int32_t msd_rope_apply(const msd_rope* r, const void* q, const void* 
   p.rot_units = r->interleaved && wide ? r->d_rot / 8 : half / w;
   const int units = p.rot_units + (r->d_head - r->d_rot) / w;
   p.by_head_units = divider(uint32_t(units));
-  p.by_token_units = divider(uint32_t(units * heads));
+  p.token_units = int(units * heads);
+  p.groups = std::max(256 / p.token_units, 1);
   const size_t lds = size_t(kTokens) * half * 8;   // d_rot 4096: 128 KB
   hipStream_t s = static_cast<hipStream_t>(stream);
   hipError_t err = hipSuccess;
