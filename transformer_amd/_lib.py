@@ -195,6 +195,11 @@ def launch(fn, what, index, *args):
         raise MsdError(rc, what)
 
 
+def current_stream(x):
+    """The handle of the current stream of x's GPU; None for a tensor in host memory."""
+    return _raw_stream(x.get_device()) if x.is_cuda else None
+
+
 def empty(x):
     """A contiguous tensor of x's shape, type and device."""
     return torch.empty_like(x, memory_format=torch.contiguous_format)

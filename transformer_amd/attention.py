@@ -11,7 +11,6 @@ backward forms the probabilities again.  Scores, softmax statistics and every su
 scores' gradients are rounded to bf16 as operands of the matrix cores, the results once to bf16.  Deterministic.
 """
 import ctypes
-import functools
 import math
 
 import torch
@@ -42,7 +41,13 @@ class Sequences:
         rows = sorted(zip(q_starts, q_lens, k_starts, k_lens), key=lambda r: -r[1] * r[3])   # the most work first
         self.host = torch.tensor(rows, dtype=torch.int32).reshape(-1, 4)
         self.table = self.host.to(device)
-        self._calls = {}
+        self._stream = _lib.current_stream(self.table)
+        self._plans = {}
+
+    def used(self):
+        """Keeps the table's memory until what has been launched on the current stream is done with it."""
+        if _lib.current_stream(self.table) != self._stream:
+            self.table.record_stream(torch.cuda.current_stream(self.table.device))
 
 
 def _ranges(lens, starts, what):
@@ -67,52 +72,79 @@ def _ranges(lens, starts, what):
     return starts, end, sum(lens)
 
 
-def _operand(x):
-    """x with contiguous heads on 16-byte boundaries, as the kernels' loads take it (copied only where it is not)."""
-    rows, heads = x.shape[-3], x.shape[-2]
-    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(n <= 1 or k % 8 == 0 for n, k in zip(x.shape, x.stride()[:-1])):
-        if 64 * x.stride(-3) * (rows > 1) + heads * x.stride(-2) * (heads > 1) < 2 ** 30:
-            return x
-    x = x.contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone()
+def _fits(shape, stride):
+    """Whether heads of these strides are contiguous, on 16-byte boundaries and within the kernels' reach."""
+    row, head = (s if n > 1 else 0 for n, s in zip(shape[-3:-1], stride[-3:-1]))
+    return ((stride[-1] == 1 or shape[-1] == 1) and all(n <= 1 or s % 8 == 0 for n, s in zip(shape, stride[:-1]))
+            and 128 * row + shape[-2] * head < 2 ** 30)
 
 
-def _strides(x):
+def _operand(x, fits):
+    """x as the kernels' loads take it, copied only where it has to be."""
+    if not fits:
+        x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(shape, stride):
     """(sequence, row, head) strides; 0 along an axis of one (or none)."""
-    s = tuple(0 if n <= 1 else k for n, k in zip(x.shape[:-1], x.stride()))
+    s = tuple(0 if n <= 1 else k for n, k in zip(shape[:-1], stride))
     return s if len(s) == 3 else (0, *s)
 
 
-def _call(q_shape, k_shape, q_stride, k_stride, v_stride, dout_stride, causal, scale, sequences=None):
-    """(arguments, bytes of the forward's and of the backward's workspace) of one shape."""
-    *_, H, D = q_shape
-    a = _lib.MsdAttn()
-    if sequences is None:
-        a.n_seqs = q_shape[0] if len(q_shape) == 4 else 1
-        a.q_len, a.k_len = q_shape[-3], k_shape[-3]
-    else:
-        a.n_seqs, a.q_len, a.k_len = sequences.n, sequences.q_longest, sequences.k_longest
-        a.seqs, a.seqs_host = sequences.table.data_ptr() or 16, sequences.host.data_ptr() or 16   # (no sequence: not read)
-    a.q_rows, a.k_rows = math.prod(q_shape[:-2]), math.prod(k_shape[:-2])
-    a.n_heads, a.n_kv_heads, a.d_head, a.causal, a.scale = H, k_shape[-2], D, causal, scale
-    for name, s in (("q_stride", q_stride), ("k_stride", k_stride), ("v_stride", v_stride), ("dout_stride", dout_stride)):
-        getattr(a, name)[:] = s
-    sizes = [_lib.check(_lib.lib().msd_attn_workspace_bytes(ctypes.byref(a), i), "msd_attn_workspace_bytes") for i in (0, 1)]
-    return ctypes.byref(a), *sizes
+def _contiguous(shape):
+    return tuple(math.prod(shape[i + 1:]) for i in range(len(shape)))
 
 
-_dense_call = functools.lru_cache(maxsize=256)(_call)
+class _Plan:
+    """How calls on operands of one layout go: the library's arguments and workspaces, for a contiguous gradient, and which
+    operands are copied first.  ``rest`` is what the output's rows lack of the sequences'."""
+
+    def __init__(self, q, k, v, causal, scale, sequences):
+        _check(q, k, v, scale, sequences)
+        self.scale, self.causal, self.sequences = scale, causal, sequences
+        self.q_shape, self.k_shape = q.shape, k.shape
+        self.fits = tuple(_fits(x.shape, x.stride()) for x in (q, k, v))
+        self.strides = tuple(_strides(x.shape, x.stride() if f else _contiguous(x.shape)) for x, f in zip((q, k, v), self.fits))
+        self.index = q.get_device()
+        self.q_zero = sequences is not None and sequences.q_count != q.shape[0]
+        self.k_zero = sequences is not None and sequences.k_count != k.shape[0]
+        self.arguments, self.forward_bytes, self.backward_bytes = self.call(_strides(q.shape, _contiguous(q.shape)))
+
+    def call(self, dout_stride, moved=(False, False, False)):
+        """(arguments, bytes of the forward's and of the backward's workspace) with these strides of dout; ``moved``: which
+        operands were copied for their place in memory."""
+        sequences, (*_, H, D) = self.sequences, self.q_shape
+        a = _lib.MsdAttn()
+        if sequences is None:
+            a.n_seqs = self.q_shape[0] if len(self.q_shape) == 4 else 1
+            a.q_len, a.k_len = self.q_shape[-3], self.k_shape[-3]
+        else:
+            a.n_seqs, a.q_len, a.k_len = sequences.n, sequences.q_longest, sequences.k_longest
+            a.seqs, a.seqs_host = sequences.table.data_ptr() or 16, sequences.host.data_ptr() or 16   # (16: nothing to read)
+        a.q_rows, a.k_rows = math.prod(self.q_shape[:-2]), math.prod(self.k_shape[:-2])
+        a.n_heads, a.n_kv_heads, a.d_head, a.causal, a.scale = H, self.k_shape[-2], D, self.causal, self.scale
+        shapes = (self.q_shape, self.k_shape, self.k_shape)
+        strides = [_strides(n, _contiguous(n)) if m else s for n, s, m in zip(shapes, self.strides, moved)]
+        for name, s in zip(("q_stride", "k_stride", "v_stride", "dout_stride"), (*strides, dout_stride)):
+            getattr(a, name)[:] = s
+        sizes = [_lib.check(_lib.lib().msd_attn_workspace_bytes(ctypes.byref(a), i), "msd_attn_workspace_bytes") for i in (0, 1)]
+        return ctypes.byref(a), *sizes
 
 
-def _arguments(q, k, v, dout_stride, causal, scale, sequences):
-    key = (q.shape, k.shape, _strides(q), _strides(k), _strides(v), dout_stride, causal, scale)
-    if sequences is None:
-        return _dense_call(*key)
-    found = sequences._calls.get(key)   # (kept with the sequences: the layers of a step make the same call)
+_plans = {}   # of calls without sequences; a Sequences keeps its own (the layers of a step make the same call)
+
+
+def _plan(q, k, v, causal, scale, sequences):
+    key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, q.device, k.device,
+           v.device, causal, scale)
+    plans = _plans if sequences is None else sequences._plans
+    found = plans.get(key)
     if found is None:
-        if len(sequences._calls) >= 64:
-            sequences._calls.clear()
-        found = sequences._calls[key] = _call(*key, sequences)
+        found = _Plan(q, k, v, causal, scale, sequences)
+        if len(plans) >= 256:
+            plans.clear()
+        plans[key] = found
     return found
 
 
@@ -129,8 +161,8 @@ def _check(q, k, v, scale, sequences):
         raise ValueError(f"d_head must be a multiple of 8 up to 128, the same for q, k and v (got {D} and {k.shape[-1]})")
     if KV == 0 or H == 0 or H % KV:
         raise ValueError(f"n_heads ({H}) must be a multiple of n_kv_heads ({KV})")
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError(f"scale must be positive (got {scale})")
+    if not 2.0 ** -60 <= scale <= 2.0 ** 60:
+        raise ValueError(f"scale must lie in [2 ** -60, 2 ** 60] (got {scale})")
     if q.dim() == 4 and q.shape[0] != k.shape[0]:
         raise ValueError(f"q holds {q.shape[0]} sequences, k and v {k.shape[0]}")
     if sequences is not None:
@@ -143,52 +175,60 @@ def _check(q, k, v, scale, sequences):
             raise ValueError(f"sequences were made for {sequences.table.device}, q is on {q.device}")
 
 
-def _empty(like, rows):
-    """A contiguous output of like's shape; zeros where the sequences leave rows out."""
+def _empty(like, zero):
+    """A contiguous output of like's shape; of zeros where the sequences leave rows out."""
     x = _lib.empty(like)
-    return x if rows is None or rows == like.shape[0] else x.zero_()
+    return x.zero_() if zero else x
 
 
-def _workspace(like, n):
-    return like.new_empty(n, dtype=torch.uint8) if n else None
-
-
-def _forward(q, k, v, causal, scale, sequences, keep):
-    q, k, v = _operand(q), _operand(k), _operand(v)
-    # dout's strides are the backward's own; a contiguous one's (out's) are put in here
-    out = _empty(q, sequences and sequences.q_count)
-    how = _arguments(q, k, v, _strides(out), causal, scale, sequences)
-    a, n, _ = how
+def _forward(q, k, v, plan, keep):
+    at = q.data_ptr() | k.data_ptr() | v.data_ptr()
+    call = plan.arguments, plan.forward_bytes, plan.backward_bytes
+    if at % 16 or plan.fits != (True, True, True):
+        operands = [_operand(x, f) for x, f in zip((q, k, v), plan.fits)]
+        moved = tuple(f and x.data_ptr() % 16 != 0 for x, f in zip((q, k, v), plan.fits))
+        q, k, v = operands
+        if any(moved):
+            call = plan.call(_strides(q.shape, _contiguous(q.shape)), moved)
+    out = _empty(q, plan.q_zero)
     lse = out.new_empty(out.shape[:-1], dtype=torch.float32) if keep else None
-    ws = _workspace(q, n)
-    _lib.launch(_lib.lib().msd_attn_forward, "msd_attn_forward", out.get_device(), a, q.data_ptr(), k.data_ptr(),
-                v.data_ptr(), out.data_ptr(), lse.data_ptr() if keep else None, ws.data_ptr() if n else None)
-    return q, k, v, out, lse, how
+    a, n, _ = call
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
+    if plan.sequences is not None:
+        plan.sequences.used()
+    _lib.launch(_lib.lib().msd_attn_forward, "msd_attn_forward", plan.index, a, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                out.data_ptr(), lse.data_ptr() if keep else None, ws.data_ptr() if n else None)
+    return q, k, v, out, lse, call
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, causal, scale, sequences):
-        q, k, v, out, lse, how = _forward(q, k, v, causal, scale, sequences, True)
+    def forward(ctx, q, k, v, plan):
+        at = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        q, k, v, out, lse, ctx.call = _forward(q, k, v, plan, True)
         ctx.save_for_backward(q, k, v, out, lse)
-        ctx.how = how, causal, scale, sequences
+        ctx.plan = plan
+        ctx.moved = tuple(f and a % 16 != 0 for a, f in zip(at, plan.fits))
         return out
 
     @staticmethod
     @_lib.first_order
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
-        (a, _, n), causal, scale, sequences = ctx.how
+        plan = ctx.plan
+        a, _, n = ctx.call
         if not dout.is_contiguous() or dout.data_ptr() % 16:
-            dout = _operand(dout)
-            a, _, n = _arguments(q, k, v, _strides(dout), causal, scale, sequences)
-        dq = _empty(q, sequences and sequences.q_count)
-        dk, dv = (_empty(x, sequences and sequences.k_count) for x in (k, v))
-        ws = _workspace(q, n)
-        _lib.launch(_lib.lib().msd_attn_backward, "msd_attn_backward", dout.get_device(), a, q.data_ptr(), k.data_ptr(),
+            dout = _operand(dout, _fits(dout.shape, dout.stride()))
+            a, _, n = plan.call(_strides(dout.shape, dout.stride()), ctx.moved)
+        dq = _empty(q, plan.q_zero)
+        dk, dv = _empty(k, plan.k_zero), _empty(v, plan.k_zero)
+        ws = q.new_empty(n, dtype=torch.uint8) if n else None
+        if plan.sequences is not None:
+            plan.sequences.used()
+        _lib.launch(_lib.lib().msd_attn_backward, "msd_attn_backward", plan.index, a, q.data_ptr(), k.data_ptr(),
                     v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
                     dv.data_ptr(), ws.data_ptr() if n else None)
-        return dq, dk, dv, None, None, None
+        return dq, dk, dv, None
 
 
 def attention(q, k, v, causal=True, scale=None, sequences=None):
@@ -201,9 +241,8 @@ def attention(q, k, v, causal=True, scale=None, sequences=None):
 
     What lies behind a sequence's own rows is not read.  Within a sequence, a key or value row that is not finite
     reaches every query that sees it, and may reach those that do not."""
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    _check(q, k, v, scale, sequences)
-    causal = bool(causal)
+    scale = q.shape[-1] ** -0.5 if scale is None and q.dim() and q.shape[-1] else float(scale or 0)
+    plan = _plan(q, k, v, bool(causal), scale, sequences)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _Attention.apply(q, k, v, causal, scale, sequences)
-    return _forward(q, k, v, causal, scale, sequences, False)[3]
+        return _Attention.apply(q, k, v, plan)
+    return _forward(q, k, v, plan, False)[3]

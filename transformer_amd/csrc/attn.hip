@@ -1002,19 +1002,19 @@ bool fits(const int64_t (&s)[3], int64_t heads) {
   for (int64_t x : s)
     if (x < 0 || x % 8) return false;
   constexpr int64_t most = int64_t(1) << 30;
-  return s[1] <= most / 64 && s[2] <= most / heads && 64 * s[1] + heads * s[2] < most;
+  return s[1] <= most / 128 && s[2] <= most / heads && 128 * s[1] + heads * s[2] < most;   // (a tile of 128 rows)
 }
 
 // whether the library takes the call, and how
 int32_t check(const msd_attn* a, bool backward, Plan& p) {
   if (!a) return MSD_E_ARG;
   if (a->n_seqs < 0 || a->q_len < 0 || a->k_len < 0 || a->n_heads <= 0 || a->n_kv_heads <= 0 || a->n_heads % a->n_kv_heads ||
-      a->d_head <= 0 || a->d_head > 128 || a->d_head % 8 || !(a->scale > 0) || !isfinite(a->scale) || a->q_rows < 0 ||
+      a->d_head <= 0 || a->d_head > 128 || a->d_head % 8 || !(a->scale >= 0x1p-60f) || !(a->scale <= 0x1p60f) || a->q_rows < 0 ||
       a->k_rows < 0)
     return MSD_E_CONFIG;
   const int64_t most = int64_t(1) << 31;
-  if (a->q_rows >= most || a->k_rows >= most || a->q_rows * a->n_heads >= most || a->k_rows * a->n_kv_heads >= most ||
-      int64_t(a->q_len) * (a->n_heads / a->n_kv_heads) >= (1 << 30) - 256 || int64_t(a->n_seqs) * a->n_kv_heads >= (1 << 20) || a->n_heads > 8192 || a->n_seqs > 65535)
+  if (a->q_rows >= most / 2 || a->k_rows >= most / 2 || a->q_rows * a->n_heads >= most || a->k_rows * a->n_kv_heads >= most ||
+      int64_t(a->q_len) * (a->n_heads / a->n_kv_heads) >= (1 << 30) - 256 || int64_t(a->n_seqs) * a->n_kv_heads >= (1 << 20) || a->n_heads > 4096 || a->n_seqs > 65535)
     return MSD_E_CONFIG;
   if (!a->seqs && (a->q_rows != int64_t(a->n_seqs) * a->q_len || a->k_rows != int64_t(a->n_seqs) * a->k_len)) return MSD_E_CONFIG;
   if (a->q_len > a->q_rows || a->k_len > a->k_rows) return MSD_E_CONFIG;

@@ -772,7 +772,7 @@ extern "C" int32_t msd_rope_apply(const msd_rope* r, const void* q, const void* 
   hipError_t err = hipSuccess;
   with_type(r->type, [&](auto t) {
     auto go = [&](auto kernel) {
-      if (lds > 65536) err = msdc::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), lds);
+      if (lds > 64000) err = msdc::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), lds);
       if (err == hipSuccess)
         hipLaunchKernelGGL(kernel, dim3(unsigned(cdiv(rows, kTokens))), dim3(256), lds, s, p);
     };

@@ -9,7 +9,6 @@ reduced to a turn before they are rounded, so far positions keep f32's precision
 table to run past).  The gradient is the same kernel turning back.
 """
 import ctypes
-import functools
 import math
 
 import torch
@@ -64,56 +63,97 @@ LAYOUTS = {"half": 0, "interleaved": 1}
 
 
 def _strides(x):
+    """(batch, token, head) strides of x with contiguous heads; 0 along an axis of one (or none)."""
     s = tuple(0 if n <= 1 else k for n, k in zip(x.shape[:-1], x.stride()))
     return s if len(s) == 3 else (0, *s)
 
 
-@functools.lru_cache(maxsize=256)
-def _call(shape, kv, q_stride, k_stride, dtype, d_rot, amplitude, interleaved, sign, pos_bytes, pos_stride, start):
-    r = _lib.MsdRope()
-    *_, r.tokens, r.n_heads, r.d_head = shape
-    r.batch = shape[0] if len(shape) == 4 else 1
-    r.n_kv_heads, r.d_rot, r.interleaved, r.type, r.sign = kv, d_rot, interleaved, _lib.TYPES[dtype], sign
-    r.position_bytes, r.amplitude, r.start = pos_bytes, amplitude, start
-    r.q_stride[:], r.k_stride[:], r.position_stride[:] = q_stride, k_stride, pos_stride
-    return r
+def _contiguous(shape):
+    s, d, h = shape[-3] * shape[-2] * shape[-1], shape[-1], shape[-2] * shape[-1]
+    return (s, h, d)
 
 
-def _heads(x):
-    return x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+def _turns_heads(x):
+    return x.shape[-1] == 1 or x.stride(-1) == 1
 
 
-def _apply(q, k, turns, amplitude, positions, start, layout, sign):
-    q, k = _heads(q), None if k is None else _heads(k)
-    pos_bytes, pos_stride = 0, (0, 0)
-    if positions is not None:
-        pos_bytes = positions.element_size()
-        pos_stride = positions.stride() if positions.dim() == 2 else (0, *positions.stride())
-    r = _call(q.shape, 0 if k is None else k.shape[-2], _strides(q), (0, 0, 0) if k is None else _strides(k), q.dtype,
-              2 * turns.numel(), amplitude, LAYOUTS[layout], sign, pos_bytes, pos_stride, start)
+class _Plan:
+    """How calls on tensors of one layout go: the library's arguments forward and, for contiguous gradients, backward."""
+
+    def __init__(self, q, k, frequencies, positions, start, layout):
+        _check(q, k, frequencies, positions, layout)
+        self.q_shape, self.kv, self.dtype, self.index = q.shape, 0 if k is None else k.shape[-2], q.dtype, q.get_device()
+        self.d_rot, self.amplitude, self.start, self.layout = frequencies.d_rot, frequencies.amplitude, start, layout
+        self.position_bytes, self.position_stride = 0, (0, 0)
+        if positions is not None:
+            self.position_bytes = positions.element_size()
+            self.position_stride = positions.stride() if positions.dim() == 2 else (0, *positions.stride())
+        self.copies = not _turns_heads(q) or (k is not None and not _turns_heads(k))
+        whole = _contiguous(q.shape), None if k is None else _contiguous(k.shape)
+        self.forward = self.call(1, *(whole if self.copies else (_strides(q), None if k is None else _strides(k))))
+        self.backward = self.call(-1, *whole)
+
+    def call(self, sign, q_stride, k_stride):
+        r = _lib.MsdRope()
+        *_, r.tokens, r.n_heads, r.d_head = self.q_shape
+        r.batch = self.q_shape[0] if len(self.q_shape) == 4 else 1
+        r.n_kv_heads, r.d_rot, r.interleaved, r.type, r.sign = self.kv, self.d_rot, LAYOUTS[self.layout], _lib.TYPES[self.dtype], sign
+        r.position_bytes, r.amplitude, r.start = self.position_bytes, self.amplitude, self.start
+        r.q_stride[:], r.k_stride[:], r.position_stride[:] = q_stride, k_stride or (0, 0, 0), self.position_stride
+        return ctypes.byref(r)
+
+
+_plans = {}
+
+
+def _plan(q, k, frequencies, positions, start, layout):
+    key = (q.shape, q.stride(), q.dtype, q.device, None if k is None else (k.shape, k.stride(), k.dtype, k.device),
+           None if positions is None else (positions.shape, positions.stride(), positions.dtype, positions.device),
+           frequencies.d_rot, frequencies.amplitude, frequencies.turns.device, start, layout)
+    found = _plans.get(key)
+    if found is None:
+        found = _Plan(q, k, frequencies, positions, start, layout)
+        if len(_plans) >= 256:
+            _plans.clear()
+        _plans[key] = found
+    return found
+
+
+def _apply(index, call, q, k, turns, positions):
     q_out = _lib.empty(q)
     k_out = None if k is None else _lib.empty(k)
-    _lib.launch(_lib.lib().msd_rope_apply, "msd_rope_apply", q.get_device(), ctypes.byref(r), q.data_ptr(),
-                None if k is None else k.data_ptr(), None if positions is None else positions.data_ptr(), turns.data_ptr(),
-                q_out.data_ptr(), None if k is None else k_out.data_ptr())
+    _lib.launch(_lib.lib().msd_rope_apply, "msd_rope_apply", index, call, q.data_ptr(), None if k is None else k.data_ptr(),
+                None if positions is None else positions.data_ptr(), turns.data_ptr(), q_out.data_ptr(),
+                None if k is None else k_out.data_ptr())
     return q_out, k_out
+
+
+def _forward(q, k, turns, positions, plan):
+    if plan.copies:
+        q, k = q.contiguous(), None if k is None else k.contiguous()
+    return _apply(plan.index, plan.forward, q, k, turns, positions)
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, turns, amplitude, positions, start, layout):
+    def forward(ctx, q, k, turns, positions, plan):
         ctx.save_for_backward(turns, positions)
-        ctx.how = amplitude, start, layout
-        q, k = _apply(q, k, turns, amplitude, positions, start, layout, 1)
+        ctx.plan = plan
+        q, k = _forward(q, k, turns, positions, plan)
         return q if k is None else (q, k)
 
     @staticmethod
     @_lib.first_order
     def backward(ctx, dq, dk=None):
         turns, positions = ctx.saved_tensors
-        amplitude, start, layout = ctx.how
-        dq, dk = _apply(dq, dk, turns, amplitude, positions, start, layout, -1)
-        return dq, dk, None, None, None, None, None
+        plan = ctx.plan
+        call = plan.backward
+        if not dq.is_contiguous() or (dk is not None and not dk.is_contiguous()):
+            if not _turns_heads(dq) or (dk is not None and not _turns_heads(dk)):
+                dq, dk = dq.contiguous(), None if dk is None else dk.contiguous()
+            call = plan.call(-1, _strides(dq), None if dk is None else _strides(dk))
+        dq, dk = _apply(plan.index, call, dq, dk, turns, positions)
+        return dq, dk, None, None, None
 
 
 def _check(q, k, frequencies, positions, layout):
@@ -143,9 +183,8 @@ def rotary(q, k, frequencies, positions=None, start=0, layout="half"):
     one GPU, any strides.  positions: (batch, tokens) or (tokens,) int32 or int64, any values; without them token t is at
     position start + t.  layout: pairs (i, i + d_rot / 2) ("half", the reference's) or (2 i, 2 i + 1) ("interleaved").
     Returns contiguous (q, k), with autograd; q alone without a k."""
-    _check(q, k, frequencies, positions, layout)
-    args = (q, k, frequencies.turns, frequencies.amplitude, positions, int(start), layout)
+    plan = _plan(q, k, frequencies, positions, int(start), layout)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotary.apply(*args)
-    q, k = _apply(*args, 1)
+        return _Rotary.apply(q, k, frequencies.turns, positions, plan)
+    q, k = _forward(q, k, frequencies.turns, positions, plan)
     return q if k is None else (q, k)
