@@ -57,14 +57,17 @@ typedef struct msd_attn {
 int64_t msd_attn_workspace_bytes(const msd_attn* a, int32_t backward);
 
 /* out = softmax(scale q k^T) v.  lse: device f32 (q_rows * n_heads), kept for the backward (its layout is the
- * library's own); may be NULL when no backward follows. */
-int32_t msd_attn_forward(const msd_attn* a, const void* q, const void* k, const void* v, void* out, float* lse,
-                         void* workspace, void* stream);
+ * library's own); out_low: a byte (q_rows * n_heads * d_head, 8-byte aligned) for what the rounding to bf16 took off each
+ * value of out, from which the backward forms rowsum(dout * out) to f32's rather than bf16's precision (dq and dk then lie
+ * a tenth nearer the exact ones).  Either may be NULL: no backward follows, or out itself will do. */
+int32_t msd_attn_forward(const msd_attn* a, const void* q, const void* k, const void* v, void* out, void* out_low,
+                         float* lse, void* workspace, void* stream);
 
-/* dq, dk, dv of the forward's arguments, `out` and `lse` its results and dout the gradient of `out`. */
+/* dq, dk, dv of the forward's arguments; `out`, `out_low` (or NULL) and `lse` are its results and dout the gradient of
+ * `out`. */
 int32_t msd_attn_backward(const msd_attn* a, const void* q, const void* k, const void* v, const void* out,
-                          const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
-                          void* stream);
+                          const void* out_low, const float* lse, const void* dout, void* dq, void* dk, void* dv,
+                          void* workspace, void* stream);
 
 /* Value types of the calls below. */
 enum { MSD_BF16 = 0, MSD_F32 = 1 };

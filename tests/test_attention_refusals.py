@@ -84,31 +84,31 @@ def test_c_refuses_shapes(kw):
     L, a = _lib.lib(), _args(**kw)
     p = ctypes.c_void_p(4096)
     assert L.msd_attn_workspace_bytes(ctypes.byref(a), 0) == _lib.MSD_E_CONFIG
-    assert L.msd_attn_forward(ctypes.byref(a), p, p, p, p, p, p, None) == _lib.MSD_E_CONFIG
-    assert L.msd_attn_backward(ctypes.byref(a), p, p, p, p, p, p, p, p, p, p, None) == _lib.MSD_E_CONFIG
+    assert L.msd_attn_forward(ctypes.byref(a), p, p, p, p, p, p, p, None) == _lib.MSD_E_CONFIG
+    assert L.msd_attn_backward(ctypes.byref(a), p, p, p, p, p, p, p, p, p, p, p, None) == _lib.MSD_E_CONFIG
 
 
 def test_c_refuses_pointers():
     L, p = _lib.lib(), ctypes.c_void_p(4096)
     assert L.msd_attn_workspace_bytes(None, 0) == _lib.MSD_E_ARG
-    assert L.msd_attn_forward(None, p, p, p, p, p, p, None) == _lib.MSD_E_ARG
+    assert L.msd_attn_forward(None, p, p, p, p, p, p, p, None) == _lib.MSD_E_ARG
     a = _args()
     for bad in (None, ctypes.c_void_p(4104)):
         for i in (0, 1, 2, 3):
-            args = [p] * 6
+            args = [p] * 7
             args[i] = bad
             assert L.msd_attn_forward(ctypes.byref(a), *args, None) == _lib.MSD_E_ARG
-        for i in range(10):
-            args = [p] * 10
+        for i in [i for i in range(11) if i != 4]:   # (out_low may be missing)
+            args = [p] * 11
             args[i] = bad
             assert L.msd_attn_backward(ctypes.byref(a), *args, None) == _lib.MSD_E_ARG
     for kw in (dict(seqs=4100), dict(seqs=16, seqs_host=None), dict(seqs=16, seqs_host=4098)):
         a = _args(**kw)
         assert L.msd_attn_workspace_bytes(ctypes.byref(a), 0) == _lib.MSD_E_ARG
     assert L.msd_attn_workspace_bytes(ctypes.byref(_args(seqs=16)), 0) >= 0
-    assert L.msd_attn_forward(ctypes.byref(a), p, p, p, p, p, p, None) == _lib.MSD_E_ARG
+    assert L.msd_attn_forward(ctypes.byref(a), p, p, p, p, p, p, p, None) == _lib.MSD_E_ARG
     a = _args(dout_stride=(1, 1, 1))
-    assert L.msd_attn_backward(ctypes.byref(a), *[p] * 10, None) == _lib.MSD_E_CONFIG
+    assert L.msd_attn_backward(ctypes.byref(a), *[p] * 11, None) == _lib.MSD_E_CONFIG
 
 
 def test_workspaces():

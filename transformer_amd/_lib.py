@@ -155,9 +155,9 @@ def lib():
     AP = ctypes.POINTER(MsdAttn)
     L.msd_attn_workspace_bytes.argtypes = [AP, I32]
     L.msd_attn_workspace_bytes.restype = I64
-    L.msd_attn_forward.argtypes = [AP, P, P, P, P, P, P, P]
+    L.msd_attn_forward.argtypes = [AP, P, P, P, P, P, P, P, P]
     L.msd_attn_forward.restype = I32
-    L.msd_attn_backward.argtypes = [AP, P, P, P, P, P, P, P, P, P, P, P]
+    L.msd_attn_backward.argtypes = [AP, P, P, P, P, P, P, P, P, P, P, P, P]
     L.msd_attn_backward.restype = I32
     F = ctypes.c_float
     L.msd_rope_apply.argtypes = [ctypes.POINTER(MsdRope), P, P, P, P, P, P, P]

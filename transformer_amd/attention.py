@@ -7,7 +7,7 @@ The reference's causal_attention (model.py:122-147) between its projections: q (
 
 What runs (``msd_attn_forward`` / ``msd_attn_backward``, ``csrc/attn.hip``): one pass over the keys with the running
 maximum and sum of the softmax, so no score matrix is stored; the forward keeps each row's logsumexp, from which the
-backward forms the probabilities again.  Scores, softmax statistics and every sum are f32; the probabilities and the
+backward forms the probabilities again, and a byte beside each value of the output for what its rounding took off.  Scores, softmax statistics and every sum are f32; the probabilities and the
 scores' gradients are rounded to bf16 as operands of the matrix cores, the results once to bf16.  Deterministic.
 """
 import ctypes
@@ -191,22 +191,25 @@ def _forward(q, k, v, plan, keep):
         if any(moved):
             call = plan.call(_strides(q.shape, _contiguous(q.shape)), moved)
     out = _empty(q, plan.q_zero)
-    lse = out.new_empty(out.shape[:-1], dtype=torch.float32) if keep else None
+    lse = low = None
+    if keep:
+        lse, low = out.new_empty(out.shape[:-1], dtype=torch.float32), torch.empty_like(out, dtype=torch.uint8)
     a, n, _ = call
     ws = q.new_empty(n, dtype=torch.uint8) if n else None
     if plan.sequences is not None:
         plan.sequences.used()
     _lib.launch(_lib.lib().msd_attn_forward, "msd_attn_forward", plan.index, a, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                out.data_ptr(), lse.data_ptr() if keep else None, ws.data_ptr() if n else None)
-    return q, k, v, out, lse, call
+                out.data_ptr(), low.data_ptr() if keep else None, lse.data_ptr() if keep else None,
+                ws.data_ptr() if n else None)
+    return q, k, v, out, low, lse, call
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, plan):
         at = q.data_ptr(), k.data_ptr(), v.data_ptr()
-        q, k, v, out, lse, ctx.call = _forward(q, k, v, plan, True)
-        ctx.save_for_backward(q, k, v, out, lse)
+        q, k, v, out, low, lse, ctx.call = _forward(q, k, v, plan, True)
+        ctx.save_for_backward(q, k, v, out, low, lse)
         ctx.plan = plan
         ctx.moved = tuple(f and a % 16 != 0 for a, f in zip(at, plan.fits))
         return out
@@ -214,7 +217,7 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @_lib.first_order
     def backward(ctx, dout):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, low, lse = ctx.saved_tensors
         plan = ctx.plan
         a, _, n = ctx.call
         if not dout.is_contiguous() or dout.data_ptr() % 16:
@@ -226,7 +229,7 @@ class _Attention(torch.autograd.Function):
         if plan.sequences is not None:
             plan.sequences.used()
         _lib.launch(_lib.lib().msd_attn_backward, "msd_attn_backward", plan.index, a, q.data_ptr(), k.data_ptr(),
-                    v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                    v.data_ptr(), out.data_ptr(), low.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
                     dv.data_ptr(), ws.data_ptr() if n else None)
         return dq, dk, dv, None
 

@@ -74,6 +74,7 @@ struct Args {
   int tile_rows, head_parts, row_parts, chunk;   // dK and dV: see KeyPart
   int64_t q_rows, k_rows;
   uint16_t *out, *dq, *dk, *dv;
+  uint8_t* low;             // what the rounding to bf16 took off each value of out (low_byte()), or null
   float* lse;
   float* stats;             // backward: (-lse / c, -D) of every row, in the order of lse
   float* part;              // forward: [splits][q_rows * H][D + 1]; backward: [2][splits][k_rows * KV][D]
@@ -110,6 +111,17 @@ __device__ __forceinline__ int div_g(const Args& p, int r) {
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
+// x is to about 2^-16 what a = bf16(x) and this byte say together: the upper eight of the sixteen bits by which x's differ
+// from a's (the rounding is to nearest, so that they are a signed byte)
+__device__ __forceinline__ uint32_t low_byte(float x, uint32_t a) { return (__float_as_uint(x) - (a << 16)) >> 8 & 0xff; }
+__device__ __forceinline__ float with_low(uint32_t a, uint32_t byte) {
+  return __uint_as_float((a << 16) + uint32_t(int32_t(byte << 24) >> 16));
+}
+// the bytes of four values and their two bf16 pairs
+__device__ __forceinline__ uint32_t low_bytes(float x0, float x1, float x2, float x3, uint32_t a01, uint32_t a23) {
+  return low_byte(x0, a01 & 0xffff) | low_byte(x1, a01 >> 16) << 8 | low_byte(x2, a23 & 0xffff) << 16 | low_byte(x3, a23 >> 16) << 24;
 }
 
 __device__ __forceinline__ bf16x8 pack8(const f32x16& s, int i) {
@@ -278,6 +290,28 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, const f32x16 (&acc)[D
     const u32x4 x = *reinterpret_cast<const u32x4*>(stage + piece_at<P>(r, c));
     uint16_t* to = dst(r);
     if (to && 8 * c < D) *reinterpret_cast<u32x4*>(to + 8 * c) = x;
+  }
+  wave_lds_order();
+}
+// Likewise the bytes that the rounding took off
+template <int DP, class F>
+__device__ __forceinline__ void store_low(uint8_t* stage, const f32x16 (&acc)[DP / 32], float by, int D, int lane, F dst) {
+  constexpr int P = DP + 8, C = DP / 8;   // (the eight spread the rows over the banks)
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float x0 = acc[b][4 * q] * by, x1 = acc[b][4 * q + 1] * by, x2 = acc[b][4 * q + 2] * by, x3 = acc[b][4 * q + 3] * by;
+      *reinterpret_cast<uint32_t*>(stage + (lane & 31) * P + 32 * b + 8 * q + 4 * (lane >> 5)) =
+          low_bytes(x0, x1, x2, x3, pack2(x0, x1), pack2(x2, x3));
+    }
+  wave_lds_order();
+#pragma unroll
+  for (int u = 0; u < 32 * C / 64; ++u) {
+    const int i = lane + 64 * u, r = i / C, c = i % C;
+    const u32x2 x = *reinterpret_cast<const u32x2*>(stage + r * P + 8 * c);
+    uint8_t* to = dst(r);
+    if (to && 8 * c < D) *reinterpret_cast<u32x2*>(to + 8 * c) = x;
   }
   wave_lds_order();
 }
@@ -467,11 +501,13 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attn_fwd(Args p, Jo
   }
   if (p.lse && j.ok && lane < 32) p.lse[stat_index(p, j)] = lse;
   const int r0 = j.r - (lane & 31);
-  store_rows<DP>(lds + wv * 32 * P, o, by, p.D, lane, [&](int r) -> uint16_t* {
-    if (r0 + r >= j.rows) return nullptr;
+  auto at = [&](int r) -> int64_t {
+    if (r0 + r >= j.rows) return -1;
     const int pos = div_g(p, r0 + r);
-    return p.out + (int64_t(j.s.qs + pos) * p.H + j.kvh * p.g + (r0 + r - pos * p.g)) * p.D;
-  });
+    return (int64_t(j.s.qs + pos) * p.H + j.kvh * p.g + (r0 + r - pos * p.g)) * p.D;
+  };
+  store_rows<DP>(lds + wv * 32 * P, o, by, p.D, lane, [&](int r) { return at(r) < 0 ? nullptr : p.out + at(r); });
+  if (p.low) store_low<DP>(lds + wv * 32 * P, o, by, p.D, lane, [&](int r) { return at(r) < 0 ? nullptr : p.low + at(r); });
 }
 
 // A row from its parts over the splits, weighted by 2^(lse_z - lse).  16 lanes a row's 8-value pieces (as many as it has), G
@@ -527,8 +563,12 @@ __global__ __launch_bounds__(kJoinLanes) void attn_join(Args p) {
   const int head = int(row) / s.qn, pos = int(row) - head * s.qn;
   u32x4 x;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = pack2(acc[2 * i] * by, acc[2 * i + 1] * by);
-  *reinterpret_cast<u32x4*>(p.out + (int64_t(s.qs + pos) * p.H + head) * p.D + 8 * c) = x;
+  for (int i = 0; i < 4; ++i) x[i] = pack2(acc[2 * i] *= by, acc[2 * i + 1] *= by);
+  const int64_t to = (int64_t(s.qs + pos) * p.H + head) * p.D + 8 * c;
+  *reinterpret_cast<u32x4*>(p.out + to) = x;
+  if (p.low)
+    *reinterpret_cast<u32x2*>(p.low + to) = u32x2{low_bytes(acc[0], acc[1], acc[2], acc[3], x[0], x[1]),
+                                                  low_bytes(acc[4], acc[5], acc[6], acc[7], x[2], x[3])};
   if (p.lse && c == 0) p.lse[at] = l == 0 ? INFINITY : m + __log2f(l);
 }
 
@@ -550,12 +590,19 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p, Jobs jobs) {
                    p.D, lane);
   float delta = 0;
   {
+    const int64_t at = (int64_t(j.s.qs + j.pos) * p.H + j.head) * p.D;
     bf16x8 o[DP / 16];
-    row_operands<DP>(o, p.o, (int64_t(j.s.qs + j.pos) * p.H + j.head) * p.D, j.ok, p.D, lane);
+    row_operands<DP>(o, p.o, at, j.ok, p.D, lane);
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks)
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const int c = 16 * ks + 8 * (lane >> 5);
+      u32x2 low{};
+      if (p.low && j.ok && c < p.D) low = *reinterpret_cast<const u32x2*>(p.low + at + c);
+      const u32x4 bits = __builtin_bit_cast(u32x4, o[ks]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) delta = fmaf(float(o[ks][i]), float(dO[ks][i]), delta);
+      for (int i = 0; i < 8; ++i)
+        delta = fmaf(with_low(bits[i >> 1] >> (16 * (i & 1)) & 0xffff, low[i >> 2] >> (8 * (i & 3)) & 0xff), float(dO[ks][i]), delta);
+    }
   }
   delta += swap_halves(delta);
   const float lse = j.ok ? p.lse[stat_index(p, j)] : INFINITY;
@@ -1086,17 +1133,20 @@ extern "C" int64_t msd_attn_workspace_bytes(const msd_attn* a, int32_t backward)
   return up(8 * a->q_rows * a->n_heads) + parts;
 }
 
-extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void* k, const void* v, void* out, float* lse,
-                                    void* workspace, void* stream) {
+extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void* k, const void* v, void* out, void* out_low,
+                                    float* lse, void* workspace, void* stream) {
   Plan pl;
   const int32_t rc = check(a, false, pl);
   if (rc != MSD_OK) return rc;
   if (a->n_seqs == 0 || a->q_len == 0) return MSD_OK;
-  if (bad(q) || bad(out) || (a->k_len && (bad(k) || bad(v)))) return MSD_E_ARG;
+  if (bad(q) || bad(out) || (a->k_len && (bad(k) || bad(v))) || reinterpret_cast<uintptr_t>(out_low) % 8 ||
+      reinterpret_cast<uintptr_t>(lse) % 16)
+    return MSD_E_ARG;
   if (pl.splits > 1 && bad(workspace)) return MSD_E_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
   Args p = args(*a, q, k, v);
   p.out = static_cast<uint16_t*>(out);
+  p.low = static_cast<uint8_t*>(out_low);
   p.lse = lse;
   p.part = static_cast<float*>(workspace);
   p.splits = pl.splits;
@@ -1115,13 +1165,14 @@ extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void
 }
 
 extern "C" int32_t msd_attn_backward(const msd_attn* a, const void* q, const void* k, const void* v, const void* out,
-                                     const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                                     const void* out_low, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
                                      void* stream) {
   Plan pl;
   const int32_t rc = check(a, true, pl);
   if (rc != MSD_OK) return rc;
   if (a->n_seqs == 0 || (a->q_len == 0 && a->k_len == 0)) return MSD_OK;
-  if ((a->q_len && (bad(q) || bad(out) || bad(lse) || bad(dout) || bad(dq))) ||
+  if ((a->q_len && (bad(q) || bad(out) || bad(lse) || bad(dout) || bad(dq) ||
+                    reinterpret_cast<uintptr_t>(out_low) % 8)) ||
       (a->k_len && (bad(k) || bad(v) || bad(dk) || bad(dv))))
     return MSD_E_ARG;
   if (bad(workspace) && (a->q_len || pl.head_parts * pl.row_parts > 1)) return MSD_E_ARG;
@@ -1129,6 +1180,7 @@ extern "C" int32_t msd_attn_backward(const msd_attn* a, const void* q, const voi
   Args p = args(*a, q, k, v);
   p.dout = view(dout, a->dout_stride);
   p.o = static_cast<const uint16_t*>(out);
+  p.low = static_cast<uint8_t*>(const_cast<void*>(out_low));
   p.lse = const_cast<float*>(lse);
   p.stats = static_cast<float*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + up(8 * a->q_rows * a->n_heads));
