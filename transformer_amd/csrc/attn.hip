@@ -316,16 +316,6 @@ __device__ __forceinline__ void store_low(uint8_t* stage, const f32x16 (&acc)[DP
   wave_lds_order();
 }
 
-// The priority of a wave with n of at most `most` pieces of work before it: the longest set how long a launch takes, and
-// otherwise share their SIMDs evenly with shorter ones that could wait
-__device__ __forceinline__ void prioritise(int n, int most) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  if (4 * n > 3 * most) __builtin_amdgcn_s_setprio(3);
-  else if (2 * n > most) __builtin_amdgcn_s_setprio(2);
-  else if (4 * n > most) __builtin_amdgcn_s_setprio(1);
-#endif
-}
-
 // The sequence that job i belongs to, and its number among that sequence's jobs
 __device__ __forceinline__ int job_sequence(const Args& p, const Jobs& jobs, int i, int& local, int lane) {
   if (!jobs.counted) {
@@ -375,7 +365,6 @@ __device__ __forceinline__ bool row_job(const Args& p, const Jobs& jobs, RowJob&
   const int per = n / p.splits, more = n % p.splits, y = blockIdx.y;
   j.t0 = per * y + min(y, more);
   j.t1 = j.t0 + per + (y < more);
-  prioritise(j.t1 - j.t0, (p.k_len + kKeys - 1) / kKeys / p.splits);
   return true;
 }
 
@@ -763,7 +752,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   if (128 * kb >= s.kn) return;
   const KeyPart w = key_part(p, s, kb, zr, n_heads);
   if (zr >= w.parts) return;   // (a block that no row sees has one, which writes its zeros)
-  prioritise(w.t1 - w.t0, p.chunk);
   const int last = s.kn - s.qn + 1;
   const uint16_t* qb = origin(p, p.q, b, s.qs, kvh * p.g + h0);
   const uint16_t* db = origin(p, p.dout, b, s.qs, kvh * p.g + h0);
