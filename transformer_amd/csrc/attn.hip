@@ -50,7 +50,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kKeys = 64;        // keys of an LDS tile
+// Keys of an LDS tile: 32 where a workgroup is one wave, so that its buffers leave room for enough others on a CU
+template <int NW>
+constexpr int tile_keys() { return NW == 1 ? 32 : 64; }
 // Rows of an LDS tile of q and dout
 template <int DP>
 constexpr int tile_rows() { return DP <= 64 ? 64 : 32; }
@@ -220,7 +222,7 @@ __device__ __forceinline__ bf16x8 cols_operand(const uint8_t* tile, int row0, in
 }
 
 // A tile of R rows on its way to LDS: wave w of NW fetches its instructions w, w + NW, ..
-template <int DP, int NW, int R = kKeys>
+template <int DP, int NW, int R>
 struct Tile {
   static constexpr int P = pitch<DP>(), C = P / 16, N = R * P / 1024 / NW;
   static_assert(64 * NW % C == 0, "an instruction's rows are a fixed number apart");
@@ -331,7 +333,7 @@ __device__ __forceinline__ int job_sequence(const Args& p, const Jobs& jobs, int
   return b;
 }
 
-// What a workgroup of row tiles works on: 32 rows a wave, keys [k_lo, k_hi) in tiles of 64
+// What a workgroup of row tiles works on: 32 rows a wave, the keys in tiles
 struct RowJob {
   Seq s;
   int b, kvh, rows, r;      // r: this lane's row
@@ -361,7 +363,7 @@ __device__ __forceinline__ bool row_job(const Args& p, const Jobs& jobs, RowJob&
   auto seen_by = [&](int r) { return p.causal ? min(max(last + div_g(p, r), 0), j.s.kn) : j.s.kn; };
   j.wave_full = seen_by(w0);
   j.wave_end = seen_by(w1);
-  const int n = (seen_by(wg) + kKeys - 1) / kKeys;
+  const int n = (seen_by(wg) + tile_keys<NW>() - 1) / tile_keys<NW>();
   const int per = n / p.splits, more = n % p.splits, y = blockIdx.y;
   j.t0 = per * y + min(y, more);
   j.t1 = j.t0 + per + (y < more);
@@ -378,14 +380,24 @@ __device__ __forceinline__ int64_t stat_index(const Args& p, const RowJob& j) {
 // product with V.  So the scores run 32 keys ahead, K one tile ahead of V: three K buffers and two of V, one barrier a tile.
 template <int DP, int NW>
 __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attn_fwd(Args p, Jobs jobs) {
-  constexpr int P = pitch<DP>(), TILE = kKeys * P;
+  constexpr int P = pitch<DP>(), KT = tile_keys<NW>(), TILE = KT * P;
   __shared__ __attribute__((aligned(16))) uint8_t lds[5 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   RowJob j;
   if (!row_job<NW>(p, jobs, j, lane, wv)) return;
   const uint16_t* kb = origin(p, p.k, j.b, j.s.ks, j.kvh);
   const uint16_t* vb = origin(p, p.v, j.b, j.s.ks, j.kvh);
-
+  Tile<DP, NW, KT> kt, vt;
+  kt.init(p.k.row, p.D, lane, wv);
+  vt.init(p.v.row, p.D, lane, wv);
+  auto load_k = [&](uint8_t* to, int t) { kt.load(to, kb + int64_t(t) * KT * p.k.row, j.s.kn - t * KT, wv); };
+  auto load_v = [&](uint8_t* to, int t) { vt.load(to, vb + int64_t(t) * KT * p.v.row, j.s.kn - t * KT, wv); };
+  uint8_t *k0 = lds, *k1 = lds + TILE, *k2 = lds + 2 * TILE, *v0 = lds + 3 * TILE, *v1 = lds + 4 * TILE;
+  if (j.t0 < j.t1) {
+    load_k(k0, j.t0);
+    load_v(v0, j.t0);
+    load_k(k1, j.t0 + 1);
+  }
   bf16x8 q[DP / 16];
   row_operands<DP>(q, origin(p, p.q, j.b, j.s.qs, 0), int64_t(j.pos) * p.q.row + int64_t(j.head) * p.q.head, j.ok, p.D, lane);
 
@@ -434,18 +446,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attn_fwd(Args p, Jo
     }
   };
 
-  Tile<DP, NW> kt, vt;
-  kt.init(p.k.row, p.D, lane, wv);
-  vt.init(p.v.row, p.D, lane, wv);
-  auto load_k = [&](uint8_t* to, int t) { kt.load(to, kb + int64_t(t) * kKeys * p.k.row, j.s.kn - t * kKeys, wv); };
-  auto load_v = [&](uint8_t* to, int t) { vt.load(to, vb + int64_t(t) * kKeys * p.v.row, j.s.kn - t * kKeys, wv); };
-  uint8_t *k0 = lds, *k1 = lds + TILE, *k2 = lds + 2 * TILE, *v0 = lds + 3 * TILE, *v1 = lds + 4 * TILE;
   f32x16 s0, s1;
-  if (j.t0 < j.t1) {
-    load_k(k0, j.t0);
-    load_v(v0, j.t0);
-    load_k(k1, j.t0 + 1);
-  }
   dma_wait();
   __syncthreads();
   if (j.t0 < j.t1) s0 = scores(k0, 0);
@@ -454,10 +455,15 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attn_fwd(Args p, Jo
       load_k(k2, t + 2);
       load_v(v1, t + 1);
     }
-    const int key0 = t * kKeys;
+    const int key0 = t * KT;
     if (key0 < j.wave_end) {
-      step(s0, s1, v0, 0, key0, k0, 32);
-      step(s1, s0, v0, 32, key0 + 32, k1, 0);
+      if constexpr (KT == 64) {
+        step(s0, s1, v0, 0, key0, k0, 32);
+        step(s1, s0, v0, 32, key0 + 32, k1, 0);
+      } else {
+        step(s0, s1, v0, 0, key0, k1, 0);
+        s0 = s1;
+      }
     }
     uint8_t* k = k0;
     k0 = k1;
@@ -565,7 +571,7 @@ __global__ __launch_bounds__(kJoinLanes) void attn_join(Args p) {
 // dQ of 32 rows a wave; also D_i = dO_i.O_i, which attn_dkv reads beside lse
 template <int DP, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p, Jobs jobs) {
-  constexpr int P = pitch<DP>(), TILE = kKeys * P;
+  constexpr int P = pitch<DP>(), KT = tile_keys<NW>(), TILE = KT * P;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   RowJob j;
@@ -573,6 +579,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p, Jobs jobs) {
   const uint16_t* kb = origin(p, p.k, j.b, j.s.ks, j.kvh);
   const uint16_t* vb = origin(p, p.v, j.b, j.s.ks, j.kvh);
 
+  Tile<DP, NW, KT> kt, vt;
+  kt.init(p.k.row, p.D, lane, wv);
+  vt.init(p.v.row, p.D, lane, wv);
+  auto load = [&](uint8_t* to, int t) {
+    kt.load(to, kb + int64_t(t) * KT * p.k.row, j.s.kn - t * KT, wv);
+    vt.load(to + TILE, vb + int64_t(t) * KT * p.v.row, j.s.kn - t * KT, wv);
+  };
+  if (j.t0 < j.t1) load(lds, j.t0);
   bf16x8 q[DP / 16], dO[DP / 16];
   row_operands<DP>(q, origin(p, p.q, j.b, j.s.qs, 0), int64_t(j.pos) * p.q.row + int64_t(j.head) * p.q.head, j.ok, p.D, lane);
   row_operands<DP>(dO, origin(p, p.dout, j.b, j.s.qs, 0), int64_t(j.pos) * p.dout.row + int64_t(j.head) * p.dout.head, j.ok,
@@ -595,17 +609,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p, Jobs jobs) {
   }
   delta += swap_halves(delta);
   const float lse = j.ok ? p.lse[stat_index(p, j)] : INFINITY;
-  if (j.ok && lane < 32) *reinterpret_cast<f32x2*>(p.stats + 2 * stat_index(p, j)) = f32x2{-lse / p.c, -delta};
+  if (j.ok && lane < 32 && blockIdx.y == 0) *reinterpret_cast<f32x2*>(p.stats + 2 * stat_index(p, j)) = f32x2{-lse / p.c, -delta};
 
   f32x16 dq[DP / 32] = {};
-  Tile<DP, NW> kt, vt;
-  kt.init(p.k.row, p.D, lane, wv);
-  vt.init(p.v.row, p.D, lane, wv);
-  auto load = [&](uint8_t* to, int t) {
-    kt.load(to, kb + int64_t(t) * kKeys * p.k.row, j.s.kn - t * kKeys, wv);
-    vt.load(to + TILE, vb + int64_t(t) * kKeys * p.v.row, j.s.kn - t * kKeys, wv);
-  };
-  if (j.t0 < j.t1) load(lds, j.t0);
   dma_wait();
   __syncthreads();
   for (int t = j.t0; t < j.t1; ++t) {
@@ -613,12 +619,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p, Jobs jobs) {
     const uint8_t* V = K + TILE;
     uint8_t* next = lds + ((t - j.t0 + 1) & 1) * 2 * TILE;
     if (t + 1 < j.t1) load(next, t + 1);
-    const int key0 = t * kKeys;
+    const int key0 = t * KT;
     if (key0 < j.wave_end) {
-      const bool edge = key0 + kKeys > j.wave_full;
+      const bool edge = key0 + KT > j.wave_full;
       const int left = j.seen - key0 - 4 * (lane >> 5);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < KT / 32; ++b) {
         f32x16 s = {}, dp = {};
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) {
@@ -642,12 +648,41 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p, Jobs jobs) {
     dma_wait();
     __syncthreads();
   }
+  if (p.splits > 1) {   // a part, joined by attn_join_dq
+    float* to = p.part + (int64_t(blockIdx.y) * p.q_rows * p.H + int64_t(j.s.qs + j.pos) * p.H + j.head) * p.D;
+    if (j.ok)
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int c = 32 * d + 8 * u + 4 * (lane >> 5);
+          if (c < p.D) *reinterpret_cast<f32x4*>(to + c) = f32x4{dq[d][4 * u], dq[d][4 * u + 1], dq[d][4 * u + 2], dq[d][4 * u + 3]};
+        }
+    return;
+  }
   const int r0 = j.r - (lane & 31);
   store_rows<DP>(lds + wv * 32 * P, dq, p.scale, p.D, lane, [&](int r) -> uint16_t* {
     if (r0 + r >= j.rows) return nullptr;
     const int pos = div_g(p, r0 + r);
     return p.dq + (int64_t(j.s.qs + pos) * p.H + j.kvh * p.g + (r0 + r - pos * p.g)) * p.D;
   });
+}
+
+// dQ as the sum of its parts over the splits, in order: 8 values a thread, of the rows of a sequence
+__global__ __launch_bounds__(256) void attn_join_dq(Args p) {
+  const Seq s = sequence(p, blockIdx.y);
+  const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 8;
+  if (i >= int64_t(s.qn) * p.H * p.D) return;
+  const int64_t n = p.q_rows * p.H * p.D, at = int64_t(s.qs) * p.H * p.D + i;
+  f32x4 x = {}, y = {};
+#pragma unroll 4
+  for (int z = 0; z < p.splits; ++z) {
+    x += *reinterpret_cast<const f32x4*>(p.part + z * n + at);
+    y += *reinterpret_cast<const f32x4*>(p.part + z * n + at + 4);
+  }
+  x *= p.scale;
+  y *= p.scale;
+  *reinterpret_cast<u32x4*>(p.dq + at) = u32x4{pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3])};
 }
 
 // Row tiles of R rows (of one head) that see a key of the 128 of block kb: [first, first + n)
@@ -954,9 +989,9 @@ void magic(uint32_t g, uint32_t& m, int& s) {
   m = uint32_t(((uint64_t(1) << (31 + s)) + g - 1) / g);
 }
 
-constexpr int kLeast = 8;    // row tiles of a part at least
+constexpr int kLeast = 16;   // row tiles of a part at least, half as many of a part of the heads
 struct Plan {
-  int waves, splits;         // of a forward or dQ workgroup; forward: splits of the keys
+  int waves, splits, dq_splits;   // of a forward or dQ workgroup; splits of the keys
   int64_t groups;            // row tiles of all sequences and K/V heads
   int key_tiles;             // of the longest
   int64_t key_groups;        // dK and dV: workgroups
@@ -997,9 +1032,10 @@ void plan(const msd_attn& a, Plan& p) {
     p.waves = 1;
     p.groups = row_groups(1);
   }
-  // few rows: the keys are split too, into at least two tiles each
-  const int64_t key_tiles = std::max<int64_t>(cdiv(a.k_len, kKeys), 1);
-  p.splits = int(p.groups >= 2 * kCus ? 1 : std::max<int64_t>(1, std::min(cdiv(4 * kCus, std::max<int64_t>(p.groups, 1)), cdiv(key_tiles, 2))));
+  // few rows: the keys are split too, into at least 128 each (dQ, whose parts are the larger share of its work: 256)
+  const int64_t few = p.groups >= 2 * kCus ? 1 : cdiv(4 * kCus, std::max<int64_t>(p.groups, 1));
+  p.splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 128))));
+  p.dq_splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 256))));
   p.key_tiles = int(cdiv(a.k_len, 128));
   // dK and dV: parts of a key block until every CU has two workgroups, four where the mask makes them uneven: the heads of a
   // group first, whose parts are alike, then the rows, as long as a part's K, V and results are worth their traffic.
@@ -1016,8 +1052,9 @@ void plan(const msd_attn& a, Plan& p) {
     p.chunk = int(std::max<int64_t>(cdiv(all * a.n_heads / (a.causal ? 2 : 1), 2 * kCus), kLeast));
   } else {
     const int64_t want = cdiv((a.causal ? 4 : 2) * kCus, std::max<int64_t>(n * a.n_kv_heads * p.key_tiles, 1));
-    p.head_parts = int(std::min<int64_t>(want, g));
-    p.chunk = int(std::max<int64_t>(cdiv(most, cdiv(want, p.head_parts)), kLeast) * cdiv(g, p.head_parts));
+    p.head_parts = int(std::max<int64_t>(1, std::min(std::min(want, g), 2 * most * g / kLeast)));
+    const int64_t n_heads = cdiv(g, p.head_parts);
+    p.chunk = int(std::max<int64_t>(cdiv(most, cdiv(want, p.head_parts)) * n_heads, kLeast));
   }
   p.row_parts = int(std::max<int64_t>(1, cdiv(most * cdiv(g, p.head_parts), p.chunk)));
   p.blocks = count(p.sums, [&](Seq s) { return cdiv(s.kn, 128); });
@@ -1117,8 +1154,9 @@ extern "C" int64_t msd_attn_workspace_bytes(const msd_attn* a, int32_t backward)
   const int32_t rc = check(a, false, pl);
   if (rc != MSD_OK) return rc;
   if (!backward) return pl.splits > 1 ? 4 * pl.splits * a->q_rows * a->n_heads * (a->d_head + 1) : 0;
+  const int64_t dq = pl.dq_splits > 1 ? up(4 * pl.dq_splits * a->q_rows * a->n_heads * a->d_head) : 0;
   const int64_t n = pl.head_parts * pl.row_parts, parts = n > 1 ? 8 * n * a->k_rows * a->n_kv_heads * a->d_head : 0;
-  return up(8 * a->q_rows * a->n_heads) + parts;
+  return up(8 * a->q_rows * a->n_heads) + std::max(dq, parts);   // (one after the other)
 }
 
 extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void* k, const void* v, void* out, void* out_low,
@@ -1146,7 +1184,7 @@ extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void
   });
   if (pl.splits > 1) {
     const int64_t rows = int64_t(a->q_len) * a->n_heads;
-    if (pl.splits > 4) hipLaunchKernelGGL(attn_join<16>, dim3(unsigned(rows), a->n_seqs), dim3(kJoinLanes), 0, s, p);
+    if (pl.splits > 8) hipLaunchKernelGGL(attn_join<16>, dim3(unsigned(rows), a->n_seqs), dim3(kJoinLanes), 0, s, p);
     else hipLaunchKernelGGL(attn_join<4>, dim3(unsigned(cdiv(rows, 4)), a->n_seqs), dim3(kJoinLanes), 0, s, p);
   }
   return launched();
@@ -1178,10 +1216,13 @@ extern "C" int32_t msd_attn_backward(const msd_attn* a, const void* q, const voi
   with_head(a->d_head, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     if (pl.groups) {
-      p.splits = 1;
-      const dim3 grid(unsigned(pl.groups));
+      p.splits = pl.dq_splits;
+      const dim3 grid(unsigned(pl.groups), pl.dq_splits);
       if (pl.waves == 4) hipLaunchKernelGGL((attn_dq<DP, 4>), grid, dim3(256), 0, s, p, pl.rows);
       else hipLaunchKernelGGL((attn_dq<DP, 1>), grid, dim3(64), 0, s, p, pl.rows);
+      if (pl.dq_splits > 1)
+        hipLaunchKernelGGL(attn_join_dq, dim3(unsigned(cdiv(int64_t(a->q_len) * a->n_heads * a->d_head, 2048)), a->n_seqs), dim3(256),
+                           0, s, p);
     }
     if (pl.key_groups) {
       p.tile_rows = pl.tile_rows;
