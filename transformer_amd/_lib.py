@@ -218,15 +218,37 @@ def first_order(backward):
 TYPES = {torch.bfloat16: 0, torch.float32: 1}
 
 
+def row_stride(shape, stride):
+    """The stride between x's rows (its last axis) where one describes them all and a row is contiguous; else None."""
+    if stride[-1] != 1 and shape[-1] > 1:
+        return None
+    row = None
+    for n, s, inner in zip(reversed(shape[:-1]), reversed(stride[:-1]), _inner(shape)):
+        if n == 1:
+            continue
+        if row is None:
+            row = s if inner == 1 else None
+            if row is None:
+                return None
+        elif s != row * inner:
+            return None
+    return shape[-1] if row is None else row
+
+
+def _inner(shape):
+    """For the leading axes from the last: how many rows of the wider ones lie within a step of each."""
+    n = 1
+    for k in reversed(shape[:-1]):
+        yield n
+        n *= k
+
+
 def rows_of(x):
-    """(x as rows of contiguous values, the stride between them): a view wherever x's strides allow one."""
-    if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1])
-    row, col = x.stride()
-    if col != 1 and x.shape[1] > 1:
-        x = x.contiguous()
-        row = x.stride(0)
-    return x, row   # (one row's stride is not used)
+    """(x or a contiguous copy, the stride between its rows)."""
+    if x.is_contiguous():
+        return x, x.shape[-1]
+    row = row_stride(x.shape, x.stride())
+    return (x.contiguous(), x.shape[-1]) if row is None else (x, row)
 
 
 def keep_bytes(rows, d, checkpoint):

@@ -8,28 +8,57 @@ What runs (``msd_swiglu_forward`` / ``msd_swiglu_backward``, ``csrc/layers.hip``
 holding on to them: half the memory of bf16 for the widest activations of a layer; the gradients are then those at the
 values that the checkpoint stands for, off by up to 1/254 of a block's largest.
 """
+import math
+
 import torch
 
 from . import _lib
 
 
-def _forward(gate, up, checkpoint, keep):
-    g, g_stride = _lib.rows_of(gate)
-    u, u_stride = _lib.rows_of(up)
-    n, d = g.shape
+class _Plan:
+    """How calls on tensors of one layout go."""
+
+    def __init__(self, gate, up, checkpoint):
+        _check(gate, up, checkpoint)
+        self.rows, self.d, self.type, self.index = math.prod(gate.shape[:-1]), gate.shape[-1], _lib.TYPES[gate.dtype], gate.get_device()
+        strides = [_lib.row_stride(x.shape, x.stride()) for x in (gate, up)]
+        self.copies = None in strides
+        self.gate_stride, self.up_stride = (self.d, self.d) if self.copies else strides
+        self.held = 2 * _lib.keep_bytes(self.rows, self.d, checkpoint)
+
+
+_plans = {}
+
+
+def _plan(gate, up, checkpoint):
+    key = gate.shape, gate.stride(), gate.dtype, gate.device, up.shape, up.stride(), up.dtype, up.device, checkpoint
+    found = _plans.get(key)
+    if found is None:
+        found = _Plan(gate, up, checkpoint)
+        if len(_plans) >= 256:
+            _plans.clear()
+        _plans[key] = found
+    return found
+
+
+def _forward(gate, up, plan, keep):
+    if plan.copies:
+        gate, up = gate.contiguous(), up.contiguous()
     y = _lib.empty(gate)
-    held = g.new_empty(2 * _lib.keep_bytes(n, d, checkpoint), dtype=torch.uint8) if keep and checkpoint else None
-    _lib.launch(_lib.lib().msd_swiglu_forward, "msd_swiglu_forward", y.get_device(), g.data_ptr(), g_stride, u.data_ptr(),
-                u_stride, n, d, _lib.TYPES[y.dtype], y.data_ptr(), None if held is None else held.data_ptr())
-    return y, g, u, held, (g_stride, u_stride)
+    held = gate.new_empty(plan.held, dtype=torch.uint8) if keep and plan.held else None
+    _lib.launch(_lib.lib().msd_swiglu_forward, "msd_swiglu_forward", plan.index, gate.data_ptr(), plan.gate_stride,
+                up.data_ptr(), plan.up_stride, plan.rows, plan.d, plan.type, y.data_ptr(),
+                None if held is None else held.data_ptr())
+    return y, gate, up, held
 
 
 class _Swiglu(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, gate, up, checkpoint):
-        y, g, u, held, ctx.strides = _forward(gate, up, checkpoint, True)
+    def forward(ctx, gate, up, plan):
+        y, gate, up, held = _forward(gate, up, plan, True)
+        ctx.plan = plan
         if held is None:
-            ctx.save_for_backward(g, u)
+            ctx.save_for_backward(gate, up)
         else:
             ctx.save_for_backward(held)
         return y
@@ -37,14 +66,12 @@ class _Swiglu(torch.autograd.Function):
     @staticmethod
     @_lib.first_order
     def backward(ctx, dy):
-        saved = ctx.saved_tensors
-        rows, stride = _lib.rows_of(dy)
-        n, d = rows.shape
+        plan, saved = ctx.plan, ctx.saved_tensors
+        dy, stride = _lib.rows_of(dy)
         dgate, dup = _lib.empty(dy), _lib.empty(dy)
-        kept = len(saved) == 1
-        g, u, held = (None, None, saved[0].data_ptr()) if kept else (saved[0].data_ptr(), saved[1].data_ptr(), None)
-        _lib.launch(_lib.lib().msd_swiglu_backward, "msd_swiglu_backward", dy.get_device(), g, ctx.strides[0], u,
-                    ctx.strides[1], held, rows.data_ptr(), stride, n, d, _lib.TYPES[dy.dtype], dgate.data_ptr(),
+        gate, up, held = (saved[0].data_ptr(), saved[1].data_ptr(), None) if len(saved) == 2 else (None, None, saved[0].data_ptr())
+        _lib.launch(_lib.lib().msd_swiglu_backward, "msd_swiglu_backward", plan.index, gate, plan.gate_stride, up,
+                    plan.up_stride, held, dy.data_ptr(), stride, plan.rows, plan.d, plan.type, dgate.data_ptr(),
                     dup.data_ptr())
         return dgate, dup, None
 
@@ -64,7 +91,7 @@ def _check(gate, up, checkpoint):
 def swiglu(gate, up, checkpoint=None):
     """gate / (1 + exp(-gate)) * up: (..., d) bf16 or f32 on one GPU, any strides (halves of one projection, say); returns
     a contiguous tensor of their shape and type.  checkpoint: None, or "int8" (see the module)."""
-    _check(gate, up, checkpoint)
+    plan = _plan(gate, up, checkpoint)
     if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
-        return _Swiglu.apply(gate, up, checkpoint)
-    return _forward(gate, up, checkpoint, False)[0]
+        return _Swiglu.apply(gate, up, plan)
+    return _forward(gate, up, plan, False)[0]
