@@ -50,9 +50,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-// Keys of an LDS tile: 32 where a workgroup is one wave, so that its buffers leave room for enough others on a CU
-template <int NW>
-constexpr int tile_keys() { return NW == 1 ? 32 : 64; }
+constexpr int kWaves = 4;        // of a workgroup, 32 rows (or keys) each
+constexpr int kKeys = 64;        // keys of an LDS tile
 // Rows of an LDS tile of q and dout
 template <int DP>
 constexpr int tile_rows() { return DP <= 64 ? 64 : 32; }
@@ -221,10 +220,10 @@ __device__ __forceinline__ bf16x8 cols_operand(const uint8_t* tile, int row0, in
 #endif
 }
 
-// A tile of R rows on its way to LDS: wave w of NW fetches its instructions w, w + NW, ..
-template <int DP, int NW, int R>
+// A tile of R rows on its way to LDS: wave w fetches its instructions w, w + kWaves, ..
+template <int DP, int R>
 struct Tile {
-  static constexpr int P = pitch<DP>(), C = P / 16, N = R * P / 1024 / NW;
+  static constexpr int P = pitch<DP>(), C = P / 16, NW = kWaves, N = R * P / 1024 / NW;
   static_assert(64 * NW % C == 0, "an instruction's rows are a fixed number apart");
   int row;            // of the first instruction
   uint32_t off[N];
@@ -344,14 +343,14 @@ struct RowJob {
   int t0, t1;               // key tiles of this split
 };
 
-template <int NW>
 __device__ __forceinline__ bool row_job(const Args& p, const Jobs& jobs, RowJob& j, int lane, int wv) {
   j.kvh = blockIdx.x % p.KV;
   int local;
   j.b = job_sequence(p, jobs, blockIdx.x / p.KV, local, lane);
   j.s = sequence(p, j.b);
   j.rows = j.s.qn * p.g;
-  const int r0 = ((j.rows + 32 * NW - 1) / (32 * NW) - 1 - local) * 32 * NW;   // the longest key ranges first
+  constexpr int kRowsWg = 32 * kWaves;
+  const int r0 = ((j.rows + kRowsWg - 1) / kRowsWg - 1 - local) * kRowsWg;   // the longest key ranges first
   if (r0 < 0) return false;
   j.r = r0 + 32 * wv + (lane & 31);
   j.ok = j.r < j.rows;
@@ -359,11 +358,11 @@ __device__ __forceinline__ bool row_job(const Args& p, const Jobs& jobs, RowJob&
   j.head = j.kvh * p.g + (j.ok ? j.r - j.pos * p.g : 0);
   const int last = j.s.kn - j.s.qn + 1;   // keys that position 0 sees
   j.seen = p.causal ? min(max(last + j.pos, 0), j.s.kn) : j.s.kn;
-  const int w0 = min(r0 + 32 * wv, j.rows - 1), w1 = min(r0 + 32 * wv + 31, j.rows - 1), wg = min(r0 + 32 * NW, j.rows) - 1;
+  const int w0 = min(r0 + 32 * wv, j.rows - 1), w1 = min(r0 + 32 * wv + 31, j.rows - 1), wg = min(r0 + kRowsWg, j.rows) - 1;
   auto seen_by = [&](int r) { return p.causal ? min(max(last + div_g(p, r), 0), j.s.kn) : j.s.kn; };
   j.wave_full = seen_by(w0);
   j.wave_end = seen_by(w1);
-  const int n = (seen_by(wg) + tile_keys<NW>() - 1) / tile_keys<NW>();
+  const int n = (seen_by(wg) + kKeys - 1) / kKeys;
   const int per = n / p.splits, more = n % p.splits, y = blockIdx.y;
   j.t0 = per * y + min(y, more);
   j.t1 = j.t0 + per + (y < more);
@@ -378,20 +377,20 @@ __device__ __forceinline__ int64_t stat_index(const Args& p, const RowJob& j) {
 // ---- forward ----
 // Per 32 keys: the scores' maximum; the probabilities, while the matrix cores form the next 32 keys' scores; then their
 // product with V.  So the scores run 32 keys ahead, K one tile ahead of V: three K buffers and two of V, one barrier a tile.
-template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attn_fwd(Args p, Jobs jobs) {
-  constexpr int P = pitch<DP>(), KT = tile_keys<NW>(), TILE = KT * P;
+template <int DP>
+__global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void attn_fwd(Args p, Jobs jobs) {
+  constexpr int P = pitch<DP>(), TILE = kKeys * P;
   __shared__ __attribute__((aligned(16))) uint8_t lds[5 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   RowJob j;
-  if (!row_job<NW>(p, jobs, j, lane, wv)) return;
+  if (!row_job(p, jobs, j, lane, wv)) return;
   const uint16_t* kb = origin(p, p.k, j.b, j.s.ks, j.kvh);
   const uint16_t* vb = origin(p, p.v, j.b, j.s.ks, j.kvh);
-  Tile<DP, NW, KT> kt, vt;
+  Tile<DP, kKeys> kt, vt;
   kt.init(p.k.row, p.D, lane, wv);
   vt.init(p.v.row, p.D, lane, wv);
-  auto load_k = [&](uint8_t* to, int t) { kt.load(to, kb + int64_t(t) * KT * p.k.row, j.s.kn - t * KT, wv); };
-  auto load_v = [&](uint8_t* to, int t) { vt.load(to, vb + int64_t(t) * KT * p.v.row, j.s.kn - t * KT, wv); };
+  auto load_k = [&](uint8_t* to, int t) { kt.load(to, kb + int64_t(t) * kKeys * p.k.row, j.s.kn - t * kKeys, wv); };
+  auto load_v = [&](uint8_t* to, int t) { vt.load(to, vb + int64_t(t) * kKeys * p.v.row, j.s.kn - t * kKeys, wv); };
   uint8_t *k0 = lds, *k1 = lds + TILE, *k2 = lds + 2 * TILE, *v0 = lds + 3 * TILE, *v1 = lds + 4 * TILE;
   if (j.t0 < j.t1) {
     load_k(k0, j.t0);
@@ -455,15 +454,10 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : 2) void attn_fwd(Args p, Jo
       load_k(k2, t + 2);
       load_v(v1, t + 1);
     }
-    const int key0 = t * KT;
+    const int key0 = t * kKeys;
     if (key0 < j.wave_end) {
-      if constexpr (KT == 64) {
-        step(s0, s1, v0, 0, key0, k0, 32);
-        step(s1, s0, v0, 32, key0 + 32, k1, 0);
-      } else {
-        step(s0, s1, v0, 0, key0, k1, 0);
-        s0 = s1;
-      }
+      step(s0, s1, v0, 0, key0, k0, 32);
+      step(s1, s0, v0, 32, key0 + 32, k1, 0);
     }
     uint8_t* k = k0;
     k0 = k1;
@@ -569,22 +563,22 @@ __global__ __launch_bounds__(kJoinLanes) void attn_join(Args p) {
 
 // ---- backward ----
 // dQ of 32 rows a wave; also D_i = dO_i.O_i, which attn_dkv reads beside lse
-template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p, Jobs jobs) {
-  constexpr int P = pitch<DP>(), KT = tile_keys<NW>(), TILE = KT * P;
+template <int DP>
+__global__ __launch_bounds__(64 * kWaves, 2) void attn_dq(Args p, Jobs jobs) {
+  constexpr int P = pitch<DP>(), TILE = kKeys * P;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TILE];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   RowJob j;
-  if (!row_job<NW>(p, jobs, j, lane, wv)) return;
+  if (!row_job(p, jobs, j, lane, wv)) return;
   const uint16_t* kb = origin(p, p.k, j.b, j.s.ks, j.kvh);
   const uint16_t* vb = origin(p, p.v, j.b, j.s.ks, j.kvh);
 
-  Tile<DP, NW, KT> kt, vt;
+  Tile<DP, kKeys> kt, vt;
   kt.init(p.k.row, p.D, lane, wv);
   vt.init(p.v.row, p.D, lane, wv);
   auto load = [&](uint8_t* to, int t) {
-    kt.load(to, kb + int64_t(t) * KT * p.k.row, j.s.kn - t * KT, wv);
-    vt.load(to + TILE, vb + int64_t(t) * KT * p.v.row, j.s.kn - t * KT, wv);
+    kt.load(to, kb + int64_t(t) * kKeys * p.k.row, j.s.kn - t * kKeys, wv);
+    vt.load(to + TILE, vb + int64_t(t) * kKeys * p.v.row, j.s.kn - t * kKeys, wv);
   };
   if (j.t0 < j.t1) load(lds, j.t0);
   bf16x8 q[DP / 16], dO[DP / 16];
@@ -619,12 +613,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_dq(Args p, Jobs jobs) {
     const uint8_t* V = K + TILE;
     uint8_t* next = lds + ((t - j.t0 + 1) & 1) * 2 * TILE;
     if (t + 1 < j.t1) load(next, t + 1);
-    const int key0 = t * KT;
+    const int key0 = t * kKeys;
     if (key0 < j.wave_end) {
-      const bool edge = key0 + KT > j.wave_full;
+      const bool edge = key0 + kKeys > j.wave_full;
       const int left = j.seen - key0 - 4 * (lane >> 5);
 #pragma unroll
-      for (int b = 0; b < KT / 32; ++b) {
+      for (int b = 0; b < kKeys / 32; ++b) {
         f32x16 s = {}, dp = {};
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) {
@@ -757,11 +751,11 @@ struct RowStream {
 // dK and dV of 128 keys, 32 a wave.  Two workgroups a CU, so that one's first loads and last stores (8 us together) are
 // behind the other's products.
 template <int DP>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_dkv(Args p, Jobs jobs) {
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_dkv(Args p, Jobs jobs) {
   constexpr int P = pitch<DP>(), R = tile_rows<DP>(), TILE = R * P, STAGE = 2 * TILE + 8 * R, S = DP <= 64 ? 3 : 2, SUB = R / 32;
-  constexpr int DB = DP / 32, LOADS = 2 * TILE / 1024 / 4 + 1;   // of a wave and stage
+  constexpr int DB = DP / 32, LOADS = 2 * TILE / 1024 / kWaves + 1;   // of a wave and stage
   __shared__ __attribute__((aligned(16))) uint8_t lds[S * STAGE + 128 * P];
-  static_assert(sizeof(lds) <= 80 * 1024 && S * STAGE >= 4 * 32 * P, "two workgroups a CU; the results' staging");
+  static_assert(sizeof(lds) <= 80 * 1024 && S * STAGE >= kWaves * 32 * P, "two workgroups a CU; the results' staging");
   uint8_t* vs = lds + S * STAGE;   // the workgroup's V rows: in registers they would spill
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   // the first keys, which the most rows see, first
@@ -795,10 +789,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const bool ok = key < s.kn;
   bf16x8 k[DP / 16];
   row_operands<DP>(k, origin(p, p.k, b, s.ks, kvh), int64_t(key) * p.k.row, ok, p.D, lane);
-  Tile<DP, 4, 128> vt;
+  Tile<DP, 128> vt;
   vt.init(p.v.row, p.D, lane, wv);
   vt.load(vs, origin(p, p.v, b, s.ks, kvh) + int64_t(128 * kb) * p.v.row, s.kn - 128 * kb, wv);
-  Tile<DP, 4, R> qt, dt;
+  Tile<DP, R> qt, dt;
   qt.init(p.q.row, p.D, lane, wv);
   dt.init(p.dout.row, p.D, lane, wv);
   // the (-lse / c, -D) pairs of a tile's rows as two rows of R: 64 lanes fetch one of them, or both of 32
@@ -991,7 +985,7 @@ void magic(uint32_t g, uint32_t& m, int& s) {
 
 constexpr int kLeast = 16;   // row tiles of a part at least, half as many of a part of the heads
 struct Plan {
-  int waves, splits, dq_splits;   // of a forward or dQ workgroup; splits of the keys
+  int splits, dq_splits;     // of the keys, forward and for dQ
   int64_t groups;            // row tiles of all sequences and K/V heads
   int key_tiles;             // of the longest
   int64_t key_groups;        // dK and dV: workgroups
@@ -1023,15 +1017,7 @@ void plan(const msd_attn& a, Plan& p) {
     }
     return all;
   };
-  auto row_groups = [&](int waves) {
-    return count(p.rows, [&](Seq s) { return cdiv(s.qn * g, 32 * waves); }) * a.n_kv_heads;
-  };
-  p.waves = 4;
-  p.groups = row_groups(4);
-  if (p.groups < kCus) {   // 32-row workgroups fill more CUs
-    p.waves = 1;
-    p.groups = row_groups(1);
-  }
+  p.groups = count(p.rows, [&](Seq s) { return cdiv(s.qn * g, 32 * kWaves); }) * a.n_kv_heads;
   // few rows: the keys are split too, into at least 128 each (dQ, whose parts are the larger share of its work: 256)
   const int64_t few = p.groups >= 2 * kCus ? 1 : cdiv(4 * kCus, std::max<int64_t>(p.groups, 1));
   p.splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 128))));
@@ -1179,8 +1165,7 @@ extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void
   const dim3 grid(unsigned(pl.groups), pl.splits);
   with_head(a->d_head, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
-    if (pl.waves == 4) hipLaunchKernelGGL((attn_fwd<DP, 4>), grid, dim3(256), 0, s, p, pl.rows);
-    else hipLaunchKernelGGL((attn_fwd<DP, 1>), grid, dim3(64), 0, s, p, pl.rows);
+    hipLaunchKernelGGL((attn_fwd<DP>), grid, dim3(64 * kWaves), 0, s, p, pl.rows);
   });
   if (pl.splits > 1) {
     const int64_t rows = int64_t(a->q_len) * a->n_heads;
@@ -1218,8 +1203,7 @@ extern "C" int32_t msd_attn_backward(const msd_attn* a, const void* q, const voi
     if (pl.groups) {
       p.splits = pl.dq_splits;
       const dim3 grid(unsigned(pl.groups), pl.dq_splits);
-      if (pl.waves == 4) hipLaunchKernelGGL((attn_dq<DP, 4>), grid, dim3(256), 0, s, p, pl.rows);
-      else hipLaunchKernelGGL((attn_dq<DP, 1>), grid, dim3(64), 0, s, p, pl.rows);
+      hipLaunchKernelGGL((attn_dq<DP>), grid, dim3(64 * kWaves), 0, s, p, pl.rows);
       if (pl.dq_splits > 1)
         hipLaunchKernelGGL(attn_join_dq, dim3(unsigned(cdiv(int64_t(a->q_len) * a->n_heads * a->d_head, 2048)), a->n_seqs), dim3(256),
                            0, s, p);
@@ -1229,7 +1213,7 @@ extern "C" int32_t msd_attn_backward(const msd_attn* a, const void* q, const voi
       p.head_parts = pl.head_parts;
       p.row_parts = pl.row_parts;
       p.chunk = pl.chunk;
-      hipLaunchKernelGGL((attn_dkv<DP>), dim3(unsigned(pl.key_groups)), dim3(256), 0, s, p, pl.keys);
+      hipLaunchKernelGGL((attn_dkv<DP>), dim3(unsigned(pl.key_groups)), dim3(64 * kWaves), 0, s, p, pl.keys);
     }
   });
   if (pl.key_groups && pl.head_parts * pl.row_parts > 1) {
