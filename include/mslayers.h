@@ -41,7 +41,9 @@ extern "C" {
  *
  * Limits: d_head a multiple of 8 up to 128; n_heads a multiple of n_kv_heads, up to 4096; scale in [2^-60, 2^60]; q_rows and
  * k_rows below 2^30, q_rows * n_heads and k_rows * n_kv_heads below 2^31; 128 consecutive rows of one head and the heads of
- * one group together span less than 2^30 elements; n_seqs up to 65535. */
+ * one group together span less than 2^30 elements; q_len times the heads of a group below 2^30 - 256; n_seqs up to 65535,
+ * n_seqs * n_kv_heads below 2^20.  Beyond 256 sequences of different lengths the launch has the longest's workgroups for
+ * each, of which the others' are empty: they must stay below 2^24. */
 typedef struct msd_attn {
   int32_t n_seqs, q_len, k_len;
   int32_t n_heads, n_kv_heads, d_head;
@@ -87,8 +89,8 @@ typedef struct msd_rope {
 } msd_rope;
 
 /* turns: device f64 (d_rot / 2); the angle is formed in f64 and reduced to less than a turn before it is rounded.
- * k and k_out may be NULL with n_kv_heads 0.  batch * tokens * (n_heads + n_kv_heads) * d_head < 2^40, d_head <= 4096,
- * n_heads + n_kv_heads <= 4096. */
+ * k and k_out may be NULL with n_kv_heads 0.  batch * tokens * (n_heads + n_kv_heads) * d_head < 2^40, batch * tokens < 2^27,
+ * d_head <= 4096, n_heads + n_kv_heads <= 4096. */
 int32_t msd_rope_apply(const msd_rope* r, const void* q, const void* k, const void* positions, const double* turns,
                        void* q_out, void* k_out, void* stream);
 
@@ -101,7 +103,8 @@ int64_t msd_checkpoint_bytes(int64_t rows, int32_t d);
 /* y = s / sqrt(mean(s^2) + eps) * scale per row of d values, s = x + residual rounded to their type (x itself without a
  * residual).  x, residual: rows of d contiguous values, `*_stride` elements apart, of `type`; y and sum (= s; NULL
  * without a residual) contiguous, of the same type; scale (d) of scale_type.  rstd: f32 (rows), or NULL when no backward
- * follows; checkpoint: NULL, or msd_checkpoint_bytes(rows, d) for s * rstd in 8 bits.  1 <= d <= 16384, rows < 2^31. */
+ * follows; checkpoint: NULL, or msd_checkpoint_bytes(rows, d) for s * rstd in 8 bits.  1 <= d <= 16384;
+ * rows below 2^26, beyond 1024 values a row 2^24, beyond 4096 values 2^22. */
 int32_t msd_rms_forward(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                         const void* scale, int32_t scale_type, int64_t rows, int32_t d, int32_t type, float eps, void* y,
                         void* sum, float* rstd, void* checkpoint, void* stream);
@@ -118,7 +121,8 @@ int32_t msd_rms_backward(const void* s, int64_t s_stride, const float* rstd, con
                          int64_t rows, int32_t d, int32_t type, void* dx, void* dscale, void* workspace, void* stream);
 
 /* y = gate / (1 + exp(-gate)) * up, rows of d contiguous values `*_stride` elements apart, y contiguous.  checkpoint:
- * NULL, or 2 msd_checkpoint_bytes(rows, d): gate's, then up's.  d >= 1, rows * d < 2^40, d < 2^24. */
+ * NULL, or 2 msd_checkpoint_bytes(rows, d): gate's, then up's.  1 <= d < 2^24, rows times d rounded up to a multiple of 128
+ * below 2^36. */
 int32_t msd_swiglu_forward(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, int64_t rows,
                            int32_t d, int32_t type, void* y, void* checkpoint, void* stream);
 

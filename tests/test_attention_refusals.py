@@ -118,3 +118,24 @@ def test_workspaces():
     many = _args(n_seqs=64, q_len=2048, k_len=2048, q_rows=64 * 2048, k_rows=64 * 2048)   # enough workgroups: no parts
     assert L.msd_attn_workspace_bytes(ctypes.byref(many), 0) == 0
     assert L.msd_attn_workspace_bytes(ctypes.byref(many), 1) == 8 * 64 * 2048 * 4
+
+
+@pytest.mark.parametrize("lens", [
+    [(2 ** 25, 2 ** 25)],                         # 2^18 x 2^20 tiles of one sequence: counts beyond 32 bits
+    [(100000, 1), (1, 10000)],                    # the parts of one sequence's rows, the keys of another
+    [(2 ** 20, 0), (1, 2 ** 20)],
+    [(0, 2 ** 25), (0, 0)],
+])
+@pytest.mark.parametrize("causal", [0, 1])
+def test_workspace_of_uneven_sequences(lens, causal):
+    """The plan's counts hold for the longest sequences, and its parts stay worth their memory."""
+    rows, q, k = [], 0, 0
+    for n, m in lens:
+        rows += [q, n, k, m]
+        q, k = q + n, k + m
+    host = (ctypes.c_int32 * len(rows))(*rows)
+    a = _args(n_seqs=len(lens), q_len=max(n for n, _ in lens), k_len=max(m for _, m in lens), n_heads=32, n_kv_heads=8, d_head=128,
+              causal=causal, q_rows=q, k_rows=k, seqs=16, seqs_host=ctypes.addressof(host),
+              q_stride=(0, 4096, 128), dout_stride=(0, 4096, 128), k_stride=(0, 1024, 128), v_stride=(0, 1024, 128))
+    n = _lib.lib().msd_attn_workspace_bytes(ctypes.byref(a), 1)
+    assert 8 * q * 32 <= n <= 8 * q * 32 + 256 + max(2 ** 31, 16 * k * 8 * 128 * (k > 2 ** 20), 4 * 5 * q * 32 * 128 * (k > 256))

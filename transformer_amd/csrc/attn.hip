@@ -1035,7 +1035,10 @@ void plan(const msd_attn& a, Plan& p) {
       all += cdiv(s.qn, p.tile_rows) * cdiv(s.kn, 128);
     }
     p.head_parts = 1;
-    p.chunk = int(std::max<int64_t>(cdiv(all * a.n_heads / (a.causal ? 2 : 1), 2 * kCus), kLeast));
+    // (a sequence far longer than the others would have more parts than their keys' share of the workspace is worth)
+    const int64_t parts = std::max<int64_t>(32 * kCus / std::max<int64_t>(cdiv(a.k_rows, 128) * a.n_kv_heads, 1), 1);
+    const int64_t chunk = std::max(cdiv(all * a.n_heads / (a.causal ? 2 : 1), 2 * kCus), cdiv(most * g, parts));
+    p.chunk = int(std::max<int64_t>(std::min(chunk, most * g), kLeast));
   } else {
     const int64_t want = cdiv((a.causal ? 4 : 2) * kCus, std::max<int64_t>(n * a.n_kv_heads * p.key_tiles, 1));
     p.head_parts = int(std::max<int64_t>(1, std::min(std::min(want, g), 2 * most * g / kLeast)));
