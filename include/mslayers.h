@@ -122,7 +122,7 @@ int32_t msd_rms_backward(const void* s, int64_t s_stride, const float* rstd, con
 
 /* y = gate / (1 + exp(-gate)) * up, rows of d contiguous values `*_stride` elements apart, y contiguous.  checkpoint:
  * NULL, or 2 msd_checkpoint_bytes(rows, d): gate's, then up's.  1 <= d < 2^24, rows times d rounded up to a multiple of 128
- * below 2^36. */
+ * below 2^35. */
 int32_t msd_swiglu_forward(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, int64_t rows,
                            int32_t d, int32_t type, void* y, void* checkpoint, void* stream);
 

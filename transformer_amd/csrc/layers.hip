@@ -5,7 +5,8 @@
 //
 // All are bound by memory: each value is read once and written once per pass, in groups of eight values a lane (16 bytes
 // of bf16), at any element alignment (the hardware takes unaligned 16-byte accesses; a row's last, partial group goes value
-// by value), and everything between is f32.
+// by value), and everything between is f32.  The rate to compare with is a large copy's, 5.2 TB/s read and written; small calls
+// are bound by the launch (3 to 4 us a kernel).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -122,6 +123,8 @@ Checkpoint checkpoint(void* p, int64_t rows, int64_t d) {
   return {q, reinterpret_cast<float*>(q + rows * padded(d)), padded(d)};
 }
 
+// Half of bf16's bytes: what a training step holds between forward and backward.  Blocks of 128 values of a row, so that a large
+// value costs its neighbours' precision only; the scale and the quotients are f32.
 // Keeps eight values of a row (group `col` / 8 of it).  All 16 lanes of a block call together; lanes past the row hold
 // zeros.  The magnitudes are compared as integers, so a NaN is the largest and makes the block's scale one.
 __device__ __forceinline__ void keep8(const Checkpoint& c, int64_t row, int col, const float (&v)[8]) {
@@ -174,7 +177,9 @@ void with_type(int type, F f) {
 
 // ---- RMSNorm ----
 // A row is held by TPR lanes, V groups of eight values each: group tid + TPR u.  One wave a row up to 1024 values (no
-// barrier), 256 lanes up to 4096, 1024 up to 16384: at most 16 values of each operand in a lane's registers.
+// barrier), 256 lanes up to 4096, 1024 up to 16384: as few lanes as hold the row with 16 values of each operand in
+// their registers.  With four times the lanes and one group each: 9.9 and 12.7 us forward and backward in place of 8.7 and
+// 9.6 (4096 rows of 1024, bf16, residual), 145 and 167 us in place of 101 and 110 (16383 rows of 4096, 8-bit checkpoint).
 template <int TPR>
 __device__ __forceinline__ float row_sum(float x, float* lds, int tid) {
   x = sum64(x);
@@ -206,6 +211,8 @@ struct RmsArgs {
   Checkpoint c;
 };
 
+// y = s rstd scale, rstd = 1 / sqrt(mean(s^2) + eps).  101 us for 16383 x 4096 (x and residual read, y, the sum and the 8-bit
+// checkpoint written: 605 MB, 6.0 TB/s, part of it out of the last-level cache); 8.7 us for 4096 x 1024; 3.5 us for 8 rows.
 template <class T, int TPR, int V>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_fwd(RmsArgs p) {
   constexpr int NT = TPR > 256 ? TPR : 256;
@@ -249,8 +256,12 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_fwd(RmsArgs p) {
   }
 }
 
+// With n = s rstd: dx = rstd (dy scale - n mean(dy scale n)) + dsum, dscale = sum over the rows of dy n.
 // A workgroup of 1024 lanes takes rows 1024 / TPR at a time and keeps dscale's sums over its rows in registers; at the end
-// they are added over its row groups through LDS, in a fixed tree, and go to part[workgroup]
+// they are added over its row groups through LDS, in a fixed tree, and go to part[workgroup]: two workgroups a CU (256 parts:
+// the same time; 1024: 116 + 7.3 us in place of 110 + 4.9 with the sum of the parts).  110 us for 16383 x 4096 from the 8-bit
+// checkpoint (473 MB, 4.3 TB/s): the row's sum stands between its loads and its stores, and loading the next row
+// ahead costs the registers of half the waves (117 us).  9.6 us for 4096 x 1024.
 template <class T, int TPR, int V>
 __global__ __launch_bounds__(1024) void rms_bwd(RmsArgs p) {
   constexpr int G = 1024 / TPR;   // row groups
@@ -322,7 +333,8 @@ __global__ __launch_bounds__(1024) void rms_bwd(RmsArgs p) {
     }
 }
 
-// dscale from the workgroups' sums: 16 columns x 16 lanes a workgroup, each lane every 16th part, then the 16 in order
+// dscale from the workgroups' sums: 16 columns x 16 lanes a workgroup, each lane every 16th part, then the 16 in order.
+// 3.0 us for 1024 columns, 4.9 us for 512 parts of 4096.
 __global__ __launch_bounds__(256) void rms_dscale(RmsArgs p, int parts) {
   __shared__ float lds[16][17];
   const int c = threadIdx.x % 16, k = threadIdx.x / 16, col = blockIdx.x * 16 + c;
@@ -384,21 +396,27 @@ __device__ __forceinline__ Place place(const Div& groups, int64_t first, int i) 
   return {row0 + r, int(8 * (at - r * groups.n))};
 }
 
-constexpr int kUnroll = 2;
+// Groups of a lane: the forward takes one (two: 176 us in place of 165 for 16384 x 8192, 5.2 in place of 4.2 for 509 x 2816; the
+// same with checkpoints), the backward one (two: 254 us in place of 243, 6.2 in place of 5.1), but two from a checkpoint, whose
+// loads are of half the size (one: 243 us in place of 229).
+constexpr int backward_groups(bool kept) { return kept ? 2 : 1; }
 
+// y = g sigmoid(g) u.  16384 x 8192 in bf16: 165 us (805 MB, 4.9 TB/s), with the 8-bit checkpoint 206 to 258 us from card to
+// card (1.08 GB, 5.2 to 4.2 TB/s).
 template <class T, bool KEEP>
 __global__ __launch_bounds__(256) void swiglu_fwd(GluArgs p) {
-  float g[kUnroll][8], u[kUnroll][8];
-  Place at[kUnroll];
+  constexpr int U = 1;
+  float g[U][8], u[U][8];
+  Place at[U];
 #pragma unroll
-  for (int k = 0; k < kUnroll; ++k) {
-    at[k] = place(p.groups, int64_t(blockIdx.x) * 256 * kUnroll, threadIdx.x + 256 * k);
+  for (int k = 0; k < U; ++k) {
+    at[k] = place(p.groups, int64_t(blockIdx.x) * 256 * U, threadIdx.x + 256 * k);
     const int n = at[k].row < p.rows ? p.d - at[k].col : 0;
     load8(static_cast<const T*>(p.gate) + at[k].row * p.gate_stride + at[k].col, n, g[k]);
     load8(static_cast<const T*>(p.up) + at[k].row * p.up_stride + at[k].col, n, u[k]);
   }
 #pragma unroll
-  for (int k = 0; k < kUnroll; ++k) {
+  for (int k = 0; k < U; ++k) {
     if (at[k].row >= p.rows) continue;   // (whole blocks of 16 lanes: a row is whole blocks)
     if constexpr (KEEP) {
       keep8(p.cg, at[k].row, at[k].col, g[k]);
@@ -410,13 +428,16 @@ __global__ __launch_bounds__(256) void swiglu_fwd(GluArgs p) {
   }
 }
 
+// With sig = sigmoid(g): du = dy g sig, dg = dy u sig (1 + g (1 - sig)).  16384 x 8192 in bf16: 243 us (1.34 GB, 5.5 TB/s), from
+// the checkpoint 210 to 249 us (1.08 GB).
 template <class T, bool KEPT>
 __global__ __launch_bounds__(256) void swiglu_bwd(GluArgs p) {
-  float g[kUnroll][8], u[kUnroll][8], dy[kUnroll][8];
-  Place at[kUnroll];
+  constexpr int U = backward_groups(KEPT);
+  float g[U][8], u[U][8], dy[U][8];
+  Place at[U];
 #pragma unroll
-  for (int k = 0; k < kUnroll; ++k) {
-    at[k] = place(p.groups, int64_t(blockIdx.x) * 256 * kUnroll, threadIdx.x + 256 * k);
+  for (int k = 0; k < U; ++k) {
+    at[k] = place(p.groups, int64_t(blockIdx.x) * 256 * U, threadIdx.x + 256 * k);
     const int n = at[k].row < p.rows ? p.d - at[k].col : 0;
     if constexpr (KEPT) {
       if (n > 0) {
@@ -430,7 +451,7 @@ __global__ __launch_bounds__(256) void swiglu_bwd(GluArgs p) {
     load8(static_cast<const T*>(p.dy) + at[k].row * p.dy_stride + at[k].col, n, dy[k]);
   }
 #pragma unroll
-  for (int k = 0; k < kUnroll; ++k) {
+  for (int k = 0; k < U; ++k) {
     if (at[k].row >= p.rows) continue;
     const int n = p.d - at[k].col;
 #pragma unroll
@@ -448,10 +469,10 @@ __global__ __launch_bounds__(256) void swiglu_bwd(GluArgs p) {
 int32_t glu_check(int64_t rows, int d, int type) {
   if (rows < 0 || d < 1 || d >= (1 << 24) || rows >= (int64_t(1) << 40) / d || (type != MSD_BF16 && type != MSD_F32)) return MSD_E_CONFIG;
   // a launch has fewer than 2^32 threads
-  return cdiv(rows * (padded(d) / 8), 256 * kUnroll) >= (int64_t(1) << 24) ? MSD_E_CONFIG : MSD_OK;
+  return cdiv(rows * (padded(d) / 8), 256) >= (int64_t(1) << 24) ? MSD_E_CONFIG : MSD_OK;
 }
 
-unsigned glu_setup(GluArgs& p, int64_t rows, int d, const void* checkpoint_) {
+unsigned glu_setup(GluArgs& p, int64_t rows, int d, const void* checkpoint_, int lane_groups) {
   p.rows = rows;
   p.d = d;
   p.groups = divider(uint32_t(checkpoint_ ? padded(d) / 8 : cdiv(d, 8)));
@@ -460,13 +481,18 @@ unsigned glu_setup(GluArgs& p, int64_t rows, int d, const void* checkpoint_) {
     p.cg = checkpoint(c, rows, d);
     p.cu = checkpoint(c + checkpoint_bytes(rows, d), rows, d);
   }
-  return unsigned(cdiv(rows * p.groups.n, 256 * kUnroll));
+  return unsigned(cdiv(rows * p.groups.n, 256 * lane_groups));
 }
 
 // ---- rotary positions ----
-// A workgroup takes kTokens tokens: their cosines and sines once, to LDS, for all heads; then units of work, a unit being
-// W values of a head's copied part, W interleaved values, or W first and W second values of pairs.  A lane keeps one unit
-// of the token (its head and place) over the tokens, kDeep of them in flight.
+// (a, c) -> (a cos - c sin, a sin + c cos) amplitude; the gradient is the same turn backwards.  The angle p turns[i] is formed
+// in f64 and reduced to less than a turn before it is rounded, so that far positions keep their precision.
+// A workgroup takes kTokens tokens: their cosines and sines once, to LDS, for all heads (the f64 product and sincospif
+// once a token and pair, not once a head); then units of work, a unit being W values of a head's copied part, W interleaved
+// values, or W first and W second values of pairs.  A lane keeps one unit of the token (its head and place) over the
+// tokens, kDeep of them in flight.  32767 tokens of 32 + 8 heads of 128 in bf16: 135 us (671 MB, 5.0 TB/s); f32 274 us; 4096 tokens
+// of 16 + 4 heads of 64: 7.0 us.  With 4 or 16 tokens a workgroup 142 us (and 9.0 us for the small call, which then has too
+// few workgroups); with 1, 2 or 8 tokens in flight within 5 % of 4 either way, by layout.
 constexpr int kTokens = 8, kDeep = 4;
 
 struct RopeArgs {
@@ -654,16 +680,14 @@ extern "C" int32_t msd_rms_backward(const void* s, int64_t s_stride, const float
   p.part = dscale ? static_cast<float*>(workspace) : nullptr;
   const int parts = rms_parts(rows, d);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipError_t err = hipSuccess;
   if (rows)
     with_type(type, [&](auto t) {
       with_row(d, [&](auto lanes, auto v) {
         constexpr int TPR = decltype(lanes)::value, V = decltype(v)::value;
-        constexpr size_t lds = size_t(1024 / TPR / 2) * 8 * TPR * V * 4;   // at most 64 KB
+        constexpr size_t lds = size_t(1024 / TPR / 2) * 8 * TPR * V * 4;   // at most 32 KB
         hipLaunchKernelGGL((rms_bwd<decltype(t), TPR, V>), dim3(parts), dim3(1024), lds, st, p);
       });
     });
-  if (err != hipSuccess) return MSD_E_HIP;
   if (dscale) hipLaunchKernelGGL(rms_dscale, dim3(unsigned(cdiv(d, 16))), dim3(256), 0, st, p, rows ? parts : 0);
   return launched();
 }
@@ -676,7 +700,7 @@ extern "C" int32_t msd_swiglu_forward(const void* gate, int64_t gate_stride, con
   if (!rows) return MSD_OK;
   if (odd(gate, type) || odd(up, type) || odd(y, type) || reinterpret_cast<uintptr_t>(checkpoint_) % 16) return MSD_E_ARG;
   GluArgs p{};
-  const unsigned blocks = glu_setup(p, rows, d, checkpoint_);
+  const unsigned blocks = glu_setup(p, rows, d, checkpoint_, 1);
   p.gate = gate;
   p.gate_stride = gate_stride;
   p.up = up;
@@ -701,7 +725,7 @@ extern "C" int32_t msd_swiglu_backward(const void* gate, int64_t gate_stride, co
       reinterpret_cast<uintptr_t>(checkpoint_) % 16)
     return MSD_E_ARG;
   GluArgs p{};
-  const unsigned blocks = glu_setup(p, rows, d, checkpoint_);
+  const unsigned blocks = glu_setup(p, rows, d, checkpoint_, backward_groups(checkpoint_ != nullptr));
   p.gate = gate;
   p.gate_stride = gate_stride;
   p.up = up;
@@ -758,7 +782,8 @@ extern "C" int32_t msd_rope_apply(const msd_rope* r, const void* q, const void* 
   p.interleaved = r->interleaved != 0;
   p.amplitude = r->amplitude;
   p.sign = float(r->sign);
-  // eight values at a time where the turning and the copied part are whole groups of them
+  // eight values at a time where the turning and the copied part are whole groups of them (one at a time is there for
+  // other sizes: 302 us in place of 135 at 32767 tokens of 40 heads of 128)
   const int half = r->d_rot / 2;
   const bool wide = (r->d_head - r->d_rot) % 8 == 0 && (r->interleaved ? r->d_rot : half) % 8 == 0;
   const int w = wide ? 8 : 1;
