@@ -20,15 +20,32 @@
 // 32, over 4 h + {0..3} and 8 + 4 h + {0..3} of each 16: the other operand, which lies in LDS row by row, is read with
 // the transposing read ds_read_b64_tr_b16 in that same order, so the probabilities are never moved between lanes.
 //
-// LDS tiles.  64 rows of 128 bytes (d_head <= 64) or 256 bytes, in 16-byte pieces; row r holds piece c at position c ^
+// LDS tiles.  Rows of 128 bytes (d_head <= 64) or 256 bytes, in 16-byte pieces; row r holds piece c at position c ^
 // f(r), with f chosen (swizzle()) so that both the plain reads (32 rows, one piece each) and the transposing reads (4
-// rows, 64 bytes each) touch every bank once.  Two buffers: the next tile is loaded to registers while this one is
-// worked on.  Rows and columns that do not exist are zeros (buffer loads outside the descriptor), so what lies
-// behind a sequence's rows is never read.
+// rows, 64 bytes each) touch every bank once.  Tiles go from memory to LDS directly, the next one or two on their way while this
+// one is worked on, one barrier a tile (through registers, at the long case below as the kernels were then: 318 us in
+// place of 300 forward, 445 in place of 390 for dQ).  Rows and columns that do not exist are zeros (buffer loads outside the
+// descriptor), so what lies behind a sequence's rows is never read.
 //
 // The backward is two kernels: attn_dq (like the forward, rows outside, keys inside) and attn_dkv (keys outside, all
 // rows of the group inside).  Each recomputes S and dP: 7 products instead of the 5 of one kernel, which would have to
 // add dQ across workgroups with atomics, in no fixed order.
+//
+// A workgroup is four waves of 32 rows (or keys) at every size: with one wave of 32 rows for few of them one token against
+// a cache took 7.0 us in place of 6.3, 333 rows against 1021 keys 23 in place of 14, and many rows twice as long (the
+// tile's fetch serves a quarter of them).
+//
+// What bounds it: the matrix cores where there are many rows.  Measured, bf16, us and the rate of the products that the
+// mask leaves (a large library product reaches 1,262 TFLOP/s on this card):
+//   rows x keys, heads / kv, d, mask          forward        dQ             dK and dV, their parts' sum
+//   8192 x 8192, 16 / 4, 128, causal          318-352 (865)  403-440 (1020) 542-579 (1014), 24     clocks fall to 2.0 GHz
+//   4096 x 4096, 32 / 32, 64, none            180 (763)      221 (933)      273 (1007)
+//   23 documents in 8191, 16 / 4, 64, causal  37             44             62, 9
+//   8 x 512 x 512, 16 / 4, 64, causal         15.9           19.0           22.3, 7.3
+//   3 x 333 x 1021, 6 / 2, 96, none           13.8, 6.9 join 16.1, 5.3 join 20.0, 4.9
+//   4 x 1 x 2000, 16 / 4, 64                  6.3, 5.2 join
+// At d_head 64 the exponentials and the other vector work fill half of the issue slots beside the products (matrix cores
+// busy 56 % of attn_dkv's time, vector units 51 %).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -85,9 +102,11 @@ struct Seq {
   int qs, qn, ks, kn;
 };
 
-// Which sequence a workgroup works on.  Sequences of one shape: `each` jobs a sequence, a sequence's in a stride of `n_seqs`
+// Which sequence a workgroup works on.  Sequences of one shape: the same number of jobs each, a sequence's in a stride of `n_seqs`
 // (the jobs of all sequences with the most work come first).  Otherwise, for up to kMostSeqs of them, the first job of each,
-// as the host has counted them; beyond that the longest's number of jobs for each, of which the others' are empty.
+// as the host has counted them (it has their lengths; 1 KB of kernel arguments); beyond that the longest's number of jobs
+// for each, of which the others' are empty: at 23 documents of 16 to 2048 rows 60, 73 and 109 us for the three kernels in
+// place of 37, 44 and 62.
 constexpr int kMostSeqs = 256;
 struct Jobs {
   int counted;              // sequences in `first`, or 0
@@ -332,6 +351,8 @@ __device__ __forceinline__ int job_sequence(const Args& p, const Jobs& jobs, int
   return b;
 }
 
+// (P and dS are rounded to bf16 as operands of the next product, to nearest: what f32 sums of bf16 operands allow.)
+
 // What a workgroup of row tiles works on: 32 rows a wave, the keys in tiles
 struct RowJob {
   Seq s;
@@ -377,6 +398,7 @@ __device__ __forceinline__ int64_t stat_index(const Args& p, const RowJob& j) {
 // ---- forward ----
 // Per 32 keys: the scores' maximum; the probabilities, while the matrix cores form the next 32 keys' scores; then their
 // product with V.  So the scores run 32 keys ahead, K one tile ahead of V: three K buffers and two of V, one barrier a tile.
+// The running maximum may lag by 2^8 before the sums are rescaled: most tiles then need no pass over the output.
 template <int DP>
 __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void attn_fwd(Args p, Jobs jobs) {
   constexpr int P = pitch<DP>(), TILE = kKeys * P;
@@ -500,7 +522,9 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void attn_fwd(Args p
 }
 
 // A row from its parts over the splits, weighted by 2^(lse_z - lse).  16 lanes a row's 8-value pieces (as many as it has), G
-// of them in turn over the splits, joined through LDS in order; 16 / G rows a workgroup.
+// of them in turn over the splits, joined through LDS in order; 16 / G rows a workgroup.  A few rows are bound by latency, and
+// more lanes share a row's splits: 16 for more than 8 splits (32 rows of 64 splits, d_head 128: 8.9 us, with 4 lanes
+// 20), 4 for more than 4 (2400 x 16 rows: 15 us, with 16 lanes 43), else 1 (3200 x 16 rows of two splits: 13.8 us, with 4 lanes 20).
 constexpr int kJoinLanes = 256;
 template <int G>
 __global__ __launch_bounds__(kJoinLanes) void attn_join(Args p) {
@@ -562,7 +586,8 @@ __global__ __launch_bounds__(kJoinLanes) void attn_join(Args p) {
 }
 
 // ---- backward ----
-// dQ of 32 rows a wave; also D_i = dO_i.O_i, which attn_dkv reads beside lse
+// dQ of 32 rows a wave; also D_i = dO_i.O_i, which attn_dkv reads beside lse.  Two workgroups a CU; operands read ahead by
+// hand, as attn_dkv does, cost a wave's registers here and were slower.
 template <int DP>
 __global__ __launch_bounds__(64 * kWaves, 2) void attn_dq(Args p, Jobs jobs) {
   constexpr int P = pitch<DP>(), TILE = kKeys * P;
@@ -748,8 +773,10 @@ struct RowStream {
   }
 };
 
-// dK and dV of 128 keys, 32 a wave.  Two workgroups a CU, so that one's first loads and last stores (8 us together) are
-// behind the other's products.
+// dK and dV of 128 keys, 32 a wave, head by head over the rows that see them, from the last rows: workgroups of one K/V head
+// run on one XCD's L2 over the same rows (the group's heads row by row, each workgroup from its own first row: 1079 us in
+// place of 675 at the long case, as the kernel was then).  Two workgroups a CU, so that one's first loads and last stores (8 us together) are behind the other's products;
+// eight waves a workgroup, one a CU, expose them.
 template <int DP>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_dkv(Args p, Jobs jobs) {
   constexpr int P = pitch<DP>(), R = tile_rows<DP>(), TILE = R * P, STAGE = 2 * TILE + 8 * R, S = DP <= 64 ? 3 : 2, SUB = R / 32;
@@ -983,7 +1010,9 @@ void magic(uint32_t g, uint32_t& m, int& s) {
   m = uint32_t(((uint64_t(1) << (31 + s)) + g - 1) / g);
 }
 
-constexpr int kLeast = 16;   // row tiles of a part at least, half as many of a part of the heads
+// Row tiles of a part at least, half as many of a part of the heads: its K, V and results are traffic of two or three tiles.
+// With 8: 25.1 us and 6.6 for the sum in place of 22.9 and 4.4 (3 x 333 x 1021)
+constexpr int kLeast = 16;
 struct Plan {
   int splits, dq_splits;     // of the keys, forward and for dQ
   int64_t groups;            // row tiles of all sequences and K/V heads
@@ -1018,14 +1047,20 @@ void plan(const msd_attn& a, Plan& p) {
     return all;
   };
   p.groups = count(p.rows, [&](Seq s) { return cdiv(s.qn * g, 32 * kWaves); }) * a.n_kv_heads;
-  // few rows: the keys are split too, into at least 128 each (dQ, whose parts are the larger share of its work: 256)
-  const int64_t few = p.groups >= 2 * kCus ? 1 : cdiv(4 * kCus, std::max<int64_t>(p.groups, 1));
+  // few rows: the keys are split too, into at least 128 each (dQ, whose parts are the larger share of its work: 256), until
+  // every CU has two workgroups (four: 54 + 17 us for the join in place of 44 + 8, dQ 70 + 12 in place of 58 + 7 at 2 x 512 rows
+  // against 4096 keys, 16 / 4 heads of 128; row tiles for one a CU left whole: 38 us in place of 31 + 10, dQ 44 in place
+  // of 38 + 6 at 2400 rows, but 75 in place of 59 + 12, dQ 94 in place of 77 + 11 at 3200 of heads of 128).  Without: one token against 2000 keys 47 us in place of 6.3 and 5.2 for the join, 333 rows
+  // against 1021 keys 36 in place of 13.8 and 6.9, dQ 33 in place of 16 and 5.
+  const int64_t few = p.groups >= 2 * kCus ? 1 : cdiv(2 * kCus, std::max<int64_t>(p.groups, 1));
   p.splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 128))));
   p.dq_splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 256))));
   p.key_tiles = int(cdiv(a.k_len, 128));
   // dK and dV: parts of a key block until every CU has two workgroups, four where the mask makes them uneven: the heads of a
-  // group first, whose parts are alike, then the rows, as long as a part's K, V and results are worth their traffic.
-  // Sequences of different lengths: parts of as many tiles as make that many of them.
+  // group first, whose parts are alike, then the rows, as long as a part's K, V and results are worth their traffic (with two
+  // under the mask: 697 us in place of 578 at 8192 rows; the heads in two parts, not four: 27.2 + 5.0 us for the sum in place
+  // of 22.5 + 7.3 at 8 x 512).  Sequences of different lengths: parts of as many tiles as make two a CU (four: 62 + 13.7 us
+  // in place of 63 + 9).
   p.tile_rows = a.d_head <= 64 ? tile_rows<64>() : tile_rows<128>();
   const int64_t most = cdiv(a.q_len, p.tile_rows);
   if (counted) {
@@ -1172,8 +1207,13 @@ extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void
   });
   if (pl.splits > 1) {
     const int64_t rows = int64_t(a->q_len) * a->n_heads;
-    if (pl.splits > 8) hipLaunchKernelGGL(attn_join<16>, dim3(unsigned(rows), a->n_seqs), dim3(kJoinLanes), 0, s, p);
-    else hipLaunchKernelGGL(attn_join<4>, dim3(unsigned(cdiv(rows, 4)), a->n_seqs), dim3(kJoinLanes), 0, s, p);
+    auto join = [&](auto lanes) {
+      constexpr int G = decltype(lanes)::value;
+      hipLaunchKernelGGL(attn_join<G>, dim3(unsigned(cdiv(rows, 16 / G)), a->n_seqs), dim3(kJoinLanes), 0, s, p);
+    };
+    if (pl.splits > 8) join(std::integral_constant<int, 16>());
+    else if (pl.splits > 4) join(std::integral_constant<int, 4>());
+    else join(std::integral_constant<int, 1>());
   }
   return launched();
 }
