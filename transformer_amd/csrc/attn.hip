@@ -40,7 +40,7 @@
 //   rows x keys, heads / kv, d, mask          forward        dQ             dK and dV, their parts' sum
 //   8192 x 8192, 16 / 4, 128, causal          318-352 (865)  403-440 (1020) 542-579 (1014), 24     clocks fall to 2.0 GHz
 //   4096 x 4096, 32 / 32, 64, none            180 (763)      221 (933)      273 (1007)
-//   23 documents in 8191, 16 / 4, 64, causal  37             44             62, 9
+//   23 documents in 8191, 16 / 4, 64, causal  37             44             54, 7.5
 //   8 x 512 x 512, 16 / 4, 64, causal         15.9           19.0           22.3, 7.3
 //   3 x 333 x 1021, 6 / 2, 96, none           13.8, 6.9 join 16.1, 5.3 join 20.0, 4.9
 //   4 x 1 x 2000, 16 / 4, 64                  6.3, 5.2 join
@@ -106,7 +106,7 @@ struct Seq {
 // (the jobs of all sequences with the most work come first).  Otherwise, for up to kMostSeqs of them, the first job of each,
 // as the host has counted them (it has their lengths; 1 KB of kernel arguments); beyond that the longest's number of jobs
 // for each, of which the others' are empty: at 23 documents of 16 to 2048 rows 60, 73 and 109 us for the three kernels in
-// place of 37, 44 and 62.
+// place of 37, 44 and 62 (with the parts of that time).
 constexpr int kMostSeqs = 256;
 struct Jobs {
   int counted;              // sequences in `first`, or 0
@@ -775,8 +775,10 @@ struct RowStream {
 
 // dK and dV of 128 keys, 32 a wave, head by head over the rows that see them, from the last rows: workgroups of one K/V head
 // run on one XCD's L2 over the same rows (the group's heads row by row, each workgroup from its own first row: 1079 us in
-// place of 675 at the long case, as the kernel was then).  Two workgroups a CU, so that one's first loads and last stores (8 us together) are behind the other's products;
-// eight waves a workgroup, one a CU, expose them.
+// place of 675 at the long case, as the kernel was then).  Part by part, block by block, so that whole parts start before the
+// rests of blocks (block by block: 97 us in place of 74 at 2400 rows of heads of 128).  Two workgroups a CU, so that one's
+// first loads and last stores (8 us together) are behind the other's products; eight waves a workgroup, one a CU, expose
+// them.
 template <int DP>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_dkv(Args p, Jobs jobs) {
   constexpr int P = pitch<DP>(), R = tile_rows<DP>(), TILE = R * P, STAGE = 2 * TILE + 8 * R, S = DP <= 64 ? 3 : 2, SUB = R / 32;
@@ -790,11 +792,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
   if (jobs.counted) {   // part by part, block by block
     kvh = blockIdx.x % p.KV;
     b = job_sequence(p, jobs, blockIdx.x / p.KV, kb, lane);
-  } else {   // workgroups of the same rows are all = n_seqs * KV * parts apart: with 8 of them, or a multiple, on one XCD
-    const int all = p.n_seqs * p.KV * p.head_parts * p.row_parts, id = blockIdx.x % all, z = id / (p.n_seqs * p.KV);
-    kb = blockIdx.x / all;
-    zh = z / p.row_parts;
-    zr = z % p.row_parts;
+  } else {   // likewise; workgroups of the same rows are all = n_seqs * KV * head_parts apart: a multiple of 8 is one XCD
+    const int all = p.n_seqs * p.KV * p.head_parts, blocks = (p.k_len + 127) / 128, id = blockIdx.x % all;
+    kb = blockIdx.x / all % blocks;
+    zr = blockIdx.x / all / blocks;
+    zh = id / (p.n_seqs * p.KV);
     b = id / p.KV % p.n_seqs;
     kvh = id % p.KV;
   }
@@ -1013,6 +1015,10 @@ void magic(uint32_t g, uint32_t& m, int& s) {
 // Row tiles of a part at least, half as many of a part of the heads: its K, V and results are traffic of two or three tiles.
 // With 8: 25.1 us and 6.6 for the sum in place of 22.9 and 4.4 (3 x 333 x 1021)
 constexpr int kLeast = 16;
+// A part's row tiles, of what there is for each of two workgroups a CU.  With 1 all of them would start at once if they were
+// alike; larger ones are fewer first loads and sums.  With 1, 1.5 and 2, the sum included: 72, 61 and 72 us (23 documents in
+// 8191), 125, 103 and 117 (the same, heads of 128), 571, 571 and 662 (8192 rows), 128, 112 and 119 (3200 rows, heads of 128)
+constexpr double kShare = 1.5;
 struct Plan {
   int splits, dq_splits;     // of the keys, forward and for dQ
   int64_t groups;            // row tiles of all sequences and K/V heads
@@ -1056,31 +1062,29 @@ void plan(const msd_attn& a, Plan& p) {
   p.splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 128))));
   p.dq_splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 256))));
   p.key_tiles = int(cdiv(a.k_len, 128));
-  // dK and dV: parts of a key block until every CU has two workgroups, four where the mask makes them uneven: the heads of a
-  // group first, whose parts are alike, then the rows, as long as a part's K, V and results are worth their traffic (with two
-  // under the mask: 697 us in place of 578 at 8192 rows; the heads in two parts, not four: 27.2 + 5.0 us for the sum in place
-  // of 22.5 + 7.3 at 8 x 512).  Sequences of different lengths: parts of as many tiles as make two a CU (four: 62 + 13.7 us
-  // in place of 63 + 9).
+  // dK and dV: parts of a key block, as many as make kShare: the heads of a group first, whose parts are alike (four heads in
+  // two parts, not four: 27.2 + 5.0 us for the sum in place of 22.5 + 7.3 at 8 x 512), then the rows, as long as a part's K,
+  // V and results are worth their traffic.  Sequences of different lengths: their heads are one list.
   p.tile_rows = a.d_head <= 64 ? tile_rows<64>() : tile_rows<128>();
   const int64_t most = cdiv(a.q_len, p.tile_rows);
+  auto pairs = [&](Seq s) {   // rows x keys that the mask leaves, about
+    const double q = s.qn, k = s.kn;
+    return !a.causal ? q * k : q <= k ? q * (k - q / 2) : k * k / 2;
+  };
+  double all = 0;
   if (counted) {
-    int64_t all = 0;
-    for (int b = 0; b < n; ++b) {
-      const Seq s = host_seq(a, b);
-      all += cdiv(s.qn, p.tile_rows) * cdiv(s.kn, 128);
-    }
-    p.head_parts = 1;
-    // (a sequence far longer than the others would have more parts than their keys' share of the workspace is worth)
-    const int64_t parts = std::max<int64_t>(32 * kCus / std::max<int64_t>(cdiv(a.k_rows, 128) * a.n_kv_heads, 1), 1);
-    const int64_t chunk = std::max(cdiv(all * a.n_heads / (a.causal ? 2 : 1), 2 * kCus), cdiv(most * g, parts));
-    p.chunk = int(std::max<int64_t>(std::min(chunk, most * g), kLeast));
+    for (int b = 0; b < n; ++b) all += pairs(host_seq(a, b));
   } else {
-    const int64_t want = cdiv((a.causal ? 4 : 2) * kCus, std::max<int64_t>(n * a.n_kv_heads * p.key_tiles, 1));
-    p.head_parts = int(std::max<int64_t>(1, std::min(std::min(want, g), 2 * most * g / kLeast)));
-    const int64_t n_heads = cdiv(g, p.head_parts);
-    p.chunk = int(std::max<int64_t>(cdiv(most, cdiv(want, p.head_parts)) * n_heads, kLeast));
+    all = double(n) * pairs(Seq{0, a.q_len, 0, a.k_len});
   }
-  p.row_parts = int(std::max<int64_t>(1, cdiv(most * cdiv(g, p.head_parts), p.chunk)));
+  const double share = kShare * all * a.n_heads / (128.0 * p.tile_rows * 2 * kCus);
+  p.head_parts = counted ? 1 : int(std::min(double(g), std::max(1.0, ceil(double(most * g) / std::max(share, kLeast / 2.0)))));
+  while (g % p.head_parts) ++p.head_parts;   // (parts of the heads are alike)
+  const int64_t list = most * cdiv(g, p.head_parts);   // row tiles of a head part
+  // (a sequence far longer than the others would have more parts than their keys' share of the workspace is worth)
+  const int64_t parts = std::max<int64_t>(32 * kCus / std::max<int64_t>(cdiv(a.k_rows, 128) * a.n_kv_heads, 1), 1);
+  p.chunk = int(std::max<int64_t>({kLeast, cdiv(list, parts), std::min(list, int64_t(std::min(share, 1e9)) + 1)}));
+  p.row_parts = int(std::max<int64_t>(1, cdiv(list, p.chunk)));
   p.blocks = count(p.sums, [&](Seq s) { return cdiv(s.kn, 128); });
   if (counted)
     p.key_groups = a.n_kv_heads * count(p.keys, [&](Seq s) {
