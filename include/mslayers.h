@@ -34,7 +34,9 @@ extern "C" {
  * n_seqs * k_len.  seqs != NULL: a device array of n_seqs (q_start, q_len, k_start, k_len), rows of one flat tensor of
  * q_rows (k_rows) rows (the sequence strides are not used), 16-byte aligned, and seqs_host the same numbers on the host,
  * read during the call; q_len and k_len here are the longest.  The ranges must lie inside the rows and not overlap one
- * another; rows outside every range are neither read nor written.  The longest sequences first run fastest.
+ * another; rows outside every range are neither read nor written.  A device entry that leaves the rows or the longest
+ * lengths (it then differs from its host copy, which is checked) counts as an empty sequence.  The longest sequences first run
+ * fastest.
  *
  * causal: query i of a sequence sees keys 0 .. k_len - q_len + i (the last query sees the last key).  A query that
  * sees nothing has output 0 and contributes to no gradient.

@@ -356,3 +356,42 @@ def test_a_cache_past_32_bit_offsets():
     _check(_grads(q, k[:, :, sub], v[:, :, sub], do), ref, tol)
     turned = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (k, v)]   # (kv head, row) order
     _check(_grads(q, turned[0][:, :, sub], turned[1][:, :, sub], do), ref, tol)
+
+
+@pytest.mark.parametrize("tk", [129, 257, 512, 700, 1024, 1100])
+def test_joins_of_two_to_many_splits(tk):
+    """Few rows whose keys are split: 2 to 4, 5 to 8 and more splits are joined by different numbers of lanes."""
+    _dense(1, 3, tk, 4, 2, 64, True, seed=tk)
+    _dense(2, 130, tk, 2, 1, 72, False, seed=tk + 1)
+
+
+@pytest.mark.parametrize("T,H,KV,D,causal", [(2500, 1, 1, 128, True), (1800, 3, 1, 64, True), (1500, 2, 1, 96, False)])
+def test_key_blocks_in_several_parts(T, H, KV, D, causal):
+    """Few heads over long sequences: the rows that see a key block are shared out to parts."""
+    _dense(1, T, T, H, KV, D, causal, seed=T)
+
+
+def test_captured_sequences_and_an_overwritten_table():
+    """Packed rows in a graph over a table made before; a table whose entries have come to leave the rows reads as empty
+    sequences, whose rows stay as they were."""
+    lens = [300, 40, 0, 129]
+    n = sum(lens)
+    x = [_rand((n + 5, h, 64), i) for i, h in enumerate((4, 2, 2, 4))]
+    seqs = Sequences(lens)
+    want = _grads(*x, sequences=seqs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _grads(*x, sequences=seqs)
+    for _ in range(3):
+        graph.replay()
+        again = _grads(*x, sequences=seqs)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, out, again))
+    assert seqs.table[:, 1].tolist() == [300, 129, 40, 0]
+    seqs.table[0, 0], seqs.table[1, 3], seqs.table[2, 1] = -7, 2 ** 30, n + 1   # start, keys, rows
+    got = _grads(*x, sequences=Sequences([], device="cuda"))
+    assert all(not g.any() for g in got)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.isfinite(a).all() for a in out)
+    assert all(not a[n:].any() for a in out)

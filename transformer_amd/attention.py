@@ -7,8 +7,9 @@ The reference's causal_attention (model.py:122-147) between its projections: q (
 
 What runs (``msd_attn_forward`` / ``msd_attn_backward``, ``csrc/attn.hip``): one pass over the keys with the running
 maximum and sum of the softmax, so no score matrix is stored; the forward keeps each row's logsumexp, from which the
-backward forms the probabilities again, and a byte beside each value of the output for what its rounding took off.  Scores, softmax statistics and every sum are f32; the probabilities and the
-scores' gradients are rounded to bf16 as operands of the matrix cores, the results once to bf16.  Deterministic.
+backward forms the probabilities again, and a byte beside each value of the output for what its rounding took off.
+Scores, softmax statistics and every sum are f32; the probabilities and the scores' gradients are rounded to bf16 as
+operands of the matrix cores, the results once to bf16.  Deterministic.
 """
 import ctypes
 import math
@@ -25,7 +26,8 @@ class Sequences:
     starts default to the sequences packed one behind the other, the keys to the queries' (self-attention).  A padded
     batch is its flat view with ``q_starts=range(0, B * T, T)`` and each sequence's own length.  Rows of no sequence are
     neither read nor attended to; their outputs and gradients are zeros.  Built once per batch from host integers
-    (checked here) and used by every layer; the device copy is made on the current stream."""
+    (checked here) and used by every layer; the device copy is made on the current stream.  A captured graph goes on
+    reading that copy: like the graph's other inputs the object has to be kept, and made before the capture."""
 
     def __init__(self, q_lens, k_lens=None, q_starts=None, k_starts=None, device="cuda"):
         q_lens = [int(n) for n in q_lens]

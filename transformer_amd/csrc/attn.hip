@@ -115,9 +115,13 @@ struct Jobs {
 
 __device__ __forceinline__ Seq sequence(const Args& p, int b) {
   if (!p.seqs) return {b * p.q_len, p.q_len, b * p.k_len, p.k_len};
-  const int4 s = reinterpret_cast<const int4*>(p.seqs)[b];
-  return {__builtin_amdgcn_readfirstlane(s.x), __builtin_amdgcn_readfirstlane(s.y), __builtin_amdgcn_readfirstlane(s.z),
-          __builtin_amdgcn_readfirstlane(s.w)};
+  const int4 x = reinterpret_cast<const int4*>(p.seqs)[b];
+  const Seq s = {__builtin_amdgcn_readfirstlane(x.x), __builtin_amdgcn_readfirstlane(x.y), __builtin_amdgcn_readfirstlane(x.z),
+                 __builtin_amdgcn_readfirstlane(x.w)};
+  // (the host has checked its own numbers; a device table that has been overwritten since must not lead out of the rows)
+  const bool ok = s.qs >= 0 && s.qn >= 0 && s.ks >= 0 && s.kn >= 0 && s.qn <= p.q_len && s.kn <= p.k_len &&
+                  s.qs <= p.q_rows - s.qn && s.ks <= p.k_rows - s.kn;
+  return ok ? s : Seq{0, 0, 0, 0};
 }
 
 // The first element of row 0, head `head` of sequence b, whose rows start at `start`.
