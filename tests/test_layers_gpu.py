@@ -12,6 +12,7 @@ import math
 import pytest
 import torch
 
+from transformer_amd.attention import attention
 from transformer_amd.norm import rms_norm
 from transformer_amd.rotary import RotaryFrequencies, rotary, rotary_frequencies
 from transformer_amd.swiglu import swiglu
@@ -239,10 +240,12 @@ def test_the_checkpoint_lets_go_of_the_activations():
     for keep in (None, "int8"):
         g, u, r = (_rand((256, 4096), i).requires_grad_() for i in range(3))
         w = _rand((4096,), 4).requires_grad_()
-        y = swiglu(g * 1, u * 1, checkpoint=keep)
-        n, _ = rms_norm(r * 1, w, r * 1, checkpoint=keep)
+        g, u, r, saved = g * 1, u * 1, r * 1, []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: saved.append(t) or t, lambda t: t):
+            y = swiglu(g, u, checkpoint=keep)
+            n, _ = rms_norm(r, w, r, checkpoint=keep)
         # (summed here: the allocator's own figure counts the whole of a block whose rest is too small to split off)
-        held.append(sum(t.nbytes for x in (y, n) for t in x.grad_fn.saved_tensors))
+        held.append(sum(t.nbytes for t in saved))
     saved = 256 * 4096 * (2 - 1 - 4 / 128) * 3
     assert abs(held[0] - held[1] - saved) < 1e5, held
 
@@ -482,3 +485,41 @@ def test_frequencies_object():
     f = rotary_frequencies(64)
     q = _rand((3, 2, 64), 1)
     assert torch.equal(rotary(q, None, f), rotary(q, None, RotaryFrequencies(f.turns)))
+
+
+def _strided_calls():
+    """(operator, its strided leaves): each reads them where they lie."""
+    freq = rotary_frequencies(64)
+    both, wide = _rand((40, 512), 1), _rand((6, 50, 8, 64), 2)
+    q, k, v = wide[:, :, :4], wide[:, :, 4:6], wide[:, :, 6:]
+    return [
+        (lambda g, u: swiglu(g, u), (both[:, :256], both[:, 256:])),
+        (lambda x, w: rms_norm(x, w), (both[:, :200], _rand((200,), 3))),
+        (lambda x, w, r: sum(rms_norm(x, w, r, checkpoint="int8")), (both[:, :200], _rand((200,), 3), both[:, 300:500])),
+        (lambda q, k, v: attention(q, k, v), (q, k, v)),
+        (lambda q, k: sum(t.sum(2) for t in rotary(q, k, freq)), (q, k)),
+    ]
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_saved_tensors_that_hooks_move(which):
+    """What is saved may come back with other strides (here by way of host memory): the same gradients."""
+    f, leaves = _strided_calls()[which]
+    leaves = [x.detach().requires_grad_() for x in leaves]
+    want = torch.autograd.grad(f(*leaves).float().sin().sum(), leaves)
+    with torch.autograd.graph.save_on_cpu():
+        y = f(*leaves)
+    got = torch.autograd.grad(y.float().sin().sum(), leaves)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_second_derivatives_are_refused(which):
+    """Gradients may be recorded, and give the same values; differentiating them raises."""
+    f, leaves = _strided_calls()[which]
+    leaves = [x.detach().requires_grad_() for x in leaves]
+    want = torch.autograd.grad(f(*leaves).float().sin().sum(), leaves)
+    got = torch.autograd.grad(f(*leaves).float().sin().sum(), leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        sum(x.float().sum() for x in got).backward()

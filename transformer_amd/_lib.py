@@ -8,10 +8,10 @@ import ctypes
 import os
 
 import torch  # noqa: F401  (load torch's HIP runtime before the library)
-from torch.autograd.function import once_differentiable
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmsdecode.so")
+OPS_PATH = os.path.join(HERE, "_ops.so")
 
 MSD_OK = 0
 MSD_E_CONFIG = -1
@@ -178,77 +178,28 @@ def lib():
     return L
 
 
-# The raw handle of the current stream and the current device, without the objects around them: an operator's backward runs in
-# the autograd engine's thread, where every such call costs several times what it does elsewhere
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-
-
-def launch(fn, what, index, *args):
-    """fn(*args, stream) on the current torch stream of GPU ``index``, with that GPU current; raises for its error code."""
-    if _device() == index:
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
-    if rc < 0:
-        raise MsdError(rc, what)
-
-
 def current_stream(x):
     """The handle of the current stream of x's GPU; None for a tensor in host memory."""
-    return _raw_stream(x.get_device()) if x.is_cuda else None
+    return torch.cuda.current_stream(x.device).cuda_stream if x.is_cuda else None
 
 
-def empty(x):
-    """A contiguous tensor of x's shape, type and device."""
-    return torch.empty_like(x, memory_format=torch.contiguous_format)
+_ops = None
 
 
-def first_order(backward):
-    """once_differentiable, without its cost where no second derivative is asked for (gradients are not recorded then)."""
-    slow = once_differentiable(backward)
-
-    def f(ctx, *grads):
-        return slow(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return f
+def ops():
+    """The torch calls of the training-layer operators (csrc/torch_ops.cpp), over the library."""
+    global _ops
+    if _ops is None:
+        lib()
+        if not os.path.exists(OPS_PATH):
+            raise RuntimeError(f"{OPS_PATH} not built: run python -m transformer_amd.build (or __graft_entry__.build())")
+        from . import _ops as loaded
+        _ops = loaded
+    return _ops
 
 
 # Value types of the layer operators (include/mslayers.h)
 TYPES = {torch.bfloat16: 0, torch.float32: 1}
-
-
-def row_stride(shape, stride):
-    """The stride between x's rows (its last axis) where one describes them all and a row is contiguous; else None."""
-    if stride[-1] != 1 and shape[-1] > 1:
-        return None
-    row = None
-    for n, s, inner in zip(reversed(shape[:-1]), reversed(stride[:-1]), _inner(shape)):
-        if n == 1:
-            continue
-        if row is None:
-            row = s if inner == 1 else None
-            if row is None:
-                return None
-        elif s != row * inner:
-            return None
-    return shape[-1] if row is None else row
-
-
-def _inner(shape):
-    """For the leading axes from the last: how many rows of the wider ones lie within a step of each."""
-    n = 1
-    for k in reversed(shape[:-1]):
-        yield n
-        n *= k
-
-
-def rows_of(x):
-    """(x or a contiguous copy, the stride between its rows)."""
-    if x.is_contiguous():
-        return x, x.shape[-1]
-    row = row_stride(x.shape, x.stride())
-    return (x.contiguous(), x.shape[-1]) if row is None else (x, row)
 
 
 def keep_bytes(rows, d, checkpoint):

@@ -43,13 +43,8 @@ class Sequences:
         rows = sorted(zip(q_starts, q_lens, k_starts, k_lens), key=lambda r: -r[1] * r[3])   # the most work first
         self.host = torch.tensor(rows, dtype=torch.int32).reshape(-1, 4)
         self.table = self.host.to(device)
-        self._stream = _lib.current_stream(self.table)
+        self.stream = _lib.current_stream(self.table)
         self._plans = {}
-
-    def used(self):
-        """Keeps the table's memory until what has been launched on the current stream is done with it."""
-        if _lib.current_stream(self.table) != self._stream:
-            self.table.record_stream(torch.cuda.current_stream(self.table.device))
 
 
 def _ranges(lens, starts, what):
@@ -81,57 +76,38 @@ def _fits(shape, stride):
             and 128 * row + shape[-2] * head < 2 ** 30)
 
 
-def _operand(x, fits):
-    """x as the kernels' loads take it, copied only where it has to be."""
-    if not fits:
-        x = x.contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
-
-
 def _strides(shape, stride):
     """(sequence, row, head) strides; 0 along an axis of one (or none)."""
     s = tuple(0 if n <= 1 else k for n, k in zip(shape[:-1], stride))
     return s if len(s) == 3 else (0, *s)
 
 
-def _contiguous(shape):
-    return tuple(math.prod(shape[i + 1:]) for i in range(len(shape)))
-
-
 class _Plan:
-    """How calls on operands of one layout go: the library's arguments and workspaces, for a contiguous gradient, and which
-    operands are copied first.  ``rest`` is what the output's rows lack of the sequences'."""
+    """How calls on operands of one layout go.  ``fits``: which operands can be read where they lie; ``native``: the library's
+    arguments and workspaces, where all can."""
 
     def __init__(self, q, k, v, causal, scale, sequences):
         _check(q, k, v, scale, sequences)
-        self.scale, self.causal, self.sequences = scale, causal, sequences
-        self.q_shape, self.k_shape = q.shape, k.shape
         self.fits = tuple(_fits(x.shape, x.stride()) for x in (q, k, v))
-        self.strides = tuple(_strides(x.shape, x.stride() if f else _contiguous(x.shape)) for x, f in zip((q, k, v), self.fits))
-        self.index = q.get_device()
-        self.q_zero = sequences is not None and sequences.q_count != q.shape[0]
-        self.k_zero = sequences is not None and sequences.k_count != k.shape[0]
-        self.arguments, self.forward_bytes, self.backward_bytes = self.call(_strides(q.shape, _contiguous(q.shape)))
+        self.native = self._native(q, k, v, causal, scale, sequences) if all(self.fits) else None
 
-    def call(self, dout_stride, moved=(False, False, False)):
-        """(arguments, bytes of the forward's and of the backward's workspace) with these strides of dout; ``moved``: which
-        operands were copied for their place in memory."""
-        sequences, (*_, H, D) = self.sequences, self.q_shape
+    @staticmethod
+    def _native(q, k, v, causal, scale, sequences):
         a = _lib.MsdAttn()
         if sequences is None:
-            a.n_seqs = self.q_shape[0] if len(self.q_shape) == 4 else 1
-            a.q_len, a.k_len = self.q_shape[-3], self.k_shape[-3]
+            a.n_seqs, a.q_len, a.k_len = q.shape[0] if q.dim() == 4 else 1, q.shape[-3], k.shape[-3]
         else:
             a.n_seqs, a.q_len, a.k_len = sequences.n, sequences.q_longest, sequences.k_longest
             a.seqs, a.seqs_host = sequences.table.data_ptr() or 16, sequences.host.data_ptr() or 16   # (16: nothing to read)
-        a.q_rows, a.k_rows = math.prod(self.q_shape[:-2]), math.prod(self.k_shape[:-2])
-        a.n_heads, a.n_kv_heads, a.d_head, a.causal, a.scale = H, self.k_shape[-2], D, self.causal, self.scale
-        shapes = (self.q_shape, self.k_shape, self.k_shape)
-        strides = [_strides(n, _contiguous(n)) if m else s for n, s, m in zip(shapes, self.strides, moved)]
-        for name, s in zip(("q_stride", "k_stride", "v_stride", "dout_stride"), (*strides, dout_stride)):
-            getattr(a, name)[:] = s
+        a.q_rows, a.k_rows = math.prod(q.shape[:-2]), math.prod(k.shape[:-2])
+        a.n_heads, a.n_kv_heads, a.d_head, a.causal, a.scale = q.shape[-2], k.shape[-2], q.shape[-1], causal, scale
+        for name, x in (("q_stride", q), ("k_stride", k), ("v_stride", v)):
+            getattr(a, name)[:] = _strides(x.shape, x.stride())
         sizes = [_lib.check(_lib.lib().msd_attn_workspace_bytes(ctypes.byref(a), i), "msd_attn_workspace_bytes") for i in (0, 1)]
-        return ctypes.byref(a), *sizes
+        if sequences is None:
+            return _lib.ops().AttnPlan(ctypes.addressof(a), *sizes, False, False, None, None, 0)
+        return _lib.ops().AttnPlan(ctypes.addressof(a), *sizes, sequences.q_count != q.shape[0], sequences.k_count != k.shape[0],
+                                   sequences.table, sequences.host, sequences.stream or 0)
 
 
 _plans = {}   # of calls without sequences; a Sequences keeps its own (the layers of a step make the same call)
@@ -177,65 +153,6 @@ def _check(q, k, v, scale, sequences):
             raise ValueError(f"sequences were made for {sequences.table.device}, q is on {q.device}")
 
 
-def _empty(like, zero):
-    """A contiguous output of like's shape; of zeros where the sequences leave rows out."""
-    x = _lib.empty(like)
-    return x.zero_() if zero else x
-
-
-def _forward(q, k, v, plan, keep):
-    at = q.data_ptr() | k.data_ptr() | v.data_ptr()
-    call = plan.arguments, plan.forward_bytes, plan.backward_bytes
-    if at % 16 or plan.fits != (True, True, True):
-        operands = [_operand(x, f) for x, f in zip((q, k, v), plan.fits)]
-        moved = tuple(f and x.data_ptr() % 16 != 0 for x, f in zip((q, k, v), plan.fits))
-        q, k, v = operands
-        if any(moved):
-            call = plan.call(_strides(q.shape, _contiguous(q.shape)), moved)
-    out = _empty(q, plan.q_zero)
-    lse = low = None
-    if keep:
-        lse, low = out.new_empty(out.shape[:-1], dtype=torch.float32), torch.empty_like(out, dtype=torch.uint8)
-    a, n, _ = call
-    ws = q.new_empty(n, dtype=torch.uint8) if n else None
-    if plan.sequences is not None:
-        plan.sequences.used()
-    _lib.launch(_lib.lib().msd_attn_forward, "msd_attn_forward", plan.index, a, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                out.data_ptr(), low.data_ptr() if keep else None, lse.data_ptr() if keep else None,
-                ws.data_ptr() if n else None)
-    return q, k, v, out, low, lse, call
-
-
-class _Attention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, plan):
-        at = q.data_ptr(), k.data_ptr(), v.data_ptr()
-        q, k, v, out, low, lse, ctx.call = _forward(q, k, v, plan, True)
-        ctx.save_for_backward(q, k, v, out, low, lse)
-        ctx.plan = plan
-        ctx.moved = tuple(f and a % 16 != 0 for a, f in zip(at, plan.fits))
-        return out
-
-    @staticmethod
-    @_lib.first_order
-    def backward(ctx, dout):
-        q, k, v, out, low, lse = ctx.saved_tensors
-        plan = ctx.plan
-        a, _, n = ctx.call
-        if not dout.is_contiguous() or dout.data_ptr() % 16:
-            dout = _operand(dout, _fits(dout.shape, dout.stride()))
-            a, _, n = plan.call(_strides(dout.shape, dout.stride()), ctx.moved)
-        dq = _empty(q, plan.q_zero)
-        dk, dv = _empty(k, plan.k_zero), _empty(v, plan.k_zero)
-        ws = q.new_empty(n, dtype=torch.uint8) if n else None
-        if plan.sequences is not None:
-            plan.sequences.used()
-        _lib.launch(_lib.lib().msd_attn_backward, "msd_attn_backward", plan.index, a, q.data_ptr(), k.data_ptr(),
-                    v.data_ptr(), out.data_ptr(), low.data_ptr(), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-                    dv.data_ptr(), ws.data_ptr() if n else None)
-        return dq, dk, dv, None
-
-
 def attention(q, k, v, causal=True, scale=None, sequences=None):
     """softmax(scale q k^T) v for every head, q head h with k/v head h // (n_heads // n_kv_heads).
 
@@ -248,6 +165,8 @@ def attention(q, k, v, causal=True, scale=None, sequences=None):
     reaches every query that sees it, and may reach those that do not."""
     scale = q.shape[-1] ** -0.5 if scale is None and q.dim() and q.shape[-1] else float(scale or 0)
     plan = _plan(q, k, v, bool(causal), scale, sequences)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _Attention.apply(q, k, v, plan)
-    return _forward(q, k, v, plan, False)[3]
+    if plan.native is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        q, k, v = (x if f and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
+                   for x, f in zip((q, k, v), plan.fits))
+        plan = _plan(q, k, v, bool(causal), scale, sequences)
+    return _lib.ops().attention(q, k, v, plan.native)

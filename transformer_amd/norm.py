@@ -17,19 +17,19 @@ from . import _lib
 
 
 class _Plan:
-    """How calls on tensors of one layout go."""
+    """How calls on tensors of one layout go; ``native``: the library's arguments, where one stride describes the rows of
+    each."""
 
     def __init__(self, x, scale, residual, eps, checkpoint):
         _check(x, scale, residual, eps, checkpoint)
-        self.rows, self.d, self.type, self.index = math.prod(x.shape[:-1]), x.shape[-1], _lib.TYPES[x.dtype], x.get_device()
-        self.scale_type, self.eps = _lib.TYPES[scale.dtype], eps
-        strides = [0 if t is None else _lib.row_stride(t.shape, t.stride()) for t in (x, residual)]
-        self.copies = None in strides
-        self.x_stride, self.residual_stride = (self.d, self.d) if self.copies else strides
-        self.sums = residual is not None
-        self.held = _lib.keep_bytes(self.rows, self.d, checkpoint)
-        self.kept_stride = self.x_stride if residual is None else self.d   # of what the backward reads: x, or the sum
-        self.parts = _lib.check(_lib.lib().msd_rms_workspace_bytes(self.rows, self.d), "msd_rms_workspace_bytes") // 4
+        self.native = None
+        strides = [0 if t is None else _lib.ops().row_stride(t) for t in (x, residual)]
+        if None in strides:
+            return
+        rows, d = math.prod(x.shape[:-1]), x.shape[-1]
+        parts = _lib.check(_lib.lib().msd_rms_workspace_bytes(rows, d), "msd_rms_workspace_bytes") // 4
+        self.native = _lib.ops().RmsPlan(rows, d, _lib.TYPES[x.dtype], _lib.TYPES[scale.dtype], eps, *strides,
+                                         _lib.keep_bytes(rows, d, checkpoint), parts)
 
 
 _plans = {}
@@ -45,50 +45,6 @@ def _plan(x, scale, residual, eps, checkpoint):
             _plans.clear()
         _plans[key] = found
     return found
-
-
-def _forward(x, scale, residual, plan, keep):
-    if plan.copies:
-        x, residual = x.contiguous(), None if residual is None else residual.contiguous()
-    scale = scale.contiguous()
-    y = _lib.empty(x)
-    total = None if residual is None else _lib.empty(x)
-    rstd = x.new_empty(plan.rows, dtype=torch.float32) if keep else None
-    held = x.new_empty(plan.held, dtype=torch.uint8) if keep and plan.held else None
-    _lib.launch(_lib.lib().msd_rms_forward, "msd_rms_forward", plan.index, x.data_ptr(), plan.x_stride,
-                None if residual is None else residual.data_ptr(), plan.residual_stride, scale.data_ptr(), plan.scale_type,
-                plan.rows, plan.d, plan.type, plan.eps, y.data_ptr(), None if total is None else total.data_ptr(),
-                None if rstd is None else rstd.data_ptr(), None if held is None else held.data_ptr())
-    return y, total, x, scale, rstd, held
-
-
-class _RmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, scale, residual, plan):
-        ctx.scale_grad = scale.requires_grad
-        y, total, x, scale, rstd, held = _forward(x, scale, residual, plan, True)
-        ctx.save_for_backward(x if held is None and total is None else total if held is None else held, scale, rstd)
-        ctx.plan, ctx.held = plan, held is not None
-        ctx.set_materialize_grads(False)
-        return y if total is None else (y, total)
-
-    @staticmethod
-    @_lib.first_order
-    def backward(ctx, dy, dtotal=None):
-        if dy is None:   # only the sum was used: the norm adds nothing
-            return dtotal, None, dtotal, None   # (there is a residual then)
-        plan = ctx.plan
-        kept, scale, rstd = ctx.saved_tensors
-        dy, dy_stride = _lib.rows_of(dy)
-        ds, ds_stride = (None, 0) if dtotal is None else _lib.rows_of(dtotal)
-        dx = _lib.empty(dy)
-        dscale, ws = (torch.empty_like(scale), rstd.new_empty(plan.parts)) if ctx.scale_grad else (None, None)
-        at = kept.data_ptr()
-        _lib.launch(_lib.lib().msd_rms_backward, "msd_rms_backward", plan.index, None if ctx.held else at, plan.kept_stride,
-                    rstd.data_ptr(), at if ctx.held else None, scale.data_ptr(), plan.scale_type, dy.data_ptr(), dy_stride,
-                    None if ds is None else ds.data_ptr(), ds_stride, plan.rows, plan.d, plan.type, dx.data_ptr(),
-                    None if dscale is None else dscale.data_ptr(), None if ws is None else ws.data_ptr())
-        return dx, dscale, dx if plan.sums else None, None
 
 
 def _check(x, scale, residual, eps, checkpoint):
@@ -116,7 +72,8 @@ def rms_norm(x, scale, residual=None, eps=1e-5, checkpoint=None):
     x (..., d) bf16 or f32 on one GPU, any strides, d up to 16384; residual of x's shape and type; scale (d,) bf16 or f32.
     checkpoint: None, or "int8" (see the module)."""
     plan = _plan(x, scale, residual, float(eps), checkpoint)
-    if torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or (residual is not None and residual.requires_grad)):
-        return _RmsNorm.apply(x, scale, residual, plan)
-    y, total, *_ = _forward(x, scale, residual, plan, False)
-    return y if total is None else (y, total)
+    if plan.native is None:
+        x, residual = x.contiguous(), None if residual is None else residual.contiguous()
+        plan = _plan(x, scale, residual, float(eps), checkpoint)
+    out = _lib.ops().rms_norm(x, scale, residual, plan.native)
+    return out[0] if residual is None else tuple(out)

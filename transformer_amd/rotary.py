@@ -68,39 +68,25 @@ def _strides(x):
     return s if len(s) == 3 else (0, *s)
 
 
-def _contiguous(shape):
-    s, d, h = shape[-3] * shape[-2] * shape[-1], shape[-1], shape[-2] * shape[-1]
-    return (s, h, d)
-
-
-def _turns_heads(x):
-    return x.shape[-1] == 1 or x.stride(-1) == 1
-
-
 class _Plan:
-    """How calls on tensors of one layout go: the library's arguments forward and, for contiguous gradients, backward."""
+    """How calls on tensors of one layout go; ``native``: the library's arguments, where the heads are contiguous."""
 
     def __init__(self, q, k, frequencies, positions, start, layout):
         _check(q, k, frequencies, positions, layout)
-        self.q_shape, self.kv, self.dtype, self.index = q.shape, 0 if k is None else k.shape[-2], q.dtype, q.get_device()
-        self.d_rot, self.amplitude, self.start, self.layout = frequencies.d_rot, frequencies.amplitude, start, layout
-        self.position_bytes, self.position_stride = 0, (0, 0)
-        if positions is not None:
-            self.position_bytes = positions.element_size()
-            self.position_stride = positions.stride() if positions.dim() == 2 else (0, *positions.stride())
-        self.copies = not _turns_heads(q) or (k is not None and not _turns_heads(k))
-        whole = _contiguous(q.shape), None if k is None else _contiguous(k.shape)
-        self.forward = self.call(1, *(whole if self.copies else (_strides(q), None if k is None else _strides(k))))
-        self.backward = self.call(-1, *whole)
-
-    def call(self, sign, q_stride, k_stride):
-        r = _lib.MsdRope()
-        *_, r.tokens, r.n_heads, r.d_head = self.q_shape
-        r.batch = self.q_shape[0] if len(self.q_shape) == 4 else 1
-        r.n_kv_heads, r.d_rot, r.interleaved, r.type, r.sign = self.kv, self.d_rot, LAYOUTS[self.layout], _lib.TYPES[self.dtype], sign
-        r.position_bytes, r.amplitude, r.start = self.position_bytes, self.amplitude, self.start
-        r.q_stride[:], r.k_stride[:], r.position_stride[:] = q_stride, k_stride or (0, 0, 0), self.position_stride
-        return ctypes.byref(r)
+        self.native = None
+        if not all(x is None or x.shape[-1] == 1 or x.stride(-1) == 1 for x in (q, k)):
+            return
+        r = [_lib.MsdRope(), _lib.MsdRope()]   # forward, and for gradients, whose strides are set when they are known
+        for r_, sign in zip(r, (1, -1)):
+            *_, r_.tokens, r_.n_heads, r_.d_head = q.shape
+            r_.batch = q.shape[0] if q.dim() == 4 else 1
+            r_.n_kv_heads, r_.d_rot = 0 if k is None else k.shape[-2], frequencies.d_rot
+            r_.interleaved, r_.type, r_.sign, r_.amplitude, r_.start = LAYOUTS[layout], _lib.TYPES[q.dtype], sign, frequencies.amplitude, start
+            if positions is not None:
+                r_.position_bytes = positions.element_size()
+                r_.position_stride[:] = positions.stride() if positions.dim() == 2 else (0, *positions.stride())
+        r[0].q_stride[:], r[0].k_stride[:] = _strides(q), (0, 0, 0) if k is None else _strides(k)
+        self.native = _lib.ops().RopePlan(*map(ctypes.addressof, r))
 
 
 _plans = {}
@@ -117,43 +103,6 @@ def _plan(q, k, frequencies, positions, start, layout):
             _plans.clear()
         _plans[key] = found
     return found
-
-
-def _apply(index, call, q, k, turns, positions):
-    q_out = _lib.empty(q)
-    k_out = None if k is None else _lib.empty(k)
-    _lib.launch(_lib.lib().msd_rope_apply, "msd_rope_apply", index, call, q.data_ptr(), None if k is None else k.data_ptr(),
-                None if positions is None else positions.data_ptr(), turns.data_ptr(), q_out.data_ptr(),
-                None if k is None else k_out.data_ptr())
-    return q_out, k_out
-
-
-def _forward(q, k, turns, positions, plan):
-    if plan.copies:
-        q, k = q.contiguous(), None if k is None else k.contiguous()
-    return _apply(plan.index, plan.forward, q, k, turns, positions)
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, turns, positions, plan):
-        ctx.save_for_backward(turns, positions)
-        ctx.plan = plan
-        q, k = _forward(q, k, turns, positions, plan)
-        return q if k is None else (q, k)
-
-    @staticmethod
-    @_lib.first_order
-    def backward(ctx, dq, dk=None):
-        turns, positions = ctx.saved_tensors
-        plan = ctx.plan
-        call = plan.backward
-        if not dq.is_contiguous() or (dk is not None and not dk.is_contiguous()):
-            if not _turns_heads(dq) or (dk is not None and not _turns_heads(dk)):
-                dq, dk = dq.contiguous(), None if dk is None else dk.contiguous()
-            call = plan.call(-1, _strides(dq), None if dk is None else _strides(dk))
-        dq, dk = _apply(plan.index, call, dq, dk, turns, positions)
-        return dq, dk, None, None, None
 
 
 def _check(q, k, frequencies, positions, layout):
@@ -184,7 +133,8 @@ def rotary(q, k, frequencies, positions=None, start=0, layout="half"):
     position start + t.  layout: pairs (i, i + d_rot / 2) ("half", the reference's) or (2 i, 2 i + 1) ("interleaved").
     Returns contiguous (q, k), with autograd; q alone without a k."""
     plan = _plan(q, k, frequencies, positions, int(start), layout)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotary.apply(q, k, frequencies.turns, positions, plan)
-    q, k = _forward(q, k, frequencies.turns, positions, plan)
-    return q if k is None else (q, k)
+    if plan.native is None:
+        q, k = q.contiguous(), None if k is None else k.contiguous()
+        plan = _plan(q, k, frequencies, positions, int(start), layout)
+    out = _lib.ops().rotary(q, k, frequencies.turns, positions, plan.native)
+    return out[0] if k is None else tuple(out)

@@ -16,15 +16,16 @@ from . import _lib
 
 
 class _Plan:
-    """How calls on tensors of one layout go."""
+    """How calls on tensors of one layout go; ``native``: the library's arguments, where one stride describes the rows of
+    each."""
 
     def __init__(self, gate, up, checkpoint):
         _check(gate, up, checkpoint)
-        self.rows, self.d, self.type, self.index = math.prod(gate.shape[:-1]), gate.shape[-1], _lib.TYPES[gate.dtype], gate.get_device()
-        strides = [_lib.row_stride(x.shape, x.stride()) for x in (gate, up)]
-        self.copies = None in strides
-        self.gate_stride, self.up_stride = (self.d, self.d) if self.copies else strides
-        self.held = 2 * _lib.keep_bytes(self.rows, self.d, checkpoint)
+        self.native = None
+        strides = [_lib.ops().row_stride(x) for x in (gate, up)]
+        if None not in strides:
+            rows, d = math.prod(gate.shape[:-1]), gate.shape[-1]
+            self.native = _lib.ops().GluPlan(rows, d, _lib.TYPES[gate.dtype], *strides, 2 * _lib.keep_bytes(rows, d, checkpoint))
 
 
 _plans = {}
@@ -39,41 +40,6 @@ def _plan(gate, up, checkpoint):
             _plans.clear()
         _plans[key] = found
     return found
-
-
-def _forward(gate, up, plan, keep):
-    if plan.copies:
-        gate, up = gate.contiguous(), up.contiguous()
-    y = _lib.empty(gate)
-    held = gate.new_empty(plan.held, dtype=torch.uint8) if keep and plan.held else None
-    _lib.launch(_lib.lib().msd_swiglu_forward, "msd_swiglu_forward", plan.index, gate.data_ptr(), plan.gate_stride,
-                up.data_ptr(), plan.up_stride, plan.rows, plan.d, plan.type, y.data_ptr(),
-                None if held is None else held.data_ptr())
-    return y, gate, up, held
-
-
-class _Swiglu(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, gate, up, plan):
-        y, gate, up, held = _forward(gate, up, plan, True)
-        ctx.plan = plan
-        if held is None:
-            ctx.save_for_backward(gate, up)
-        else:
-            ctx.save_for_backward(held)
-        return y
-
-    @staticmethod
-    @_lib.first_order
-    def backward(ctx, dy):
-        plan, saved = ctx.plan, ctx.saved_tensors
-        dy, stride = _lib.rows_of(dy)
-        dgate, dup = _lib.empty(dy), _lib.empty(dy)
-        gate, up, held = (saved[0].data_ptr(), saved[1].data_ptr(), None) if len(saved) == 2 else (None, None, saved[0].data_ptr())
-        _lib.launch(_lib.lib().msd_swiglu_backward, "msd_swiglu_backward", plan.index, gate, plan.gate_stride, up,
-                    plan.up_stride, held, dy.data_ptr(), stride, plan.rows, plan.d, plan.type, dgate.data_ptr(),
-                    dup.data_ptr())
-        return dgate, dup, None
 
 
 def _check(gate, up, checkpoint):
@@ -92,6 +58,7 @@ def swiglu(gate, up, checkpoint=None):
     """gate / (1 + exp(-gate)) * up: (..., d) bf16 or f32 on one GPU, any strides (halves of one projection, say); returns
     a contiguous tensor of their shape and type.  checkpoint: None, or "int8" (see the module)."""
     plan = _plan(gate, up, checkpoint)
-    if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
-        return _Swiglu.apply(gate, up, plan)
-    return _forward(gate, up, plan, False)[0]
+    if plan.native is None:
+        gate, up = gate.contiguous(), up.contiguous()
+        plan = _plan(gate, up, checkpoint)
+    return _lib.ops().swiglu(gate, up, plan.native)
