@@ -40,7 +40,7 @@
 //   rows x keys, heads / kv, d, mask          forward        dQ             dK and dV, their parts' sum
 //   8192 x 8192, 16 / 4, 128, causal          318-352 (865)  403-440 (1020) 542-579 (1014), 24     clocks fall to 2.0 GHz
 //   4096 x 4096, 32 / 32, 64, none            180 (763)      221 (933)      273 (1007)
-//   23 documents in 8191, 16 / 4, 64, causal  37             44             54, 7.5
+//   24 documents in 8191, 16 / 4, 64, causal  37             44             54, 7.5
 //   8 x 512 x 512, 16 / 4, 64, causal         15.9           19.0           22.3, 7.3
 //   3 x 333 x 1021, 6 / 2, 96, none           13.8, 6.9 join 16.1, 5.3 join 20.0, 4.9
 //   4 x 1 x 2000, 16 / 4, 64                  6.3, 5.2 join
@@ -105,7 +105,7 @@ struct Seq {
 // Which sequence a workgroup works on.  Sequences of one shape: the same number of jobs each, a sequence's in a stride of `n_seqs`
 // (the jobs of all sequences with the most work come first).  Otherwise, for up to kMostSeqs of them, the first job of each,
 // as the host has counted them (it has their lengths; 1 KB of kernel arguments); beyond that the longest's number of jobs
-// for each, of which the others' are empty: at 23 documents of 16 to 2048 rows 60, 73 and 109 us for the three kernels in
+// for each, of which the others' are empty: at 24 documents of 3 to 1596 rows 60, 73 and 109 us for the three kernels in
 // place of 37, 44 and 62 (with the parts of that time).
 constexpr int kMostSeqs = 256;
 struct Jobs {
@@ -1020,7 +1020,7 @@ void magic(uint32_t g, uint32_t& m, int& s) {
 // With 8: 25.1 us and 6.6 for the sum in place of 22.9 and 4.4 (3 x 333 x 1021)
 constexpr int kLeast = 16;
 // A part's row tiles, of what there is for each of two workgroups a CU.  With 1 all of them would start at once if they were
-// alike; larger ones are fewer first loads and sums.  With 1, 1.5 and 2, the sum included: 72, 61 and 72 us (23 documents in
+// alike; larger ones are fewer first loads and sums.  With 1, 1.5 and 2, the sum included: 72, 61 and 72 us (24 documents in
 // 8191), 125, 103 and 117 (the same, heads of 128), 571, 571 and 662 (8192 rows), 128, 112 and 119 (3200 rows, heads of 128)
 constexpr double kShare = 1.5;
 struct Plan {
