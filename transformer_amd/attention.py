@@ -137,8 +137,8 @@ def _check(q, k, v, scale, sequences):
     D, H, KV = q.shape[-1], q.shape[-2], k.shape[-2]
     if k.shape[-1] != D or D % 8 or not 0 < D <= 128:
         raise ValueError(f"d_head must be a multiple of 8 up to 128, the same for q, k and v (got {D} and {k.shape[-1]})")
-    if KV == 0 or H == 0 or H % KV:
-        raise ValueError(f"n_heads ({H}) must be a multiple of n_kv_heads ({KV})")
+    if KV == 0 or H == 0 or H % KV or H > 4096:
+        raise ValueError(f"n_heads ({H}) must be a multiple of n_kv_heads ({KV}), up to 4096")
     if not 2.0 ** -60 <= scale <= 2.0 ** 60:
         raise ValueError(f"scale must lie in [2 ** -60, 2 ** 60] (got {scale})")
     if q.dim() == 4 and q.shape[0] != k.shape[0]:
