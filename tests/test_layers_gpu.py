@@ -523,3 +523,37 @@ def test_second_derivatives_are_refused(which):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     with pytest.raises(RuntimeError, match="differentiable once"):
         sum(x.float().sum() for x in got).backward()
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_parts_of_the_gradients_and_twice(which):
+    """Only some leaves want gradients; a graph that is kept gives them again; nothing is recorded without a wish for it."""
+    f, leaves = _strided_calls()[which]
+    whole = [x.detach().requires_grad_() for x in leaves]
+    y = f(*whole).float().sin().sum()
+    want = torch.autograd.grad(y, whole, retain_graph=True)
+    again = torch.autograd.grad(y, whole)
+    assert all(torch.equal(a, b) for a, b in zip(want, again))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, whole)
+    for i in range(len(leaves)):
+        some = [x.detach().requires_grad_(i == j) for j, x in enumerate(leaves)]
+        got, = torch.autograd.grad(f(*some).float().sin().sum(), some[i:i + 1])
+        assert torch.equal(got, want[i])
+    with torch.no_grad():
+        assert not f(*whole).requires_grad
+    with torch.inference_mode():
+        assert torch.equal(f(*leaves), f(*whole))
+
+
+def test_rotary_heads_of_4096():
+    """The most cosines and sines that a workgroup keeps."""
+    q, freq = _rand((5, 1, 4096), 3), rotary_frequencies(4096)
+    got = rotary(q, None, freq, start=7)
+    pos = torch.arange(7, 12, dtype=torch.int64, device="cuda")
+    turn = (pos.double()[:, None] * freq.turns) % 1.0 * (2 * math.pi)
+    a, b = q[:, 0, :2048].double(), q[:, 0, 2048:].double()
+    want = torch.cat((a * turn.cos() - b * turn.sin(), a * turn.sin() + b * turn.cos()), -1)
+    # the result's rounding, and the f32 angle, cosine and products: a few 2^-24 of the pair
+    tol = 2.0 ** -8 * want.abs() + 2.0 ** -20 * torch.cat((a.abs() + b.abs(),) * 2, -1)
+    assert ((got[:, 0].double() - want).abs() <= tol).all()

@@ -32,7 +32,8 @@ def hipcc():
 
 
 def ops_command(out):
-    """The host compiler's command for _ops.so, over libmsdecode.so beside it."""
+    """The host compiler's command for _ops.so, over libmsdecode.so beside it (HIP's headers want to be told their platform
+    by a compiler that is not hipcc)."""
     import torch
     base = os.path.dirname(torch.__file__)
     include = [os.path.join(base, "include"), os.path.join(base, "include/torch/csrc/api/include"),
