@@ -258,10 +258,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_fwd(RmsArgs p) {
 
 // With n = s rstd: dx = rstd (dy scale - n mean(dy scale n)) + dsum, dscale = sum over the rows of dy n.
 // A workgroup of 1024 lanes takes rows 1024 / TPR at a time and keeps dscale's sums over its rows in registers; at the end
-// they are added over its row groups through LDS, in a fixed tree, and go to part[workgroup]: two workgroups a CU (256 parts:
-// the same time; 1024: 116 + 7.3 us in place of 110 + 4.9 with the sum of the parts).  110 us for 16383 x 4096 from the 8-bit
-// checkpoint (473 MB, 4.3 TB/s): the row's sum stands between its loads and its stores, and loading the next row
-// ahead costs the registers of half the waves (117 us).  9.6 us for 4096 x 1024.
+// they are added over its row groups through LDS, in a fixed tree, and go to part[workgroup].  At most 512 parts (256: the
+// same time; 1024: 116 + 7.3 us in place of 110 + 4.9 with the sum of the parts).  110 us for 16383 x 4096 from the 8-bit
+// checkpoint (473 MB, 4.3 TB/s): the row's sum stands between its loads and its stores; loading the next row ahead costs
+// the registers of half the waves (117 us), and workgroups of 512 lanes, whose rows wait for fewer others, gain nothing
+// (112).  9.6 us for 4096 x 1024.
 template <class T, int TPR, int V>
 __global__ __launch_bounds__(1024) void rms_bwd(RmsArgs p) {
   constexpr int G = 1024 / TPR;   // row groups
