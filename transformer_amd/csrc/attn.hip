@@ -175,18 +175,19 @@ __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
 // 64 lanes' 16 bytes at byte offsets `off` from `base` (wave-uniform) straight to the 1 KB of LDS at byte address `to`
 // (lane after lane); kOutside gives zeros.  In assembly, because the compiler would wait for it before
 // every LDS read that follows; dma_wait() is the wait, and what the workgroup's other waves fetched needs its barrier too.
-// (m0, the LDS base, is set in the same statement: the compiler has no use of its own for it in these kernels.)
+// m0, the LDS base, is set in the same statement; the load may take it one wait state after the scalar write, which nothing
+// puts between the two inside a statement but the s_nop.
 __device__ __forceinline__ void dma(const uint16_t* base, uint32_t off, uint32_t to) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, 0x7fffffff, 0x00020000);
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(r));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(r) : "m0");
 #endif
 }
 // 64 lanes' 4 bytes to the 256 bytes of LDS at `to`
 __device__ __forceinline__ void dma4(const float* base, uint32_t off, uint32_t to) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, 0x7fffffff, 0x00020000);
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(r));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(r) : "m0");
 #endif
 }
 // Until at most N of this wave's loads are outstanding (they return in order).  The compiler counts it, so that its own
