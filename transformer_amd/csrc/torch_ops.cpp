@@ -177,7 +177,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Attn& 
 
 // ---- rotary positions ----
 struct RopePlan : torch::CustomClassHolder {
-  msd_rope forward, backward;   // the latter of contiguous gradients
+  msd_rope forward, backward;   // (the strides of gradients and of the saved positions are set in the call)
 };
 using Rope = c10::intrusive_ptr<RopePlan>;
 
@@ -206,12 +206,17 @@ struct Rotary : torch::autograd::Function<Rotary> {
     const auto x = ctx->get_saved_variables();
     const auto capsule = ctx->saved_data["plan"].toCapsule();
     msd_rope r = static_cast<const RopePlan&>(*capsule).backward;
+    const Tensor positions = x[1];   // (hooks on saved tensors may have given them other strides)
+    if (positions.defined()) {
+      r.position_stride[0] = positions.dim() == 2 ? positions.stride(0) : 0;
+      r.position_stride[1] = positions.stride(-1);
+    }
     Tensor dq = g[0], dk = g.size() > 1 ? g[1] : Tensor();
     if (!heads_contiguous(dq)) dq = dq.contiguous();
     if (dk.defined() && !heads_contiguous(dk)) dk = dk.contiguous();
     head_strides(dq, r.q_stride);
     if (dk.defined()) head_strides(dk, r.k_stride);
-    auto [a, b] = rope_run(r, dq, dk, x[0], x[1]);
+    auto [a, b] = rope_run(r, dq, dk, x[0].contiguous(), positions);
     return first_order({a, b, Tensor(), Tensor(), Tensor()}, recorded);
   }
 };
