@@ -25,3 +25,9 @@ def test_replaced_frequencies(turns):
     """A vector that is not what the plan was made for would be read past its end."""
     with pytest.raises(ValueError, match="float64"):
         _lib.ops().rotary(torch.zeros(4, 2, 8), None, turns, None, _rope())
+
+
+def test_frequencies_that_want_a_gradient():
+    """They would get none, without a word."""
+    with pytest.raises(ValueError, match="no gradient"):
+        _lib.ops().rotary(torch.zeros(4, 2, 8), None, _turns().requires_grad_(), None, _rope())

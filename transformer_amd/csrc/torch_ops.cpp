@@ -227,6 +227,8 @@ variable_list rotary(const Tensor& q, const MaybeTensor& k, const Tensor& turns,
   if (turns.scalar_type() != at::kDouble || turns.dim() != 1 || turns.numel() != p->forward.d_rot / 2 || !turns.is_contiguous() ||
       turns.device() != q.device())
     throw std::invalid_argument("turns must be a contiguous float64 vector of d_rot / 2 values on q's GPU");
+  if (at::GradMode::is_enabled() && turns.requires_grad())
+    throw std::invalid_argument("the frequencies take no gradient: hand over turns.detach()");
   if (at::GradMode::is_enabled() && (wanted(q) || (k && wanted(*k)))) return Rotary::apply(q, k, turns, positions, p);
   auto [a, b] = rope_run(p->forward, q, k.value_or(Tensor()), turns, positions.value_or(Tensor()));
   if (!b.defined()) return {a};

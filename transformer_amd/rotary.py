@@ -17,7 +17,8 @@ from . import _lib
 
 
 class RotaryFrequencies:
-    """Turns per position of each pair (device float64, d_rot / 2) and the amplitude of the rotated values."""
+    """Turns per position of each pair (device float64, d_rot / 2) and the amplitude of the rotated values.  They take no
+    gradient: ``rotary`` refuses turns that want one while gradients are recorded."""
 
     def __init__(self, turns, amplitude=1.0):
         if turns.dim() != 1 or turns.numel() == 0 or turns.dtype != torch.float64 or not turns.is_contiguous():
