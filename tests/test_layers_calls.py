@@ -4,6 +4,8 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from transformer_amd import _lib
 
@@ -31,3 +33,44 @@ def test_frequencies_that_want_a_gradient():
     """They would get none, without a word."""
     with pytest.raises(ValueError, match="no gradient"):
         _lib.ops().rotary(torch.zeros(4, 2, 8), None, _turns().requires_grad_(), None, _rope())
+
+
+def _calls():
+    """(call, its operands) of every operator: host tensors and plans of their shapes."""
+    ops, x = _lib.ops(), [torch.linspace(-1, 1, 64).reshape(4, 16) * (i + 1) for i in range(3)]
+    a = _lib.MsdAttn()
+    h = [t.to(torch.bfloat16).reshape(4, 2, 8) for t in x]
+    attn = ops.AttnPlan(ctypes.addressof(a), 0, 0, False, False, None, None, 0)
+    rms, glu, rope = ops.RmsPlan(4, 16, 1, 1, 1e-5, 16, 16, 0, 16), ops.GluPlan(4, 16, 1, 16, 16, 0), _rope()
+    return [
+        (lambda q, k, v: ops.attention(q, k, v, attn), h),
+        (lambda q: ops.rotary(q, None, _turns(), None, rope)[0], [x[0].reshape(4, 2, 8)]),
+        (lambda s, w: ops.rms_norm(s, w, None, rms)[0], [x[0], x[1][0]]),
+        (lambda s, w, r: ops.rms_norm(s, w, r, rms)[0], [x[0], x[1][0], x[2]]),
+        (lambda g, u: ops.swiglu(g, u, glu), x[:2]),
+    ]
+
+
+@pytest.mark.parametrize("which", range(5))
+@pytest.mark.parametrize("recorded", [False, True])
+def test_forward_mode(which, recorded):
+    """An operand with a tangent, whichever it is: a result without one would stand for a tangent of zero."""
+    f, x = _calls()[which]
+    for i in range(len(x)):
+        with fwd.dual_level(), torch.set_grad_enabled(recorded):
+            y = [t.clone().requires_grad_(recorded) for t in x]
+            y[i] = fwd.make_dual(y[i], torch.ones_like(y[i]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f(*y)
+
+
+@pytest.mark.parametrize("which", range(5))
+@pytest.mark.parametrize("recorded", [False, True])
+def test_traces(which, recorded):
+    """A trace would keep the outputs' allocation and none of the kernels."""
+    f, x = _calls()[which]
+    x = tuple(t.clone().requires_grad_(recorded) for t in x)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(f, x, check_trace=False)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(f)(*x)

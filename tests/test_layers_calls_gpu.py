@@ -1,9 +1,13 @@
-"""Calls of the layer operators that their first tests leave out: saved tensors with other strides."""
-
+"""Calls of the layer operators that their first tests leave out: saved tensors with other strides, forward-mode
+differentiation and traces."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
+from transformer_amd.attention import attention
+from transformer_amd.norm import rms_norm
 from transformer_amd.rotary import rotary, rotary_frequencies
+from transformer_amd.swiglu import swiglu
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +33,29 @@ def test_rotary_positions_whose_saved_copy_has_other_strides(kind):
                 y = rotary(leaf, None, freq, positions.contiguous())
             grads += torch.autograd.grad(y, leaf, dx)
         assert torch.equal(*grads)
+
+
+def _calls():
+    freq = rotary_frequencies(64)
+    h, x = [_rand((2, 5, 2, 64), i) for i in range(3)], [_rand((5, 64), i) for i in range(3)]
+    return [(attention, h), (lambda q, k: rotary(q, k, freq)[0], h[:2]), (lambda q: rotary(q, None, freq), h[:1]),
+            (lambda s, w, r: rms_norm(s, w[0], r)[0], x), (lambda s, w: rms_norm(s, w[0], checkpoint="int8"), x[:2]), (swiglu, x[:2])]
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_forward_mode_and_traces_are_refused(which):
+    """By the public calls and by the gradients, which then go on as before."""
+    f, x = _calls()[which]
+    want = f(*x)
+    for recorded in (False, True):
+        y = [t.detach().requires_grad_(recorded) for t in x]
+        with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            f(fwd.make_dual(y[0], torch.ones_like(y[0])), *y[1:])
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, tuple(y), check_trace=False)
+    out = f(*y)
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        torch.autograd.grad(out, y, fwd.make_dual(torch.ones_like(out), torch.ones_like(out)), retain_graph=True)
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(out, y, torch.ones_like(out)))
+    with torch.no_grad():
+        assert torch.equal(f(*x), want)

@@ -7,8 +7,10 @@
 // over operands that the kernels take as they lie.
 #include <torch/extension.h>
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <memory>
 #include <optional>
@@ -39,6 +41,18 @@ void* at_(const Tensor& x) { return x.defined() ? x.data_ptr() : nullptr; }
 Tensor contiguous_like(const Tensor& x) { return at::empty_like(x, x.options(), at::MemoryFormat::Contiguous); }
 Tensor bytes(const Tensor& x, int64_t n) { return at::empty({n}, x.options().dtype(at::kByte)); }
 bool wanted(const Tensor& x) { return x.defined() && x.requires_grad(); }
+
+// A call is launches of the library, which neither a trace records (it would keep the outputs' allocation and nothing else) nor
+// forward-mode differentiation sees (an output without a tangent stands for a tangent of zero): refused, in the backward too.
+bool has_tangent(const Tensor& x) { return x.defined() && x._fw_grad(0).defined(); }
+bool has_tangent(const MaybeTensor& x) { return x && has_tangent(*x); }
+template <class... X>
+void only_run(const char* what, const X&... x) {
+  using c10::impl::TorchDispatchModeKey;
+  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY))
+    throw std::runtime_error(std::string(what) + " cannot be traced: a trace does not record its kernels");
+  if ((has_tangent(x) || ...)) throw std::runtime_error(std::string(what) + " has no forward-mode derivative");
+}
 
 // The calls go to x's device, with its current stream
 struct Place {
@@ -152,6 +166,7 @@ struct Attention : torch::autograd::Function<Attention> {
     return {out};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    only_run("the gradient of attention", g[0]);
     const bool recorded = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
     const auto x = ctx->get_saved_variables();   // (with the strides that hooks on saved tensors have given them, if any)
@@ -172,6 +187,7 @@ struct Attention : torch::autograd::Function<Attention> {
 };
 
 Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Attn& p) {
+  only_run("attention", q, k, v);
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v))) return Attention::apply(q, k, v, p)[0];
   return attn_run(q, k, v, *p, nullptr, nullptr);
 }
@@ -202,6 +218,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     return {a, b};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    only_run("the gradient of rotary", g[0], g.size() > 1 ? g[1] : Tensor());
     const bool recorded = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
     const auto x = ctx->get_saved_variables();
@@ -223,6 +240,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
 };
 
 variable_list rotary(const Tensor& q, const MaybeTensor& k, const Tensor& turns, const MaybeTensor& positions, const Rope& p) {
+  only_run("rotary", q, k, turns);
   // (a RotaryFrequencies can be given another vector after its own checks, and the plan knows its length only)
   if (turns.scalar_type() != at::kDouble || turns.dim() != 1 || turns.numel() != p->forward.d_rot / 2 || !turns.is_contiguous() ||
       turns.device() != q.device())
@@ -271,6 +289,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     return {o.y, o.sum};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    only_run("the gradient of rms_norm", g[0], g.size() > 1 ? g[1] : Tensor());
     const bool recorded = at::GradMode::is_enabled(), sums = g.size() > 1;
     at::NoGradGuard no_grad;
     const Tensor dsum = sums ? g[1] : Tensor();
@@ -298,6 +317,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
 };
 
 variable_list rms_norm(const Tensor& x, const Tensor& scale, const MaybeTensor& residual, const Rms& p) {
+  only_run("rms_norm", x, scale, residual);
   if (at::GradMode::is_enabled() && (wanted(x) || wanted(scale) || (residual && wanted(*residual))))
     return RmsNorm::apply(x, scale, residual, p);
   RmsOut o = rms_run(x, scale.contiguous(), residual.value_or(Tensor()), *p, false);
@@ -330,6 +350,7 @@ struct Swiglu : torch::autograd::Function<Swiglu> {
     return {y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    only_run("the gradient of swiglu", g[0]);
     const bool recorded = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
     const auto s = ctx->get_saved_variables();
@@ -349,6 +370,7 @@ struct Swiglu : torch::autograd::Function<Swiglu> {
 };
 
 Tensor swiglu(const Tensor& gate, const Tensor& up, const Glu& p) {
+  only_run("swiglu", gate, up);
   if (at::GradMode::is_enabled() && (wanted(gate) || wanted(up))) return Swiglu::apply(gate, up, p)[0];
   return glu_run(gate, up, *p, nullptr);
 }
