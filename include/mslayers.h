@@ -62,8 +62,8 @@ int64_t msd_attn_workspace_bytes(const msd_attn* a, int32_t backward);
 
 /* out = softmax(scale q k^T) v.  lse: device f32 (q_rows * n_heads), kept for the backward (its layout is the
  * library's own); out_low: a byte (q_rows * n_heads * d_head, 8-byte aligned) for what the rounding to bf16 took off each
- * value of out, from which the backward forms rowsum(dout * out) to f32's rather than bf16's precision (dq and dk then lie
- * a tenth nearer the exact ones).  Either may be NULL: no backward follows, or out itself will do. */
+ * value of out, from which the backward forms rowsum(dout * out) with values of out to 2^-15 rather than bf16's 2^-8 (dq and dk
+ * then lie a tenth nearer the exact ones).  Either may be NULL: no backward follows, or out itself will do. */
 int32_t msd_attn_forward(const msd_attn* a, const void* q, const void* k, const void* v, void* out, void* out_low,
                          float* lse, void* workspace, void* stream);
 

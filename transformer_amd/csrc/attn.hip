@@ -137,9 +137,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
-// x is to about 2^-16 what a = bf16(x) and this byte say together: the upper eight of the sixteen bits by which x's differ
-// from a's (the rounding is to nearest, so that they are a signed byte)
-__device__ __forceinline__ uint32_t low_byte(float x, uint32_t a) { return (__float_as_uint(x) - (a << 16)) >> 8 & 0xff; }
+// x is to 2^-15 what a = bf16(x) and this byte say together: the upper eight of the sixteen bits by which x's differ from a's.
+// The rounding is to nearest, so the difference lies in [-0x8000, 0x8000] and its upper byte is a signed one but for the
+// upper end, a tie that is rounded down (means of two or four values often are one): that takes the largest byte, which is
+// off by 0x100 of x's bits as any other may be.
+__device__ __forceinline__ uint32_t low_byte(float x, uint32_t a) {
+  return uint32_t(min(int32_t(__float_as_uint(x) - (a << 16)), 0x7fff)) >> 8 & 0xff;
+}
 __device__ __forceinline__ float with_low(uint32_t a, uint32_t byte) {
   return __uint_as_float((a << 16) + uint32_t(int32_t(byte << 24) >> 16));
 }
