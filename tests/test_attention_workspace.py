@@ -1,0 +1,47 @@
+"""Workspaces of attention over sequences that leave rows out, on the CPU: they follow the sequences' rows, not the tensors'."""
+import ctypes
+
+import pytest
+
+from transformer_amd import _lib
+
+
+def workspace(q_lens, k_lens=None, gap=0, H=32, KV=8, D=128, causal=1):
+    """(forward's, backward's) bytes of sequences in rows of `gap` each (0: packed), and the bytes of the statistics of all rows."""
+    k_lens, rows, q, k = k_lens or q_lens, [], 0, 0
+    for n, m in zip(q_lens, k_lens):
+        rows += [q, n, k, m]
+        q, k = q + (gap or n), k + (gap or m)
+    host, a = (ctypes.c_int32 * len(rows))(*rows), _lib.MsdAttn()
+    a.n_seqs, a.q_len, a.k_len, a.q_rows, a.k_rows = len(q_lens), max(q_lens), max(k_lens), q, k
+    a.n_heads, a.n_kv_heads, a.d_head, a.causal, a.scale = H, KV, D, causal, D ** -0.5
+    a.q_stride[:], a.dout_stride[:] = [(0, H * D, D)] * 2
+    a.k_stride[:], a.v_stride[:] = [(0, KV * D, D)] * 2
+    a.seqs, a.seqs_host = 16, ctypes.addressof(host)
+    n = [_lib.check(_lib.lib().msd_attn_workspace_bytes(ctypes.byref(a), i), "workspace") for i in (0, 1)]
+    return *n, (8 * q * H + 255) // 256 * 256
+
+
+@pytest.mark.parametrize("q_lens,k_lens,gap", [
+    ([1] * 16, [4096] * 16, 4096),       # a new row of each sequence of a padded batch
+    ([4] * 64, [2048] * 64, 2048),
+    ([300] * 2, None, 4096),
+    ([1], [100000], 131072),
+    ([1], [1], 131072),
+    ([700, 20, 3], None, 50000),
+    ([3000, 1], [1, 3000], 60000),
+    ([1] * 256, [129] * 256, 4096),
+])
+@pytest.mark.parametrize("H,KV,D", [(32, 8, 128), (16, 1, 64), (4, 4, 8)])
+@pytest.mark.parametrize("causal", [0, 1])
+def test_padding_takes_no_workspace(q_lens, k_lens, gap, H, KV, D, causal):
+    packed, padded = (workspace(q_lens, k_lens, g, H, KV, D, causal) for g in (0, gap))
+    assert padded[0] == packed[0] and padded[1] - padded[2] == packed[1] - packed[2]
+    # splits times workgroups of 128 rows: below 2 x 512; two tensors of 8192 parts of 128 keys
+    assert padded[0] <= 1024 * 128 * 4 * (D + 1) and padded[1] - padded[2] <= 2 ** 30
+
+
+def test_sizes_of_one_new_row_each():
+    forward, backward, stats = workspace([1] * 16, [4096] * 16, 4096)
+    assert forward == 4 * 4 * (16 * 8) * 4 * (128 + 1)   # floats, splits, workgroups, rows of a workgroup, values of a row
+    assert backward == stats + forward // (128 + 1) * 128

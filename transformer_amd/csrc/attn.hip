@@ -89,14 +89,24 @@ struct Args {
   int g_shift;
   float c, scale;
   int splits;               // forward: of the keys
+  int64_t groups, blocks;   // workgroups of rows; blocks of 128 keys of all sequences (see Parts)
+  int row_slots, key_slots;
   int tile_rows, head_parts, row_parts, chunk;   // dK and dV: see KeyPart
   int64_t q_rows, k_rows;
   uint16_t *out, *dq, *dk, *dv;
   uint8_t* low;             // what the rounding to bf16 took off each value of out (low_byte()), or null
   float* lse;
   float* stats;             // backward: (-lse / c, -D) of every row, in the order of lse
-  float* part;              // forward: [splits][q_rows * H][D + 1]; backward: [2][splits][k_rows * KV][D]
+  float* part;              // see Parts
 };
+
+// Parts.  What the splits of the keys leave of a row, and what the parts of a key block leave of its dK and dV, lies workgroup by
+// workgroup: row r of workgroup x at x row_slots + r % 128, key k of block i (as attn_sum_parts counts them) at i key_slots +
+// k % 128; the slots are 128, or as many as the longest sequence has.  So they take the memory of what the sequences hold, not
+// of the tensors' rows: 1 MB for a new row in each of 16 x 4096 padded ones, 32 / 8 heads of 128 over 4096 keys (4.3 GB by the
+// tensors' rows).  The rows' take 68 MB at most, as splits times workgroups stay below 4 kCus, the keys' 1 GB (plan()).
+//   forward: [splits][groups row_slots][D], then [splits][groups row_slots] logsumexps; dQ: [splits][groups row_slots][D]
+//   dK and dV: [2][parts][blocks key_slots][KV][D]
 
 struct Seq {
   int qs, qn, ks, kn;
@@ -404,6 +414,25 @@ __device__ __forceinline__ int64_t stat_index(const Args& p, const RowJob& j) {
   return int64_t(j.s.qs) * p.H + int64_t(j.head) * j.s.qn + j.pos;
 }
 
+// Row `row` of a sequence's H qn, by K/V heads: where it lies and where its parts do
+struct JoinRow {
+  bool ok;
+  int pos, head;
+  int64_t slot;
+};
+__device__ __forceinline__ JoinRow join_row(const Args& p, const Jobs& jobs, const Seq& s, int b, int64_t row) {
+  const int n = s.qn * p.g;
+  JoinRow j{};
+  if (row >= int64_t(n) * p.KV) return j;
+  const int kvh = int(row) / n, r = int(row) - kvh * n, local = (n - 1) / (32 * kWaves) - r / (32 * kWaves);   // (see row_job)
+  j.pos = div_g(p, r);
+  j.head = kvh * p.g + r - j.pos * p.g;
+  const int64_t x = (jobs.counted ? jobs.first[b] + local : int64_t(local) * p.n_seqs + b) * p.KV + kvh;
+  j.ok = x < p.groups;   // (else a device table that has been overwritten: the host has counted fewer rows)
+  j.slot = x * p.row_slots + r % (32 * kWaves);
+  return j;
+}
+
 // ---- forward ----
 // Per 32 keys: the scores' maximum; the probabilities, while the matrix cores form the next 32 keys' scores; then their
 // product with V.  So the scores run 32 keys ahead, K one tile ahead of V: three K buffers and two of V, one barrier a tile.
@@ -505,8 +534,8 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void attn_fwd(Args p
   const float lse = l == 0 ? INFINITY : m + __log2f(l);   // +inf: 2^(c s - lse) is 0 for a row that sees nothing
   if (p.splits > 1) {   // normalised part and its weight, joined by attn_join
     if (j.ok) {
-      const int64_t row = stat_index(p, j);
-      float* to = p.part + (int64_t(blockIdx.y) * p.q_rows * p.H + row) * p.D;
+      const int64_t slots = p.groups * p.row_slots, row = blockIdx.y * slots + int64_t(blockIdx.x) * p.row_slots + 32 * wv + (lane & 31);
+      float* to = p.part + row * p.D;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -515,7 +544,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void attn_fwd(Args p
           if (c < p.D)
             *reinterpret_cast<f32x4*>(to + c) = f32x4{o[d][4 * u] * by, o[d][4 * u + 1] * by, o[d][4 * u + 2] * by, o[d][4 * u + 3] * by};
         }
-      if (lane < 32) p.part[int64_t(p.splits) * p.q_rows * p.H * p.D + int64_t(blockIdx.y) * p.q_rows * p.H + row] = lse;
+      if (lane < 32) p.part[p.splits * slots * p.D + row] = lse;
     }
     return;
   }
@@ -536,20 +565,20 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void attn_fwd(Args p
 // 20), 4 for more than 4 (2400 x 16 rows: 15 us, with 16 lanes 43), else 1 (3200 x 16 rows of two splits: 13.8 us, with 4 lanes 20).
 constexpr int kJoinLanes = 256;
 template <int G>
-__global__ __launch_bounds__(kJoinLanes) void attn_join(Args p) {
+__global__ __launch_bounds__(kJoinLanes) void attn_join(Args p, Jobs jobs) {
   __shared__ float lds[kJoinLanes][11];
   const int tid = threadIdx.x, c = tid % 16, zg = tid / 16 % G;
   const Seq s = sequence(p, blockIdx.y);
-  const int64_t n = p.q_rows * p.H, rows = int64_t(s.qn) * p.H, row = int64_t(blockIdx.x) * (kJoinLanes / 16 / G) + tid / 16 / G;
-  const int64_t at = int64_t(s.qs) * p.H + row;   // in the statistics' order
-  const bool ok = row < rows && 8 * c < p.D;
-  const float* w = p.part + int64_t(p.splits) * n * p.D;
+  const int64_t n = p.groups * p.row_slots;
+  const JoinRow j = join_row(p, jobs, s, blockIdx.y, int64_t(blockIdx.x) * (kJoinLanes / 16 / G) + tid / 16 / G);
+  const bool ok = j.ok && 8 * c < p.D;
+  const float* w = p.part + p.splits * n * p.D;
   float m = -INFINITY, l = 0, acc[8] = {};
   if (ok)
 #pragma unroll 2
     for (int z = zg; z < p.splits; z += G) {
-      const float x = w[z * n + at];
-      const float* from = p.part + (z * n + at) * p.D + 8 * c;
+      const float x = w[z * n + j.slot];
+      const float* from = p.part + (z * n + j.slot) * p.D + 8 * c;
       const f32x4 a = *reinterpret_cast<const f32x4*>(from), b = *reinterpret_cast<const f32x4*>(from + 4);
       if (x == INFINITY) continue;   // nothing seen in this part
       const float mn = fmaxf(m, x), old = exp2_hw(m - mn), e = exp2_hw(x - mn);   // (a NaN stays one through e)
@@ -582,16 +611,15 @@ __global__ __launch_bounds__(kJoinLanes) void attn_join(Args p) {
     for (int i = 0; i < 8; ++i) acc[i] = fmaf(e, x[2 + i], acc[i]);
   }
   const float by = l == 0 ? 0.0f : 1.0f / l;
-  const int head = int(row) / s.qn, pos = int(row) - head * s.qn;
   u32x4 x;
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = pack2(acc[2 * i] *= by, acc[2 * i + 1] *= by);
-  const int64_t to = (int64_t(s.qs + pos) * p.H + head) * p.D + 8 * c;
+  const int64_t to = (int64_t(s.qs + j.pos) * p.H + j.head) * p.D + 8 * c;
   *reinterpret_cast<u32x4*>(p.out + to) = x;
   if (p.low)
     *reinterpret_cast<u32x2*>(p.low + to) = u32x2{low_bytes(acc[0], acc[1], acc[2], acc[3], x[0], x[1]),
                                                   low_bytes(acc[4], acc[5], acc[6], acc[7], x[2], x[3])};
-  if (p.lse && c == 0) p.lse[at] = l == 0 ? INFINITY : m + __log2f(l);
+  if (p.lse && c == 0) p.lse[int64_t(s.qs) * p.H + int64_t(j.head) * s.qn + j.pos] = l == 0 ? INFINITY : m + __log2f(l);
 }
 
 // ---- backward ----
@@ -677,7 +705,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_dq(Args p, Jobs jobs) {
     __syncthreads();
   }
   if (p.splits > 1) {   // a part, joined by attn_join_dq
-    float* to = p.part + (int64_t(blockIdx.y) * p.q_rows * p.H + int64_t(j.s.qs + j.pos) * p.H + j.head) * p.D;
+    float* to = p.part + ((blockIdx.y * p.groups + blockIdx.x) * p.row_slots + 32 * wv + (lane & 31)) * p.D;
     if (j.ok)
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d)
@@ -697,20 +725,23 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_dq(Args p, Jobs jobs) {
 }
 
 // dQ as the sum of its parts over the splits, in order: 8 values a thread, of the rows of a sequence
-__global__ __launch_bounds__(256) void attn_join_dq(Args p) {
+__global__ __launch_bounds__(256) void attn_join_dq(Args p, Jobs jobs) {
   const Seq s = sequence(p, blockIdx.y);
-  const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 8;
-  if (i >= int64_t(s.qn) * p.H * p.D) return;
-  const int64_t n = p.q_rows * p.H * p.D, at = int64_t(s.qs) * p.H * p.D + i;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x, row = i / (uint32_t(p.D) / 8), c = i - row * (uint32_t(p.D) / 8);
+  const JoinRow j = join_row(p, jobs, s, blockIdx.y, row);
+  if (!j.ok) return;
+  const int64_t n = p.groups * p.row_slots;
+  const float* from = p.part + j.slot * p.D + 8 * c;
   f32x4 x = {}, y = {};
 #pragma unroll 4
   for (int z = 0; z < p.splits; ++z) {
-    x += *reinterpret_cast<const f32x4*>(p.part + z * n + at);
-    y += *reinterpret_cast<const f32x4*>(p.part + z * n + at + 4);
+    x += *reinterpret_cast<const f32x4*>(from + z * n * p.D);
+    y += *reinterpret_cast<const f32x4*>(from + z * n * p.D + 4);
   }
   x *= p.scale;
   y *= p.scale;
-  *reinterpret_cast<u32x4*>(p.dq + at) = u32x4{pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3])};
+  *reinterpret_cast<u32x4*>(p.dq + (int64_t(s.qs + j.pos) * p.H + j.head) * p.D + 8 * c) =
+      u32x4{pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3])};
 }
 
 // Row tiles of R rows (of one head) that see a key of the 128 of block kb: [first, first + n)
@@ -789,7 +820,7 @@ struct RowStream {
 // first loads and last stores (8 us together) are behind the other's products; eight waves a workgroup, one a CU, expose
 // them.
 template <int DP>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_dkv(Args p, Jobs jobs) {
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_dkv(Args p, Jobs jobs, Jobs sums) {
   constexpr int P = pitch<DP>(), R = tile_rows<DP>(), TILE = R * P, STAGE = 2 * TILE + 8 * R, S = DP <= 64 ? 3 : 2, SUB = R / 32;
   constexpr int DB = DP / 32, LOADS = 2 * TILE / 1024 / kWaves + 1;   // of a wave and stage
   __shared__ __attribute__((aligned(16))) uint8_t lds[S * STAGE + 128 * P];
@@ -963,9 +994,10 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
   dma_wait();
   __syncthreads();
   if (parts > 1 && (p.head_parts > 1 || w.parts > 1)) {
-    float* to = p.part + ((int64_t(z) * p.k_rows + s.ks + key) * p.KV + kvh) * p.D;
-    const int64_t all = parts * p.k_rows * p.KV * p.D;
-    if (ok)
+    const int64_t block = jobs.counted ? sums.first[b] + kb : int64_t(kb) * p.n_seqs + b;
+    float* to = p.part + (((z * p.blocks + block) * p.key_slots + 32 * wv + (lane & 31)) * p.KV + kvh) * p.D;
+    const int64_t all = parts * p.blocks * p.key_slots * p.KV * p.D;
+    if (ok && block < p.blocks)   // (more: a device table that has been overwritten)
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -993,8 +1025,8 @@ __global__ __launch_bounds__(256) void attn_sum_parts(Args p, Jobs jobs) {
   const int width = p.KV * p.D, i = (blockIdx.y * 256 + threadIdx.x) * 8, row = i / width;
   if (row >= 128 || 128 * kb + row >= s.kn) return;
   const bool v = blockIdx.z;
-  const int64_t n = p.k_rows * width, at = int64_t(s.ks + 128 * kb) * width + i;
-  const float* from = p.part + (v ? p.head_parts * p.row_parts * n : 0) + at;
+  const int64_t n = p.blocks * p.key_slots * width, at = int64_t(s.ks + 128 * kb) * width + i;
+  const float* from = p.part + (v ? p.head_parts * p.row_parts * n : 0) + int64_t(blockIdx.x) * p.key_slots * width + i;
   f32x4 x = {}, y = {};
   for (int zh = 0; zh < p.head_parts; ++zh) {
     const KeyPart w = key_part(p, s, kb, 0, (zh + 1) * p.g / p.head_parts - zh * p.g / p.head_parts);
@@ -1031,6 +1063,7 @@ constexpr double kShare = 1.5;
 struct Plan {
   int splits, dq_splits;     // of the keys, forward and for dQ
   int64_t groups;            // row tiles of all sequences and K/V heads
+  int row_slots, key_slots;  // see Parts
   int key_tiles;             // of the longest
   int64_t key_groups;        // dK and dV: workgroups
   int tile_rows, head_parts, row_parts, chunk;   // see KeyPart
@@ -1070,7 +1103,10 @@ void plan(const msd_attn& a, Plan& p) {
   const int64_t few = p.groups >= 2 * kCus ? 1 : cdiv(2 * kCus, std::max<int64_t>(p.groups, 1));
   p.splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 128))));
   p.dq_splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 256))));
+  p.row_slots = int(std::min<int64_t>(a.q_len * g, 32 * kWaves));
+  p.key_slots = std::min(a.k_len, 128);
   p.key_tiles = int(cdiv(a.k_len, 128));
+  p.blocks = count(p.sums, [&](Seq s) { return cdiv(s.kn, 128); });
   // dK and dV: parts of a key block, as many as make kShare: the heads of a group first, whose parts are alike (four heads in
   // two parts, not four: 27.2 + 5.0 us for the sum in place of 22.5 + 7.3 at 8 x 512), then the rows, as long as a part's K,
   // V and results are worth their traffic.  Sequences of different lengths: their heads are one list.
@@ -1091,10 +1127,9 @@ void plan(const msd_attn& a, Plan& p) {
   while (g % p.head_parts) ++p.head_parts;   // (parts of the heads are alike)
   const int64_t list = most * cdiv(g, p.head_parts);   // row tiles of a head part
   // (a sequence far longer than the others would have more parts than their keys' share of the workspace is worth)
-  const int64_t parts = std::max<int64_t>(32 * kCus / std::max<int64_t>(cdiv(a.k_rows, 128) * a.n_kv_heads, 1), 1);
+  const int64_t parts = std::max<int64_t>(32 * kCus / std::max<int64_t>(cdiv(p.blocks * p.key_slots, 128) * a.n_kv_heads, 1), 1);
   p.chunk = int(std::max<int64_t>({kLeast, cdiv(list, parts), std::min(list, int64_t(std::min(share, 1e9)) + 1)}));
   p.row_parts = int(std::max<int64_t>(1, cdiv(list, p.chunk)));
-  p.blocks = count(p.sums, [&](Seq s) { return cdiv(s.kn, 128); });
   if (counted)
     p.key_groups = a.n_kv_heads * count(p.keys, [&](Seq s) {
       int64_t all = 0;
@@ -1147,8 +1182,12 @@ bool bad(const void* p) { return !p || reinterpret_cast<uintptr_t>(p) % 16; }
 
 View view(const void* p, const int64_t (&s)[3]) { return {static_cast<const uint16_t*>(p), s[0], s[1], s[2]}; }
 
-Args args(const msd_attn& a, const void* q, const void* k, const void* v) {
+Args args(const msd_attn& a, const Plan& pl, const void* q, const void* k, const void* v) {
   Args p{};
+  p.groups = pl.groups;
+  p.blocks = pl.blocks;
+  p.row_slots = pl.row_slots;
+  p.key_slots = pl.key_slots;
   p.q = view(q, a.q_stride);
   p.k = view(k, a.k_stride);
   p.v = view(v, a.v_stride);
@@ -1190,9 +1229,11 @@ extern "C" int64_t msd_attn_workspace_bytes(const msd_attn* a, int32_t backward)
   Plan pl;
   const int32_t rc = check(a, false, pl);
   if (rc != MSD_OK) return rc;
-  if (!backward) return pl.splits > 1 ? 4 * pl.splits * a->q_rows * a->n_heads * (a->d_head + 1) : 0;
-  const int64_t dq = pl.dq_splits > 1 ? up(4 * pl.dq_splits * a->q_rows * a->n_heads * a->d_head) : 0;
-  const int64_t n = pl.head_parts * pl.row_parts, parts = n > 1 ? 8 * n * a->k_rows * a->n_kv_heads * a->d_head : 0;
+  const int64_t slots = pl.groups * pl.row_slots;
+  if (!backward) return pl.splits > 1 ? 4 * pl.splits * slots * (a->d_head + 1) : 0;
+  const int64_t dq = pl.dq_splits > 1 ? up(4 * pl.dq_splits * slots * a->d_head) : 0;
+  const int64_t n = pl.head_parts * pl.row_parts;
+  const int64_t parts = n > 1 ? 8 * n * pl.blocks * pl.key_slots * a->n_kv_heads * a->d_head : 0;
   return up(8 * a->q_rows * a->n_heads) + std::max(dq, parts);   // (one after the other)
 }
 
@@ -1207,7 +1248,7 @@ extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void
     return MSD_E_ARG;
   if (pl.splits > 1 && bad(workspace)) return MSD_E_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  Args p = args(*a, q, k, v);
+  Args p = args(*a, pl, q, k, v);
   p.out = static_cast<uint16_t*>(out);
   p.low = static_cast<uint8_t*>(out_low);
   p.lse = lse;
@@ -1222,7 +1263,7 @@ extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void
     const int64_t rows = int64_t(a->q_len) * a->n_heads;
     auto join = [&](auto lanes) {
       constexpr int G = decltype(lanes)::value;
-      hipLaunchKernelGGL(attn_join<G>, dim3(unsigned(cdiv(rows, 16 / G)), a->n_seqs), dim3(kJoinLanes), 0, s, p);
+      hipLaunchKernelGGL(attn_join<G>, dim3(unsigned(cdiv(rows, 16 / G)), a->n_seqs), dim3(kJoinLanes), 0, s, p, pl.rows);
     };
     if (pl.splits > 8) join(std::integral_constant<int, 16>());
     else if (pl.splits > 4) join(std::integral_constant<int, 4>());
@@ -1244,7 +1285,7 @@ extern "C" int32_t msd_attn_backward(const msd_attn* a, const void* q, const voi
     return MSD_E_ARG;
   if (bad(workspace) && (a->q_len || pl.head_parts * pl.row_parts > 1)) return MSD_E_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  Args p = args(*a, q, k, v);
+  Args p = args(*a, pl, q, k, v);
   p.dout = view(dout, a->dout_stride);
   p.o = static_cast<const uint16_t*>(out);
   p.low = static_cast<uint8_t*>(const_cast<void*>(out_low));
@@ -1262,14 +1303,14 @@ extern "C" int32_t msd_attn_backward(const msd_attn* a, const void* q, const voi
       hipLaunchKernelGGL((attn_dq<DP>), grid, dim3(64 * kWaves), 0, s, p, pl.rows);
       if (pl.dq_splits > 1)
         hipLaunchKernelGGL(attn_join_dq, dim3(unsigned(cdiv(int64_t(a->q_len) * a->n_heads * a->d_head, 2048)), a->n_seqs), dim3(256),
-                           0, s, p);
+                           0, s, p, pl.rows);
     }
     if (pl.key_groups) {
       p.tile_rows = pl.tile_rows;
       p.head_parts = pl.head_parts;
       p.row_parts = pl.row_parts;
       p.chunk = pl.chunk;
-      hipLaunchKernelGGL((attn_dkv<DP>), dim3(unsigned(pl.key_groups)), dim3(64 * kWaves), 0, s, p, pl.keys);
+      hipLaunchKernelGGL((attn_dkv<DP>), dim3(unsigned(pl.key_groups)), dim3(64 * kWaves), 0, s, p, pl.keys, pl.sums);
     }
   });
   if (pl.key_groups && pl.head_parts * pl.row_parts > 1) {
