@@ -44,8 +44,8 @@ extern "C" {
  * Limits: d_head a multiple of 8 up to 128; n_heads a multiple of n_kv_heads, up to 4096; scale in [2^-60, 2^60]; q_rows and
  * k_rows below 2^30, q_rows * n_heads and k_rows * n_kv_heads below 2^31; 128 consecutive rows of one head and the heads of
  * one group together span less than 2^30 elements; q_len times the heads of a group below 2^30 - 256; n_seqs up to 65535,
- * n_seqs * n_kv_heads below 2^20.  Beyond 256 sequences of different lengths the launch has the longest's workgroups for
- * each, of which the others' are empty: they must stay below 2^24. */
+ * n_seqs * n_kv_heads below 2^20; a launch's workgroups (of up to 256 sequences, or of more whose lengths are alike) below
+ * 2^24. */
 typedef struct msd_attn {
   int32_t n_seqs, q_len, k_len;
   int32_t n_heads, n_kv_heads, d_head;

@@ -67,3 +67,53 @@ def test_a_new_row_in_each_sequence_of_a_large_padded_batch():
     assert torch.equal(got[0][T - 1::T], v[T - 1::T].repeat_interleave(H // KV, 1))
     want = q[:1].double().reshape(KV, H // KV, D).sum(1) / T
     assert ((got[3].double() - want).abs() <= 2.0 ** -7 * q[:1].double().abs().reshape(KV, H // KV, D).sum(1) / T).all()
+
+
+# Past 256 sequences: launches of 256, and one of all that follow where their lengths are alike
+MANY = {
+    "one long": [900] + [1 + i % 40 for i in range(500)],
+    "long ones": [300 + i % 50 for i in range(300)] + [1 + 7 * i % 23 for i in range(300)],
+    "alike": [20 + i % 7 for i in range(400)],
+    "257": [400] + [3] * 256,
+    "none but one": [0] * 300 + [130] + [0] * 300,
+}
+
+
+@pytest.mark.parametrize("lens", MANY)
+@pytest.mark.parametrize("H,KV,D,causal", [(4, 1, 64, True), (2, 2, 72, False)])
+def test_many_sequences(lens, H, KV, D, causal):
+    lens = MANY[lens]
+    q, k, v, do = (_rand((sum(lens) + 3, h, D), i) for i, h in enumerate((H, KV, KV, H)))
+    ref, tol = _reference(q, k, v, do, causal, D ** -0.5, [(a, n, a, n) for a, n in zip(_starts(lens), lens)])
+    got = _grads(q, k, v, do, causal=causal, sequences=Sequences(lens))
+    _check(got, ref, tol)
+    turned = Sequences(lens)   # the shortest first, as a C caller may have them
+    turned.host = turned.host.flip(0).contiguous()
+    turned.table.copy_(turned.host)
+    _check(_grads(q, k, v, do, causal=causal, sequences=turned), ref, tol)
+
+
+def test_many_sequences_of_their_own_keys():
+    """One new row of each over caches of different lengths, a long one among them, and rows of a padded batch."""
+    k_lens = [5000] + [1 + 13 * i % 90 for i in range(400)]
+    q_lens = [1 + i % 3 for i in range(401)]
+    q, do = (_rand((sum(q_lens), 4, 64), i) for i in (1, 2))
+    k, v = (_rand((sum(k_lens), 2, 64), i) for i in (3, 4))
+    got = _grads(q, k, v, do, sequences=Sequences(q_lens, k_lens))
+    ref, tol = _reference(q, k, v, do, True, 0.125, list(zip(_starts(q_lens), q_lens, _starts(k_lens), k_lens)))
+    _check(got, ref, tol)
+
+
+def test_many_sequences_captured_and_replayed():
+    lens = MANY["one long"]
+    x = [_rand((sum(lens), h, 64), i) for i, h in enumerate((4, 2, 2, 4))]
+    seqs = Sequences(lens)
+    want = _grads(*x, sequences=seqs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _grads(*x, sequences=seqs)
+    for i in range(3):
+        graph.replay()
+        again = _grads(*x, sequences=seqs)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, out, again)), i

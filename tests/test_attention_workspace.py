@@ -45,3 +45,12 @@ def test_sizes_of_one_new_row_each():
     forward, backward, stats = workspace([1] * 16, [4096] * 16, 4096)
     assert forward == 4 * 4 * (16 * 8) * 4 * (128 + 1)   # floats, splits, workgroups, rows of a workgroup, values of a row
     assert backward == stats + forward // (128 + 1) * 128
+
+
+@pytest.mark.parametrize("lens", [[32768] + [64] * 2299, [65536] + [64] * 1099, [64] * 300 + [32768] + [64] * 2000,
+                                  [4096] * 257 + [1] * 40000, [1] * 65535], ids=len)
+def test_many_sequences_and_a_long_one(lens):
+    """Launches of as many workgroups as the sequences have, not of the longest's for each: 2300 times 1024 of 8 K/V heads each
+    would be more than a launch can hold."""
+    forward, backward, stats = workspace(lens, H=32, KV=8, D=128)
+    assert forward <= 1024 * 128 * 4 * 129 and backward - stats <= 2 ** 30

@@ -113,10 +113,11 @@ struct Seq {
 };
 
 // Which sequence a workgroup works on.  Sequences of one shape: the same number of jobs each, a sequence's in a stride of `n_seqs`
-// (the jobs of all sequences with the most work come first).  Otherwise, for up to kMostSeqs of them, the first job of each,
-// as the host has counted them (it has their lengths; 1 KB of kernel arguments); beyond that the longest's number of jobs
-// for each, of which the others' are empty: at 24 documents of 3 to 1596 rows 60, 73 and 109 us for the three kernels in
-// place of 37, 44 and 62 (with the parts of that time).
+// (the jobs of all sequences with the most work come first).  Otherwise the first job of each of up to kMostSeqs sequences, as
+// the host has counted them (it has their lengths; 1 KB of kernel arguments): the longest's number of jobs for each, of which
+// the others' are empty, takes 60, 73 and 109 us for the three kernels in place of 37, 44 and 62 at 24 documents of 3 to 1596
+// rows (with the parts of that time).  More sequences: launches of that many, and one of the longest's jobs for each from where that
+// leaves few empty (uniform_from()).
 constexpr int kMostSeqs = 256;
 struct Jobs {
   int counted;              // sequences in `first`, or 0
@@ -1060,15 +1061,23 @@ constexpr int kLeast = 16;
 // alike; larger ones are fewer first loads and sums.  With 1, 1.5 and 2, the sum included: 72, 61 and 72 us (24 documents in
 // 8191), 125, 103 and 117 (the same, heads of 128), 571, 571 and 662 (8192 rows), 128, 112 and 119 (3200 rows, heads of 128)
 constexpr double kShare = 1.5;
+
+// What a launch works on: the sequences from `first` on, with counted jobs at most kMostSeqs of them
+struct Launch {
+  int first, n, q_len, k_len;   // the longest of them
+  int row_parts;                // of the longest's row tiles
+  int64_t groups, blocks, key_groups;
+  Jobs rows, keys, sums;
+};
 struct Plan {
   int splits, dq_splits;     // of the keys, forward and for dQ
-  int64_t groups;            // row tiles of all sequences and K/V heads
+  int uniform;               // the sequences from here on are one launch of the longest's jobs for each; those before it are counted
+  int64_t groups;            // row tiles of a launch's sequences and K/V heads, at most
   int row_slots, key_slots;  // see Parts
-  int key_tiles;             // of the longest
-  int64_t key_groups;        // dK and dV: workgroups
+  int64_t key_groups;        // dK and dV: workgroups of a launch, at most
   int tile_rows, head_parts, row_parts, chunk;   // see KeyPart
-  int64_t blocks;            // of 128 keys, of all sequences
-  Jobs rows, keys, sums;
+  int64_t blocks;            // of 128 keys, of a launch's sequences, at most
+  Launch one;                // the first
 };
 
 constexpr int kCus = 256;
@@ -1080,48 +1089,116 @@ Seq host_seq(const msd_attn& a, int b) {
   return {s[0], s[1], s[2], s[3]};
 }
 
-void plan(const msd_attn& a, Plan& p) {
-  const int64_t g = a.n_heads / a.n_kv_heads, n = a.n_seqs;
-  const bool counted = a.seqs && n <= kMostSeqs;
-  // jobs of all sequences, f(sequence) each
-  auto count = [&](Jobs& jobs, auto f) {
-    jobs.counted = counted ? int(n) : 0;
-    if (!counted) return int64_t(n * f(Seq{0, a.q_len, 0, a.k_len}));
+// Jobs of a launch's sequences, f(sequence) each; how many
+template <class F>
+int64_t count(const msd_attn& a, const Plan& p, const Launch& l, Jobs& jobs, F f) {
+  jobs.counted = l.first < p.uniform ? l.n : 0;
+  if (!jobs.counted) return int64_t(l.n) * f(Seq{0, l.q_len, 0, l.k_len});
+  int64_t all = 0;
+  for (int b = 0; b < l.n; ++b) {
+    jobs.first[b] = int(std::min<int64_t>(all, INT32_MAX));
+    all += f(host_seq(a, l.first + b));
+  }
+  return all;
+}
+
+int64_t row_tiles(const msd_attn& a, int qn) { return cdiv(int64_t(qn) * (a.n_heads / a.n_kv_heads), 32 * kWaves); }
+
+void rows_and_blocks(const msd_attn& a, const Plan& p, int first, Launch& l) {
+  l.first = first;
+  l.n = first < p.uniform ? std::min(kMostSeqs, a.n_seqs - first) : a.n_seqs - first;
+  l.q_len = a.seqs ? 0 : a.q_len;
+  l.k_len = a.seqs ? 0 : a.k_len;
+  for (int b = 0; a.seqs && b < l.n; ++b) {
+    const Seq s = host_seq(a, first + b);
+    l.q_len = std::max(l.q_len, s.qn);
+    l.k_len = std::max(l.k_len, s.kn);
+  }
+  l.groups = a.n_kv_heads * count(a, p, l, l.rows, [&](Seq s) { return row_tiles(a, s.qn); });
+  l.blocks = count(a, p, l, l.sums, [&](Seq s) { return cdiv(s.kn, 128); });
+}
+
+void key_jobs(const msd_attn& a, const Plan& p, Launch& l) {
+  const int g = a.n_heads / a.n_kv_heads;
+  l.row_parts = int(std::max<int64_t>(1, cdiv(cdiv(l.q_len, p.tile_rows) * cdiv(g, p.head_parts), p.chunk)));
+  l.key_groups = a.n_kv_heads * count(a, p, l, l.keys, [&](Seq s) {
+    if (l.first >= p.uniform) return cdiv(s.kn, 128) * p.head_parts * l.row_parts;
     int64_t all = 0;
-    for (int b = 0; b < n; ++b) {
-      jobs.first[b] = int(std::min<int64_t>(all, INT32_MAX));
-      all += f(host_seq(a, b));
-    }
+    for (int z = 0, blocks = 1; z < l.row_parts && blocks; ++z)   // (fewer from part to part)
+      all += blocks = blocks_with_part(s, z, g, p.tile_rows, p.chunk, a.causal != 0);
     return all;
-  };
-  p.groups = count(p.rows, [&](Seq s) { return cdiv(s.qn * g, 32 * kWaves); }) * a.n_kv_heads;
-  // few rows: the keys are split too, into at least 128 each (dQ, whose parts are the larger share of its work: 256), until
-  // every CU has two workgroups (four: 54 + 17 us for the join in place of 44 + 8, dQ 70 + 12 in place of 58 + 7 at 2 x 512 rows
-  // against 4096 keys, 16 / 4 heads of 128; row tiles for one a CU left whole: 38 us in place of 31 + 10, dQ 44 in place
-  // of 38 + 6 at 2400 rows, but 75 in place of 59 + 12, dQ 94 in place of 77 + 11 at 3200 of heads of 128).  Without: one token against 2000 keys 47 us in place of 6.3 and 5.2 for the join, 333 rows
-  // against 1021 keys 36 in place of 13.8 and 6.9, dQ 33 in place of 16 and 5.
-  const int64_t few = p.groups >= 2 * kCus ? 1 : cdiv(2 * kCus, std::max<int64_t>(p.groups, 1));
-  p.splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 128))));
-  p.dq_splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 256))));
-  p.row_slots = int(std::min<int64_t>(a.q_len * g, 32 * kWaves));
-  p.key_slots = std::min(a.k_len, 128);
-  p.key_tiles = int(cdiv(a.k_len, 128));
-  p.blocks = count(p.sums, [&](Seq s) { return cdiv(s.kn, 128); });
-  // dK and dV: parts of a key block, as many as make kShare: the heads of a group first, whose parts are alike (four heads in
-  // two parts, not four: 27.2 + 5.0 us for the sum in place of 22.5 + 7.3 at 8 x 512), then the rows, as long as a part's K,
-  // V and results are worth their traffic.  Sequences of different lengths: their heads are one list.
-  p.tile_rows = a.d_head <= 64 ? tile_rows<64>() : tile_rows<128>();
-  const int64_t most = cdiv(a.q_len, p.tile_rows);
+  });
+}
+
+// Jobs of the longest for all sequences from `first` on are up to this many times their own jobs: one such launch then takes
+// what counted launches take (512 sequences of 16 to 1024 rows, 4.0 times: 360 us and 1350 with the gradients in place of 340 and
+// 1310; 4096 of 16 rows, once: 128 and 667 in place of 235 and 1024; one of 8192 rows before 299 of 64, 57 times: 653 and
+// 2306 in place of 186 and 831).
+constexpr int kMostEmpty = 4;
+
+int uniform_from(const msd_attn& a) {
+  if (!a.seqs) return 0;
+  int from = a.n_seqs, q_len = 0, k_len = 0;
+  int64_t jobs = 0;
+  for (int b = a.n_seqs - 1; b >= 0; --b) {
+    const Seq s = host_seq(a, b);
+    q_len = std::max(q_len, s.qn);
+    k_len = std::max(k_len, s.kn);
+    jobs += row_tiles(a, s.qn) + cdiv(s.kn, 128);
+    const int n = a.n_seqs - b;
+    if (b % kMostSeqs == 0 && n > kMostSeqs && n * (row_tiles(a, q_len) + cdiv(k_len, 128)) <= kMostEmpty * jobs) from = b;
+  }
+  return from;
+}
+
+// f(launch) of every launch of the call, from the first; p.one is the first one's before and the last one's afterwards
+template <class F>
+void launches(const msd_attn& a, Plan& p, F f) {
+  for (int first = 0; first < a.n_seqs; first += p.one.n) {
+    if (first) {
+      rows_and_blocks(a, p, first, p.one);
+      key_jobs(a, p, p.one);
+    }
+    f(p.one);
+  }
+}
+
+void plan(const msd_attn& a, Plan& p) {
+  const int64_t g = a.n_heads / a.n_kv_heads;
+  p.uniform = uniform_from(a);
+  const bool counted = p.uniform > 0;
   auto pairs = [&](Seq s) {   // rows x keys that the mask leaves, about
     const double q = s.qn, k = s.kn;
     return !a.causal ? q * k : q <= k ? q * (k - q / 2) : k * k / 2;
   };
   double all = 0;
-  if (counted) {
-    for (int b = 0; b < n; ++b) all += pairs(host_seq(a, b));
-  } else {
-    all = double(n) * pairs(Seq{0, a.q_len, 0, a.k_len});
+  p.groups = p.blocks = p.key_groups = 0;
+  rows_and_blocks(a, p, 0, p.one);
+  for (int first = 0; first < a.n_seqs; first += p.one.n) {
+    if (first) rows_and_blocks(a, p, first, p.one);
+    p.groups = std::max(p.groups, p.one.groups);
+    p.blocks = std::max(p.blocks, p.one.blocks);
+    double sum = a.seqs ? 0 : double(a.n_seqs) * pairs(Seq{0, a.q_len, 0, a.k_len});
+    for (int b = first; a.seqs && b < first + p.one.n; ++b) sum += pairs(host_seq(a, b));
+    all = std::max(all, sum);
   }
+  const bool several = p.one.first > 0;
+  // few rows: the keys are split too, into at least 128 each (dQ, whose parts are the larger share of its work: 256), until
+  // every CU has two workgroups (four: 54 + 17 us for the join in place of 44 + 8, dQ 70 + 12 in place of 58 + 7 at 2 x 512 rows
+  // against 4096 keys, 16 / 4 heads of 128; row tiles for one a CU left whole: 38 us in place of 31 + 10, dQ 44 in place
+  // of 38 + 6 at 2400 rows, but 75 in place of 59 + 12, dQ 94 in place of 77 + 11 at 3200 of heads of 128).  Without: one token
+  // against 2000 keys 47 us in place of 6.3 and 4.2 for the join, 333 rows against 1021 keys 36 in place of 13.8 and 6.9, dQ 33 in
+  // place of 16 and 5.
+  const int64_t few = p.groups >= 2 * kCus ? 1 : cdiv(2 * kCus, std::max<int64_t>(p.groups, 1));
+  p.splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 128))));
+  p.dq_splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 256))));
+  p.row_slots = int(std::min<int64_t>(a.q_len * g, 32 * kWaves));
+  p.key_slots = std::min(a.k_len, 128);
+  // dK and dV: parts of a key block, as many as make kShare: the heads of a group first, whose parts are alike (four heads in
+  // two parts, not four: 27.2 + 5.0 us for the sum in place of 22.5 + 7.3 at 8 x 512), then the rows, as long as a part's K,
+  // V and results are worth their traffic.  Sequences of different lengths: their heads are one list.
+  p.tile_rows = a.d_head <= 64 ? tile_rows<64>() : tile_rows<128>();
+  const int64_t most = cdiv(a.q_len, p.tile_rows);
   const double share = kShare * all * a.n_heads / (128.0 * p.tile_rows * 2 * kCus);
   p.head_parts = counted ? 1 : int(std::min(double(g), std::max(1.0, ceil(double(most * g) / std::max(share, kLeast / 2.0)))));
   while (g % p.head_parts) ++p.head_parts;   // (parts of the heads are alike)
@@ -1130,15 +1207,12 @@ void plan(const msd_attn& a, Plan& p) {
   const int64_t parts = std::max<int64_t>(32 * kCus / std::max<int64_t>(cdiv(p.blocks * p.key_slots, 128) * a.n_kv_heads, 1), 1);
   p.chunk = int(std::max<int64_t>({kLeast, cdiv(list, parts), std::min(list, int64_t(std::min(share, 1e9)) + 1)}));
   p.row_parts = int(std::max<int64_t>(1, cdiv(list, p.chunk)));
-  if (counted)
-    p.key_groups = a.n_kv_heads * count(p.keys, [&](Seq s) {
-      int64_t all = 0;
-      for (int z = 0; z < p.row_parts; ++z) all += blocks_with_part(s, z, int(g), p.tile_rows, p.chunk, a.causal != 0);
-      return all;
-    });
-  else {
-    p.keys.counted = 0;
-    p.key_groups = n * a.n_kv_heads * p.key_tiles * p.head_parts * p.row_parts;
+  if (several) rows_and_blocks(a, p, 0, p.one);
+  key_jobs(a, p, p.one);
+  launches(a, p, [&](const Launch& l) { p.key_groups = std::max(p.key_groups, l.key_groups); });
+  if (several) {
+    rows_and_blocks(a, p, 0, p.one);
+    key_jobs(a, p, p.one);
   }
 }
 
@@ -1184,17 +1258,11 @@ View view(const void* p, const int64_t (&s)[3]) { return {static_cast<const uint
 
 Args args(const msd_attn& a, const Plan& pl, const void* q, const void* k, const void* v) {
   Args p{};
-  p.groups = pl.groups;
-  p.blocks = pl.blocks;
   p.row_slots = pl.row_slots;
   p.key_slots = pl.key_slots;
   p.q = view(q, a.q_stride);
   p.k = view(k, a.k_stride);
   p.v = view(v, a.v_stride);
-  p.seqs = a.seqs;
-  p.n_seqs = a.n_seqs;
-  p.q_len = a.q_len;
-  p.k_len = a.k_len;
   p.H = a.n_heads;
   p.KV = a.n_kv_heads;
   p.g = a.n_heads / a.n_kv_heads;
@@ -1205,6 +1273,17 @@ Args args(const msd_attn& a, const Plan& pl, const void* q, const void* k, const
   p.c = a.scale * kLog2e;
   p.q_rows = a.q_rows;
   p.k_rows = a.k_rows;
+  return p;
+}
+
+Args args(Args p, const msd_attn& a, const Launch& l) {
+  p.seqs = a.seqs ? a.seqs + 4 * l.first : nullptr;
+  p.n_seqs = l.n;
+  p.q_len = l.q_len;
+  p.k_len = l.k_len;
+  p.groups = l.groups;
+  p.blocks = l.blocks;
+  p.row_parts = l.row_parts;
   return p;
 }
 
@@ -1254,21 +1333,23 @@ extern "C" int32_t msd_attn_forward(const msd_attn* a, const void* q, const void
   p.lse = lse;
   p.part = static_cast<float*>(workspace);
   p.splits = pl.splits;
-  const dim3 grid(unsigned(pl.groups), pl.splits);
-  with_head(a->d_head, [&](auto dp) {
-    constexpr int DP = decltype(dp)::value;
-    hipLaunchKernelGGL((attn_fwd<DP>), grid, dim3(64 * kWaves), 0, s, p, pl.rows);
-  });
-  if (pl.splits > 1) {
-    const int64_t rows = int64_t(a->q_len) * a->n_heads;
+  launches(*a, pl, [&](const Launch& l) {
+    if (!l.groups) return;
+    const Args x = args(p, *a, l);
+    with_head(a->d_head, [&](auto dp) {
+      constexpr int DP = decltype(dp)::value;
+      hipLaunchKernelGGL((attn_fwd<DP>), dim3(unsigned(l.groups), pl.splits), dim3(64 * kWaves), 0, s, x, l.rows);
+    });
+    if (pl.splits == 1) return;
+    const int64_t rows = int64_t(l.q_len) * a->n_heads;
     auto join = [&](auto lanes) {
       constexpr int G = decltype(lanes)::value;
-      hipLaunchKernelGGL(attn_join<G>, dim3(unsigned(cdiv(rows, 16 / G)), a->n_seqs), dim3(kJoinLanes), 0, s, p, pl.rows);
+      hipLaunchKernelGGL(attn_join<G>, dim3(unsigned(cdiv(rows, 16 / G)), l.n), dim3(kJoinLanes), 0, s, x, l.rows);
     };
     if (pl.splits > 8) join(std::integral_constant<int, 16>());
     else if (pl.splits > 4) join(std::integral_constant<int, 4>());
     else join(std::integral_constant<int, 1>());
-  }
+  });
   return launched();
 }
 
@@ -1295,27 +1376,27 @@ extern "C" int32_t msd_attn_backward(const msd_attn* a, const void* q, const voi
   p.dq = static_cast<uint16_t*>(dq);
   p.dk = static_cast<uint16_t*>(dk);
   p.dv = static_cast<uint16_t*>(dv);
-  with_head(a->d_head, [&](auto dp) {
-    constexpr int DP = decltype(dp)::value;
-    if (pl.groups) {
-      p.splits = pl.dq_splits;
-      const dim3 grid(unsigned(pl.groups), pl.dq_splits);
-      hipLaunchKernelGGL((attn_dq<DP>), grid, dim3(64 * kWaves), 0, s, p, pl.rows);
-      if (pl.dq_splits > 1)
-        hipLaunchKernelGGL(attn_join_dq, dim3(unsigned(cdiv(int64_t(a->q_len) * a->n_heads * a->d_head, 2048)), a->n_seqs), dim3(256),
-                           0, s, p, pl.rows);
-    }
-    if (pl.key_groups) {
-      p.tile_rows = pl.tile_rows;
-      p.head_parts = pl.head_parts;
-      p.row_parts = pl.row_parts;
-      p.chunk = pl.chunk;
-      hipLaunchKernelGGL((attn_dkv<DP>), dim3(unsigned(pl.key_groups)), dim3(64 * kWaves), 0, s, p, pl.keys, pl.sums);
+  p.splits = pl.dq_splits;
+  p.tile_rows = pl.tile_rows;
+  p.head_parts = pl.head_parts;
+  p.chunk = pl.chunk;
+  launches(*a, pl, [&](const Launch& l) {
+    const Args x = args(p, *a, l);
+    with_head(a->d_head, [&](auto dp) {
+      constexpr int DP = decltype(dp)::value;
+      if (l.groups) {
+        hipLaunchKernelGGL((attn_dq<DP>), dim3(unsigned(l.groups), pl.dq_splits), dim3(64 * kWaves), 0, s, x, l.rows);
+        if (pl.dq_splits > 1)
+          hipLaunchKernelGGL(attn_join_dq, dim3(unsigned(cdiv(int64_t(l.q_len) * a->n_heads * a->d_head, 2048)), l.n), dim3(256), 0, s, x,
+                             l.rows);
+      }
+      if (l.key_groups)
+        hipLaunchKernelGGL((attn_dkv<DP>), dim3(unsigned(l.key_groups)), dim3(64 * kWaves), 0, s, x, l.keys, l.sums);
+    });
+    if (l.key_groups && pl.head_parts * l.row_parts > 1) {
+      const int64_t slices = cdiv(128 * int64_t(a->n_kv_heads) * a->d_head, 2048);
+      hipLaunchKernelGGL(attn_sum_parts, dim3(unsigned(l.blocks), unsigned(slices), 2), dim3(256), 0, s, x, l.sums);
     }
   });
-  if (pl.key_groups && pl.head_parts * pl.row_parts > 1) {
-    const int64_t slices = cdiv(128 * int64_t(a->n_kv_heads) * a->d_head, 2048);
-    hipLaunchKernelGGL(attn_sum_parts, dim3(unsigned(pl.blocks), unsigned(slices), 2), dim3(256), 0, s, p, pl.sums);
-  }
   return launched();
 }
