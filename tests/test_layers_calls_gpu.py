@@ -1,9 +1,10 @@
 """Calls of the layer operators that their first tests leave out: saved tensors with other strides, forward-mode
-differentiation and traces."""
+differentiation and traces, and norms of so many rows that the backward's workgroups take several each."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
+from test_layers_gpu import E, ROWS_E, U, _int8, _near
 from transformer_amd.attention import attention
 from transformer_amd.norm import rms_norm
 from transformer_amd.rotary import rotary, rotary_frequencies
@@ -59,3 +60,36 @@ def test_forward_mode_and_traces_are_refused(which):
     assert all(torch.isfinite(g).all() for g in torch.autograd.grad(out, y, torch.ones_like(out)))
     with torch.no_grad():
         assert torch.equal(f(*x), want)
+
+
+@pytest.mark.parametrize("rows,d", [(8195, 100), (24591, 8), (2051, 1100), (6147, 2049), (515, 4100), (1537, 5000), (513, 16384)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("keep", [None, "int8"])
+def test_rms_norm_of_several_rows_a_group(rows, d, dtype, keep):
+    """At most 512 workgroups of 16, 4 or 1 rows (d up to 1024, 4096, 16384): past 8192, 2048 and 512 rows each takes a second and
+    third row, the last with groups that have none.  The scale's gradient then is sums of up to 4 rows a lane, 4 steps of a tree,
+    32 parts a lane and 16 lanes: 56 additions of 2^-24 each are within the 2^-18 allowed.  The other tolerances are those of
+    test_layers_gpu.py with one term more: a kept value that is off by o (a quotient between two integers, rounded to either) makes
+    dx = rstd (t - n m) + ds, m = mean(t n), differ by rstd (o m + n mean(t o) + o mean(t o)), and in short f32 rows the last
+    product counts (4e-6 of 4e-4 at 100 values)."""
+    x, r = _rand((rows, d), d, dtype) * 0.5, _rand((rows, d), d + 1, dtype) * 2
+    w = (1 + 0.2 * _rand((d,), d + 2, torch.float32)).to(dtype)
+    dy, ds = _rand((rows, d), d + 3, dtype), _rand((rows, d), d + 4, dtype)
+    leaves = [t.requires_grad_() for t in (x, w, r)]
+    y, s = rms_norm(*leaves, checkpoint=keep)
+    dx, dw, dr = torch.autograd.grad((y, s), leaves, (dy, ds))
+    assert torch.equal(dx, dr) and torch.equal(s, (x.float() + r.float()).to(dtype))
+    u, w64, t, add = U[dtype], w.detach().double(), dy.double() * w.detach().double(), ds.double()
+    rstd = 1 / (s.detach().double().square().mean(1, keepdim=True) + 1e-5).sqrt()
+    n = s.detach().double() * rstd
+    _near(y.detach(), n * w64, (u + E) * (n * w64).abs(), "y")
+    off = torch.zeros_like(n)
+    if keep:
+        n, step, tie = _int8(n)
+        off = step * tie + E * (n.abs() + step)
+    m, shift = (t * n).mean(1, keepdim=True), (t.abs() * off).mean(1, keepdim=True)
+    ref = rstd * (t - n * m) + add
+    tol = u * ref.abs() + E * (rstd * (t.abs() + n.abs() * (t * n).abs().mean(1, keepdim=True)) + add.abs())
+    _near(dx, ref, tol + rstd * (off * m.abs() + n.abs() * shift + off * shift), "dx")
+    part = dy.double() * n
+    _near(dw, part.sum(0), u * part.sum(0).abs() + ROWS_E * part.abs().sum(0) + (dy.double().abs() * off).sum(0), "dscale")
