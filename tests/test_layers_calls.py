@@ -8,6 +8,7 @@ import torch.autograd.forward_ad as fwd
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from transformer_amd import _lib
+from transformer_amd.rotary import rotary, rotary_frequencies
 
 
 def _rope(tokens=4, heads=2, d=8, rot=8):
@@ -74,3 +75,18 @@ def test_traces(which, recorded):
         torch.jit.trace(f, x, check_trace=False)
     with pytest.raises(RuntimeError, match="cannot be traced"):
         make_fx(f)(*x)
+
+
+@pytest.mark.parametrize("shape", [(2 ** 27, 1, 8), (2 ** 32 + 5, 1, 8), (2 ** 32 + 1, 3, 2, 8), (3, 2 ** 32 + 1, 2, 8), (4, 4097, 8),
+                                   (2 ** 20, 2 ** 12, 2 ** 8), (2, 2, 4104)])
+def test_more_tokens_or_heads_than_the_library_counts(shape):
+    """2^32 + 5 tokens would be 5 in 32 bits: the others' outputs would stay whatever the memory held."""
+    q = torch.zeros(1, dtype=torch.bfloat16).expand(shape)
+    with pytest.raises(ValueError, match=r"2 \*\* 27 tokens"):
+        rotary(q, None, rotary_frequencies(8, device="cpu"))
+
+
+@pytest.mark.parametrize("start", [2 ** 62 + 1, 2 ** 64 + 3, -2 ** 63])
+def test_starts_past_64_bits(start):
+    with pytest.raises(ValueError, match="start"):
+        rotary(torch.zeros(4, 2, 8), None, rotary_frequencies(8, device="cpu"), start=start)

@@ -73,7 +73,7 @@ class _Plan:
     """How calls on tensors of one layout go; ``native``: the library's arguments, where the heads are contiguous."""
 
     def __init__(self, q, k, frequencies, positions, start, layout):
-        _check(q, k, frequencies, positions, layout)
+        _check(q, k, frequencies, positions, start, layout)
         self.native = None
         if not all(x is None or x.shape[-1] == 1 or x.stride(-1) == 1 for x in (q, k)):
             return
@@ -106,11 +106,17 @@ def _plan(q, k, frequencies, positions, start, layout):
     return found
 
 
-def _check(q, k, frequencies, positions, layout):
+def _check(q, k, frequencies, positions, start, layout):
     if q.dim() not in (3, 4):
         raise ValueError(f"q (batch, tokens, heads, d_head) or (tokens, heads, d_head) expected, got {tuple(q.shape)}")
     if k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1] or k.dtype != q.dtype):
         raise ValueError(f"k must be q's tokens, d_head and type, got {tuple(k.shape)} {k.dtype} beside {tuple(q.shape)} {q.dtype}")
+    rows, heads, d = math.prod(q.shape[:-2]), q.shape[-2] + (0 if k is None else k.shape[-2]), q.shape[-1]
+    if rows >= 2 ** 27 or heads > 4096 or d > 4096 or rows * heads * d >= 2 ** 40:   # (the library takes 32-bit counts)
+        raise ValueError(f"fewer than 2 ** 27 tokens, up to 4096 heads of q and k together, heads of up to 4096 values and fewer than "
+                         f"2 ** 40 values in all expected, got {rows} tokens and {heads} heads of {d}")
+    if not -2 ** 62 <= start <= 2 ** 62:
+        raise ValueError(f"start must lie in [-2 ** 62, 2 ** 62] (got {start})")
     if q.dtype not in _lib.TYPES:
         raise ValueError("q and k must be bfloat16 or float32")
     if layout not in LAYOUTS:
