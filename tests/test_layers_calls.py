@@ -9,6 +9,7 @@ from torch.fx.experimental.proxy_tensor import make_fx
 
 from transformer_amd import _lib
 from transformer_amd.rotary import rotary, rotary_frequencies
+from transformer_amd.swiglu import swiglu
 
 
 def _rope(tokens=4, heads=2, d=8, rot=8):
@@ -90,3 +91,11 @@ def test_more_tokens_or_heads_than_the_library_counts(shape):
 def test_starts_past_64_bits(start):
     with pytest.raises(ValueError, match="start"):
         rotary(torch.zeros(4, 2, 8), None, rotary_frequencies(8, device="cpu"), start=start)
+
+
+@pytest.mark.parametrize("d", [2 ** 24, 2 ** 32 + 128])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_rows_longer_than_the_library_counts(d, checkpoint):
+    x = torch.zeros(1, dtype=torch.bfloat16).expand(2, d)
+    with pytest.raises(ValueError, match=r"2 \*\* 24"):
+        swiglu(x, x, checkpoint=checkpoint)

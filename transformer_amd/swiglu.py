@@ -46,6 +46,8 @@ def _check(gate, up, checkpoint):
     if gate.dim() < 1 or gate.shape != up.shape or gate.dtype != up.dtype or gate.shape[-1] == 0:
         raise ValueError(f"gate and up of one shape (..., d) and type expected, got {tuple(gate.shape)} {gate.dtype} and "
                          f"{tuple(up.shape)} {up.dtype}")
+    if gate.shape[-1] >= 2 ** 24:
+        raise ValueError(f"rows of up to 2 ** 24 - 1 values expected (got {gate.shape[-1]})")
     if gate.dtype not in _lib.TYPES:
         raise ValueError("gate and up must be bfloat16 or float32")
     if checkpoint not in (None, "int8"):
