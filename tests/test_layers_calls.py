@@ -99,3 +99,13 @@ def test_rows_longer_than_the_library_counts(d, checkpoint):
     x = torch.zeros(1, dtype=torch.bfloat16).expand(2, d)
     with pytest.raises(ValueError, match=r"2 \*\* 24"):
         swiglu(x, x, checkpoint=checkpoint)
+
+
+@pytest.mark.parametrize("back", [torch.zeros(4, 6).half(), torch.zeros(24), torch.zeros(6, 4), torch.zeros(4, 5),
+                                  torch.zeros(4, 6, device="meta")])
+def test_saved_tensors_that_come_back_as_others(back):
+    """The check that every backward begins with (test_layers_calls_gpu.py): anything but other strides."""
+    saved = torch.zeros(4, 6)
+    _lib.ops().restored(torch.zeros(6, 4).t(), saved)
+    with pytest.raises(RuntimeError, match="saved tensor"):
+        _lib.ops().restored(back, saved)

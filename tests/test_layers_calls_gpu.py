@@ -93,3 +93,28 @@ def test_rms_norm_of_several_rows_a_group(rows, d, dtype, keep):
     _near(dx, ref, tol + rstd * (off * m.abs() + n.abs() * shift + off * shift), "dx")
     part = dy.double() * n
     _near(dw, part.sum(0), u * part.sum(0).abs() + ROWS_E * part.abs().sum(0) + (dy.double().abs() * off).sum(0), "dscale")
+
+
+@pytest.mark.parametrize("which", range(7))
+def test_saved_tensors_that_hooks_change(which):
+    """Other types, shapes or devices raise instead of being read as what was saved; the same values elsewhere do."""
+    freq, at = rotary_frequencies(64), torch.arange(10, dtype=torch.int32, device="cuda").reshape(2, 5)
+    calls = _calls() + [(lambda q: rotary(q, None, freq, at), [_rand((2, 5, 2, 64), 1)])]
+    f, x = calls[which]
+    x = [t.detach().requires_grad_() for t in x]
+    want = torch.autograd.grad(f(*x), x, torch.ones_like(f(*x)))
+    saved = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: saved.append(t) or t, lambda t: t):
+        f(*x)
+    for i in range(len(saved)):
+        for change in (lambda t: t.cpu(), lambda t: t.reshape(-1)[:-1], lambda t: t.to(torch.float16), lambda t: t.clone(),
+                       lambda t: t[None].expand(2, *t.shape).transpose(0, -1).contiguous().transpose(0, -1)[0]):
+            n = []
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: n.append(t) or (len(n) - 1, t), lambda p: change(p[1]) if p[0] == i else p[1]):
+                out = f(*x)
+            same = (u := change(saved[i])).dtype == saved[i].dtype and u.shape == saved[i].shape and u.is_cuda
+            if same:
+                assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, x, torch.ones_like(out)), want))
+            else:
+                with pytest.raises(RuntimeError, match="saved tensor"):
+                    torch.autograd.grad(out, x, torch.ones_like(out))

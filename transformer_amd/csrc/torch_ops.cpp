@@ -61,6 +61,14 @@ struct Place {
   explicit Place(const Tensor& x) : guard(x.device()), stream(c10::hip::getCurrentHIPStream(x.get_device()).stream()) {}
 };
 
+// Hooks on saved tensors hand them back as they like: strides are taken as they come, all else has to be what was saved (the
+// kernels would read other values, or past the end).
+void restored(const Tensor& x, at::ScalarType type, at::IntArrayRef sizes, at::Device device) {
+  if (!x.defined() || x.scalar_type() != type || x.sizes() != sizes || x.device() != device)
+    throw std::runtime_error("a saved tensor has come back with another type, shape or device");
+}
+at::ScalarType scalar_type(int32_t type) { return type == MSD_F32 ? at::kFloat : at::kBFloat16; }
+
 // What a backward node returns.  Second derivatives are refused where one is asked for, not where gradients are only recorded.
 variable_list first_order(variable_list g, bool recorded) {
   if (!recorded) return g;
@@ -172,8 +180,15 @@ struct Attention : torch::autograd::Function<Attention> {
     const auto x = ctx->get_saved_variables();   // (with the strides that hooks on saved tensors have given them, if any)
     const auto capsule = ctx->saved_data["plan"].toCapsule();
     const AttnPlan& p = static_cast<const AttnPlan&>(*capsule);
-    Place on(g[0]);
     msd_attn a = p.a;
+    const auto q_sizes = g[0].sizes();
+    const int64_t dense[4] = {a.n_seqs, a.k_len, a.n_kv_heads, a.d_head}, flat[3] = {a.k_rows, a.n_kv_heads, a.d_head};
+    const auto k_sizes = g[0].dim() == 4 ? at::IntArrayRef(dense) : at::IntArrayRef(flat);
+    for (int i : {0, 3}) restored(x[i], at::kBFloat16, q_sizes, g[0].device());
+    for (int i : {1, 2}) restored(x[i], at::kBFloat16, k_sizes, g[0].device());
+    restored(x[4], at::kByte, q_sizes, g[0].device());
+    restored(x[5], at::kFloat, q_sizes.slice(0, q_sizes.size() - 1), g[0].device());
+    Place on(g[0]);
     const Tensor q = attn_operand(x[0], a.q_stride), k = attn_operand(x[1], a.k_stride), v = attn_operand(x[2], a.v_stride);
     const Tensor dout = attn_operand(g[0], a.dout_stride), out = x[3].contiguous(), low = x[4].contiguous(), lse = x[5].contiguous();
     Tensor dq = attn_output(q, p.q_zero), dk = attn_output(k, p.k_zero), dv = attn_output(v, p.k_zero), ws;
@@ -224,8 +239,12 @@ struct Rotary : torch::autograd::Function<Rotary> {
     const auto x = ctx->get_saved_variables();
     const auto capsule = ctx->saved_data["plan"].toCapsule();
     msd_rope r = static_cast<const RopePlan&>(*capsule).backward;
-    const Tensor positions = x[1];   // (hooks on saved tensors may have given them other strides)
-    if (positions.defined()) {
+    restored(x[0], at::kDouble, r.d_rot / 2, g[0].device());
+    const Tensor positions = x[1];
+    if (r.position_bytes) {
+      const int64_t sizes[2] = {r.batch, r.tokens};
+      restored(positions, r.position_bytes == 8 ? at::kLong : at::kInt,
+               at::IntArrayRef(sizes).slice(positions.defined() && positions.dim() == 2 ? 0 : 1), g[0].device());
       r.position_stride[0] = positions.dim() == 2 ? positions.stride(0) : 0;
       r.position_stride[1] = positions.stride(-1);
     }
@@ -298,9 +317,13 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     const auto s = ctx->get_saved_variables();
     const auto capsule = ctx->saved_data["plan"].toCapsule();
     const RmsPlan& p = static_cast<const RmsPlan&>(*capsule);
+    if (p.held) restored(s[0], at::kByte, p.held, g[0].device());
+    else restored(s[0], scalar_type(p.type), g[0].sizes(), g[0].device());
+    restored(s[1], scalar_type(p.scale_type), int64_t(p.d), g[0].device());
+    restored(s[2], at::kFloat, p.rows, g[0].device());
     Place on(g[0]);
-    const auto [kept, kept_stride] = p.held ? std::pair<Tensor, int64_t>{s[0], 0} : rows_of(s[0]);
-    const Tensor scale = s[1].contiguous(), rstd = s[2];
+    const auto [kept, kept_stride] = p.held ? std::pair<Tensor, int64_t>{s[0].contiguous(), 0} : rows_of(s[0]);
+    const Tensor scale = s[1].contiguous(), rstd = s[2].contiguous();
     const auto [dy, dy_stride] = rows_of(g[0]);
     const auto [ds, ds_stride] = dsum.defined() ? rows_of(dsum) : std::pair<Tensor, int64_t>{Tensor(), 0};
     Tensor dx = contiguous_like(dy), dscale, ws;
@@ -356,13 +379,16 @@ struct Swiglu : torch::autograd::Function<Swiglu> {
     const auto s = ctx->get_saved_variables();
     const auto capsule = ctx->saved_data["plan"].toCapsule();
     const GluPlan& p = static_cast<const GluPlan&>(*capsule);
+    if (p.held) restored(s[0], at::kByte, p.held, g[0].device());
+    for (size_t i = 0; !p.held && i < 2; ++i) restored(s[i], scalar_type(p.type), g[0].sizes(), g[0].device());
     Place on(g[0]);
     const std::pair<Tensor, int64_t> none;
     const auto [gate, gate_stride] = p.held ? none : rows_of(s[0]);
     const auto [up, up_stride] = p.held ? none : rows_of(s[1]);
     const auto [dy, stride] = rows_of(g[0]);
+    const Tensor held = p.held ? s[0].contiguous() : Tensor();
     Tensor dgate = contiguous_like(dy), dup = contiguous_like(dy);
-    check(msd_swiglu_backward(at_(gate), gate_stride, at_(up), up_stride, p.held ? at_(s[0]) : nullptr, at_(dy), stride, p.rows, p.d,
+    check(msd_swiglu_backward(at_(gate), gate_stride, at_(up), up_stride, p.held ? at_(held) : nullptr, at_(dy), stride, p.rows, p.d,
                               p.type, at_(dgate), at_(dup), on.stream),
           "msd_swiglu_backward");
     return first_order({dgate, dup, Tensor()}, recorded);
@@ -439,4 +465,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_norm", &rms_norm, free_threads);
   m.def("swiglu", &swiglu, free_threads);
   m.def("row_stride", &row_stride);
+  m.def("restored", [](const Tensor& x, const Tensor& saved) { restored(x, saved.scalar_type(), saved.sizes(), saved.device()); });
 }
