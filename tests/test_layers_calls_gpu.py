@@ -118,3 +118,17 @@ def test_saved_tensors_that_hooks_change(which):
             else:
                 with pytest.raises(RuntimeError, match="saved tensor"):
                     torch.autograd.grad(out, x, torch.ones_like(out))
+
+
+@pytest.mark.parametrize("which", range(7))
+def test_inside_a_compiled_function(which):
+    """torch.compile breaks its graph at the calls and runs them, with their gradients."""
+    at = torch.arange(10, dtype=torch.int32, device="cuda").reshape(2, 5)
+    f, x = (_calls() + [(lambda q: rotary(q, None, rotary_frequencies(64), at, layout="interleaved"), [_rand((2, 5, 2, 64), 1)])])[which]
+    got = []
+    torch._dynamo.reset()
+    for g in (f, torch.compile(f, backend="eager")):
+        leaves = [t.clone().requires_grad_() for t in x]
+        y = g(*[t * 2 for t in leaves])
+        got.append([y, *torch.autograd.grad(y, leaves, torch.ones_like(y))])
+    assert all(torch.equal(a, b) for a, b in zip(*got))

@@ -69,6 +69,10 @@ def _strides(x):
     return s if len(s) == 3 else (0, *s)
 
 
+def _set(struct, name, values):
+    getattr(struct, name)[:] = values   # (by name: torch.compile, which runs these lines itself, cannot assign to struct.name[:])
+
+
 class _Plan:
     """How calls on tensors of one layout go; ``native``: the library's arguments, where the heads are contiguous."""
 
@@ -85,8 +89,9 @@ class _Plan:
             r_.interleaved, r_.type, r_.sign, r_.amplitude, r_.start = LAYOUTS[layout], _lib.TYPES[q.dtype], sign, frequencies.amplitude, start
             if positions is not None:
                 r_.position_bytes = positions.element_size()
-                r_.position_stride[:] = positions.stride() if positions.dim() == 2 else (0, *positions.stride())
-        r[0].q_stride[:], r[0].k_stride[:] = _strides(q), (0, 0, 0) if k is None else _strides(k)
+                _set(r_, "position_stride", positions.stride() if positions.dim() == 2 else (0, *positions.stride()))
+        _set(r[0], "q_stride", _strides(q))
+        _set(r[0], "k_stride", (0, 0, 0) if k is None else _strides(k))
         self.native = _lib.ops().RopePlan(*map(ctypes.addressof, r))
 
 
