@@ -39,7 +39,7 @@ extern "C" {
  * fastest.
  *
  * causal: query i of a sequence sees keys 0 .. k_len - q_len + i (the last query sees the last key).  A query that
- * sees nothing has output 0 and contributes to no gradient.
+ * sees nothing has output 0 and, where its dout is finite, contributes to no gradient.
  *
  * Limits: d_head a multiple of 8 up to 128; n_heads a multiple of n_kv_heads, up to 4096; scale in [2^-60, 2^60]; q_rows and
  * k_rows below 2^30, q_rows * n_heads and k_rows * n_kv_heads below 2^31; 128 consecutive rows of one head and the heads of

@@ -162,7 +162,8 @@ def attention(q, k, v, causal=True, scale=None, sequences=None):
     A query that sees nothing has output 0.  ``scale`` defaults to d_head ** -0.5.  Returns q's shape, contiguous.
 
     What lies behind a sequence's own rows is not read.  Within a sequence, a key or value row that is not finite
-    reaches every query that sees it, and may reach those that do not."""
+    reaches every query that sees it, and may reach those that do not; a row of the incoming gradient likewise the
+    gradients of keys and values (a masked probability is a zero that is multiplied)."""
     scale = q.shape[-1] ** -0.5 if scale is None and q.dim() and q.shape[-1] else float(scale or 0)
     plan = _plan(q, k, v, bool(causal), scale, sequences)
     if plan.native is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:

@@ -819,7 +819,8 @@ struct RowStream {
 // place of 675 at the long case, as the kernel was then).  Part by part, block by block, so that whole parts start before the
 // rests of blocks (block by block: 97 us in place of 74 at 2400 rows of heads of 128).  Two workgroups a CU, so that one's
 // first loads and last stores (8 us together) are behind the other's products; eight waves a workgroup, one a CU, expose
-// them.
+// them.  Heads of 97 to 128 need four registers more than the 256 of two waves a SIMD: three are kept in scratch over the loop; one,
+// which the diagonal's mask takes, is read back there, where the wait for it is one for the tile on its way too.
 template <int DP>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_dkv(Args p, Jobs jobs, Jobs sums) {
   constexpr int P = pitch<DP>(), R = tile_rows<DP>(), TILE = R * P, STAGE = 2 * TILE + 8 * R, S = DP <= 64 ? 3 : 2, SUB = R / 32;
