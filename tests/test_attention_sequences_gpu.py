@@ -1,12 +1,12 @@
 """Attention over sequences that leave rows out, with few rows, whose keys and rows are split: the same bits as packed, and the
-formulas' values (tolerances: test_attention_gpu.py)."""
+formulas' values (tolerances: test_attention_gpu.py); and over a cache of a million rows a head."""
 import math
 
 import pytest
 import torch
 
 from test_attention_gpu import _check, _grads, _rand, _reference
-from transformer_amd.attention import Sequences
+from transformer_amd.attention import Sequences, _fits, attention
 
 pytestmark = pytest.mark.gpu
 
@@ -117,3 +117,30 @@ def test_many_sequences_captured_and_replayed():
         again = _grads(*x, sequences=seqs)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, out, again)), i
+
+
+def test_a_cache_of_a_million_rows_a_head_is_read_where_it_lies():
+    """(kv head, row) order, 8 heads of 128: the heads together span 2^30 elements and more, each by itself does not."""
+    rows, KV, H, D = 2 ** 20 + 16, 8, 16, 128
+    caches = [torch.empty((1, KV, rows, D), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for i, c in enumerate(caches):
+        c[:, :, :3000] = _rand((1, KV, 3000, D), i)
+    k, v = (c.transpose(1, 2)[:, :3000] for c in caches)
+    assert _fits(k.shape, k.stride(), 1) and not _fits(k.shape, k.stride(), KV)
+    q, do = _rand((1, 2, H, D), 2), _rand((1, 2, H, D), 3)
+    want = _grads(q, k.contiguous(), v.contiguous(), do)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    assert torch.equal(attention(q, k, v), want[0])
+    taken = torch.cuda.max_memory_allocated() - before
+    assert taken < k.numel() * 2, taken   # (no copy)
+    assert all(torch.equal(a, b) for a, b in zip(_grads(q, k, v, do), want))
+    whole = [c.transpose(1, 2) for c in caches]
+    for c in caches:
+        c[:, :, 3000:] = 0
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = attention(q, *whole)
+    taken = torch.cuda.max_memory_allocated() - before
+    assert taken < 100e6 and torch.isfinite(out).all()

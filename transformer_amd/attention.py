@@ -69,11 +69,12 @@ def _ranges(lens, starts, what):
     return starts, end, sum(lens)
 
 
-def _fits(shape, stride):
-    """Whether heads of these strides are contiguous, on 16-byte boundaries and within the kernels' reach."""
+def _fits(shape, stride, group):
+    """Whether heads of these strides are contiguous, on 16-byte boundaries and within the kernels' reach: 128 rows and the heads
+    that share a K/V head."""
     row, head = (s if n > 1 else 0 for n, s in zip(shape[-3:-1], stride[-3:-1]))
     return ((stride[-1] == 1 or shape[-1] == 1) and all(n <= 1 or s % 8 == 0 for n, s in zip(shape, stride[:-1]))
-            and 128 * row + shape[-2] * head < 2 ** 30)
+            and 128 * row + group * head < 2 ** 30)
 
 
 def _strides(shape, stride):
@@ -88,7 +89,8 @@ class _Plan:
 
     def __init__(self, q, k, v, causal, scale, sequences):
         _check(q, k, v, scale, sequences)
-        self.fits = tuple(_fits(x.shape, x.stride()) for x in (q, k, v))
+        group = q.shape[-2] // k.shape[-2]
+        self.fits = tuple(_fits(x.shape, x.stride(), heads) for x, heads in ((q, group), (k, 1), (v, 1)))
         self.native = self._native(q, k, v, causal, scale, sequences) if all(self.fits) else None
 
     @staticmethod

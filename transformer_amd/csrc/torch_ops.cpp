@@ -128,20 +128,20 @@ struct AttnPlan : torch::CustomClassHolder {
 };
 using Attn = c10::intrusive_ptr<AttnPlan>;
 
-// Whether x can be read where it lies: heads contiguous, on 16-byte boundaries, within reach
-bool attn_reads(const Tensor& x) {
+// Whether x can be read where it lies: heads contiguous, on 16-byte boundaries, within reach (128 rows and `group` heads)
+bool attn_reads(const Tensor& x, int64_t group) {
   if (x.is_contiguous()) return reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
   const int64_t n = x.dim();
   if (!heads_contiguous(x) || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16) return false;
   for (int64_t i = 0; i + 1 < n; ++i)
     if (x.size(i) > 1 && x.stride(i) % 8) return false;
   const int64_t row = x.size(n - 3) > 1 ? x.stride(n - 3) : 0, head = x.size(n - 2) > 1 ? x.stride(n - 2) : 0;
-  return 128 * row + x.size(n - 2) * head < int64_t(1) << 30;
+  return 128 * row + group * head < int64_t(1) << 30;
 }
 
 // x, or a copy that can be read, and its strides
-Tensor attn_operand(const Tensor& x, int64_t (&s)[3]) {
-  const Tensor y = attn_reads(x) ? x : x.clone(at::MemoryFormat::Contiguous);
+Tensor attn_operand(const Tensor& x, int64_t group, int64_t (&s)[3]) {
+  const Tensor y = attn_reads(x, group) ? x : x.clone(at::MemoryFormat::Contiguous);
   head_strides(y, s);
   return y;
 }
@@ -189,8 +189,9 @@ struct Attention : torch::autograd::Function<Attention> {
     restored(x[4], at::kByte, q_sizes, g[0].device());
     restored(x[5], at::kFloat, q_sizes.slice(0, q_sizes.size() - 1), g[0].device());
     Place on(g[0]);
-    const Tensor q = attn_operand(x[0], a.q_stride), k = attn_operand(x[1], a.k_stride), v = attn_operand(x[2], a.v_stride);
-    const Tensor dout = attn_operand(g[0], a.dout_stride), out = x[3].contiguous(), low = x[4].contiguous(), lse = x[5].contiguous();
+    const int64_t group = a.n_heads / a.n_kv_heads;
+    const Tensor q = attn_operand(x[0], group, a.q_stride), k = attn_operand(x[1], 1, a.k_stride), v = attn_operand(x[2], 1, a.v_stride);
+    const Tensor dout = attn_operand(g[0], group, a.dout_stride), out = x[3].contiguous(), low = x[4].contiguous(), lse = x[5].contiguous();
     Tensor dq = attn_output(q, p.q_zero), dk = attn_output(k, p.k_zero), dv = attn_output(v, p.k_zero), ws;
     if (p.backward_bytes) ws = bytes(q, p.backward_bytes);
     p.use_table(on.stream);
