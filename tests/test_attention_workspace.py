@@ -1,5 +1,6 @@
 """Workspaces of attention over sequences that leave rows out, on the CPU: they follow the sequences' rows, not the tensors'."""
 import ctypes
+import random
 
 import pytest
 
@@ -54,3 +55,36 @@ def test_many_sequences_and_a_long_one(lens):
     would be more than a launch can hold."""
     forward, backward, stats = workspace(lens, H=32, KV=8, D=128)
     assert forward <= 1024 * 128 * 4 * 129 and backward - stats <= 2 ** 30
+
+
+@pytest.mark.parametrize("seed", range(300))
+def test_sizes_stay_bounded(seed):
+    """Any lengths, packed: uneven and even ones, empty ones, rows without keys, few heads and many."""
+    rng = random.Random(seed)
+    n, longest = int(2 ** rng.uniform(0, 11)), 2 ** rng.uniform(1, 14)
+
+    def lens(longest):
+        power = rng.choice([1, 1, 0.1])   # (mostly short, or mostly long)
+        return [int(longest * rng.random() ** (1 / power) if power < 1 else longest ** rng.random()) * (rng.random() < 0.9) for _ in range(n)]
+
+    q_lens, k_lens = lens(longest), None if rng.random() < 0.5 else lens(2 ** rng.uniform(1, 15))
+    KV = rng.choice([1, 2, 4, 8, 32])
+    H, D = KV * rng.choice([1, 2, 4, 7, 16]), rng.choice([8, 64, 72, 128])
+    if not sum(q_lens) * H < 2 ** 31:
+        pytest.skip("more rows than the library counts")
+    forward, backward, stats = workspace(q_lens, k_lens, 0, H, KV, D, rng.randint(0, 1))
+    assert forward <= 1024 * 128 * 4 * (D + 1) and backward - stats <= 2 ** 30 + 256
+
+
+@pytest.mark.parametrize("q,k,H,KV,D", [(100000, 1000, 4096, 1, 128), (100000, 128, 512, 1, 128), (120, 120, 56, 8, 128), (1, 1, 4096, 1, 128),
+                                        (5000, 1, 4096, 4, 128), (30000, 30000, 64, 1, 128)])
+@pytest.mark.parametrize("B", [1, 3])
+@pytest.mark.parametrize("causal", [0, 1])
+def test_sizes_of_dense_batches(q, k, H, KV, D, B, causal):
+    a = _lib.MsdAttn()
+    a.n_seqs, a.q_len, a.k_len, a.q_rows, a.k_rows = B, q, k, B * q, B * k
+    a.n_heads, a.n_kv_heads, a.d_head, a.causal, a.scale = H, KV, D, causal, 0.1
+    a.q_stride[:], a.dout_stride[:] = [(q * H * D, H * D, D)] * 2
+    a.k_stride[:], a.v_stride[:] = [(k * KV * D, KV * D, D)] * 2
+    n = [_lib.check(_lib.lib().msd_attn_workspace_bytes(ctypes.byref(a), i), "workspace") for i in (0, 1)]
+    assert n[0] <= 1024 * 128 * 4 * (D + 1) and n[1] <= 8 * B * q * H + 2 ** 30 + 512

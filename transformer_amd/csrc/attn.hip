@@ -1167,7 +1167,6 @@ void launches(const msd_attn& a, Plan& p, F f) {
 void plan(const msd_attn& a, Plan& p) {
   const int64_t g = a.n_heads / a.n_kv_heads;
   p.uniform = uniform_from(a);
-  const bool counted = p.uniform > 0;
   auto pairs = [&](Seq s) {   // rows x keys that the mask leaves, about
     const double q = s.qn, k = s.kn;
     return !a.causal ? q * k : q <= k ? q * (k - q / 2) : k * k / 2;
@@ -1197,16 +1196,18 @@ void plan(const msd_attn& a, Plan& p) {
   p.key_slots = std::min(a.k_len, 128);
   // dK and dV: parts of a key block, as many as make kShare: the heads of a group first, whose parts are alike (four heads in
   // two parts, not four: 27.2 + 5.0 us for the sum in place of 22.5 + 7.3 at 8 x 512), then the rows, as long as a part's K,
-  // V and results are worth their traffic.  Sequences of different lengths: their heads are one list.
+  // V and results are worth their traffic.  Of sequences in a table the heads are one list.
   p.tile_rows = a.d_head <= 64 ? tile_rows<64>() : tile_rows<128>();
   const int64_t most = cdiv(a.q_len, p.tile_rows);
   const double share = kShare * all * a.n_heads / (128.0 * p.tile_rows * 2 * kCus);
-  p.head_parts = counted ? 1 : int(std::min(double(g), std::max(1.0, ceil(double(most * g) / std::max(share, kLeast / 2.0)))));
-  while (g % p.head_parts) ++p.head_parts;   // (parts of the heads are alike)
-  const int64_t list = most * cdiv(g, p.head_parts);   // row tiles of a head part
-  // (a sequence far longer than the others would have more parts than their keys' share of the workspace is worth)
+  // (a sequence far longer than the others, or one of few keys, would have more parts than their keys' share of the workspace is
+  // worth: up to 8192 blocks of a part and K/V head)
   const int64_t parts = std::max<int64_t>(32 * kCus / std::max<int64_t>(cdiv(p.blocks * p.key_slots, 128) * a.n_kv_heads, 1), 1);
-  p.chunk = int(std::max<int64_t>({kLeast, cdiv(list, parts), std::min(list, int64_t(std::min(share, 1e9)) + 1)}));
+  p.head_parts = a.seqs ? 1 : int(std::min(double(g), std::max(1.0, ceil(double(most * g) / std::max(share, kLeast / 2.0)))));
+  while (g % p.head_parts) ++p.head_parts;   // (parts of the heads are alike)
+  while (p.head_parts > parts || g % p.head_parts) --p.head_parts;
+  const int64_t list = most * cdiv(g, p.head_parts);   // row tiles of a head part
+  p.chunk = int(std::max<int64_t>({kLeast, cdiv(list, std::max<int64_t>(parts / p.head_parts, 1)), std::min(list, int64_t(std::min(share, 1e9)) + 1)}));
   p.row_parts = int(std::max<int64_t>(1, cdiv(list, p.chunk)));
   if (several) rows_and_blocks(a, p, 0, p.one);
   key_jobs(a, p, p.one);
