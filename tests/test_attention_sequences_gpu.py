@@ -119,6 +119,16 @@ def test_many_sequences_captured_and_replayed():
         assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, out, again)), i
 
 
+def test_host_numbers_that_change_after_the_first_call():
+    """Each call reads the numbers that its workspaces were made for."""
+    lens = [1, 1, 1, 700]
+    x = [_rand((sum(lens), h, 64), i) for i, h in enumerate((4, 2, 2, 4))]
+    seqs = Sequences(lens)
+    want = _grads(*x, sequences=seqs)
+    seqs.host[1:] = torch.tensor([3, 700, 3, 700], dtype=torch.int32)
+    assert all(torch.equal(a, b) for a, b in zip(_grads(*x, sequences=seqs), want))
+
+
 def test_a_cache_of_a_million_rows_a_head_is_read_where_it_lies():
     """(kv head, row) order, 8 heads of 128: the heads together span 2^30 elements and more, each by itself does not."""
     rows, KV, H, D = 2 ** 20 + 16, 8, 16, 128

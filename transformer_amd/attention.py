@@ -100,7 +100,8 @@ class _Plan:
             a.n_seqs, a.q_len, a.k_len = q.shape[0] if q.dim() == 4 else 1, q.shape[-3], k.shape[-3]
         else:
             a.n_seqs, a.q_len, a.k_len = sequences.n, sequences.q_longest, sequences.k_longest
-            a.seqs, a.seqs_host = sequences.table.data_ptr() or 16, sequences.host.data_ptr() or 16   # (16: nothing to read)
+            host = sequences.host.clone()   # (the plan's own: its workspaces are as large as these numbers ask)
+            a.seqs, a.seqs_host = sequences.table.data_ptr() or 16, host.data_ptr() or 16   # (16: nothing to read)
         a.q_rows, a.k_rows = math.prod(q.shape[:-2]), math.prod(k.shape[:-2])
         a.n_heads, a.n_kv_heads, a.d_head, a.causal, a.scale = q.shape[-2], k.shape[-2], q.shape[-1], causal, scale
         for name, x in (("q_stride", q), ("k_stride", k), ("v_stride", v)):
@@ -109,7 +110,7 @@ class _Plan:
         if sequences is None:
             return _lib.ops().AttnPlan(ctypes.addressof(a), *sizes, False, False, None, None, 0)
         return _lib.ops().AttnPlan(ctypes.addressof(a), *sizes, sequences.q_count != q.shape[0], sequences.k_count != k.shape[0],
-                                   sequences.table, sequences.host, sequences.stream or 0)
+                                   sequences.table, host, sequences.stream or 0)
 
 
 _plans = {}   # of calls without sequences; a Sequences keeps its own (the layers of a step make the same call)
