@@ -40,10 +40,10 @@
 //   rows x keys, heads / kv, d, mask          forward        dQ             dK and dV, their parts' sum
 //   8192 x 8192, 16 / 4, 128, causal          318-352 (865)  403-440 (1020) 542-579 (1014), 24     clocks fall to 2.0 GHz
 //   4096 x 4096, 32 / 32, 64, none            180 (763)      221 (933)      273 (1007)
-//   24 documents in 8191, 16 / 4, 64, causal  37             44             54, 7.5
-//   8 x 512 x 512, 16 / 4, 64, causal         15.9           19.0           22.3, 7.3
-//   3 x 333 x 1021, 6 / 2, 96, none           13.8, 6.9 join 16.1, 5.3 join 20.0, 4.9
-//   4 x 1 x 2000, 16 / 4, 64                  6.3, 5.2 join
+//   24 documents in 8191, 16 / 4, 64, causal  38             45             54, 8.0
+//   8 x 512 x 512, 16 / 4, 64, causal         16.7           19.8           22.6, 7.4
+//   3 x 333 x 1021, 6 / 2, 96, none           13.2, 7.3 join 15.8, 4.2 join 20.0, 4.9
+//   4 x 1 x 2000, 16 / 4, 64                  6.2, 4.4 join
 // At d_head 64 the exponentials and the other vector work fill half of the issue slots beside the products (matrix cores
 // busy 56 % of attn_dkv's time, vector units 51 %).
 #include <hip/hip_runtime.h>
@@ -1187,8 +1187,8 @@ void plan(const msd_attn& a, Plan& p) {
   // every CU has two workgroups (four: 54 + 17 us for the join in place of 44 + 8, dQ 70 + 12 in place of 58 + 7 at 2 x 512 rows
   // against 4096 keys, 16 / 4 heads of 128; row tiles for one a CU left whole: 38 us in place of 31 + 10, dQ 44 in place
   // of 38 + 6 at 2400 rows, but 75 in place of 59 + 12, dQ 94 in place of 77 + 11 at 3200 of heads of 128).  Without: one token
-  // against 2000 keys 47 us in place of 6.3 and 4.2 for the join, 333 rows against 1021 keys 36 in place of 13.8 and 6.9, dQ 33 in
-  // place of 16 and 5.
+  // against 2000 keys 47 us in place of 6.2 and 4.4 for the join, 333 rows against 1021 keys 36 in place of 13 and 7, dQ 33 in
+  // place of 16 and 4.
   const int64_t few = p.groups >= 2 * kCus ? 1 : cdiv(2 * kCus, std::max<int64_t>(p.groups, 1));
   p.splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 128))));
   p.dq_splits = int(std::max<int64_t>(1, std::min(few, cdiv(a.k_len, 256))));
