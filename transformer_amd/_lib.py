@@ -31,7 +31,8 @@ EXPORTS = ("msd_packed_weight_elems", "msd_workspace_bytes", "msd_default_workgr
            "msd_xent_targets", "msd_xent_forward", "msd_xent_backward",
            "msd_attn_workspace_bytes", "msd_attn_forward", "msd_attn_backward", "msd_rope_apply",
            "msd_checkpoint_bytes", "msd_rms_forward", "msd_rms_workspace_bytes", "msd_rms_backward",
-           "msd_swiglu_forward", "msd_swiglu_backward")
+           "msd_swiglu_forward", "msd_swiglu_backward", "msd_paged_plan", "msd_paged_append",
+           "msd_paged_attn_workspace_bytes", "msd_paged_attn", "msd_paged_evict_workspace_bytes", "msd_paged_evict")
 
 # Paths of the library (bits of msd_config_support)
 PATHS = {"decode": 1, "prefill": 2, "verify": 4, "batched": 8, "sample": 16, "batched_step": 32}
@@ -61,6 +62,13 @@ class MsdRope(ctypes.Structure):
                                               "type", "sign", "position_bytes")]
     _fields_ += [("amplitude", ctypes.c_float), ("start", ctypes.c_int64), ("q_stride", ctypes.c_int64 * 3),
                  ("k_stride", ctypes.c_int64 * 3), ("position_stride", ctypes.c_int64 * 2)]
+
+
+class MsdPaged(ctypes.Structure):
+    """One call on the paged cache (include/mspaged.h): q_stride is (row, head), k_stride and v_stride (head, position)."""
+    _fields_ = [("d_head", ctypes.c_int32), ("scale", ctypes.c_float), ("q_rows", ctypes.c_int64), ("positions", ctypes.c_int64)]
+    _fields_ += [(k, ctypes.c_int64 * 2) for k in ("q_stride", "k_stride", "v_stride")]
+    _fields_ += [("plan", ctypes.c_void_p), ("plan_host", ctypes.c_void_p)]
 
 
 class MsdError(RuntimeError):
@@ -174,6 +182,19 @@ def lib():
     L.msd_swiglu_forward.restype = I32
     L.msd_swiglu_backward.argtypes = [P, I64, P, I64, P, P, I64, I64, I32, I32, P, P, P]
     L.msd_swiglu_backward.restype = I32
+    GP = ctypes.POINTER(MsdPaged)
+    L.msd_paged_plan.argtypes = [I32, P, P, I32, I32, I32, I32, P, I64]
+    L.msd_paged_plan.restype = I64
+    L.msd_paged_append.argtypes = [GP, P, P, P, P, P, P, P]
+    L.msd_paged_append.restype = I32
+    L.msd_paged_attn_workspace_bytes.argtypes = [GP, I32]
+    L.msd_paged_attn_workspace_bytes.restype = I64
+    L.msd_paged_attn.argtypes = [GP, P, P, P, P, P, I32, P, P, P]
+    L.msd_paged_attn.restype = I32
+    L.msd_paged_evict_workspace_bytes.argtypes = [GP, I32, I32]
+    L.msd_paged_evict_workspace_bytes.restype = I64
+    L.msd_paged_evict.argtypes = [GP, I32, I64, I64, P, P, P, I32, I32, I32, P, I32, P, P, P, P]
+    L.msd_paged_evict.restype = I32
     _lib = L
     return L
 

@@ -2,7 +2,7 @@
 
 Each library is one ``hipcc -shared`` over its sources in ``csrc/``; the output
 ``.so`` sits next to this file and is what ``_lib.py`` loads.  ``_ops.so`` (host C++, the
-training-layer operators' torch calls with autograd) is built over the library.
+operators' torch calls) is built over the library.
 """
 import os
 import shutil
@@ -20,7 +20,7 @@ HIPCC_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-shared", f"--offload-arch={ARCH}"
 
 LIBS = {
     "libmsdecode.so": ["csrc/msdecode.hip", "csrc/sample.hip", "csrc/prefill.hip", "csrc/batched.hip",
-                       "csrc/xent.hip", "csrc/attn.hip", "csrc/layers.hip"],
+                       "csrc/xent.hip", "csrc/attn.hip", "csrc/layers.hip", "csrc/paged.hip"],
 }
 
 

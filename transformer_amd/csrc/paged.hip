@@ -1,0 +1,1257 @@
+// The paged cache's operators (gfx950): a step's keys and values into their pages, attention of each sequence's newest tokens
+// over its pages with or without the weight that each position receives, and eviction.
+//
+// Reference: model.py:122-147 (attention), :212-215 (the cache); the paged cache itself is only described there.
+//
+// New token i of a sequence of length L with n of them stands at position L - n + i and sees positions j <= L - n + i.  With
+// c = scale log2(e), for every query head and its K/V head:
+//   P_ij = 2^(c q_i.k_j - L_i), L_i = log2 sum_j 2^(c q_i.k_j);   O_i = sum_j P_ij v_j;   W'_j = W_j + sum_i P_ij
+//
+// Work is shared out on the host (msd_paged_plan), which has the lengths: lists of jobs that the device reads, with all that a
+// job needs beside the pages, so that no workgroup is empty and none counts sequences.  Row r of a sequence's group is position r / g,
+// head r % g (see attn.hip, whose tiles these kernels use).
+//   few rows (up to 32 of a group: a token, a few drafts): paged_few, then paged_finish where the keys are split or weights counted
+//   more (a chunk of a prompt): paged_many, paged_finish where the keys are split, paged_weights where weights are counted
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include <algorithm>
+#include <vector>
+
+#include "../../include/mspaged.h"
+#include "attn_tiles.h"
+#include "internal.h"
+
+namespace msp {
+using namespace msa;
+
+constexpr int kPage = MSD_PAGE;
+constexpr int kFewRows = 32;      // of a group: paged_few
+constexpr int kFewKeys = 32;      // keys of its tiles
+constexpr int kManyRows = 32 * kWaves;
+constexpr int32_t kMagic = 0x70616731;
+
+// Words of a plan behind the public ones: launches' sizes, then where the lists lie
+enum {
+  N_FEW = MSD_PLAN_RESERVED + 1, N_MANY, N_FEWS, N_TILES, N_MANYS, N_APPENDS, FEW_PARTS, MANY_PARTS, SCORES,
+  AT_SEQS, AT_FEW, AT_MANY, AT_FEWS, AT_TILES, AT_MANYS, AT_APPENDS, AT_TABLES, END
+};
+static_assert(END <= MSD_PLAN_HEADER, "the header's words");
+
+// A piece of a sequence's keys against 32 of its rows (few) or 128 (many): tiles t0 .. t1 of 32 or 64 keys
+struct Job {
+  int q0, n, len, seq;
+  int row0, t0, t1, slot;         // slot: where its part lies; paged_few: the lowest bit of row0 says whether it is the only one,
+};                                // the others where the sequence's scores lie; paged_many: row0 < 0: the only one, of row -row0 - 1
+struct SeqOf { int q0, n, len, zero; };
+struct Few { int q0, n, len, seq, slot, parts, scores, zero; };
+struct RowTile { int q0, n, len, seq, row0, slot, parts, tiles; };
+struct Append { int row, count, position, zero; };   // rows `row` .. to the pool's positions `position` ..
+static_assert(sizeof(Job) == 32 && sizeof(Few) == 32 && sizeof(RowTile) == 32 && sizeof(Append) == 16 && sizeof(SeqOf) == 16, "");
+
+struct Pages {
+  const uint16_t* p;
+  int64_t head, row;              // strides in elements
+};
+
+struct Args {
+  const uint16_t* q;
+  int64_t q_row, q_head;
+  Pages k, v;
+  int D, H, KV, g;
+  uint32_t g_magic;
+  int g_shift;
+  float c;
+  int64_t q_rows;
+  int n_seqs, width, longest, n_pages;
+  const int32_t* plan;
+  const int32_t* tables;
+  const Job* jobs;                // of the launch
+  int n_few, n_many;
+  uint16_t* out;
+  float *few_part, *few_lse;      // [slot][kv head][32] rows of D, logsumexps
+  float *many_part, *many_lse;    // [slot][kv head][128]
+  float* lse;                     // of every row of many, sequence by sequence, head by head, or null
+  float* scores;                  // c q.k of few rows, [sequence][kv head][row][keys up to a multiple of 32], or null
+  int64_t score_words;
+  const float* weights;
+  int weights_width;
+  float* weights_out;
+};
+
+// Scalar loads of what a plan says (it does not change while a kernel runs)
+template <class T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef const __attribute__((address_space(4))) uint32_t word;
+  T x;
+  uint32_t w[sizeof(T) / 4];
+  word* from = (word*)(uintptr_t)p;
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(T) / 4; ++i) w[i] = __builtin_amdgcn_readfirstlane(from[i]);
+  __builtin_memcpy(&x, w, sizeof(T));
+  return x;
+#else
+  return *p;
+#endif
+}
+
+__device__ __forceinline__ int pick(int i, int a, int b, int c, int d) {   // (of values: of members it would become an array in memory)
+  const int low = i & 1 ? b : a, high = i & 1 ? d : c;
+  return i & 2 ? high : low;
+}
+
+// The host has checked its own numbers; device words that have been overwritten since must not lead out of anything.
+__device__ __forceinline__ bool sound(const Args& p, int q0, int n, int len, int seq) {
+  return q0 >= 0 && n >= 0 && q0 <= p.q_rows - n && len >= n && len <= p.longest && seq >= 0 && seq < p.n_seqs;
+}
+
+__device__ __forceinline__ int tiles_of(int len, int keys) { return len / keys + (len % keys != 0); }
+
+__device__ __forceinline__ int div_g(const Args& p, int r) { return div_by(r, p.g_magic, p.g_shift); }
+
+__device__ __forceinline__ const uint16_t* row_at(const Args& p, int q0, int kvh, int pos, int of_group) {
+  return p.q + int64_t(q0 + pos) * p.q_row + int64_t(kvh * p.g + of_group) * p.q_head;
+}
+
+// A tile of R positions on its way from pages to LDS, NW waves: an instruction's rows are 8 (or 4) of one page.
+template <int DP, int R, int NW>
+struct PagedTile {
+  static constexpr int P = pitch<DP>(), C = P / 16, N = R * P / 1024 / NW, ROWS = 64 / C;   // rows of an instruction
+  static constexpr int KINDS = NW * ROWS >= kPage ? 1 : kPage / (NW * ROWS);                // of offsets: the same rows of a page
+  int row;               // of the first instruction
+  uint32_t off[KINDS];   // from the page's start
+  __device__ __forceinline__ void init(int64_t row_stride, int D, int lane, int wv) {
+    row = ROWS * wv + lane / C;
+#pragma unroll
+    for (int u = 0; u < KINDS; ++u) {
+      const int r = row + ROWS * NW * u, c = lane % C ^ swizzle<P>(r);
+      off[u] = 8 * c < D ? uint32_t(r % kPage) * uint32_t(row_stride) * 2 + 16 * c : kOutside;
+    }
+  }
+  // page(i): the tile's page i, of a head's pages at `head`; `left` of the tile's rows exist, the others are zeros
+  template <class F>
+  __device__ __forceinline__ void load(uint32_t to, int left, int wv, const uint16_t* head, int64_t row_stride, int n_pages, F page) const {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const uint32_t at = page((ROWS * wv + ROWS * NW * u) / kPage);
+      const bool there = at < uint32_t(n_pages);
+      dma(head + int64_t(there ? at : 0) * (kPage * row_stride), row + ROWS * NW * u < (there ? left : 0) ? off[u % KINDS] : kOutside,
+          to + 1024 * (wv + NW * u));
+    }
+  }
+};
+
+// LDS reads of this wave are done (their memory may be written)
+__device__ __forceinline__ void reads_done() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  wave_lds_order();
+  __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt 0
+  wave_lds_order();
+#endif
+}
+template <int N>
+__device__ __forceinline__ void landed() {
+  wave_lds_order();
+  dma_wait<N>();
+  wave_lds_order();
+}
+
+// One tile of 32 keys against 32 rows: scores, running maximum and sum, product with V.  The running maximum may lag by 2^8
+// before the sums are rescaled.
+template <int DP>
+struct Rows {
+  f32x16 o[DP / 32];
+  float m, l;
+  __device__ __forceinline__ void start() {
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) o[d] = f32x16{};
+    m = -INFINITY;
+    l = 0;
+  }
+  // s: c-scaled or raw scores of this lane's row against 16 keys
+  __device__ __forceinline__ float new_maximum(const f32x16& s, float c) {
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+    top = fmaxf(top, swap_halves(top)) * c;
+    if (__any(top > m + 8.0f)) {
+      const float mn = fmaxf(m, top), by = mn == -INFINITY ? 1.0f : exp2_hw(m - mn);
+      m = mn;
+      l *= by;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) o[d] *= by;
+    }
+    return m == -INFINITY ? 0.0f : m;
+  }
+  __device__ __forceinline__ void probabilities(f32x16& s, float c, float sub) {
+    float sum = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = exp2_hw(fmaf(s[i], c, -sub));
+      sum += s[i];
+    }
+    l += sum;
+  }
+  __device__ __forceinline__ void add(const f32x16& s, const uint8_t* V, int row0, int lane) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const bf16x8 pr = pack8(s, 8 * h);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) o[d] = mfma(cols_operand<pitch<DP>()>(V, row0 + 16 * h, d, lane), pr, o[d]);
+    }
+  }
+};
+
+template <int DP>
+__device__ __forceinline__ f32x16 scores_of(const uint8_t* K, int row0, const bf16x8 (&q)[DP / 16], int lane) {
+  f32x16 s = {};
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) s = mfma(rows_operand<pitch<DP>()>(K, row0, ks, lane), q[ks], s);
+  return s;
+}
+
+// ---- few rows ----
+// The waves of a workgroup take a job's tiles in turn, each with LDS of its own that it fills itself, so that none waits for
+// another before the end, where they are joined.
+template <int DP>
+constexpr int few_waves() { return DP <= 64 ? 4 : 2; }
+
+template <int DP>
+__global__ __launch_bounds__(64 * few_waves<DP>()) void paged_few(Args p) {
+  constexpr int P = pitch<DP>(), W = few_waves<DP>(), TILE = kFewKeys * P, OROW = DP + 4;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[W * 4 * TILE];
+  __shared__ float stats[W][2][32];
+  static_assert(4 * TILE >= 4 * 32 * OROW, "a wave's part of the output");
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = blockIdx.x % p.KV;
+  const Job j = scalar_load(p.jobs + blockIdx.x / p.KV);
+  const int R = j.n * p.g;
+  if (!sound(p, j.q0, j.n, j.len, j.seq) || R > kFewRows || j.t0 < 0 || j.t1 > tiles_of(j.len, kFewKeys) || j.slot < 0 || j.slot >= p.n_few)
+    return;
+  uint8_t* mine = lds + wv * 4 * TILE;
+  const uint32_t to = lds_address(mine);
+  const uint16_t *kb = p.k.p + kvh * p.k.head, *vb = p.v.p + kvh * p.v.head;
+  const int32_t* table = p.tables + int64_t(j.seq) * p.width;
+  PagedTile<DP, kFewKeys, 1> kt, vt;
+  kt.init(p.k.row, p.D, lane, 0);
+  vt.init(p.v.row, p.D, lane, 0);
+  constexpr int HALF = decltype(kt)::N;
+  auto load = [&](int t, int stage) {
+    const int2 pages = scalar_load(reinterpret_cast<const int2*>(table) + t);
+    const int left = j.len - t * kFewKeys;
+    auto page = [&](int i) { return pick(i, pages.x, pages.y, 0, 0); };
+    kt.load(to + stage * 2 * TILE, left, 0, kb, p.k.row, p.n_pages, page);
+    vt.load(to + stage * 2 * TILE + TILE, left, 0, vb, p.v.row, p.n_pages, page);
+  };
+  int t = j.t0 + wv;
+  if (t < j.t1) load(t, 0);
+  const int r = lane & 31, pos = div_g(p, min(r, R - 1));
+  const bool ok = r < R;
+  bf16x8 q[DP / 16];
+  row_operands<DP>(q, p.q, row_at(p, j.q0, kvh, pos, ok ? r - pos * p.g : 0) - p.q, ok, p.D, lane);
+  const int first = j.len - j.n + 1, seen = first + pos;   // keys that the first row sees, that this one sees
+  const int padded = tiles_of(j.len, kFewKeys) * kFewKeys;
+  float* scores = nullptr;
+  if (p.scores) {
+    const int64_t at = int64_t(j.row0 >> 1) * kFewKeys * p.KV + int64_t(kvh) * R * padded;
+    if (at >= 0 && at + int64_t(R) * padded <= p.score_words) scores = p.scores + at + int64_t(r) * padded + 4 * (lane >> 5);
+  }
+
+  Rows<DP> x;
+  x.start();
+  dma_wait();   // (for q, so that the compiler does not wait for all loads in the loop)
+  for (int stage = 0; t < j.t1; t += W, stage ^= 1) {
+    const uint8_t *K = mine + stage * 2 * TILE, *V = K + TILE;
+    const bool more = t + W < j.t1;
+    if (more) {
+      reads_done();
+      load(t + W, stage ^ 1);
+      landed<3 * HALF>();
+    } else {
+      landed<HALF>();
+    }
+    f32x16 s = scores_of<DP>(K, 0, q, lane);
+    const int key0 = t * kFewKeys;
+    if (key0 + kFewKeys > first) {
+      const int left = seen - key0 - 4 * (lane >> 5);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i >> 2) + (i & 3) >= left) s[i] = -INFINITY;
+    }
+    const float sub = x.new_maximum(s, p.c);
+    if (scores && ok)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<f32x4*>(scores + key0 + 8 * u) = f32x4{s[4 * u] * p.c, s[4 * u + 1] * p.c, s[4 * u + 2] * p.c, s[4 * u + 3] * p.c};
+    x.probabilities(s, p.c, sub);
+    if (more) landed<2 * HALF>();
+    else landed<0>();
+    x.add(s, V, 0, lane);
+  }
+  x.l += swap_halves(x.l);
+  // the waves' parts, joined
+  reads_done();
+  float* part = reinterpret_cast<float*>(mine);
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      *reinterpret_cast<f32x4*>(part + r * OROW + 32 * d + 8 * u + 4 * (lane >> 5)) =
+          f32x4{x.o[d][4 * u], x.o[d][4 * u + 1], x.o[d][4 * u + 2], x.o[d][4 * u + 3]};
+  if (lane < 32) {
+    stats[wv][0][r] = x.m;
+    stats[wv][1][r] = x.l;
+  }
+  __syncthreads();
+  const bool only = j.row0 & 1;
+  if (!only && !p.few_part) return;   // (overwritten device words)
+  const int64_t slot = (int64_t(j.slot) * p.KV + kvh) * kFewRows;
+  const int pieces = p.D / 4;
+  for (int i = tid; i < R * pieces; i += 64 * W) {
+    const int row = i / pieces, c = i - row * pieces;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) m = fmaxf(m, stats[w][0][row]);
+    float l = 0;
+    f32x4 o = {};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float lw = stats[w][1][row], e = lw == 0 ? 0.0f : exp2_hw(stats[w][0][row] - m);   // (a NaN sum stays one)
+      l = fmaf(e, lw, l);
+      o += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * 4 * TILE) + row * OROW + 4 * c) * e;
+    }
+    o *= l == 0 ? 0.0f : 1.0f / l;
+    if (!only) {
+      *reinterpret_cast<f32x4*>(p.few_part + (slot + row) * p.D + 4 * c) = o;
+    } else {
+      const int at = div_g(p, row);
+      *reinterpret_cast<u32x2*>(p.out + (int64_t(j.q0 + at) * p.H + kvh * p.g + row - at * p.g) * p.D + 4 * c) =
+          u32x2{pack2(o[0], o[1]), pack2(o[2], o[3])};
+    }
+    if (c == 0 && (!only || p.scores)) p.few_lse[slot + row] = l == 0 ? INFINITY : m + __log2f(l);
+  }
+}
+
+// ---- many rows ----
+// As attn.hip's forward: scores 32 keys ahead, K one tile ahead of V, three K buffers and two of V, one barrier a tile.
+template <int DP>
+__global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void paged_many(Args p) {
+  constexpr int P = pitch<DP>(), TILE = kKeys * P;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[5 * TILE];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = blockIdx.x % p.KV;
+  const Job j = scalar_load(p.jobs + blockIdx.x / p.KV);
+  const int rows = j.n * p.g, row0 = j.row0 < 0 ? -j.row0 - 1 : j.row0, tiles = tiles_of(j.len, kKeys);
+  const bool only = j.row0 < 0;
+  if (!sound(p, j.q0, j.n, j.len, j.seq) || row0 >= rows || j.t0 < 0 || j.t1 > tiles || j.slot < 0 || j.slot >= p.n_many) return;
+  const uint16_t *kb = p.k.p + kvh * p.k.head, *vb = p.v.p + kvh * p.v.head;
+  const int4* table = reinterpret_cast<const int4*>(p.tables + int64_t(j.seq) * p.width);
+  PagedTile<DP, kKeys, kWaves> kt, vt;
+  kt.init(p.k.row, p.D, lane, wv);
+  vt.init(p.v.row, p.D, lane, wv);
+  auto load_k = [&](uint8_t* to, int t, int4 pages) {
+    kt.load(lds_address(to), j.len - t * kKeys, wv, kb, p.k.row, p.n_pages, [&](int i) { return pick(i, pages.x, pages.y, pages.z, pages.w); });
+  };
+  auto load_v = [&](uint8_t* to, int t, int4 pages) {
+    vt.load(lds_address(to), j.len - t * kKeys, wv, vb, p.v.row, p.n_pages, [&](int i) { return pick(i, pages.x, pages.y, pages.z, pages.w); });
+  };
+  auto pages_of = [&](int t) { return scalar_load(table + min(t, tiles - 1)); };
+  uint8_t *k0 = lds, *k1 = lds + TILE, *k2 = lds + 2 * TILE, *v0 = lds + 3 * TILE, *v1 = lds + 4 * TILE;
+  int4 next{}, after{};   // the pages of tiles t + 1 and t + 2
+  if (j.t0 < j.t1) {
+    const int4 now = pages_of(j.t0);
+    next = pages_of(j.t0 + 1);
+    after = pages_of(j.t0 + 2);
+    load_k(k0, j.t0, now);
+    load_v(v0, j.t0, now);
+    load_k(k1, j.t0 + 1, next);
+  }
+  const int r = row0 + 32 * wv + (lane & 31), pos = div_g(p, min(r, rows - 1));
+  const bool ok = r < rows;
+  bf16x8 q[DP / 16];
+  row_operands<DP>(q, p.q, row_at(p, j.q0, kvh, pos, ok ? r - pos * p.g : 0) - p.q, ok, p.D, lane);
+  const int first = j.len - j.n + 1, seen = first + pos;
+  const int wave_full = first + div_g(p, min(row0 + 32 * wv, rows - 1)), wave_end = first + div_g(p, min(row0 + 32 * wv + 31, rows - 1));
+
+  Rows<DP> x;
+  x.start();
+  // s: the scores of 32 keys from key0, which lie from row0 of V; next: where the next 32 keys' K rows lie
+  auto step = [&](f32x16& s, f32x16& ahead, const uint8_t* V, int v_row, int key0, const uint8_t* next_k, int next_row) {
+    if (key0 + 32 > wave_full) {   // the diagonal or the end
+      const int left = seen - key0 - 4 * (lane >> 5);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i >> 2) + (i & 3) >= left) s[i] = -INFINITY;
+    }
+    const float sub = x.new_maximum(s, p.c);
+    ahead = scores_of<DP>(next_k, next_row, q, lane);
+    x.probabilities(s, p.c, sub);
+    x.add(s, V, v_row, lane);
+  };
+
+  f32x16 s0, s1;
+  dma_wait();
+  __syncthreads();
+  if (j.t0 < j.t1) s0 = scores_of<DP>(k0, 0, q, lane);
+  for (int t = j.t0; t < j.t1; ++t) {
+    if (t + 1 < j.t1) {
+      load_k(k2, t + 2, after);
+      load_v(v1, t + 1, next);
+      next = after;
+      after = pages_of(t + 3);
+    }
+    const int key0 = t * kKeys;
+    if (key0 < wave_end) {
+      step(s0, s1, v0, 0, key0, k0, 32);
+      step(s1, s0, v0, 32, key0 + 32, k1, 0);
+    }
+    uint8_t* k = k0;
+    k0 = k1;
+    k1 = k2;
+    k2 = k;
+    uint8_t* v = v0;
+    v0 = v1;
+    v1 = v;
+    dma_wait();
+    __syncthreads();
+  }
+  float l = x.l + swap_halves(x.l);
+  const float by = l == 0 ? 0.0f : 1.0f / l;   // (a NaN sum stays one)
+  const float lse = l == 0 ? INFINITY : x.m + __log2f(l);
+  if (!only) {   // a normalised part and its weight, joined by paged_finish
+    if (ok && p.many_part) {
+      const int64_t row = (int64_t(j.slot) * p.KV + kvh) * kManyRows + 32 * wv + (lane & 31);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int c = 32 * d + 8 * u + 4 * (lane >> 5);
+          if (c < p.D)
+            *reinterpret_cast<f32x4*>(p.many_part + row * p.D + c) =
+                f32x4{x.o[d][4 * u] * by, x.o[d][4 * u + 1] * by, x.o[d][4 * u + 2] * by, x.o[d][4 * u + 3] * by};
+        }
+      if (lane < 32) p.many_lse[row] = lse;
+    }
+    return;
+  }
+  if (p.lse && ok && lane < 32) p.lse[int64_t(j.q0) * p.H + int64_t(kvh * p.g + r - pos * p.g) * j.n + pos] = lse;
+  const int r0 = r - (lane & 31);
+  store_rows<DP>(lds + wv * 32 * P, x.o, by, p.D, lane, [&](int i) -> uint16_t* {
+    if (r0 + i >= rows) return nullptr;
+    const int at = div_g(p, r0 + i);
+    return p.out + (int64_t(j.q0 + at) * p.H + kvh * p.g + (r0 + i - at * p.g)) * p.D;
+  });
+}
+
+// ---- what is left ----
+// Workgroups, in this order: 32 rows of a row tile of many; the rows of a sequence of few; 1024 positions' weights of such.
+constexpr int kFinish = 256, kWeightKeys = 4 * kFinish;
+
+// Rows `rows` (up to 32) from their parts' normalised outputs, weighted by 2^(lse_z - lse): 16 lanes a row's 8-value
+// pieces, G of them in turn over the parts, joined through LDS in order.
+__device__ __forceinline__ void join(const Args& p, float (*lds)[11], const float* part, const float* lse, int64_t stride, int parts, int rows,
+                                     int q0, int n, int row0, int kvh, bool keep) {
+  const int tid = threadIdx.x, c = tid % 16;
+  const int G = rows >= 16 ? 1 : rows > 8 ? 1 : rows > 4 ? 2 : rows > 2 ? 4 : rows > 1 ? 8 : 16;
+  const int per = 16 / G, zg = tid / 16 % G;
+  for (int first = 0; first < rows; first += per) {
+    const int row = first + tid / 16 / G;
+    const bool ok = row < rows && 8 * c < p.D;
+    float m = -INFINITY, l = 0, acc[8] = {};
+    if (ok)
+#pragma unroll 4
+      for (int z = zg; z < parts; z += G) {
+        const float x = lse[z * stride + row];
+        const float* from = part + (z * stride + row) * p.D + 8 * c;
+        const f32x4 a = *reinterpret_cast<const f32x4*>(from), b = *reinterpret_cast<const f32x4*>(from + 4);
+        if (x == INFINITY) continue;   // nothing seen in this part
+        const float mn = fmaxf(m, x), old = exp2_hw(m - mn), e = exp2_hw(x - mn);   // (a NaN stays one through e)
+        m = mn;
+        l = fmaf(l, old, e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[i] = fmaf(acc[i], old, e * a[i]);
+          acc[4 + i] = fmaf(acc[4 + i], old, e * b[i]);
+        }
+      }
+    __syncthreads();
+    lds[tid][0] = m;
+    lds[tid][1] = l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lds[tid][2 + i] = acc[i];
+    __syncthreads();
+    if (zg || !ok) continue;
+    m = -INFINITY;
+    for (int g = 0; g < G; ++g) m = fmaxf(m, lds[tid + 16 * g][0]);
+    l = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = 0;
+    for (int g = 0; g < G; ++g) {
+      const float* x = lds[tid + 16 * g];
+      const float e = x[1] == 0 ? 0.0f : exp2_hw(x[0] - m);
+      l = fmaf(e, x[1], l);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = fmaf(e, x[2 + i], acc[i]);
+    }
+    const float by = l == 0 ? 0.0f : 1.0f / l;
+    u32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = pack2(acc[2 * i] * by, acc[2 * i + 1] * by);
+    const int pos = div_g(p, row0 + row), head = kvh * p.g + row0 + row - pos * p.g;
+    *reinterpret_cast<u32x4*>(p.out + (int64_t(q0 + pos) * p.H + head) * p.D + 8 * c) = x;
+    if (keep && c == 0) p.lse[int64_t(q0) * p.H + int64_t(head) * n + pos] = l == 0 ? INFINITY : m + __log2f(l);
+  }
+}
+
+__global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* tiles, int n_tiles, const Few* fews, int n_fews) {
+  __shared__ float lds[kFinish][11];
+  __shared__ float row_lse[kFewRows];
+  const int tid = threadIdx.x;
+  int64_t id = blockIdx.x;
+  if (id < int64_t(n_tiles) * p.KV * kWaves) {
+    const int kvh = id % p.KV, sub = id / p.KV % kWaves;
+    const RowTile t = scalar_load(tiles + id / p.KV / kWaves);
+    const int rows = min(t.n * p.g - t.row0 - 32 * sub, 32);
+    if (!sound(p, t.q0, t.n, t.len, t.seq) || t.row0 < 0 || rows <= 0 || t.parts < 2 || t.slot < 0 || t.slot > p.n_many - t.parts) return;
+    const int64_t at = (int64_t(t.slot) * p.KV + kvh) * kManyRows + 32 * sub;
+    join(p, lds, p.many_part + at * p.D, p.many_lse + at, int64_t(p.KV) * kManyRows, t.parts, rows, t.q0, t.n, t.row0 + 32 * sub, kvh, p.lse);
+    return;
+  }
+  id -= int64_t(n_tiles) * p.KV * kWaves;
+  const bool weigh = id >= int64_t(n_fews) * p.KV;
+  if (weigh) id -= int64_t(n_fews) * p.KV;
+  const int kvh = id % p.KV;
+  const Few f = scalar_load(fews + id / p.KV % n_fews);
+  const int R = f.n * p.g;
+  if (!sound(p, f.q0, f.n, f.len, f.seq) || R > kFewRows || f.parts < 0 || f.slot < 0 || f.slot > p.n_few - f.parts) return;
+  const int64_t at = (int64_t(f.slot) * p.KV + kvh) * kFewRows, stride = int64_t(p.KV) * kFewRows;
+  if (!weigh) {
+    if (f.parts > 1) join(p, lds, p.few_part + at * p.D, p.few_lse + at, stride, f.parts, R, f.q0, f.n, 0, kvh, false);
+    return;
+  }
+  // the rows' logsumexps, from their parts': eight lanes a row
+  {
+    const int row = tid / 8;
+    float m = -INFINITY, l = 0;
+    if (row < R)
+      for (int z = tid % 8; z < f.parts; z += 8) {
+        const float x = p.few_lse[at + z * stride + row];
+        if (x == INFINITY) continue;
+        const float mn = fmaxf(m, x);
+        l = fmaf(l, exp2_hw(m - mn), exp2_hw(x - mn));
+        m = mn;
+      }
+#pragma unroll
+    for (int w = 1; w < 8; w *= 2) {
+      const float m2 = __shfl_xor(m, w), l2 = __shfl_xor(l, w), mn = fmaxf(m, m2);
+      l = (l == 0 ? 0.0f : l * exp2_hw(m - mn)) + (l2 == 0 ? 0.0f : l2 * exp2_hw(m2 - mn));
+      m = mn;
+    }
+    if (row < kFewRows && tid % 8 == 0) row_lse[row] = l == 0 ? INFINITY : m + __log2f(l);
+  }
+  __syncthreads();
+  const int key = int(id / p.KV / n_fews) * kWeightKeys + 4 * tid;
+  if (key >= p.longest) return;
+  const int padded = tiles_of(f.len, kFewKeys) * kFewKeys;
+  float w[4] = {};
+  if (key < f.len) {
+    const int64_t row = int64_t(f.seq) * p.KV + kvh;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (key + i < f.len - f.n && key + i < p.weights_width) w[i] = p.weights[row * p.weights_width + key + i];
+    const int64_t base = int64_t(f.scores) * kFewKeys * p.KV + int64_t(kvh) * R * padded;
+    if (base >= 0 && base + int64_t(R) * padded <= p.score_words) {
+      f32x4 sum = {};
+#pragma unroll 4
+      for (int r = 0; r < R; ++r) {
+        const f32x4 s = *reinterpret_cast<const f32x4*>(p.scores + base + int64_t(r) * padded + key);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += exp2_hw(s[i] - row_lse[r]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (key + i < f.len) w[i] += sum[i];
+    }
+  }
+  float* out = p.weights_out + (int64_t(f.seq) * p.KV + kvh) * p.longest + key;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (key + i < p.longest) out[i] = w[i];
+}
+
+// ---- the weights of many rows ----
+// 128 keys a workgroup, 32 a wave in registers, over the group's heads and the rows that see them: S = Q K^T, a lane holds one
+// key's scores against 16 rows, so that its sum stays in the lane.
+template <int DP>
+__global__ __launch_bounds__(64 * kWaves) void paged_weights(Args p, const Job* seqs, int n_seqs) {
+  constexpr int P = pitch<DP>(), R = DP <= 64 ? 64 : 32, TILE = R * P, STAGE = TILE + 256, SUB = R / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = blockIdx.x % p.KV, kb = blockIdx.x / p.KV / n_seqs;
+  const Job j = scalar_load(seqs + blockIdx.x / p.KV % n_seqs);
+  if (!sound(p, j.q0, j.n, j.len, j.seq)) return;
+  const int k0 = 128 * kb + 32 * wv, key = k0 + (lane & 31);
+  float sum = 0;
+  if (128 * kb < j.len) {
+    const uint16_t* kbase = p.k.p + kvh * p.k.head;
+    const int page = key < j.len ? p.tables[int64_t(j.seq) * p.width + key / kPage] : -1;
+    bf16x8 k[DP / 16];
+    row_operands<DP>(k, kbase, (int64_t(page) * kPage + key % kPage) * p.k.row, uint32_t(page) < uint32_t(p.n_pages), p.D, lane);
+    const int pos0 = max(128 * kb - (j.len - j.n), 0) / R * R, n = (j.n - pos0 + R - 1) / R, all = n * p.g;   // row tiles a head, of the group
+    Tile<DP, R> qt;
+    qt.init(p.q_row, p.D, lane, wv);
+    const uint16_t* q0 = p.q + int64_t(j.q0) * p.q_row + int64_t(kvh * p.g) * p.q_head;
+    const float* l0 = p.lse + int64_t(j.q0) * p.H + int64_t(kvh * p.g) * j.n;
+    auto load = [&](int i, int stage) {
+      const int head = i / n, pos = pos0 + (i - head * n) * R, left = j.n - pos;
+      uint8_t* to = lds + stage * STAGE;
+      qt.load(to, q0 + int64_t(pos) * p.q_row + int64_t(head) * p.q_head, left, wv);
+      if (wv == 0) dma4(l0 + int64_t(head) * j.n + pos, lane < min(left, R) ? 4 * lane : kOutside, lds_address(to + TILE));
+    };
+    load(0, 0);
+    for (int i = 0; i < all; ++i) {
+      dma_wait();
+      __syncthreads();
+      if (i + 1 < all) load(i + 1, (i + 1) & 1);
+      const uint8_t* Q = lds + (i & 1) * STAGE;
+      const float* lse = reinterpret_cast<const float*>(Q + TILE);
+      const int pos = pos0 + i % n * R;
+#pragma unroll
+      for (int a = 0; a < SUB; ++a) {
+        f32x16 s = {};
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) s = mfma(rows_operand<P>(Q, 32 * a, ks, lane), k[ks], s);
+        const int row = pos + 32 * a + 4 * (lane >> 5);
+        if (j.len - j.n + pos + 32 * a < k0 + 31 || pos + 32 * a + 32 > j.n) {   // the diagonal, the last rows
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int at = row + 8 * (v >> 2) + (v & 3);
+            if (at >= j.n || key > j.len - j.n + at) s[v] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const f32x4 l = *reinterpret_cast<const f32x4*>(lse + 32 * a + 8 * u + 4 * (lane >> 5));
+#pragma unroll
+          for (int v = 0; v < 4; ++v) sum += exp2_hw(fmaf(s[4 * u + v], p.c, -l[v]));
+        }
+      }
+    }
+  }
+  sum += swap_halves(sum);
+  if (lane >= 32 || key >= p.longest) return;
+  const int64_t row = int64_t(j.seq) * p.KV + kvh;
+  float w = 0;
+  if (key < j.len) w = (key < j.len - j.n && key < p.weights_width ? p.weights[row * p.weights_width + key] : 0.0f) + sum;
+  p.weights_out[row * p.longest + key] = w;
+}
+
+// ---- append ----
+struct AppendArgs {
+  const uint16_t *k_new, *v_new;
+  int64_t k_new_row, k_new_head, v_new_row, v_new_head;
+  uint16_t *k, *v;
+  int64_t k_head, k_row, v_head, v_row;
+  const Append* jobs;
+  int KV, pieces;      // 16-byte pieces of a head
+  int64_t q_rows, positions;
+};
+
+// The rows of one page and sequence: memory bound, a head's rows one behind the other as the pool's layout has them.
+__global__ __launch_bounds__(256) void paged_append(AppendArgs p) {
+  const Append a = scalar_load(p.jobs + blockIdx.x);
+  if (a.row < 0 || a.count <= 0 || a.count > kPage || a.row > p.q_rows - a.count || a.position < 0 || a.position > p.positions - a.count)
+    return;
+  const int head_pieces = a.count * p.pieces, all = p.KV * head_pieces;
+  for (int i = threadIdx.x; i < 2 * all; i += 256) {
+    const bool value = i >= all;
+    const int at = value ? i - all : i, head = at / head_pieces, in = at - head * head_pieces, r = in / p.pieces, c = in - r * p.pieces;
+    const uint16_t* from = value ? p.v_new + (a.row + r) * p.v_new_row + head * p.v_new_head : p.k_new + (a.row + r) * p.k_new_row + head * p.k_new_head;
+    uint16_t* to = value ? p.v + (a.position + r) * p.v_row + head * p.v_head : p.k + (a.position + r) * p.k_row + head * p.k_head;
+    *reinterpret_cast<u32x4*>(to + 8 * c) = *reinterpret_cast<const u32x4*>(from + 8 * c);
+  }
+}
+
+// ---- eviction ----
+struct EvictArgs {
+  uint16_t *k, *v;
+  int64_t k_layer, k_head, k_row, v_layer, v_head, v_row;
+  const float* weights;
+  int weights_width, keep, recent;
+  const SeqOf* seqs;
+  const int32_t *tables, *to;
+  int width, to_width, n_pages, longest;
+  int n_seqs, KV, pieces;
+  float* weights_out;
+  int32_t *kept, *source;      // source: the pool's positions of the kept rows, or -1
+};
+
+// Weights in the order of eviction as unsigned numbers: larger is kept first; -0 is 0, a NaN the largest.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(x == 0 ? 0.0f : x);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// The kept positions of one sequence, layer and head: the key of the least kept weight by four passes of 8 bits over the
+// candidates (counts in LDS, one set a wave), then the kept positions in order, by counts of those before each.
+template <int T>
+__global__ __launch_bounds__(T) void paged_select(EvictArgs p) {
+  constexpr int W = T / 64;
+  __shared__ uint32_t counts[W][256];
+  __shared__ uint32_t state[4];    // key so far, how many are still to be taken
+  __shared__ uint32_t sums[W][2];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, s = blockIdx.y, kvh = blockIdx.x % p.KV;
+  const SeqOf q = scalar_load(p.seqs + s);
+  const int64_t row = (int64_t(blockIdx.x / p.KV) * p.n_seqs + s) * p.KV + kvh;
+  const int len = q.len < 0 || q.len > p.longest ? 0 : q.len, held = min(len, p.keep);
+  const int old = len - min(p.recent, len), heavy = held - (len - old);   // candidates, how many of them stay
+  const float* w = p.weights + row * p.weights_width;
+  auto key_of = [&](int j) { return order_of(j < p.weights_width ? w[j] : 0.0f); };
+  uint32_t key = 0, need = heavy;
+  if (heavy > 0 && heavy < old) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (int i = tid; i < W * 256; i += T) (&counts[0][0])[i] = 0;
+      __syncthreads();
+      for (int j = tid; j < old; j += T) {
+        const uint32_t x = key_of(j);
+        if (shift == 24 || x >> (shift + 8) == key >> (shift + 8)) atomicAdd(&counts[wv][x >> shift & 255], 1u);
+      }
+      __syncthreads();
+      for (int i = tid; i < 256; i += T) {
+        uint32_t n = 0;
+        for (int v = 0; v < W; ++v) n += counts[v][i];
+        counts[0][i] = n;
+      }
+      __syncthreads();
+      if (wv == 0) {   // from the largest digit down: lane l has digits 255 - 4 l .. 252 - 4 l
+        uint32_t n[4], mine = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine += n[i] = counts[0][255 - 4 * lane - i];
+        uint32_t before = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const uint32_t x = __shfl_up(before, d);
+          if (lane >= d) before += x;
+        }
+        before -= mine;
+        if (before < need && before + mine >= need) {
+          int i = 0;
+          while (before + n[i] < need) before += n[i++];
+          state[0] = key | uint32_t(255 - 4 * lane - i) << shift;
+          state[1] = need - before;
+        }
+      }
+      __syncthreads();
+      key = state[0];
+      need = state[1];
+      __syncthreads();
+    }
+  }
+  // keys above `key` stay, and the first `need` of those equal to it
+  const bool all = heavy >= old;
+  const int32_t* table = p.tables + int64_t(s) * p.width;
+  uint32_t n_kept = 0, n_equal = 0;   // before this round
+  for (int j0 = 0; j0 < len; j0 += T) {
+    const int j = j0 + tid;
+    bool above = false, equal = false;
+    float weight = 0;
+    if (j < len) {
+      weight = j < p.weights_width ? w[j] : 0.0f;
+      const uint32_t x = order_of(weight);
+      above = j >= old || all || (heavy > 0 && x > key);
+      equal = !above && heavy > 0 && x == key;
+    }
+    const uint64_t below = (uint64_t(1) << lane) - 1, ea = __ballot(equal);
+    if (lane == 0) sums[wv][0] = __popcll(ea);
+    __syncthreads();
+    uint32_t rank = n_equal + __popcll(ea & below), equals = 0;
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+      const uint32_t x = sums[v][0];
+      equals += x;
+      if (v < wv) rank += x;
+    }
+    const bool stays = above || (equal && rank < need);
+    const uint64_t ka = __ballot(stays);
+    if (lane == 0) sums[wv][1] = __popcll(ka);
+    __syncthreads();
+    uint32_t at = n_kept + __popcll(ka & below), kepts = 0;
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+      const uint32_t x = sums[v][1];
+      kepts += x;
+      if (v < wv) at += x;
+    }
+    if (stays && at < uint32_t(p.keep)) {
+      const int page = table[j / kPage];
+      p.kept[row * p.keep + at] = j;
+      p.weights_out[row * p.keep + at] = weight;
+      p.source[row * p.keep + at] = uint32_t(page) < uint32_t(p.n_pages) ? page * kPage + j % kPage : -1;
+    }
+    n_kept += kepts;
+    n_equal += equals;
+  }
+  for (int i = held + tid; i < p.keep; i += T) {
+    p.kept[row * p.keep + i] = -1;
+    p.weights_out[row * p.keep + i] = 0;
+    p.source[row * p.keep + i] = -1;
+  }
+}
+
+// The kept rows to their new places: 16-byte pieces, four in flight a thread; K (blockIdx.z 0) and V.
+constexpr int kMove = 4;
+__global__ __launch_bounds__(256) void paged_move(EvictArgs p, int blocks) {
+  const int s = blockIdx.x / blocks, layer = blockIdx.y / p.KV, kvh = blockIdx.y % p.KV;
+  const bool value = blockIdx.z;
+  const int64_t row_stride = value ? p.v_row : p.k_row;
+  uint16_t* base = value ? p.v + layer * p.v_layer + kvh * p.v_head : p.k + layer * p.k_layer + kvh * p.k_head;
+  const int32_t* source = p.source + ((int64_t(layer) * p.n_seqs + s) * p.KV + kvh) * p.keep;
+  const int64_t first = int64_t(blockIdx.x % blocks) * 256 * kMove;
+  u32x4 x[kMove];
+  uint16_t* to[kMove];
+#pragma unroll
+  for (int u = 0; u < kMove; ++u) {
+    const int64_t i = first + u * 256 + threadIdx.x;
+    const int j = int(i / p.pieces), c = int(i - int64_t(j) * p.pieces);
+    to[u] = nullptr;
+    if (j >= p.keep) continue;
+    const int from = source[j], page = p.to[int64_t(s) * p.to_width + j / kPage];
+    if (from < 0 || uint32_t(page) >= uint32_t(p.n_pages)) continue;
+    x[u] = *reinterpret_cast<const u32x4*>(base + int64_t(from) * row_stride + 8 * c);
+    to[u] = base + (int64_t(page) * kPage + j % kPage) * row_stride + 8 * c;
+  }
+#pragma unroll
+  for (int u = 0; u < kMove; ++u)
+    if (to[u]) *reinterpret_cast<u32x4*>(to[u]) = x[u];
+}
+
+// ---- host: the plan ----
+// Workgroups that a launch is shared out to, about, and tiles of a job at least.
+constexpr int kFewGroups = 1024, kManyGroups = 512;
+constexpr int kFewLeast = 4, kManyLeast = 2;
+
+struct Pieces {
+  int64_t each;
+  // of a list of `tiles`: one until it has half as much again as the others' pieces
+  int of(int64_t tiles) const { return 2 * tiles <= 3 * each ? 1 : int(cdiv(tiles, each)); }
+};
+Pieces pieces(int64_t tiles, int n_kv, int groups, int least) {
+  return {std::max<int64_t>(least, cdiv(tiles * n_kv, groups))};
+}
+
+struct Writer {
+  int32_t* words;   // or null: counting
+  int64_t at = MSD_PLAN_HEADER;
+  int64_t list(int64_t n, int64_t each) {
+    const int64_t from = at;
+    at += (n * each + 3) / 4 * 4;
+    return from;
+  }
+};
+
+int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_width, int H, int KV, int longest, int32_t* words, int64_t room) {
+  if (n_seqs < 0 || n_seqs > 65535 || H <= 0 || KV <= 0 || H % KV || H > 4096 || table_width < 0 || longest < 0 ||
+      table_width > (INT32_MAX / kPage))
+    return MSD_E_CONFIG;
+  if (n_seqs && (!seqs || (table_width && !tables))) return MSD_E_ARG;
+  const int64_t g = H / KV;
+  int most = 0;
+  int64_t q_end = 0, q_count = 0;
+  std::vector<int> few, many;   // sequences
+  int64_t few_tiles = 0, many_tiles = 0, row_tiles = 0, appends = 0, scores = 0;
+  auto seen = [&](const int32_t* s, int64_t row) { return s[2] - s[1] + 1 + row / g; };   // positions that the row sees
+  for (int b = 0; b < n_seqs; ++b) {
+    const int32_t* s = seqs + 3 * b;
+    const int64_t rows = s[1] * g;
+    if (s[0] < 0 || s[1] < 0 || s[2] < s[1] || s[2] > int64_t(table_width) * kPage || (longest && s[2] > longest) || s[0] > INT32_MAX - s[1] ||
+        rows >= (1 << 30) - 256)
+      return MSD_E_CONFIG;
+    most = std::max(most, s[2]);
+    if (s[1]) q_end = std::max<int64_t>(q_end, int64_t(s[0]) + s[1]);
+    q_count += s[1];
+    if (rows <= kFewRows) {
+      few.push_back(b);
+      if (rows) few_tiles += cdiv(s[2], kFewKeys);
+      scores += rows * cdiv(longest ? longest : s[2], kFewKeys);
+    } else {
+      many.push_back(b);
+      for (int64_t r = 0; r < rows; r += kManyRows, ++row_tiles) many_tiles += cdiv(seen(s, std::min(r + kManyRows, rows) - 1), kKeys);
+    }
+    if (longest) appends += s[1] ? cdiv(s[1], kPage) + 1 : 0;
+    else if (s[1]) appends += cdiv(s[2], kPage) - (s[2] - s[1]) / kPage;
+  }
+  if (longest > int64_t(table_width) * kPage) return MSD_E_CONFIG;
+  const Pieces fp = pieces(few_tiles, KV, kFewGroups, kFewLeast), mp = pieces(many_tiles, KV, kManyGroups, kManyLeast);
+  int64_t n_few = 0, n_many = 0, few_active = 0;
+  bool few_parts = false, many_parts = false;
+  for (int b : few) {
+    if (!seqs[3 * b + 1]) continue;
+    const int n = fp.of(cdiv(seqs[3 * b + 2], kFewKeys));
+    ++few_active;
+    n_few += n;
+    few_parts |= n > 1;
+  }
+  for (int b : many)
+    for (int64_t r = 0, rows = seqs[3 * b + 1] * g; r < rows; r += kManyRows) {
+      const int n = mp.of(cdiv(seen(seqs + 3 * b, std::min(r + kManyRows, rows) - 1), kKeys));
+      n_many += n;
+      many_parts |= n > 1;
+    }
+  if (longest) {   // as many as any lengths up to it give: at most one piece more than whole ones for each list
+    n_few = few_active ? few_active + cdiv(kFewGroups, KV) : 0;
+    n_many = row_tiles ? row_tiles + cdiv(kManyGroups, KV) : 0;
+    few_parts = few_active;
+    many_parts = row_tiles;
+  }
+  const int width = int(cdiv(table_width, 4) * 4);
+  Writer w{words};
+  const int64_t at_seqs = w.list(n_seqs, 4), at_few = w.list(n_few, 8), at_many = w.list(n_many, 8), at_fews = w.list(few.size(), 8),
+                at_tiles = w.list(row_tiles, 8), at_manys = w.list(many.size(), 8), at_appends = w.list(appends, 4),
+                at_tables = w.list(n_seqs, width);
+  if (w.at >= (int64_t(1) << 28) || scores >= (int64_t(1) << 30) || (n_few + int64_t(few.size())) * KV >= (1 << 24) ||
+      (n_many + 4 * row_tiles) * KV >= (1 << 24))
+    return MSD_E_CONFIG;
+  if (!words) return w.at;
+  if (room < w.at) return MSD_E_ARG;
+  memset(words, 0, size_t(at_tables) * 4);
+  // empty jobs, of a sequence that there is not
+  for (int64_t i = 0; i < n_few; ++i) words[at_few + 8 * i + 3] = -1;
+  for (int64_t i = 0; i < n_many; ++i) words[at_many + 8 * i + 3] = -1;
+  words[MSD_PLAN_MAGIC] = kMagic;
+  words[MSD_PLAN_WORDS] = int32_t(w.at);
+  words[MSD_PLAN_SEQS] = n_seqs;
+  words[MSD_PLAN_HEADS] = H;
+  words[MSD_PLAN_KV_HEADS] = KV;
+  words[MSD_PLAN_WIDTH] = width;
+  words[MSD_PLAN_LONGEST] = longest ? longest : most;
+  words[MSD_PLAN_Q_END] = int32_t(q_end);
+  words[MSD_PLAN_Q_COUNT] = int32_t(q_count);
+  words[MSD_PLAN_RESERVED] = longest != 0;
+  words[N_FEW] = int32_t(n_few);
+  words[N_MANY] = int32_t(n_many);
+  words[N_FEWS] = int32_t(few.size());
+  words[N_TILES] = int32_t(row_tiles);
+  words[N_MANYS] = int32_t(many.size());
+  words[N_APPENDS] = int32_t(appends);
+  words[FEW_PARTS] = few_parts;
+  words[MANY_PARTS] = many_parts;
+  words[SCORES] = int32_t(scores);
+  words[AT_SEQS] = int32_t(at_seqs);
+  words[AT_FEW] = int32_t(at_few);
+  words[AT_MANY] = int32_t(at_many);
+  words[AT_FEWS] = int32_t(at_fews);
+  words[AT_TILES] = int32_t(at_tiles);
+  words[AT_MANYS] = int32_t(at_manys);
+  words[AT_APPENDS] = int32_t(at_appends);
+  words[AT_TABLES] = int32_t(at_tables);
+
+  // pages: what is behind a sequence's length is 0 on the device
+  int pages = 0;
+  for (int b = 0; b < n_seqs; ++b) {
+    int32_t* row = words + at_tables + int64_t(b) * width;
+    const int used = int(cdiv(seqs[3 * b + 2], kPage));
+    for (int i = 0; i < used; ++i) {
+      const int x = tables[int64_t(b) * table_width + i];
+      if (x < 0 || x > INT32_MAX / kPage - 1) return MSD_E_CONFIG;
+      row[i] = x;
+      pages = std::max(pages, x + 1);
+    }
+    std::fill(row + used, row + width, 0);
+  }
+  words[MSD_PLAN_PAGES] = pages;
+  std::vector<uint8_t> uses(pages, 0);   // 0, 1, more
+  for (int b = 0; b < n_seqs; ++b)
+    for (int i = 0; i < int(cdiv(seqs[3 * b + 2], kPage)); ++i) {
+      uint8_t& x = uses[words[at_tables + int64_t(b) * width + i]];
+      x = std::min(x + 1, 2);
+    }
+  bool shared = false;
+  Append* append = reinterpret_cast<Append*>(words + at_appends);
+  for (int b = 0; b < n_seqs; ++b) {
+    const int32_t *s = seqs + 3 * b, *row = words + at_tables + int64_t(b) * width;
+    memcpy(words + at_seqs + 4 * b, s, 12);
+    for (int at = s[2] - s[1]; at < s[2];) {
+      const int end = std::min(s[2], (at / kPage + 1) * kPage);
+      *append++ = {s[0] + at - (s[2] - s[1]), end - at, row[at / kPage] * kPage + at % kPage, 0};
+      shared |= uses[row[at / kPage]] > 1;
+      at = end;
+    }
+  }
+  words[MSD_PLAN_SHARED] = shared;
+
+  // jobs, the longest first
+  struct List { int64_t each; int index; };
+  std::vector<List> order;
+  Job* job = reinterpret_cast<Job*>(words + at_few);
+  Few* f = reinterpret_cast<Few*>(words + at_fews);
+  int slot = 0, score = 0;
+  for (size_t i = 0; i < few.size(); ++i) {
+    const int32_t* s = seqs + 3 * few[i];
+    const int64_t tiles = cdiv(s[2], kFewKeys);
+    const int n = s[1] ? fp.of(tiles) : 0;
+    f[i] = {s[0], s[1], s[2], few[i], slot, n, score, 0};
+    slot += n;
+    score += int(s[1] * g * cdiv(longest ? longest : s[2], kFewKeys));
+    if (n) order.push_back({cdiv(tiles, n), int(i)});
+  }
+  auto longest_first = [](const List& a, const List& b) { return a.each > b.each; };
+  std::stable_sort(order.begin(), order.end(), longest_first);
+  for (const List& o : order) {
+    const Few& x = f[o.index];
+    const int64_t tiles = cdiv(x.len, kFewKeys);
+    for (int z = 0; z < x.parts; ++z)
+      *job++ = {x.q0, x.n, x.len, x.seq, 2 * x.scores + (x.parts == 1), int(tiles * z / x.parts), int(tiles * (z + 1) / x.parts), x.slot + z};
+  }
+  order.clear();
+  job = reinterpret_cast<Job*>(words + at_many);
+  RowTile* t = reinterpret_cast<RowTile*>(words + at_tiles);
+  Job* m = reinterpret_cast<Job*>(words + at_manys);
+  slot = 0;
+  int index = 0;
+  for (int b : many) {
+    const int32_t* s = seqs + 3 * b;
+    *m++ = {s[0], s[1], s[2], b, 0, 0, 0, 0};
+    const int64_t rows = s[1] * g;
+    for (int64_t r = (rows - 1) / kManyRows * kManyRows; r >= 0; r -= kManyRows, ++index) {   // the longest of a sequence first
+      const int64_t tiles = cdiv(seen(s, std::min(r + kManyRows, rows) - 1), kKeys);
+      const int n = mp.of(tiles);
+      t[index] = {s[0], s[1], s[2], b, int(r), slot, n, int(tiles)};
+      slot += n;
+      order.push_back({cdiv(tiles, n), index});
+    }
+  }
+  std::stable_sort(order.begin(), order.end(), longest_first);
+  for (const List& o : order) {
+    const RowTile& x = t[o.index];
+    const int64_t tiles = x.tiles;
+    for (int z = 0; z < x.parts; ++z)
+      *job++ = {x.q0, x.n, x.len, x.seq, x.parts == 1 ? -x.row0 - 1 : x.row0, int(tiles * z / x.parts), int(tiles * (z + 1) / x.parts), x.slot + z};
+  }
+  return w.at;
+}
+
+// ---- host: the calls ----
+bool bad(const void* p) { return !p || reinterpret_cast<uintptr_t>(p) % 16; }
+int32_t launched() { return hipGetLastError() == hipSuccess ? MSD_OK : MSD_E_HIP; }
+int64_t up(int64_t x) { return cdiv(x, 256) * 256; }
+
+// strides of rows that come in tiles of up to `rows`, and of `heads` heads
+bool fits(int64_t row, int64_t head, int64_t rows, int64_t heads) {
+  constexpr int64_t most = int64_t(1) << 30;
+  return row >= 0 && head >= 0 && row % 8 == 0 && head % 8 == 0 && row <= most / rows && head <= most / heads && rows * row + heads * head < most;
+}
+
+int32_t check(const msd_paged* a) {
+  if (!a || bad(a->plan) || !a->plan_host || reinterpret_cast<uintptr_t>(a->plan_host) % 4) return MSD_E_ARG;
+  const int32_t* h = a->plan_host;
+  if (h[MSD_PLAN_MAGIC] != kMagic) return MSD_E_ARG;
+  if (a->d_head <= 0 || a->d_head > 128 || a->d_head % 8 || !(a->scale >= 0x1p-60f) || !(a->scale <= 0x1p60f) || a->q_rows < 0 ||
+      a->q_rows > INT32_MAX || a->positions < 0 || a->positions > INT32_MAX || a->positions % kPage)
+    return MSD_E_CONFIG;
+  const int64_t g = h[MSD_PLAN_HEADS] / h[MSD_PLAN_KV_HEADS];
+  if (a->q_rows * h[MSD_PLAN_HEADS] > INT32_MAX || h[MSD_PLAN_Q_END] > a->q_rows || h[MSD_PLAN_PAGES] > a->positions / kPage)
+    return MSD_E_CONFIG;
+  if (!fits(a->q_stride[0], a->q_stride[1], 128, g)) return MSD_E_CONFIG;
+  for (const int64_t* s : {a->k_stride, a->v_stride})
+    if (s[0] < 0 || s[0] % 8 || s[0] > (int64_t(1) << 40) || !fits(s[1], 0, kPage, 1)) return MSD_E_CONFIG;
+  return MSD_OK;
+}
+
+// Where a workspace's parts begin, in bytes
+struct Space {
+  int64_t few_part, few_lse, many_part, many_lse, lse, scores, end;
+};
+Space space(const msd_paged& a, bool weighted) {
+  const int32_t* h = a.plan_host;
+  const int64_t few = int64_t(h[N_FEW]) * h[MSD_PLAN_KV_HEADS] * kFewRows, many = int64_t(h[N_MANY]) * h[MSD_PLAN_KV_HEADS] * kManyRows;
+  Space s{};
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t from = at;
+    at += up(bytes);
+    return from;
+  };
+  s.few_part = take(h[FEW_PARTS] ? 4 * few * a.d_head : 0);
+  s.few_lse = take(h[FEW_PARTS] || weighted ? 4 * few : 0);
+  s.many_part = take(h[MANY_PARTS] ? 4 * many * a.d_head : 0);
+  s.many_lse = take(h[MANY_PARTS] ? 4 * many : 0);
+  s.lse = take(weighted && h[N_MANYS] ? 4 * a.q_rows * h[MSD_PLAN_HEADS] : 0);
+  s.scores = take(weighted ? 4 * int64_t(h[SCORES]) * kFewKeys * h[MSD_PLAN_KV_HEADS] : 0);
+  s.end = at;
+  return s;
+}
+
+}  // namespace msp
+
+using namespace msp;
+
+extern "C" int64_t msd_paged_plan(int32_t n_seqs, const int32_t* seqs, const int32_t* tables, int32_t table_width, int32_t n_heads,
+                                  int32_t n_kv_heads, int32_t longest, int32_t* words, int64_t room) {
+  try {
+    return plan(n_seqs, seqs, tables, table_width, n_heads, n_kv_heads, longest, words, room);
+  } catch (...) {   // (no memory for its lists)
+    return MSD_E_CONFIG;
+  }
+}
+
+extern "C" int32_t msd_paged_append(const msd_paged* a, const void* k_new, const int64_t* k_new_stride, const void* v_new,
+                                    const int64_t* v_new_stride, void* k, void* v, void* stream) {
+  const int32_t rc = check(a);
+  if (rc != MSD_OK) return rc;
+  if (!k_new_stride || !v_new_stride) return MSD_E_ARG;
+  const int32_t* h = a->plan_host;
+  const int64_t KV = h[MSD_PLAN_KV_HEADS];
+  if (!fits(k_new_stride[0], k_new_stride[1], 128, KV) || !fits(v_new_stride[0], v_new_stride[1], 128, KV)) return MSD_E_CONFIG;
+  if (h[MSD_PLAN_SHARED]) return MSD_E_CONFIG;
+  if (!h[N_APPENDS]) return MSD_OK;
+  if (bad(k_new) || bad(v_new) || bad(k) || bad(v)) return MSD_E_ARG;
+  AppendArgs p{static_cast<const uint16_t*>(k_new), static_cast<const uint16_t*>(v_new), k_new_stride[0], k_new_stride[1], v_new_stride[0],
+               v_new_stride[1], static_cast<uint16_t*>(k), static_cast<uint16_t*>(v), a->k_stride[0], a->k_stride[1], a->v_stride[0],
+               a->v_stride[1], reinterpret_cast<const Append*>(a->plan + h[AT_APPENDS]), int(KV), a->d_head / 8, a->q_rows, a->positions};
+  hipLaunchKernelGGL(paged_append, dim3(h[N_APPENDS]), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+  return launched();
+}
+
+extern "C" int64_t msd_paged_attn_workspace_bytes(const msd_paged* a, int32_t weighted) {
+  const int32_t rc = check(a);
+  return rc != MSD_OK ? rc : space(*a, weighted).end;
+}
+
+extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void* k, const void* v, void* out, const float* weights,
+                                  int32_t weights_width, float* weights_out, void* workspace, void* stream) {
+  const int32_t rc = check(a);
+  if (rc != MSD_OK) return rc;
+  const int32_t* h = a->plan_host;
+  const bool weighted = weights_out != nullptr;
+  if (weights_width < 0) return MSD_E_CONFIG;
+  if (weighted && weights_width && (!weights || reinterpret_cast<uintptr_t>(weights) % 4)) return MSD_E_ARG;
+  if (reinterpret_cast<uintptr_t>(weights_out) % 4) return MSD_E_ARG;
+  const int64_t KV = h[MSD_PLAN_KV_HEADS], longest = h[MSD_PLAN_LONGEST], most = (int64_t(1) << 32) / 256 - 1;
+  const int64_t key_blocks = cdiv(longest, 128), weight_blocks = weighted ? cdiv(longest, kWeightKeys) : 0;
+  const int64_t finish = (h[MANY_PARTS] ? int64_t(h[N_TILES]) * KV * kWaves : 0) + int64_t(h[N_FEWS]) * KV * (1 + weight_blocks);
+  if (finish > most || key_blocks * KV * h[N_MANYS] > most) return MSD_E_CONFIG;
+  if (h[MSD_PLAN_Q_COUNT] && (bad(q) || bad(k) || bad(v) || bad(out))) return MSD_E_ARG;
+  const Space at = space(*a, weighted);
+  if (at.end && bad(workspace)) return MSD_E_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  auto floats = [&](int64_t x) { return reinterpret_cast<float*>(ws + x); };
+  Args p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_row = a->q_stride[0];
+  p.q_head = a->q_stride[1];
+  p.k = {static_cast<const uint16_t*>(k), a->k_stride[0], a->k_stride[1]};
+  p.v = {static_cast<const uint16_t*>(v), a->v_stride[0], a->v_stride[1]};
+  p.D = a->d_head;
+  p.H = h[MSD_PLAN_HEADS];
+  p.KV = int(KV);
+  p.g = p.H / p.KV;
+  magic(uint32_t(p.g), p.g_magic, p.g_shift);
+  p.c = a->scale * kLog2e;
+  p.q_rows = a->q_rows;
+  p.n_seqs = h[MSD_PLAN_SEQS];
+  p.width = h[MSD_PLAN_WIDTH];
+  p.longest = int(longest);
+  p.n_pages = int(a->positions / kPage);
+  p.plan = a->plan;
+  p.tables = a->plan + h[AT_TABLES];
+  p.n_few = h[N_FEW];
+  p.n_many = h[N_MANY];
+  p.out = static_cast<uint16_t*>(out);
+  p.few_part = h[FEW_PARTS] ? floats(at.few_part) : nullptr;
+  p.few_lse = floats(at.few_lse);
+  p.many_part = h[MANY_PARTS] ? floats(at.many_part) : nullptr;
+  p.many_lse = floats(at.many_lse);
+  p.lse = weighted ? floats(at.lse) : nullptr;
+  p.scores = weighted ? floats(at.scores) : nullptr;
+  p.score_words = int64_t(h[SCORES]) * kFewKeys * KV;
+  p.weights = weights;
+  p.weights_width = weights_width;
+  p.weights_out = weights_out;
+  const Job* manys = reinterpret_cast<const Job*>(a->plan + h[AT_MANYS]);
+  with_head(a->d_head, [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    if (h[N_FEW]) {
+      p.jobs = reinterpret_cast<const Job*>(a->plan + h[AT_FEW]);
+      hipLaunchKernelGGL((paged_few<DP>), dim3(unsigned(h[N_FEW] * KV)), dim3(64 * few_waves<DP>()), 0, s, p);
+    }
+    if (h[N_MANY]) {
+      p.jobs = reinterpret_cast<const Job*>(a->plan + h[AT_MANY]);
+      hipLaunchKernelGGL((paged_many<DP>), dim3(unsigned(h[N_MANY] * KV)), dim3(64 * kWaves), 0, s, p);
+    }
+  });
+  const int n_tiles = h[MANY_PARTS] ? h[N_TILES] : 0, n_fews = h[FEW_PARTS] || weighted ? h[N_FEWS] : 0;
+  const int64_t groups = int64_t(n_tiles) * KV * kWaves + int64_t(n_fews) * KV * (1 + weight_blocks);
+  if (groups)
+    hipLaunchKernelGGL(paged_finish, dim3(unsigned(groups)), dim3(kFinish), 0, s, p, reinterpret_cast<const RowTile*>(a->plan + h[AT_TILES]),
+                       n_tiles, reinterpret_cast<const Few*>(a->plan + h[AT_FEWS]), n_fews);
+  if (weighted && h[N_MANYS] && key_blocks)
+    with_head(a->d_head, [&](auto dp) {
+      constexpr int DP = decltype(dp)::value;
+      hipLaunchKernelGGL((paged_weights<DP>), dim3(unsigned(key_blocks * KV * h[N_MANYS])), dim3(64 * kWaves), 0, s, p, manys, h[N_MANYS]);
+    });
+  return launched();
+}
+
+extern "C" int64_t msd_paged_evict_workspace_bytes(const msd_paged* a, int32_t n_layers, int32_t keep) {
+  const int32_t rc = check(a);
+  if (rc != MSD_OK) return rc;
+  const int32_t* h = a->plan_host;
+  if (n_layers < 0 || keep < 0 || int64_t(n_layers) * h[MSD_PLAN_KV_HEADS] >= 65536 ||
+      int64_t(n_layers) * h[MSD_PLAN_KV_HEADS] * h[MSD_PLAN_SEQS] * std::max(keep, 1) >= int64_t(1) << 40)
+    return MSD_E_CONFIG;
+  return 4 * int64_t(n_layers) * h[MSD_PLAN_KV_HEADS] * h[MSD_PLAN_SEQS] * keep;
+}
+
+extern "C" int32_t msd_paged_evict(const msd_paged* a, int32_t n_layers, int64_t k_layer, int64_t v_layer, void* k, void* v,
+                                   const float* weights, int32_t weights_width, int32_t keep, int32_t recent, const int32_t* to,
+                                   int32_t to_width, float* weights_out, int32_t* kept, void* workspace, void* stream) {
+  const int64_t bytes = msd_paged_evict_workspace_bytes(a, n_layers, keep);
+  if (bytes < 0) return int32_t(bytes);
+  const int32_t* h = a->plan_host;
+  if (weights_width < 0 || recent < 0 || recent > keep || to_width < 0 || keep > int64_t(to_width) * kPage || k_layer % 8 || v_layer % 8 ||
+      k_layer < 0 || v_layer < 0 || k_layer > (int64_t(1) << 44) || v_layer > (int64_t(1) << 44))
+    return MSD_E_CONFIG;
+  if (!bytes) return MSD_OK;
+  if (bad(k) || bad(v) || (weights_width && (!weights || reinterpret_cast<uintptr_t>(weights) % 4)) || !to || reinterpret_cast<uintptr_t>(to) % 4 ||
+      !weights_out || reinterpret_cast<uintptr_t>(weights_out) % 4 || !kept || reinterpret_cast<uintptr_t>(kept) % 4 || bad(workspace))
+    return MSD_E_ARG;
+  EvictArgs p{};
+  p.k = static_cast<uint16_t*>(k);
+  p.v = static_cast<uint16_t*>(v);
+  p.k_layer = k_layer;
+  p.k_head = a->k_stride[0];
+  p.k_row = a->k_stride[1];
+  p.v_layer = v_layer;
+  p.v_head = a->v_stride[0];
+  p.v_row = a->v_stride[1];
+  p.weights = weights;
+  p.weights_width = weights_width;
+  p.keep = keep;
+  p.recent = recent;
+  p.seqs = reinterpret_cast<const SeqOf*>(a->plan + h[AT_SEQS]);
+  p.tables = a->plan + h[AT_TABLES];
+  p.to = to;
+  p.width = h[MSD_PLAN_WIDTH];
+  p.to_width = to_width;
+  p.n_pages = int(a->positions / kPage);
+  p.longest = h[MSD_PLAN_LONGEST];
+  p.n_seqs = h[MSD_PLAN_SEQS];
+  p.KV = h[MSD_PLAN_KV_HEADS];
+  p.pieces = a->d_head / 8;
+  p.weights_out = weights_out;
+  p.kept = kept;
+  p.source = static_cast<int32_t*>(workspace);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 rows(n_layers * p.KV, p.n_seqs);
+  const int64_t blocks = cdiv(int64_t(keep) * p.pieces, 256 * kMove);
+  if (blocks * p.n_seqs * 256 >= int64_t(1) << 32) return MSD_E_CONFIG;
+  if (p.longest <= 4096) hipLaunchKernelGGL(paged_select<256>, rows, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL(paged_select<1024>, rows, dim3(1024), 0, s, p);
+  hipLaunchKernelGGL(paged_move, dim3(unsigned(blocks * p.n_seqs), n_layers * p.KV, 2), dim3(256), 0, s, p, int(blocks));
+  return launched();
+}

@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "../../include/mslayers.h"
+#include "../../include/mspaged.h"
 
 namespace {
 
@@ -402,6 +403,85 @@ Tensor swiglu(const Tensor& gate, const Tensor& up, const Glu& p) {
   return glu_run(gate, up, *p, nullptr);
 }
 
+// ---- the paged cache ----
+struct PagedPlan : torch::CustomClassHolder {
+  msd_paged a;
+  int64_t k_new[2], v_new[2];   // strides of new rows (row, head)
+  Tensor table, host;           // of the sequences
+  uint64_t table_stream;        // that the table was made on
+};
+using Paged = c10::intrusive_ptr<PagedPlan>;
+
+// keeps a table's memory until what is launched on stream s is done with it
+void use_table(const Tensor& table, uint64_t made_on, hipStream_t s) {
+  if (reinterpret_cast<uint64_t>(s) != made_on)
+    table.record_stream(c10::impl::VirtualGuardImpl(table.device().type()).getStream(table.device()));
+}
+
+template <class... X>
+void no_gradient(const char* what, const X&... x) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || ...))
+    throw std::invalid_argument(std::string(what) + " has no gradient: call it under torch.no_grad(), or hand over detached tensors");
+}
+
+void paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Paged& p) {
+  only_run("paged_append", k, v, k_pages, v_pages);
+  no_gradient("paged_append", k, v, k_pages, v_pages);
+  Place on(k_pages);
+  use_table(p->table, p->table_stream, on.stream);
+  check(msd_paged_append(&p->a, at_(k), p->k_new, at_(v), p->v_new, at_(k_pages), at_(v_pages), on.stream), "msd_paged_append");
+  k_pages.unsafeGetTensorImpl()->bump_version();
+  v_pages.unsafeGetTensorImpl()->bump_version();
+}
+
+variable_list paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const MaybeTensor& weights, const Paged& p) {
+  only_run("paged_attention", q, k_pages, v_pages, weights);
+  no_gradient("paged_attention", q, k_pages, v_pages);
+  if (weights) no_gradient("paged_attention", *weights);
+  Place on(q);
+  const int32_t* h = p->host.data_ptr<int32_t>();
+  Tensor out = attn_output(q, h[MSD_PLAN_Q_COUNT] != q.size(0)), held, counted, ws;
+  if (weights) {
+    held = weights->contiguous();
+    counted = at::empty({h[MSD_PLAN_SEQS], h[MSD_PLAN_KV_HEADS], h[MSD_PLAN_LONGEST]}, held.options());
+  }
+  const int64_t n = msd_paged_attn_workspace_bytes(&p->a, counted.defined());
+  if (n < 0) check(int32_t(n), "msd_paged_attn_workspace_bytes");
+  if (n) ws = bytes(q, n);
+  use_table(p->table, p->table_stream, on.stream);
+  check(msd_paged_attn(&p->a, at_(q), at_(k_pages), at_(v_pages), at_(out), static_cast<const float*>(at_(held)),
+                       held.defined() ? int32_t(held.size(2)) : 0, static_cast<float*>(at_(counted)), at_(ws), on.stream),
+        "msd_paged_attn");
+  if (!weights) return {out};
+  return {out, counted};
+}
+
+variable_list paged_evict(const Tensor& k_pages, const Tensor& v_pages, const Tensor& weights, const Tensor& to, int32_t keep, int32_t recent,
+                          uint64_t to_stream, const Paged& p) {
+  only_run("paged_evict", k_pages, v_pages, weights);
+  no_gradient("paged_evict", k_pages, v_pages, weights);
+  Place on(k_pages);
+  const Tensor w = weights.contiguous();
+  auto sizes = w.sizes().vec();
+  sizes.back() = keep;
+  Tensor out = at::empty(sizes, w.options()), kept = at::empty(sizes, w.options().dtype(at::kInt)), ws;
+  const bool layers = k_pages.dim() == 4;
+  const int32_t n_layers = layers ? int32_t(k_pages.size(0)) : 1;
+  const int64_t n = msd_paged_evict_workspace_bytes(&p->a, n_layers, keep);
+  if (n < 0) check(int32_t(n), "msd_paged_evict_workspace_bytes");
+  if (n) ws = bytes(k_pages, n);
+  use_table(p->table, p->table_stream, on.stream);
+  use_table(to, to_stream, on.stream);
+  auto layer = [&](const Tensor& x) { return n_layers > 1 ? x.stride(0) : 0; };
+  check(msd_paged_evict(&p->a, n_layers, layer(k_pages), layer(v_pages), at_(k_pages), at_(v_pages), static_cast<const float*>(at_(w)),
+                        int32_t(w.size(-1)), keep, recent, static_cast<const int32_t*>(at_(to)), int32_t(to.size(1)),
+                        static_cast<float*>(at_(out)), static_cast<int32_t*>(at_(kept)), at_(ws), on.stream),
+        "msd_paged_evict");
+  k_pages.unsafeGetTensorImpl()->bump_version();
+  v_pages.unsafeGetTensorImpl()->bump_version();
+  return {out, kept};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -461,10 +541,25 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         p->held = held;
         return p;
       }));
+  py::class_<PagedPlan, Paged>(m, "PagedPlan")
+      .def(py::init([](uintptr_t a, const Tensor& table, const Tensor& host, uint64_t table_stream, int64_t k_row, int64_t k_head,
+                       int64_t v_row, int64_t v_head) {
+        auto p = c10::make_intrusive<PagedPlan>();
+        p->a = *reinterpret_cast<const msd_paged*>(a);
+        p->table = table;
+        p->host = host;
+        p->table_stream = table_stream;
+        p->k_new[0] = k_row, p->k_new[1] = k_head;
+        p->v_new[0] = v_row, p->v_new[1] = v_head;
+        return p;
+      }));
   m.def("attention", &attention, free_threads);
   m.def("rotary", &rotary, free_threads);
   m.def("rms_norm", &rms_norm, free_threads);
   m.def("swiglu", &swiglu, free_threads);
+  m.def("paged_append", &paged_append, free_threads);
+  m.def("paged_attention", &paged_attention, free_threads);
+  m.def("paged_evict", &paged_evict, free_threads);
   m.def("row_stride", &row_stride);
   m.def("restored", [](const Tensor& x, const Tensor& saved) { restored(x, saved.scalar_type(), saved.sizes(), saved.device()); });
 }
