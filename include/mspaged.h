@@ -43,7 +43,7 @@ enum {
  * words NULL: returns how many there are; otherwise writes them (`room` of them are there) and returns that.  Word MSD_PLAN_Q_END:
  * one past the last row; Q_COUNT: rows of all sequences; PAGES: one past the largest page in use; SHARED: whether a page
  * that takes new rows is in use elsewhere too.
- * Limits: 0 <= q_len <= length <= longest <= 16 table_width; n_heads a multiple of n_kv_heads, up to 4096; n_seqs up to 65535,
+ * Limits: 0 <= q_len <= length <= longest <= 16 table_width, below 2^31 - 2^16; n_heads a multiple of n_kv_heads, up to 4096; n_seqs up to 65535,
  * rows and pool positions below 2^31; q_len times the heads of a group below 2^30 - 256; the words below 2^28. */
 int64_t msd_paged_plan(int32_t n_seqs, const int32_t* seqs, const int32_t* tables, int32_t table_width, int32_t n_heads,
                        int32_t n_kv_heads, int32_t longest, int32_t* words, int64_t room);

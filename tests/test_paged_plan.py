@@ -12,8 +12,8 @@ from transformer_amd.paged_attention import PagedEviction, PagedSequences, paged
 
 # words of a plan: the public ones, then the launches' sizes and where the lists lie
 (MAGIC, WORDS, SEQS, HEADS, KV_HEADS, WIDTH, LONGEST, Q_END, Q_COUNT, PAGES, SHARED, RESERVED,
- N_FEW, N_MANY, N_FEWS, N_TILES, N_MANYS, N_APPENDS, FEW_PARTS, MANY_PARTS, SCORES,
- AT_SEQS, AT_FEW, AT_MANY, AT_FEWS, AT_TILES, AT_MANYS, AT_APPENDS, AT_TABLES) = range(29)
+ N_FEW, N_MANY, N_FEWS, N_TILES, N_MANYS, N_APPENDS, FEW_PARTS, MANY_PARTS, FEW_ROWS, SCORES,
+ AT_SEQS, AT_FEW, AT_MANY, AT_FEWS, AT_TILES, AT_MANYS, AT_APPENDS, AT_TABLES) = range(30)
 
 
 def tables_of(lengths, seed=0):

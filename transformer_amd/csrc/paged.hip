@@ -31,11 +31,12 @@ constexpr int kPage = MSD_PAGE;
 constexpr int kFewRows = 32;      // of a group: paged_few
 constexpr int kFewKeys = 32;      // keys of its tiles
 constexpr int kManyRows = 32 * kWaves;
+constexpr int kLongest = INT32_MAX - 65536;
 constexpr int32_t kMagic = 0x70616731;
 
 // Words of a plan behind the public ones: launches' sizes, then where the lists lie
 enum {
-  N_FEW = MSD_PLAN_RESERVED + 1, N_MANY, N_FEWS, N_TILES, N_MANYS, N_APPENDS, FEW_PARTS, MANY_PARTS, SCORES,
+  N_FEW = MSD_PLAN_RESERVED + 1, N_MANY, N_FEWS, N_TILES, N_MANYS, N_APPENDS, FEW_PARTS, MANY_PARTS, FEW_ROWS, SCORES,
   AT_SEQS, AT_FEW, AT_MANY, AT_FEWS, AT_TILES, AT_MANYS, AT_APPENDS, AT_TABLES, END
 };
 static_assert(END <= MSD_PLAN_HEADER, "the header's words");
@@ -220,7 +221,7 @@ template <int DP>
 constexpr int few_waves() { return DP <= 64 ? 4 : 2; }
 
 template <int DP>
-__global__ __launch_bounds__(64 * few_waves<DP>()) void paged_few(Args p) {
+__global__ __launch_bounds__(64 * few_waves<DP>(), 2) void paged_few(Args p) {
   constexpr int P = pitch<DP>(), W = few_waves<DP>(), TILE = kFewKeys * P, OROW = DP + 4;
   __shared__ __attribute__((aligned(16))) uint8_t lds[W * 4 * TILE];
   __shared__ float stats[W][2][32];
@@ -336,102 +337,256 @@ __global__ __launch_bounds__(64 * few_waves<DP>()) void paged_few(Args p) {
 }
 
 // ---- many rows ----
-// As attn.hip's forward: scores 32 keys ahead, K one tile ahead of V, three K buffers and two of V, one barrier a tile.
+// 128 rows a workgroup, 32 a wave, tiles of 64 keys, each in two halves.  While the softmax of a half is formed (vector units), the
+// matrix cores form the scores of the half behind it and the product of the half before it with V: three independent pieces of
+// work in one stretch of code.  A wave issues an instruction every four cycles or more, and two of them share a SIMD, so what is not a
+// product counts by its instructions.  Hence: each wave fetches from one page of a tile, whose descriptor ends with the rows that
+// exist; LDS places are constants (the loop's body is there for even and odd tiles); addresses within a place are kept.
+//
+// Wave w fetches page w of a tile, rows r of it with r < 8 to the tile's first half and the others to its second: instruction u of
+// ROWS rows lies, in the half, behind those of the waves before it.  So the first half's keys are the first eight of each
+// page.  In a half, LDS row x (a score's register and lane half) is key key_of(x) of the tile, plus 8 in the second.
+template <int DP>
+struct HalfTile {
+  static constexpr int P = pitch<DP>(), C = P / 16, ROWS = 64 / C, N = kPage / 2 / ROWS, BYTES = 32 * P;   // N instructions a wave
+  uint32_t off, step;   // of this lane in a page, and from one instruction's rows to the next
+  __device__ __forceinline__ void init(int64_t row_stride, int D, int lane, int wv) {
+    const int i = lane / C, c = lane % C ^ swizzle<P>(ROWS * wv + i);
+    step = ROWS * uint32_t(row_stride) * 2;
+    off = 8 * c < D ? uint32_t(i) * uint32_t(row_stride) * 2 + 16 * c : kOutside;
+  }
+  // the key of register i (of a score) of lanes 0 .. 31; those of the others lie kLanes behind
+  static constexpr int kLanes = P == 128 ? 4 : kPage;
+  static constexpr int key_of(int i) { return P == 128 ? kPage * (i / 4) + i % 4 : kPage * 2 * (i / 4 % 2) + 4 * (i / 8) + i % 4; }
+};
+// Rows `rows` (0 .. 16) of a page's positions of a head, as a buffer
+struct PageRows {
+  const uint16_t* p;
+  uint32_t bytes;
+};
+template <int DP, int HALF>
+__device__ __forceinline__ void load_half(const HalfTile<DP>& x, const PageRows& page, uint32_t to) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(page.p), 0, page.bytes, 0x00020000);
+#pragma unroll
+  for (int u = 0; u < HalfTile<DP>::N; ++u)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to + 4096 * u),
+                 "v"(x.off + (HALF * HalfTile<DP>::N + u) * x.step), "s"(r) : "m0");
+#endif
+}
+
+// Nothing moves across
+__device__ __forceinline__ void order_steps() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+
 template <int DP>
 __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void paged_many(Args p) {
-  constexpr int P = pitch<DP>(), TILE = kKeys * P;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[5 * TILE];
+  using Half = HalfTile<DP>;
+  constexpr int P = pitch<DP>(), BYTES = Half::BYTES, KS = DP / 16, DB = DP / 32;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[8 * BYTES];   // four halves of K, four of V
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % p.KV;
   const Job j = scalar_load(p.jobs + blockIdx.x / p.KV);
-  const int rows = j.n * p.g, row0 = j.row0 < 0 ? -j.row0 - 1 : j.row0, tiles = tiles_of(j.len, kKeys);
+  const int rows = j.n * p.g, row0 = j.row0 < 0 ? -j.row0 - 1 : j.row0;
   const bool only = j.row0 < 0;
-  if (!sound(p, j.q0, j.n, j.len, j.seq) || row0 >= rows || j.t0 < 0 || j.t1 > tiles || j.slot < 0 || j.slot >= p.n_many) return;
+  if (!sound(p, j.q0, j.n, j.len, j.seq) || row0 >= rows || j.t0 < 0 || j.t1 <= j.t0 || j.t1 > tiles_of(j.len, kKeys) || j.slot < 0 || j.slot >= p.n_many)
+    return;
   const uint16_t *kb = p.k.p + kvh * p.k.head, *vb = p.v.p + kvh * p.v.head;
-  const int4* table = reinterpret_cast<const int4*>(p.tables + int64_t(j.seq) * p.width);
-  PagedTile<DP, kKeys, kWaves> kt, vt;
+  const int32_t* table = p.tables + int64_t(j.seq) * p.width;
+  Half kt, vt;
   kt.init(p.k.row, p.D, lane, wv);
   vt.init(p.v.row, p.D, lane, wv);
-  auto load_k = [&](uint8_t* to, int t, int4 pages) {
-    kt.load(lds_address(to), j.len - t * kKeys, wv, kb, p.k.row, p.n_pages, [&](int i) { return pick(i, pages.x, pages.y, pages.z, pages.w); });
+  const uint32_t k_row = uint32_t(p.k.row) * 2, v_row = uint32_t(p.v.row) * 2;   // (16 rows span less than 2^31 bytes)
+  auto page_of = [&](int t) { return scalar_load(table + min(t * (kKeys / kPage) + wv, p.width - 1)); };
+  // this wave's page of tile t: rows that the job reads
+  auto rows_in = [&](int t, int page) {
+    return t < j.t0 || t >= j.t1 || uint32_t(page) >= uint32_t(p.n_pages) ? 0 : min(max(j.len - t * kKeys - kPage * wv, 0), kPage);
   };
-  auto load_v = [&](uint8_t* to, int t, int4 pages) {
-    vt.load(lds_address(to), j.len - t * kKeys, wv, vb, p.v.row, p.n_pages, [&](int i) { return pick(i, pages.x, pages.y, pages.z, pages.w); });
+  auto page_rows = [&](const uint16_t* head, uint32_t row, int page, int n) {
+    return PageRows{head + (uint64_t(uint32_t(n ? page : 0)) * (kPage * row) >> 1), n * row};
   };
-  auto pages_of = [&](int t) { return scalar_load(table + min(t, tiles - 1)); };
-  uint8_t *k0 = lds, *k1 = lds + TILE, *k2 = lds + 2 * TILE, *v0 = lds + 3 * TILE, *v1 = lds + 4 * TILE;
-  int4 next{}, after{};   // the pages of tiles t + 1 and t + 2
-  if (j.t0 < j.t1) {
-    const int4 now = pages_of(j.t0);
-    next = pages_of(j.t0 + 1);
-    after = pages_of(j.t0 + 2);
-    load_k(k0, j.t0, now);
-    load_v(v0, j.t0, now);
-    load_k(k1, j.t0 + 1, next);
+  auto k_page = [&](int t, int page) { return page_rows(kb, k_row, page, rows_in(t, page)); };
+  auto v_page = [&](int t, int page) { return page_rows(vb, v_row, page, rows_in(t, page)); };
+  const uint32_t mine = lds_address(lds) + 1024 * wv;
+  auto k_place = [&](int i) { return mine + (i & 3) * BYTES; };
+  auto v_place = [&](int i) { return mine + (4 + (i & 3)) * BYTES; };
+  // half i of K and V (counted from the job's first tile) lies in place i % 4; an iteration reads K's halves 2 t + 1 and 2 t + 2, V's
+  // 2 t - 1 (zeros before the first) and 2 t, and fetches the next two of each
+  int page1 = page_of(j.t0 + 1), page2 = page_of(j.t0 + 2);
+  PageRows k1, v0;   // of tile t + 1 and t
+  {
+    const int page = page_of(j.t0);
+    const PageRows k0 = k_page(j.t0, page);
+    v0 = v_page(j.t0, page);
+    k1 = k_page(j.t0 + 1, page1);
+    load_half<DP, 0>(kt, k0, k_place(0));
+    load_half<DP, 1>(kt, k0, k_place(1));
+    load_half<DP, 0>(kt, k1, k_place(2));
+    load_half<DP, 1>(vt, PageRows{vb, 0}, v_place(3));
+    load_half<DP, 0>(vt, v0, v_place(0));
   }
   const int r = row0 + 32 * wv + (lane & 31), pos = div_g(p, min(r, rows - 1));
   const bool ok = r < rows;
-  bf16x8 q[DP / 16];
+  bf16x8 q[KS];
   row_operands<DP>(q, p.q, row_at(p, j.q0, kvh, pos, ok ? r - pos * p.g : 0) - p.q, ok, p.D, lane);
-  const int first = j.len - j.n + 1, seen = first + pos;
-  const int wave_full = first + div_g(p, min(row0 + 32 * wv, rows - 1)), wave_end = first + div_g(p, min(row0 + 32 * wv + 31, rows - 1));
+  const int first = j.len - j.n + 1, seen = first + pos, wave_full = first + div_g(p, min(row0 + 32 * wv, rows - 1));
 
-  Rows<DP> x;
-  x.start();
-  // s: the scores of 32 keys from key0, which lie from row0 of V; next: where the next 32 keys' K rows lie
-  auto step = [&](f32x16& s, f32x16& ahead, const uint8_t* V, int v_row, int key0, const uint8_t* next_k, int next_row) {
-    if (key0 + 32 > wave_full) {   // the diagonal or the end
-      const int left = seen - key0 - 4 * (lane >> 5);
+  // where this lane reads in a half's rows: the operands of 32 keys (K), of 32 columns (V: the first and the second eight rows)
+  uint32_t k_at[KS], v_at[2][DB];
+  const uint32_t base = lds_address(lds);
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) k_at[ks] = base + piece_at<P>(lane & 31, 2 * ks + (lane >> 5));
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int t = lane & 15, x = 8 * h + 4 * (lane >> 5) + (t >> 2), c = 4 * d + 2 * ((lane >> 4) & 1) + ((t & 3) >> 1);
+      v_at[h][d] = base + 4 * BYTES + piece_at<P>(x, c) + 8 * (t & 1);
+    }
+#if defined(__HIP_DEVICE_COMPILE__)   // (kept in registers: formed again at each read they cost a quarter of the loop's vector instructions)
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm("" : "+v"(k_at[ks]));
+#pragma unroll
+  for (int d = 0; d < 2 * DB; ++d) asm("" : "+v"(v_at[d / DB][d % DB]));
+#endif
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  typedef __attribute__((address_space(3))) const bf16x8 lds_bf16x8;
+#else
+  typedef s16x4 lds_s16x4;
+  typedef const bf16x8 lds_bf16x8;
+#endif
+  f32x16 o[DB] = {};
+  float m = -INFINITY, l = 0;   // running maximum of c s, up to 2^8 too small; sum of 2^(c s - m) over this lane's keys
+  bf16x8 pr[2] = {};            // the half before, as operands
+  // operand n of a half: K's for the scores, then V's for the product
+  auto operand = [&](int n, int k, int v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if (n < KS) return *(lds_bf16x8*)(k_at[n] + k * BYTES);
+    const int h = (n - KS) / DB, d = (n - KS) % DB;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(v_at[0][d] + v * BYTES + 16 * h * P));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(v_at[1][d] + v * BYTES + 16 * h * P));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#else
+    return bf16x8{};
+#endif
+  };
+  auto scores = [&](int place) {
+    f32x16 s = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = mfma(operand(ks, place, 0), q[ks], s);
+    return s;
+  };
+  auto product = [&](int place) {
+#pragma unroll
+    for (int n = 0; n < 2 * DB; ++n) o[n % DB] = mfma(operand(KS + n, 0, place), pr[n / DB], o[n % DB]);
+  };
+  // s: the scores of half `second` of tile t; ahead: those of the half behind it, in K's place k; the half before is V's place v.
+  // Step by step: a matrix product, the operand of the one after the next, a share of the softmax (left to itself the compiler waits
+  // for each operand in turn and forms the softmax after all products).
+  constexpr int STEPS = KS + 2 * DB, AHEAD = 2;
+  auto half = [&](f32x16& s, f32x16& ahead, int t, int second, int k, int v) {
+    if (t * kKeys + kKeys > wave_full) {   // the diagonal or the end
+      const int left = seen - t * kKeys - 8 * second - Half::kLanes * (lane >> 5);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (8 * (i >> 2) + (i & 3) >= left) s[i] = -INFINITY;
+        if (Half::key_of(i) >= left) s[i] = -INFINITY;
     }
-    const float sub = x.new_maximum(s, p.c);
-    ahead = scores_of<DP>(next_k, next_row, q, lane);
-    x.probabilities(s, p.c, sub);
-    x.add(s, V, v_row, lane);
+    bf16x8 f[AHEAD + 1], next[2];
+    float top = s[0], sum = 0, by = 1, sub = 0;
+    bool grown = false;
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) f[n] = operand(n, k, v);
+    ahead = f32x16{};
+#pragma unroll
+    for (int n = 0; n < STEPS; ++n) {
+      if (n + AHEAD < STEPS) f[(n + AHEAD) % (AHEAD + 1)] = operand(n + AHEAD, k, v);
+      const bf16x8 x = f[n % (AHEAD + 1)];
+      if (n < KS) ahead = mfma(x, q[n], ahead);
+      else o[(n - KS) % DB] = mfma(x, pr[(n - KS) / DB], o[(n - KS) % DB]);
+      if (n < 2) {
+#pragma unroll
+        for (int i = 8 * n + (n == 0); i < 8 * n + 8; ++i) top = __builtin_elementwise_maximum(top, s[i]);
+      } else if (n == 2) {
+        top = __builtin_elementwise_maximum(top, swap_halves(top)) * p.c;
+        grown = __any(top > m + 8.0f);   // rescaling by less than 2^8 can wait: f32 sums and bf16 P keep their precision
+        const float mn = grown ? fmaxf(m, top) : m;
+        by = mn == -INFINITY ? 1.0f : exp2_hw(m - mn);
+        sub = mn == -INFINITY ? 0.0f : mn;
+        m = mn;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (3 + i * (STEPS - 3) / 16 == n) {
+            s[i] = exp2_hw(fmaf(s[i], p.c, -sub));
+            sum += s[i];
+            if (i == 7) next[0] = pack8(s, 0);
+            if (i == 15) next[1] = pack8(s, 8);
+          }
+      }
+      order_steps();
+    }
+    l = fmaf(l, by, sum);
+    pr[0] = next[0];
+    pr[1] = next[1];
+#if defined(__HIP_DEVICE_COMPILE__)   // (formed above, not behind the branch)
+    asm volatile("" : "+v"(pr[0]), "+v"(pr[1]), "+v"(l));
+#endif
+    if (grown)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] *= by;
   };
 
   f32x16 s0, s1;
-  dma_wait();
+  dma_wait();   // (for q too, so that the compiler does not wait for all loads in the loop)
   __syncthreads();
-  if (j.t0 < j.t1) s0 = scores_of<DP>(k0, 0, q, lane);
-  for (int t = j.t0; t < j.t1; ++t) {
-    if (t + 1 < j.t1) {
-      load_k(k2, t + 2, after);
-      load_v(v1, t + 1, next);
-      next = after;
-      after = pages_of(t + 3);
-    }
-    const int key0 = t * kKeys;
-    if (key0 < wave_end) {
-      step(s0, s1, v0, 0, key0, k0, 32);
-      step(s1, s0, v0, 32, key0 + 32, k1, 0);
-    }
-    uint8_t* k = k0;
-    k0 = k1;
+  s0 = scores(0);
+  __syncthreads();   // (the first place is fetched to next)
+  auto tile = [&](auto odd, int t) {
+    constexpr int X = 2 * decltype(odd)::value;
+    const PageRows k2 = k_page(t + 2, page2), v1 = v_page(t + 1, page1);
+    load_half<DP, 1>(kt, k1, k_place(X + 3));
+    load_half<DP, 0>(kt, k2, k_place(X + 4));
+    load_half<DP, 1>(vt, v0, v_place(X + 1));
+    load_half<DP, 0>(vt, v1, v_place(X + 2));
     k1 = k2;
-    k2 = k;
-    uint8_t* v = v0;
     v0 = v1;
-    v1 = v;
+    page1 = page2;
+    page2 = page_of(t + 3);
+    half(s0, s1, t, 0, X + 1, (X + 3) & 3);
+    half(s1, s0, t, 1, (X + 2) & 3, X);
     dma_wait();
     __syncthreads();
+  };
+  int t = j.t0;
+  for (; t + 1 < j.t1; t += 2) {
+    tile(std::integral_constant<int, 0>(), t);
+    tile(std::integral_constant<int, 1>(), t + 1);
   }
-  float l = x.l + swap_halves(x.l);
+  if (t < j.t1) {
+    tile(std::integral_constant<int, 0>(), t);
+    product(1);
+  } else {
+    product(3);
+  }
+  __syncthreads();   // (the tiles are read, the rows are staged in their place)
+  l += swap_halves(l);
   const float by = l == 0 ? 0.0f : 1.0f / l;   // (a NaN sum stays one)
-  const float lse = l == 0 ? INFINITY : x.m + __log2f(l);
+  const float lse = l == 0 ? INFINITY : m + __log2f(l);
   if (!only) {   // a normalised part and its weight, joined by paged_finish
     if (ok && p.many_part) {
       const int64_t row = (int64_t(j.slot) * p.KV + kvh) * kManyRows + 32 * wv + (lane & 31);
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d)
+      for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int c = 32 * d + 8 * u + 4 * (lane >> 5);
           if (c < p.D)
             *reinterpret_cast<f32x4*>(p.many_part + row * p.D + c) =
-                f32x4{x.o[d][4 * u] * by, x.o[d][4 * u + 1] * by, x.o[d][4 * u + 2] * by, x.o[d][4 * u + 3] * by};
+                f32x4{o[d][4 * u] * by, o[d][4 * u + 1] * by, o[d][4 * u + 2] * by, o[d][4 * u + 3] * by};
         }
       if (lane < 32) p.many_lse[row] = lse;
     }
@@ -439,97 +594,97 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void paged_many(Args
   }
   if (p.lse && ok && lane < 32) p.lse[int64_t(j.q0) * p.H + int64_t(kvh * p.g + r - pos * p.g) * j.n + pos] = lse;
   const int r0 = r - (lane & 31);
-  store_rows<DP>(lds + wv * 32 * P, x.o, by, p.D, lane, [&](int i) -> uint16_t* {
+  store_rows<DP>(lds + wv * 32 * P, o, by, p.D, lane, [&](int i) -> uint16_t* {
     if (r0 + i >= rows) return nullptr;
     const int at = div_g(p, r0 + i);
-    return p.out + (int64_t(j.q0 + at) * p.H + kvh * p.g + (r0 + i - at * p.g)) * p.D;
+    return p.out + (int64_t(j.q0 + at) * p.H + (kvh * p.g + (r0 + i - at * p.g))) * p.D;
   });
 }
 
 // ---- what is left ----
-// Workgroups, in this order: 32 rows of a row tile of many; the rows of a sequence of few; 1024 positions' weights of such.
-constexpr int kFinish = 256, kWeightKeys = 4 * kFinish;
+// Workgroups, in this order: four rows of a row tile of many; four rows of a sequence of few; 1024 positions' weights of such.
+constexpr int kFinish = 256, kWeightKeys = 4 * kFinish, kJoinRows = 4;
 
-// Rows `rows` (up to 32) from their parts' normalised outputs, weighted by 2^(lse_z - lse): 16 lanes a row's 8-value
+// Rows `rows` (up to four) from their parts' normalised outputs, weighted by 2^(lse_z - lse): 16 lanes a row's 8-value
 // pieces, G of them in turn over the parts, joined through LDS in order.
 __device__ __forceinline__ void join(const Args& p, float (*lds)[11], const float* part, const float* lse, int64_t stride, int parts, int rows,
                                      int q0, int n, int row0, int kvh, bool keep) {
   const int tid = threadIdx.x, c = tid % 16;
-  const int G = rows >= 16 ? 1 : rows > 8 ? 1 : rows > 4 ? 2 : rows > 2 ? 4 : rows > 1 ? 8 : 16;
-  const int per = 16 / G, zg = tid / 16 % G;
-  for (int first = 0; first < rows; first += per) {
-    const int row = first + tid / 16 / G;
-    const bool ok = row < rows && 8 * c < p.D;
-    float m = -INFINITY, l = 0, acc[8] = {};
-    if (ok)
+  const int shift = rows > 2 ? 2 : rows > 1 ? 3 : 4, G = 1 << shift, zg = tid / 16 % G, row = tid / 16 >> shift;
+  const bool ok = row < rows && 8 * c < p.D;
+  float m = -INFINITY, l = 0, acc[8] = {};
+  if (ok)
 #pragma unroll 4
-      for (int z = zg; z < parts; z += G) {
-        const float x = lse[z * stride + row];
-        const float* from = part + (z * stride + row) * p.D + 8 * c;
-        const f32x4 a = *reinterpret_cast<const f32x4*>(from), b = *reinterpret_cast<const f32x4*>(from + 4);
-        if (x == INFINITY) continue;   // nothing seen in this part
-        const float mn = fmaxf(m, x), old = exp2_hw(m - mn), e = exp2_hw(x - mn);   // (a NaN stays one through e)
-        m = mn;
-        l = fmaf(l, old, e);
+    for (int z = zg; z < parts; z += G) {
+      const float x = lse[z * stride + row];
+      const float* from = part + (z * stride + row) * p.D + 8 * c;
+      const f32x4 a = *reinterpret_cast<const f32x4*>(from), b = *reinterpret_cast<const f32x4*>(from + 4);
+      // (infinite: nothing seen in this part; no branch, so that the next parts' loads need not wait; a NaN stays one through e)
+      const float mn = x == INFINITY ? m : fmaxf(m, x);
+      const float old = m == -INFINITY ? 0.0f : exp2_hw(m - mn), e = x == INFINITY ? 0.0f : exp2_hw(x - mn);
+      m = mn;
+      l = fmaf(l, old, e);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[i] = fmaf(acc[i], old, e * a[i]);
-          acc[4 + i] = fmaf(acc[4 + i], old, e * b[i]);
-        }
+      for (int i = 0; i < 4; ++i) {
+        acc[i] = fmaf(acc[i], old, e * a[i]);
+        acc[4 + i] = fmaf(acc[4 + i], old, e * b[i]);
       }
-    __syncthreads();
-    lds[tid][0] = m;
-    lds[tid][1] = l;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) lds[tid][2 + i] = acc[i];
-    __syncthreads();
-    if (zg || !ok) continue;
-    m = -INFINITY;
-    for (int g = 0; g < G; ++g) m = fmaxf(m, lds[tid + 16 * g][0]);
-    l = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = 0;
-    for (int g = 0; g < G; ++g) {
-      const float* x = lds[tid + 16 * g];
-      const float e = x[1] == 0 ? 0.0f : exp2_hw(x[0] - m);
-      l = fmaf(e, x[1], l);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] = fmaf(e, x[2 + i], acc[i]);
     }
-    const float by = l == 0 ? 0.0f : 1.0f / l;
-    u32x4 x;
+  lds[tid][0] = m;
+  lds[tid][1] = l;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = pack2(acc[2 * i] * by, acc[2 * i + 1] * by);
-    const int pos = div_g(p, row0 + row), head = kvh * p.g + row0 + row - pos * p.g;
-    *reinterpret_cast<u32x4*>(p.out + (int64_t(q0 + pos) * p.H + head) * p.D + 8 * c) = x;
-    if (keep && c == 0) p.lse[int64_t(q0) * p.H + int64_t(head) * n + pos] = l == 0 ? INFINITY : m + __log2f(l);
+  for (int i = 0; i < 8; ++i) lds[tid][2 + i] = acc[i];
+  __syncthreads();
+  if (zg || !ok) return;
+  m = -INFINITY;
+  for (int g = 0; g < G; ++g) m = fmaxf(m, lds[tid + 16 * g][0]);
+  l = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0;
+  for (int g = 0; g < G; ++g) {
+    const float* x = lds[tid + 16 * g];
+    const float e = x[1] == 0 ? 0.0f : exp2_hw(x[0] - m);
+    l = fmaf(e, x[1], l);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = fmaf(e, x[2 + i], acc[i]);
   }
+  const float by = l == 0 ? 0.0f : 1.0f / l;
+  u32x4 x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = pack2(acc[2 * i] * by, acc[2 * i + 1] * by);
+  const int pos = div_g(p, row0 + row), head = kvh * p.g + row0 + row - pos * p.g;
+  *reinterpret_cast<u32x4*>(p.out + (int64_t(q0 + pos) * p.H + head) * p.D + 8 * c) = x;
+  if (keep && c == 0) p.lse[int64_t(q0) * p.H + int64_t(head) * n + pos] = l == 0 ? INFINITY : m + __log2f(l);
 }
 
-__global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* tiles, int n_tiles, const Few* fews, int n_fews) {
+__global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* tiles, int n_tiles, const Few* fews, int n_fews, int few_joins) {
   __shared__ float lds[kFinish][11];
   __shared__ float row_lse[kFewRows];
+  constexpr int kSubs = kManyRows / kJoinRows;
   const int tid = threadIdx.x;
-  int64_t id = blockIdx.x;
-  if (id < int64_t(n_tiles) * p.KV * kWaves) {
-    const int kvh = id % p.KV, sub = id / p.KV % kWaves;
-    const RowTile t = scalar_load(tiles + id / p.KV / kWaves);
-    const int rows = min(t.n * p.g - t.row0 - 32 * sub, 32);
+  int id = blockIdx.x;
+  if (id < n_tiles * p.KV * kSubs) {
+    const int kvh = id % p.KV, sub = id / p.KV % kSubs;
+    const RowTile t = scalar_load(tiles + id / p.KV / kSubs);
+    const int row0 = t.row0 + kJoinRows * sub, rows = min(t.n * p.g - row0, kJoinRows);
     if (!sound(p, t.q0, t.n, t.len, t.seq) || t.row0 < 0 || rows <= 0 || t.parts < 2 || t.slot < 0 || t.slot > p.n_many - t.parts) return;
-    const int64_t at = (int64_t(t.slot) * p.KV + kvh) * kManyRows + 32 * sub;
-    join(p, lds, p.many_part + at * p.D, p.many_lse + at, int64_t(p.KV) * kManyRows, t.parts, rows, t.q0, t.n, t.row0 + 32 * sub, kvh, p.lse);
+    const int64_t at = (int64_t(t.slot) * p.KV + kvh) * kManyRows + kJoinRows * sub;
+    join(p, lds, p.many_part + at * p.D, p.many_lse + at, int64_t(p.KV) * kManyRows, t.parts, rows, t.q0, t.n, row0, kvh, p.lse);
     return;
   }
-  id -= int64_t(n_tiles) * p.KV * kWaves;
-  const bool weigh = id >= int64_t(n_fews) * p.KV;
-  if (weigh) id -= int64_t(n_fews) * p.KV;
-  const int kvh = id % p.KV;
+  id -= n_tiles * p.KV * kSubs;
+  const int joins = n_fews * p.KV * few_joins;
+  const bool weigh = id >= joins;
+  if (weigh) id -= joins;
+  const int kvh = id % p.KV, nth = id / p.KV / n_fews;
   const Few f = scalar_load(fews + id / p.KV % n_fews);
   const int R = f.n * p.g;
   if (!sound(p, f.q0, f.n, f.len, f.seq) || R > kFewRows || f.parts < 0 || f.slot < 0 || f.slot > p.n_few - f.parts) return;
   const int64_t at = (int64_t(f.slot) * p.KV + kvh) * kFewRows, stride = int64_t(p.KV) * kFewRows;
   if (!weigh) {
-    if (f.parts > 1) join(p, lds, p.few_part + at * p.D, p.few_lse + at, stride, f.parts, R, f.q0, f.n, 0, kvh, false);
+    const int row0 = kJoinRows * nth, rows = min(R - row0, kJoinRows);
+    if (f.parts > 1 && rows > 0)
+      join(p, lds, p.few_part + (at + row0) * p.D, p.few_lse + at + row0, stride, f.parts, rows, f.q0, f.n, row0, kvh, false);
     return;
   }
   // the rows' logsumexps, from their parts': eight lanes a row
@@ -553,7 +708,7 @@ __global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* t
     if (row < kFewRows && tid % 8 == 0) row_lse[row] = l == 0 ? INFINITY : m + __log2f(l);
   }
   __syncthreads();
-  const int key = int(id / p.KV / n_fews) * kWeightKeys + 4 * tid;
+  const int key = nth * kWeightKeys + 4 * tid;
   if (key >= p.longest) return;
   const int padded = tiles_of(f.len, kFewKeys) * kFewKeys;
   float w[4] = {};
@@ -584,12 +739,16 @@ __global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* t
 
 // ---- the weights of many rows ----
 // 128 keys a workgroup, 32 a wave in registers, over the group's heads and the rows that see them: S = Q K^T, a lane holds one
-// key's scores against 16 rows, so that its sum stays in the lane.
+// key's scores against 16 rows, so that its sum stays in the lane.  Two halves of four waves take the row tiles in turn, so
+// that a SIMD has the products of one wave beside the exponentials of the other.
+constexpr int kHalves = 2;
 template <int DP>
-__global__ __launch_bounds__(64 * kWaves) void paged_weights(Args p, const Job* seqs, int n_seqs) {
-  constexpr int P = pitch<DP>(), R = DP <= 64 ? 64 : 32, TILE = R * P, STAGE = TILE + 256, SUB = R / 32;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+__global__ __launch_bounds__(64 * kWaves * kHalves) void paged_weights(Args p, const Job* seqs, int n_seqs) {
+  constexpr int P = pitch<DP>(), R = DP <= 64 ? 64 : 32, TILE = R * P, STAGE = TILE + 256 * kWaves, SUB = R / 32, STAGES = 4;
+  constexpr int LOADS = TILE / 1024 / kWaves + 1;   // of a wave and stage: rows, and their logsumexps, of which each wave has its own
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kHalves * STAGES * STAGE];
+  __shared__ float other[kHalves][kWaves * 32];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wv = wave % kWaves, half = wave / kWaves;
   const int kvh = blockIdx.x % p.KV, kb = blockIdx.x / p.KV / n_seqs;
   const Job j = scalar_load(seqs + blockIdx.x / p.KV % n_seqs);
   if (!sound(p, j.q0, j.n, j.len, j.seq)) return;
@@ -598,26 +757,31 @@ __global__ __launch_bounds__(64 * kWaves) void paged_weights(Args p, const Job* 
   if (128 * kb < j.len) {
     const uint16_t* kbase = p.k.p + kvh * p.k.head;
     const int page = key < j.len ? p.tables[int64_t(j.seq) * p.width + key / kPage] : -1;
-    bf16x8 k[DP / 16];
-    row_operands<DP>(k, kbase, (int64_t(page) * kPage + key % kPage) * p.k.row, uint32_t(page) < uint32_t(p.n_pages), p.D, lane);
     const int pos0 = max(128 * kb - (j.len - j.n), 0) / R * R, n = (j.n - pos0 + R - 1) / R, all = n * p.g;   // row tiles a head, of the group
     Tile<DP, R> qt;
     qt.init(p.q_row, p.D, lane, wv);
     const uint16_t* q0 = p.q + int64_t(j.q0) * p.q_row + int64_t(kvh * p.g) * p.q_head;
     const float* l0 = p.lse + int64_t(j.q0) * p.H + int64_t(kvh * p.g) * j.n;
-    auto load = [&](int i, int stage) {
-      const int head = i / n, pos = pos0 + (i - head * n) * R, left = j.n - pos;
-      uint8_t* to = lds + stage * STAGE;
+    uint8_t* mine = lds + half * STAGES * STAGE;
+    auto load = [&](int i, int stage) {   // (past the last tile too, of zeros: every stage is the same number of loads)
+      const int head = min(i / n, p.g - 1), pos = pos0 + (i % n) * R, left = i < all ? j.n - pos : 0;
+      uint8_t* to = mine + stage * STAGE;
       qt.load(to, q0 + int64_t(pos) * p.q_row + int64_t(head) * p.q_head, left, wv);
-      if (wv == 0) dma4(l0 + int64_t(head) * j.n + pos, lane < min(left, R) ? 4 * lane : kOutside, lds_address(to + TILE));
+      dma4(l0 + int64_t(head) * j.n + pos, lane < min(left, R) ? 4 * lane : kOutside, lds_address(to + TILE) + 256 * wv);
     };
-    load(0, 0);
-    for (int i = 0; i < all; ++i) {
-      dma_wait();
+    bf16x8 k[DP / 16];
+    row_operands<DP>(k, kbase, (int64_t(page) * kPage + key % kPage) * p.k.row, uint32_t(page) < uint32_t(p.n_pages), p.D, lane);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) load(half + kHalves * i, i);
+    dma_wait();   // (for k, so that the compiler does not wait for all loads in the loop)
+    for (int i = half, stage = 0; i - half < all; i += kHalves) {
+      dma_wait<(STAGES - 2) * LOADS>();
       __syncthreads();
-      if (i + 1 < all) load(i + 1, (i + 1) & 1);
-      const uint8_t* Q = lds + (i & 1) * STAGE;
-      const float* lse = reinterpret_cast<const float*>(Q + TILE);
+      load(i + kHalves * (STAGES - 1), stage == 0 ? STAGES - 1 : stage - 1);
+      const uint8_t* Q = mine + stage * STAGE;
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      if (i >= all) continue;
+      const float* lse = reinterpret_cast<const float*>(Q + TILE + 256 * wv);
       const int pos = pos0 + i % n * R;
 #pragma unroll
       for (int a = 0; a < SUB; ++a) {
@@ -640,9 +804,14 @@ __global__ __launch_bounds__(64 * kWaves) void paged_weights(Args p, const Job* 
         }
       }
     }
+    dma_wait();
   }
   sum += swap_halves(sum);
-  if (lane >= 32 || key >= p.longest) return;
+  if (lane < 32) other[half][32 * wv + lane] = sum;
+  __syncthreads();
+  if (half || lane >= 32 || key >= p.longest) return;
+#pragma unroll
+  for (int h = 1; h < kHalves; ++h) sum += other[h][32 * wv + lane];
   const int64_t row = int64_t(j.seq) * p.KV + kvh;
   float w = 0;
   if (key < j.len) w = (key < j.len - j.n && key < p.weights_width ? p.weights[row * p.weights_width + key] : 0.0f) + sum;
@@ -696,105 +865,116 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// The kept positions of one sequence, layer and head: the key of the least kept weight by four passes of 8 bits over the
-// candidates (counts in LDS, one set a wave), then the kept positions in order, by counts of those before each.
-template <int T>
+// The kept positions of one sequence, layer and head.  The candidates are those before the newest; wave w has them from w S on,
+// S a multiple of 64, as keys in IT registers a lane (IT 0: read again each time), 0 where there is none, which no weight's key
+// is.  The least kept key comes digit by digit (11, 11 and 10 bits) from counts in LDS; what is above it stays, and of what is
+// equal the first ones.  Each wave then counts what stays of its own, and writes it behind what stays of the waves before it.
+template <int T, int IT>
 __global__ __launch_bounds__(T) void paged_select(EvictArgs p) {
-  constexpr int W = T / 64;
-  __shared__ uint32_t counts[W][256];
-  __shared__ uint32_t state[4];    // key so far, how many are still to be taken
+  constexpr int W = T / 64, kBins = 2048, B = kBins / T;
+  __shared__ uint32_t counts[kBins];
+  __shared__ uint32_t state[2];    // key so far, how many equal ones are still to be taken
   __shared__ uint32_t sums[W][2];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, s = blockIdx.y, kvh = blockIdx.x % p.KV;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), s = blockIdx.y, kvh = blockIdx.x % p.KV;
   const SeqOf q = scalar_load(p.seqs + s);
   const int64_t row = (int64_t(blockIdx.x / p.KV) * p.n_seqs + s) * p.KV + kvh;
   const int len = q.len < 0 || q.len > p.longest ? 0 : q.len, held = min(len, p.keep);
   const int old = len - min(p.recent, len), heavy = held - (len - old);   // candidates, how many of them stay
+  const int read = min(old, p.weights_width);
   const float* w = p.weights + row * p.weights_width;
-  auto key_of = [&](int j) { return order_of(j < p.weights_width ? w[j] : 0.0f); };
-  uint32_t key = 0, need = heavy;
+  const int its = tiles_of(old, T), first = wv * its * 64 + lane;
+  auto load = [&](int j) { return j < read ? order_of(w[j]) : j < old ? order_of(0.0f) : 0u; };
+  uint32_t x[IT ? IT : 1];
+  if constexpr (IT) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) x[i] = i < its ? load(first + 64 * i) : 0;
+  }
+  auto each = [&](auto f) {   // f(position, key)
+    if constexpr (IT) {
+#pragma unroll
+      for (int i = 0; i < IT; ++i)
+        if (i < its) f(first + 64 * i, x[i]);
+    } else {
+      for (int i = 0; i < its; ++i) f(first + 64 * i, load(first + 64 * i));
+    }
+  };
+  uint32_t key = heavy > 0 ? 0 : 0xffffffffu, need = 0;   // (all candidates, or none, stay)
   if (heavy > 0 && heavy < old) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < W * 256; i += T) (&counts[0][0])[i] = 0;
-      __syncthreads();
-      for (int j = tid; j < old; j += T) {
-        const uint32_t x = key_of(j);
-        if (shift == 24 || x >> (shift + 8) == key >> (shift + 8)) atomicAdd(&counts[wv][x >> shift & 255], 1u);
-      }
-      __syncthreads();
-      for (int i = tid; i < 256; i += T) {
-        uint32_t n = 0;
-        for (int v = 0; v < W; ++v) n += counts[v][i];
-        counts[0][i] = n;
-      }
-      __syncthreads();
-      if (wv == 0) {   // from the largest digit down: lane l has digits 255 - 4 l .. 252 - 4 l
-        uint32_t n[4], mine = 0;
+    need = heavy;
+    auto digit = [&](int shift, uint32_t mask, uint32_t above) {   // above: the key's bits that are settled
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mine += n[i] = counts[0][255 - 4 * lane - i];
-        uint32_t before = mine;
+      for (int i = 0; i < B; ++i) counts[tid + T * i] = 0;
+      __syncthreads();
+      each([&](int, uint32_t k) {
+        if (!above || (k & above) == key) atomicAdd(&counts[k >> shift & mask], 1u);
+      });
+      __syncthreads();
+      uint32_t n[B], mine = 0;   // from the largest digit down
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const uint32_t x = __shfl_up(before, d);
-          if (lane >= d) before += x;
-        }
-        before -= mine;
-        if (before < need && before + mine >= need) {
-          int i = 0;
-          while (before + n[i] < need) before += n[i++];
-          state[0] = key | uint32_t(255 - 4 * lane - i) << shift;
-          state[1] = need - before;
+      for (int i = 0; i < B; ++i) mine += n[i] = counts[kBins - 1 - B * tid - i];
+      uint32_t before = mine;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const uint32_t y = __shfl_up(before, d);
+        if (lane >= d) before += y;
+      }
+      if (lane == 63) sums[wv][0] = before;
+      __syncthreads();
+      for (int v = 0; v < wv; ++v) before += sums[v][0];
+      before -= mine;
+      if (before < need && before + mine >= need) {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+          if (before < need && before + n[i] >= need) {
+            state[0] = key | uint32_t(kBins - 1 - B * tid - i) << shift;
+            state[1] = need - before;
+          }
+          before += n[i];
         }
       }
       __syncthreads();
       key = state[0];
       need = state[1];
-      __syncthreads();
-    }
+    };
+    digit(21, 2047, 0);
+    digit(10, 2047, 0xffe00000u);
+    digit(0, 1023, 0xfffffc00u);
   }
-  // keys above `key` stay, and the first `need` of those equal to it
-  const bool all = heavy >= old;
+  uint32_t aboves = 0, equals = 0;
+  each([&](int, uint32_t k) {
+    aboves += __popcll(__ballot(k > key));
+    equals += __popcll(__ballot(k == key));
+  });
+  __syncthreads();
+  if (lane == 0) {
+    sums[wv][0] = aboves;
+    sums[wv][1] = equals;
+  }
+  __syncthreads();
+  uint32_t at = 0, rank = 0;   // of what stays before, of equal ones before
+  for (int v = 0; v < wv; ++v) {
+    at += sums[v][0];
+    rank += sums[v][1];
+  }
+  at += min(rank, need);
   const int32_t* table = p.tables + int64_t(s) * p.width;
-  uint32_t n_kept = 0, n_equal = 0;   // before this round
-  for (int j0 = 0; j0 < len; j0 += T) {
-    const int j = j0 + tid;
-    bool above = false, equal = false;
-    float weight = 0;
-    if (j < len) {
-      weight = j < p.weights_width ? w[j] : 0.0f;
-      const uint32_t x = order_of(weight);
-      above = j >= old || all || (heavy > 0 && x > key);
-      equal = !above && heavy > 0 && x == key;
-    }
-    const uint64_t below = (uint64_t(1) << lane) - 1, ea = __ballot(equal);
-    if (lane == 0) sums[wv][0] = __popcll(ea);
-    __syncthreads();
-    uint32_t rank = n_equal + __popcll(ea & below), equals = 0;
-#pragma unroll
-    for (int v = 0; v < W; ++v) {
-      const uint32_t x = sums[v][0];
-      equals += x;
-      if (v < wv) rank += x;
-    }
-    const bool stays = above || (equal && rank < need);
-    const uint64_t ka = __ballot(stays);
-    if (lane == 0) sums[wv][1] = __popcll(ka);
-    __syncthreads();
-    uint32_t at = n_kept + __popcll(ka & below), kepts = 0;
-#pragma unroll
-    for (int v = 0; v < W; ++v) {
-      const uint32_t x = sums[v][1];
-      kepts += x;
-      if (v < wv) at += x;
-    }
-    if (stays && at < uint32_t(p.keep)) {
-      const int page = table[j / kPage];
-      p.kept[row * p.keep + at] = j;
-      p.weights_out[row * p.keep + at] = weight;
-      p.source[row * p.keep + at] = uint32_t(page) < uint32_t(p.n_pages) ? page * kPage + j % kPage : -1;
-    }
-    n_kept += kepts;
-    n_equal += equals;
-  }
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  auto write = [&](uint32_t to, int j) {
+    const int page = table[j / kPage];
+    p.kept[row * p.keep + to] = j;
+    p.weights_out[row * p.keep + to] = j < p.weights_width ? w[j] : 0.0f;
+    p.source[row * p.keep + to] = uint32_t(page) < uint32_t(p.n_pages) ? page * kPage + j % kPage : -1;
+  };
+  each([&](int j, uint32_t k) {
+    const uint64_t e = __ballot(k == key);
+    const bool stays = k > key || (k == key && rank + __popcll(e & below) < need);
+    rank += __popcll(e);
+    const uint64_t kept = __ballot(stays);
+    const uint32_t to = at + __popcll(kept & below);
+    at += __popcll(kept);
+    if (stays && to < uint32_t(p.keep)) write(to, j);
+  });
+  for (int i = max(heavy, 0) + tid; i < held; i += T) write(i, len - held + i);   // the newest
   for (int i = held + tid; i < p.keep; i += T) {
     p.kept[row * p.keep + i] = -1;
     p.weights_out[row * p.keep + i] = 0;
@@ -832,7 +1012,7 @@ __global__ __launch_bounds__(256) void paged_move(EvictArgs p, int blocks) {
 // ---- host: the plan ----
 // Workgroups that a launch is shared out to, about, and tiles of a job at least.
 constexpr int kFewGroups = 1024, kManyGroups = 512;
-constexpr int kFewLeast = 4, kManyLeast = 2;
+constexpr int kFewLeast = 4, kManyLeast = 8;
 
 struct Pieces {
   int64_t each;
@@ -859,15 +1039,15 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
     return MSD_E_CONFIG;
   if (n_seqs && (!seqs || (table_width && !tables))) return MSD_E_ARG;
   const int64_t g = H / KV;
-  int most = 0;
+  int most = 0;   // (lengths up to kLongest: the next tile's first position is a number too)
   int64_t q_end = 0, q_count = 0;
   std::vector<int> few, many;   // sequences
-  int64_t few_tiles = 0, many_tiles = 0, row_tiles = 0, appends = 0, scores = 0;
+  int64_t few_tiles = 0, few_rows = 0, many_tiles = 0, row_tiles = 0, appends = 0, scores = 0;
   auto seen = [&](const int32_t* s, int64_t row) { return s[2] - s[1] + 1 + row / g; };   // positions that the row sees
   for (int b = 0; b < n_seqs; ++b) {
     const int32_t* s = seqs + 3 * b;
     const int64_t rows = s[1] * g;
-    if (s[0] < 0 || s[1] < 0 || s[2] < s[1] || s[2] > int64_t(table_width) * kPage || (longest && s[2] > longest) || s[0] > INT32_MAX - s[1] ||
+    if (s[0] < 0 || s[1] < 0 || s[2] < s[1] || s[2] > std::min<int64_t>(int64_t(table_width) * kPage, kLongest) || (longest && s[2] > longest) || s[0] > INT32_MAX - s[1] ||
         rows >= (1 << 30) - 256)
       return MSD_E_CONFIG;
     most = std::max(most, s[2]);
@@ -876,6 +1056,7 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
     if (rows <= kFewRows) {
       few.push_back(b);
       if (rows) few_tiles += cdiv(s[2], kFewKeys);
+      few_rows = std::max(few_rows, rows);
       scores += rows * cdiv(longest ? longest : s[2], kFewKeys);
     } else {
       many.push_back(b);
@@ -884,7 +1065,7 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
     if (longest) appends += s[1] ? cdiv(s[1], kPage) + 1 : 0;
     else if (s[1]) appends += cdiv(s[2], kPage) - (s[2] - s[1]) / kPage;
   }
-  if (longest > int64_t(table_width) * kPage) return MSD_E_CONFIG;
+  if (longest > std::min<int64_t>(int64_t(table_width) * kPage, kLongest)) return MSD_E_CONFIG;
   const Pieces fp = pieces(few_tiles, KV, kFewGroups, kFewLeast), mp = pieces(many_tiles, KV, kManyGroups, kManyLeast);
   int64_t n_few = 0, n_many = 0, few_active = 0;
   bool few_parts = false, many_parts = false;
@@ -939,6 +1120,7 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
   words[N_APPENDS] = int32_t(appends);
   words[FEW_PARTS] = few_parts;
   words[MANY_PARTS] = many_parts;
+  words[FEW_ROWS] = int32_t(few_rows);
   words[SCORES] = int32_t(scores);
   words[AT_SEQS] = int32_t(at_seqs);
   words[AT_FEW] = int32_t(at_few);
@@ -1132,7 +1314,9 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
   if (reinterpret_cast<uintptr_t>(weights_out) % 4) return MSD_E_ARG;
   const int64_t KV = h[MSD_PLAN_KV_HEADS], longest = h[MSD_PLAN_LONGEST], most = (int64_t(1) << 32) / 256 - 1;
   const int64_t key_blocks = cdiv(longest, 128), weight_blocks = weighted ? cdiv(longest, kWeightKeys) : 0;
-  const int64_t finish = (h[MANY_PARTS] ? int64_t(h[N_TILES]) * KV * kWaves : 0) + int64_t(h[N_FEWS]) * KV * (1 + weight_blocks);
+  const int n_tiles = h[MANY_PARTS] ? h[N_TILES] : 0, n_fews = h[FEW_PARTS] || weighted ? h[N_FEWS] : 0;
+  const int few_joins = h[FEW_PARTS] ? int(cdiv(h[FEW_ROWS], kJoinRows)) : 0;
+  const int64_t finish = int64_t(n_tiles) * KV * (kManyRows / kJoinRows) + int64_t(n_fews) * KV * (few_joins + weight_blocks);
   if (finish > most || key_blocks * KV * h[N_MANYS] > most) return MSD_E_CONFIG;
   if (h[MSD_PLAN_Q_COUNT] && (bad(q) || bad(k) || bad(v) || bad(out))) return MSD_E_ARG;
   const Space at = space(*a, weighted);
@@ -1184,15 +1368,13 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
       hipLaunchKernelGGL((paged_many<DP>), dim3(unsigned(h[N_MANY] * KV)), dim3(64 * kWaves), 0, s, p);
     }
   });
-  const int n_tiles = h[MANY_PARTS] ? h[N_TILES] : 0, n_fews = h[FEW_PARTS] || weighted ? h[N_FEWS] : 0;
-  const int64_t groups = int64_t(n_tiles) * KV * kWaves + int64_t(n_fews) * KV * (1 + weight_blocks);
-  if (groups)
-    hipLaunchKernelGGL(paged_finish, dim3(unsigned(groups)), dim3(kFinish), 0, s, p, reinterpret_cast<const RowTile*>(a->plan + h[AT_TILES]),
-                       n_tiles, reinterpret_cast<const Few*>(a->plan + h[AT_FEWS]), n_fews);
+  if (finish)
+    hipLaunchKernelGGL(paged_finish, dim3(unsigned(finish)), dim3(kFinish), 0, s, p, reinterpret_cast<const RowTile*>(a->plan + h[AT_TILES]),
+                       n_tiles, reinterpret_cast<const Few*>(a->plan + h[AT_FEWS]), n_fews, few_joins);
   if (weighted && h[N_MANYS] && key_blocks)
     with_head(a->d_head, [&](auto dp) {
       constexpr int DP = decltype(dp)::value;
-      hipLaunchKernelGGL((paged_weights<DP>), dim3(unsigned(key_blocks * KV * h[N_MANYS])), dim3(64 * kWaves), 0, s, p, manys, h[N_MANYS]);
+      hipLaunchKernelGGL((paged_weights<DP>), dim3(unsigned(key_blocks * KV * h[N_MANYS])), dim3(64 * kWaves * kHalves), 0, s, p, manys, h[N_MANYS]);
     });
   return launched();
 }
@@ -1250,8 +1432,10 @@ extern "C" int32_t msd_paged_evict(const msd_paged* a, int32_t n_layers, int64_t
   const dim3 rows(n_layers * p.KV, p.n_seqs);
   const int64_t blocks = cdiv(int64_t(keep) * p.pieces, 256 * kMove);
   if (blocks * p.n_seqs * 256 >= int64_t(1) << 32) return MSD_E_CONFIG;
-  if (p.longest <= 4096) hipLaunchKernelGGL(paged_select<256>, rows, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL(paged_select<1024>, rows, dim3(1024), 0, s, p);
+  if (p.longest <= 2048) hipLaunchKernelGGL((paged_select<256, 8>), rows, dim3(256), 0, s, p);
+  else if (p.longest <= 8192) hipLaunchKernelGGL((paged_select<1024, 8>), rows, dim3(1024), 0, s, p);
+  else if (p.longest <= 32768) hipLaunchKernelGGL((paged_select<1024, 32>), rows, dim3(1024), 0, s, p);
+  else hipLaunchKernelGGL((paged_select<1024, 0>), rows, dim3(1024), 0, s, p);
   hipLaunchKernelGGL(paged_move, dim3(unsigned(blocks * p.n_seqs), n_layers * p.KV, 2), dim3(256), 0, s, p, int(blocks));
   return launched();
 }

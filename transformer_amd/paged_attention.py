@@ -27,6 +27,8 @@ from . import _lib
 from .attention import _fits, _ranges
 from .paged import PAGE
 
+LONGEST = 2 ** 31 - 2 ** 16 - 1   # positions of a sequence
+
 
 def _words(q_lens, lengths, q_starts, tables, n_heads, n_kv_heads, longest):
     """The library's plan of a step as an int32 tensor on the host."""
@@ -85,8 +87,8 @@ class PagedSequences:
         self.n, self.n_heads, self.n_kv_heads = len(self.q_lens), int(n_heads), int(n_kv_heads)
         if self.n_kv_heads < 1 or self.n_heads < 1 or self.n_heads % self.n_kv_heads or self.n_heads > 4096:
             raise ValueError(f"n_heads ({n_heads}) must be a multiple of n_kv_heads ({n_kv_heads}), up to 4096")
-        if longest is not None and not 1 <= longest < 2 ** 31 - PAGE:
-            raise ValueError(f"longest must lie in [1, 2**31 - {PAGE}) (got {longest})")
+        if longest is not None and not 1 <= longest <= LONGEST:
+            raise ValueError(f"longest must lie in [1, {LONGEST}] (got {longest})")
         self._reserved = 0 if longest is None else int(longest)
         self.host = self._plan(lengths, tables)
         self.table = self.host.to(device)
@@ -99,8 +101,8 @@ class PagedSequences:
             raise ValueError(f"{self.n} lengths of new tokens, {len(lengths)} lengths")
         if any(n < q for n, q in zip(lengths, self.q_lens)):
             raise ValueError("a length counts the new tokens and cannot be less")
-        if max(lengths, default=0) >= 2 ** 31 - PAGE or self._reserved and max(lengths, default=0) > self._reserved:
-            raise ValueError(f"length {max(lengths)} outside [0, {self._reserved or 2 ** 31 - PAGE}]")
+        if max(lengths, default=0) > (self._reserved or LONGEST):
+            raise ValueError(f"length {max(lengths)} outside [0, {self._reserved or LONGEST}]")
         pages = _tables(tables, [-(-n // PAGE) for n in lengths], "tables")
         if self._reserved:
             pages = np.pad(pages, ((0, 0), (0, -(-self._reserved // PAGE) - pages.shape[1])))
@@ -130,7 +132,7 @@ class PagedEviction:
     def __init__(self, sequences, keep, recent, tables):
         self.sequences, self.version = sequences, sequences.version
         self.keep, self.recent = int(keep), int(recent)
-        if not 0 <= self.recent <= self.keep < 2 ** 31 - PAGE:
+        if not 0 <= self.recent <= self.keep <= LONGEST:
             raise ValueError(f"0 <= recent <= keep expected (got {recent} and {keep})")
         self.lengths = [min(n, self.keep) for n in sequences.lengths]
         needed = [-(-n // PAGE) for n in self.lengths]
