@@ -258,8 +258,7 @@ def test_c_calls_outside_the_limits(bad):
     assert L.msd_paged_attn_workspace_bytes(p, 0) == _lib.MSD_E_CONFIG
     assert L.msd_paged_attn(p, 256, 256, 256, 256, None, 0, None, 256, None) == _lib.MSD_E_CONFIG
     assert L.msd_paged_append(p, 256, stride, 256, stride, 256, 256, None) == _lib.MSD_E_CONFIG
-    assert L.msd_paged_evict_workspace_bytes(p, 1, 16) == _lib.MSD_E_CONFIG
-    assert L.msd_paged_evict(p, 1, 0, 0, 256, 256, 256, 40, 16, 4, 256, 1, 256, 256, 256, None) == _lib.MSD_E_CONFIG
+    assert L.msd_paged_evict(p, 1, 0, 0, 256, 256, 256, 40, 16, 4, 256, 1, 256, 256, None) == _lib.MSD_E_CONFIG
 
 
 def test_c_calls_with_bad_pointers():
@@ -279,9 +278,9 @@ def test_c_calls_with_bad_pointers():
     assert L.msd_paged_attn(p, 256, 256, 256, 256, 256, -1, 256, 256, None) == _lib.MSD_E_CONFIG
     assert L.msd_paged_append(p, 256, None, 256, stride, 256, 256, None) == A
     assert L.msd_paged_append(p, 256, odd, 256, stride, 256, 256, None) == _lib.MSD_E_CONFIG
-    evict = lambda k=256, v=256, w=256, to=256, out=256, kept=256, ws=256, keep=16, recent=4, width=1, layers=1, layer=0: L.msd_paged_evict(  # noqa: E731
-        p, layers, layer, layer, k, v, w, 40, keep, recent, to, width, out, kept, ws, None)
-    for name in ("k", "v", "w", "to", "out", "kept", "ws"):
+    evict = lambda k=256, v=256, w=256, to=256, out=256, kept=256, keep=16, recent=4, width=1, layers=1, layer=0: L.msd_paged_evict(  # noqa: E731
+        p, layers, layer, layer, k, v, w, 40, keep, recent, to, width, out, kept, None)
+    for name in ("k", "v", "w", "to", "out", "kept"):
         assert evict(**{name: None}) == A and evict(**{name: 257}) == A
     for bad in (dict(recent=17), dict(recent=-1), dict(keep=17), dict(keep=-1, recent=-1), dict(width=-1), dict(layers=-1), dict(layers=32768), dict(layer=4), dict(layer=-8)):
         assert evict(**bad) == _lib.MSD_E_CONFIG, bad

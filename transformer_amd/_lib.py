@@ -32,7 +32,7 @@ EXPORTS = ("msd_packed_weight_elems", "msd_workspace_bytes", "msd_default_workgr
            "msd_attn_workspace_bytes", "msd_attn_forward", "msd_attn_backward", "msd_rope_apply",
            "msd_checkpoint_bytes", "msd_rms_forward", "msd_rms_workspace_bytes", "msd_rms_backward",
            "msd_swiglu_forward", "msd_swiglu_backward", "msd_paged_plan", "msd_paged_append",
-           "msd_paged_attn_workspace_bytes", "msd_paged_attn", "msd_paged_evict_workspace_bytes", "msd_paged_evict")
+           "msd_paged_attn_workspace_bytes", "msd_paged_attn", "msd_paged_evict")
 
 # Paths of the library (bits of msd_config_support)
 PATHS = {"decode": 1, "prefill": 2, "verify": 4, "batched": 8, "sample": 16, "batched_step": 32}
@@ -191,9 +191,7 @@ def lib():
     L.msd_paged_attn_workspace_bytes.restype = I64
     L.msd_paged_attn.argtypes = [GP, P, P, P, P, P, I32, P, P, P]
     L.msd_paged_attn.restype = I32
-    L.msd_paged_evict_workspace_bytes.argtypes = [GP, I32, I32]
-    L.msd_paged_evict_workspace_bytes.restype = I64
-    L.msd_paged_evict.argtypes = [GP, I32, I64, I64, P, P, P, I32, I32, I32, P, I32, P, P, P, P]
+    L.msd_paged_evict.argtypes = [GP, I32, I64, I64, P, P, P, I32, I32, I32, P, I32, P, P, P]
     L.msd_paged_evict.restype = I32
     _lib = L
     return L

@@ -69,12 +69,12 @@ struct Args {
   int n_seqs, width, longest, n_pages;
   const int32_t* plan;
   const int32_t* tables;
-  const Job* jobs;                // of the launch
+  const Job *few, *many;
   int n_few, n_many;
   uint16_t* out;
   float *few_part, *few_lse;      // [slot][kv head][32] rows of D, logsumexps
   float *many_part, *many_lse;    // [slot][kv head][128]
-  float* lse;                     // of every row of many, sequence by sequence, head by head, or null
+  float* lse;                     // -L_i / c of every row of many, sequence by sequence, head by head, or null
   float* scores;                  // c q.k of few rows, [sequence][kv head][row][keys up to a multiple of 32], or null
   int64_t score_words;
   const float* weights;
@@ -117,6 +117,14 @@ __device__ __forceinline__ const uint16_t* row_at(const Args& p, int q0, int kvh
   return p.q + int64_t(q0 + pos) * p.q_row + int64_t(kvh * p.g + of_group) * p.q_head;
 }
 
+// As dma(), of what is read once
+__device__ __forceinline__ void dma_once(const uint16_t* base, uint32_t off, uint32_t to) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, 0x7fffffff, 0x00020000);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(to), "v"(off), "s"(r) : "m0");
+#endif
+}
+
 // A tile of R positions on its way from pages to LDS, NW waves: an instruction's rows are 8 (or 4) of one page.
 template <int DP, int R, int NW>
 struct PagedTile {
@@ -139,7 +147,7 @@ struct PagedTile {
     for (int u = 0; u < N; ++u) {
       const uint32_t at = page((ROWS * wv + ROWS * NW * u) / kPage);
       const bool there = at < uint32_t(n_pages);
-      dma(head + int64_t(there ? at : 0) * (kPage * row_stride), row + ROWS * NW * u < (there ? left : 0) ? off[u % KINDS] : kOutside,
+      dma_once(head + int64_t(there ? at : 0) * (kPage * row_stride), row + ROWS * NW * u < (there ? left : 0) ? off[u % KINDS] : kOutside,
           to + 1024 * (wv + NW * u));
     }
   }
@@ -221,14 +229,17 @@ template <int DP>
 constexpr int few_waves() { return DP <= 64 ? 4 : 2; }
 
 template <int DP>
-__global__ __launch_bounds__(64 * few_waves<DP>(), 2) void paged_few(Args p) {
+constexpr int few_lds() { return few_waves<DP>() * (4 * kFewKeys * pitch<DP>() + 256); }   // and two statistics of 32 rows a wave
+
+// Workgroup `group` of few rows
+template <int DP>
+__device__ __forceinline__ void few_rows(const Args& p, int group, uint8_t* lds) {
   constexpr int P = pitch<DP>(), W = few_waves<DP>(), TILE = kFewKeys * P, OROW = DP + 4;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[W * 4 * TILE];
-  __shared__ float stats[W][2][32];
+  float(*stats)[2][32] = reinterpret_cast<float(*)[2][32]>(lds + W * 4 * TILE);
   static_assert(4 * TILE >= 4 * 32 * OROW, "a wave's part of the output");
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kvh = blockIdx.x % p.KV;
-  const Job j = scalar_load(p.jobs + blockIdx.x / p.KV);
+  const int kvh = group % p.KV;
+  const Job j = scalar_load(p.few + group / p.KV);
   const int R = j.n * p.g;
   if (!sound(p, j.q0, j.n, j.len, j.seq) || R > kFewRows || j.t0 < 0 || j.t1 > tiles_of(j.len, kFewKeys) || j.slot < 0 || j.slot >= p.n_few)
     return;
@@ -382,14 +393,14 @@ __device__ __forceinline__ void order_steps() {
 #endif
 }
 
+// Workgroup `group` of many rows; lds: four halves of K, four of V
 template <int DP>
-__global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void paged_many(Args p) {
+__device__ __forceinline__ void many_rows(const Args& p, int group, uint8_t* lds) {
   using Half = HalfTile<DP>;
   constexpr int P = pitch<DP>(), BYTES = Half::BYTES, KS = DP / 16, DB = DP / 32;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[8 * BYTES];   // four halves of K, four of V
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kvh = blockIdx.x % p.KV;
-  const Job j = scalar_load(p.jobs + blockIdx.x / p.KV);
+  const int kvh = group % p.KV;
+  const Job j = scalar_load(p.many + group / p.KV);
   const int rows = j.n * p.g, row0 = j.row0 < 0 ? -j.row0 - 1 : j.row0;
   const bool only = j.row0 < 0;
   if (!sound(p, j.q0, j.n, j.len, j.seq) || row0 >= rows || j.t0 < 0 || j.t1 <= j.t0 || j.t1 > tiles_of(j.len, kKeys) || j.slot < 0 || j.slot >= p.n_many)
@@ -592,13 +603,37 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void paged_many(Args
     }
     return;
   }
-  if (p.lse && ok && lane < 32) p.lse[int64_t(j.q0) * p.H + int64_t(kvh * p.g + r - pos * p.g) * j.n + pos] = lse;
+  if (p.lse && ok && lane < 32) p.lse[int64_t(j.q0) * p.H + int64_t(kvh * p.g + r - pos * p.g) * j.n + pos] = -lse / p.c;
   const int r0 = r - (lane & 31);
   store_rows<DP>(lds + wv * 32 * P, o, by, p.D, lane, [&](int i) -> uint16_t* {
     if (r0 + i >= rows) return nullptr;
     const int at = div_g(p, r0 + i);
     return p.out + (int64_t(j.q0 + at) * p.H + (kvh * p.g + (r0 + i - at * p.g))) * p.D;
   });
+}
+
+template <int DP>
+__global__ __launch_bounds__(64 * few_waves<DP>(), 2) void paged_few(Args p) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds<DP>()];
+  few_rows<DP>(p, blockIdx.x, lds);
+}
+template <int DP>
+constexpr int many_lds() { return 8 * HalfTile<DP>::BYTES; }
+template <int DP>
+__global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void paged_many(Args p) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[many_lds<DP>()];
+  many_rows<DP>(p, blockIdx.x, lds);
+}
+// A step of both: tokens' workgroups, which wait for memory, spread among the chunks', which wait for the matrix cores.
+template <int DP>
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_both(Args p) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(few_lds<DP>(), many_lds<DP>())];
+  const uint32_t few = p.n_few * p.KV, b = blockIdx.x, before = uint32_t(uint64_t(b) * few / gridDim.x);
+  if (uint32_t(uint64_t(b + 1) * few / gridDim.x) > before) {
+    if (threadIdx.x < 64 * few_waves<DP>()) few_rows<DP>(p, before, lds);   // (whole waves: the others end)
+  } else {
+    many_rows<DP>(p, b - before, lds);
+  }
 }
 
 // ---- what is left ----
@@ -654,7 +689,7 @@ __device__ __forceinline__ void join(const Args& p, float (*lds)[11], const floa
   for (int i = 0; i < 4; ++i) x[i] = pack2(acc[2 * i] * by, acc[2 * i + 1] * by);
   const int pos = div_g(p, row0 + row), head = kvh * p.g + row0 + row - pos * p.g;
   *reinterpret_cast<u32x4*>(p.out + (int64_t(q0 + pos) * p.H + head) * p.D + 8 * c) = x;
-  if (keep && c == 0) p.lse[int64_t(q0) * p.H + int64_t(head) * n + pos] = l == 0 ? INFINITY : m + __log2f(l);
+  if (keep && c == 0) p.lse[int64_t(q0) * p.H + int64_t(head) * n + pos] = l == 0 ? -INFINITY : -(m + __log2f(l)) / p.c;
 }
 
 __global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* tiles, int n_tiles, const Few* fews, int n_fews, int few_joins) {
@@ -739,12 +774,13 @@ __global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* t
 
 // ---- the weights of many rows ----
 // 128 keys a workgroup, 32 a wave in registers, over the group's heads and the rows that see them: S = Q K^T, a lane holds one
-// key's scores against 16 rows, so that its sum stays in the lane.  Two halves of four waves take the row tiles in turn, so
-// that a SIMD has the products of one wave beside the exponentials of the other.
+// key's scores against 16 rows, so that its sum stays in the lane; a row's scores start as -L_i / c (what p.lse holds here).  Two
+// halves of four waves take the tiles of 64 rows in turn.  While the probabilities of 32 rows are formed, the matrix cores form the
+// next 32 rows' scores.
 constexpr int kHalves = 2;
 template <int DP>
 __global__ __launch_bounds__(64 * kWaves * kHalves) void paged_weights(Args p, const Job* seqs, int n_seqs) {
-  constexpr int P = pitch<DP>(), R = DP <= 64 ? 64 : 32, TILE = R * P, STAGE = TILE + 256 * kWaves, SUB = R / 32, STAGES = 4;
+  constexpr int P = pitch<DP>(), R = 64, TILE = R * P, STAGE = TILE + 256 * kWaves, STAGES = 3, KS = DP / 16;
   constexpr int LOADS = TILE / 1024 / kWaves + 1;   // of a wave and stage: rows, and their logsumexps, of which each wave has its own
   __shared__ __attribute__((aligned(16))) uint8_t lds[kHalves * STAGES * STAGE];
   __shared__ float other[kHalves][kWaves * 32];
@@ -757,53 +793,107 @@ __global__ __launch_bounds__(64 * kWaves * kHalves) void paged_weights(Args p, c
   if (128 * kb < j.len) {
     const uint16_t* kbase = p.k.p + kvh * p.k.head;
     const int page = key < j.len ? p.tables[int64_t(j.seq) * p.width + key / kPage] : -1;
-    const int pos0 = max(128 * kb - (j.len - j.n), 0) / R * R, n = (j.n - pos0 + R - 1) / R, all = n * p.g;   // row tiles a head, of the group
+    const int before = j.len - j.n, pos0 = max(128 * kb - before, 0) / R * R, n = (j.n - pos0 + R - 1) / R, all = n * p.g;   // tiles a head, of the group
     Tile<DP, R> qt;
     qt.init(p.q_row, p.D, lane, wv);
-    const uint16_t* q0 = p.q + int64_t(j.q0) * p.q_row + int64_t(kvh * p.g) * p.q_head;
-    const float* l0 = p.lse + int64_t(j.q0) * p.H + int64_t(kvh * p.g) * j.n;
-    uint8_t* mine = lds + half * STAGES * STAGE;
-    auto load = [&](int i, int stage) {   // (past the last tile too, of zeros: every stage is the same number of loads)
-      const int head = min(i / n, p.g - 1), pos = pos0 + (i % n) * R, left = i < all ? j.n - pos : 0;
-      uint8_t* to = mine + stage * STAGE;
-      qt.load(to, q0 + int64_t(pos) * p.q_row + int64_t(head) * p.q_head, left, wv);
-      dma4(l0 + int64_t(head) * j.n + pos, lane < min(left, R) ? 4 * lane : kOutside, lds_address(to + TILE) + 256 * wv);
+    // this half's way through the tiles, head by head
+    const uint16_t* q = p.q + int64_t(j.q0 + pos0 + half * R) * p.q_row + int64_t(kvh * p.g) * p.q_head;
+    const float* l = p.lse + int64_t(j.q0) * p.H + int64_t(kvh * p.g) * j.n + pos0 + half * R;
+    const int64_t q_on = kHalves * R * p.q_row, q_back = p.q_head - n * R * p.q_row;   // to the next tile; from behind a head's last to the next's
+    int left = j.n - pos0 - half * R, tiles = (all - half + kHalves - 1) / kHalves;     // rows from the tile on; tiles to be fetched
+    const int last = j.n - pos0 - n * R;                                                // (0 or less: of the rows behind the last tile)
+    const uint32_t mine = lds_address(lds) + half * STAGES * STAGE;
+    auto load = [&](int stage) {   // (past the last tile too, of zeros: every stage is the same number of loads)
+      while (left <= last) {
+        left += n * R;
+        q += q_back;
+        l += j.n - n * R;
+      }
+      const uint32_t to = mine + stage * STAGE + 1024 * wv;
+      const int there = tiles > 0 ? left : 0;
+      const uint16_t* from = tiles > 0 ? q : p.q;
+#pragma unroll
+      for (int u = 0; u < LOADS - 1; ++u)
+        dma(from, qt.row + 64 * kWaves / (P / 16) * u < there ? qt.off[u] : kOutside, to + 1024 * kWaves * u);
+      dma4(tiles > 0 ? l : p.lse, lane < there ? 4 * lane : kOutside, mine + stage * STAGE + TILE + 256 * wv);
+      --tiles;
+      left -= kHalves * R;
+      q += q_on;
+      l += kHalves * R;
     };
-    bf16x8 k[DP / 16];
+    bf16x8 k[KS];
     row_operands<DP>(k, kbase, (int64_t(page) * kPage + key % kPage) * p.k.row, uint32_t(page) < uint32_t(p.n_pages), p.D, lane);
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) load(half + kHalves * i, i);
+    for (int i = 0; i < STAGES - 1; ++i) load(i);
+    uint32_t q_at[KS], l_at = mine + TILE + 256 * wv + 16 * (lane >> 5);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q_at[ks] = mine + piece_at<P>(lane & 31, 2 * ks + (lane >> 5));
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm("" : "+v"(q_at[ks]));
+    asm("" : "+v"(l_at));
+    typedef __attribute__((address_space(3))) const bf16x8 lds_bf16x8;
+    typedef __attribute__((address_space(3))) const f32x4 lds_f32x4;
+#else
+    typedef const bf16x8 lds_bf16x8;
+    typedef const f32x4 lds_f32x4;
+#endif
     dma_wait();   // (for k, so that the compiler does not wait for all loads in the loop)
-    for (int i = half, stage = 0; i - half < all; i += kHalves) {
+    f32x16 s0, s1;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s1[i] = -INFINITY;
+    int pos = pos0 + half * R;   // of the tile that is worked on
+    // ahead: the scores of rows 32 a .. of the tile in a stage; s: those before, which are summed
+    auto step = [&](f32x16& ahead, const f32x16& s, int stage, int a) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const f32x4 x = *(lds_f32x4*)(uintptr_t)(l_at + stage * STAGE + 128 * a + 32 * u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ahead[4 * u + i] = x[i];
+      }
+      bf16x8 f[3];
+      auto operand = [&](int ks) { return *(lds_bf16x8*)(uintptr_t)(q_at[ks] + stage * STAGE + 32 * a * P); };
+#pragma unroll
+      for (int i = 0; i < 2; ++i) f[i] = operand(i);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (ks + 2 < KS) f[(ks + 2) % 3] = operand(ks + 2);
+        ahead = mfma(f[ks % 3], k[ks], ahead);
+#pragma unroll
+        for (int i = 16 * ks / KS; i < 16 * (ks + 1) / KS; ++i) sum += exp2_hw(s[i] * p.c);
+        order_steps();
+      }
+      const int at = pos + 32 * a;
+      if (before + at < k0 + 31 || at + 32 > j.n) {   // the diagonal, the last rows
+        const int hidden = max(key - before, 0) - at - 4 * (lane >> 5), rows = j.n - at - 4 * (lane >> 5);   // (a row sees the key from `hidden` on)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i >> 2) + (i & 3) < hidden || 8 * (i >> 2) + (i & 3) >= rows) ahead[i] = -INFINITY;
+      }
+    };
+    int work = (all - half + kHalves - 1) / kHalves;
+    auto tile = [&](int stage, int next) {
       dma_wait<(STAGES - 2) * LOADS>();
       __syncthreads();
-      load(i + kHalves * (STAGES - 1), stage == 0 ? STAGES - 1 : stage - 1);
-      const uint8_t* Q = mine + stage * STAGE;
-      stage = stage + 1 == STAGES ? 0 : stage + 1;
-      if (i >= all) continue;
-      const float* lse = reinterpret_cast<const float*>(Q + TILE + 256 * wv);
-      const int pos = pos0 + i % n * R;
-#pragma unroll
-      for (int a = 0; a < SUB; ++a) {
-        f32x16 s = {};
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) s = mfma(rows_operand<P>(Q, 32 * a, ks, lane), k[ks], s);
-        const int row = pos + 32 * a + 4 * (lane >> 5);
-        if (j.len - j.n + pos + 32 * a < k0 + 31 || pos + 32 * a + 32 > j.n) {   // the diagonal, the last rows
-#pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const int at = row + 8 * (v >> 2) + (v & 3);
-            if (at >= j.n || key > j.len - j.n + at) s[v] = -INFINITY;
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const f32x4 l = *reinterpret_cast<const f32x4*>(lse + 32 * a + 8 * u + 4 * (lane >> 5));
-#pragma unroll
-          for (int v = 0; v < 4; ++v) sum += exp2_hw(fmaf(s[4 * u + v], p.c, -l[v]));
-        }
+      load(next);
+      if (work-- > 0) {
+        while (pos - pos0 >= n * R) pos -= n * R;
+        step(s0, s1, stage, 0);
+        step(s1, s0, stage, 1);
+        pos += kHalves * R;
       }
+    };
+    static_assert(STAGES == 3, "the stages in turn");
+    for (int i = (all + kHalves - 1) / kHalves; i > 0;) {
+      tile(0, 2);
+      if (--i == 0) break;
+      tile(1, 0);
+      if (--i == 0) break;
+      tile(2, 1);
+      --i;
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += exp2_hw(s1[i] * p.c);
     dma_wait();
   }
   sum += swap_halves(sum);
@@ -829,18 +919,32 @@ struct AppendArgs {
   int64_t q_rows, positions;
 };
 
-// The rows of one page and sequence: memory bound, a head's rows one behind the other as the pool's layout has them.
+// The rows of one page and sequence, up to 256 16-byte pieces of a head: a thread has one piece of every head (of every second,
+// fourth, .. where there are fewer), K's heads, then V's.  Memory bound.  Stores that do not stay in the caches: 16383 tokens of 8
+// heads of 128 to pages that are not in them take 53 us in place of 58.
 __global__ __launch_bounds__(256) void paged_append(AppendArgs p) {
   const Append a = scalar_load(p.jobs + blockIdx.x);
   if (a.row < 0 || a.count <= 0 || a.count > kPage || a.row > p.q_rows - a.count || a.position < 0 || a.position > p.positions - a.count)
     return;
-  const int head_pieces = a.count * p.pieces, all = p.KV * head_pieces;
-  for (int i = threadIdx.x; i < 2 * all; i += 256) {
-    const bool value = i >= all;
-    const int at = value ? i - all : i, head = at / head_pieces, in = at - head * head_pieces, r = in / p.pieces, c = in - r * p.pieces;
-    const uint16_t* from = value ? p.v_new + (a.row + r) * p.v_new_row + head * p.v_new_head : p.k_new + (a.row + r) * p.k_new_row + head * p.k_new_head;
-    uint16_t* to = value ? p.v + (a.position + r) * p.v_row + head * p.v_head : p.k + (a.position + r) * p.k_row + head * p.k_head;
-    *reinterpret_cast<u32x4*>(to + 8 * c) = *reinterpret_cast<const u32x4*>(from + 8 * c);
+  const int n = a.count * p.pieces, heads = 256 / n, h0 = threadIdx.x / n, i = threadIdx.x - h0 * n, r = i / p.pieces, c = i - r * p.pieces;
+  if (h0 >= heads) return;
+  const uint16_t *k_from = p.k_new + (a.row + r) * p.k_new_row + 8 * c, *v_from = p.v_new + (a.row + r) * p.v_new_row + 8 * c;
+  uint16_t *k_to = p.k + (a.position + r) * p.k_row + 8 * c, *v_to = p.v + (a.position + r) * p.v_row + 8 * c;
+  constexpr int U = 4;
+  for (int h = h0; h < p.KV; h += U * heads) {
+    u32x4 x[2 * U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (h + u * heads < p.KV) {
+        x[2 * u] = *reinterpret_cast<const u32x4*>(k_from + (h + u * heads) * p.k_new_head);
+        x[2 * u + 1] = *reinterpret_cast<const u32x4*>(v_from + (h + u * heads) * p.v_new_head);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (h + u * heads < p.KV) {
+        __builtin_nontemporal_store(x[2 * u], reinterpret_cast<u32x4*>(k_to + (h + u * heads) * p.k_head));
+        __builtin_nontemporal_store(x[2 * u + 1], reinterpret_cast<u32x4*>(v_to + (h + u * heads) * p.v_head));
+      }
   }
 }
 
@@ -855,14 +959,16 @@ struct EvictArgs {
   int width, to_width, n_pages, longest;
   int n_seqs, KV, pieces;
   float* weights_out;
-  int32_t *kept, *source;      // source: the pool's positions of the kept rows, or -1
+  int32_t* kept;
 };
 
 // Weights in the order of eviction as unsigned numbers: larger is kept first; -0 is 0, a NaN the largest.
 __device__ __forceinline__ uint32_t order_of(float x) {
-  if (x != x) return 0xffffffffu;
-  const uint32_t b = __float_as_uint(x == 0 ? 0.0f : x);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const uint32_t b = __float_as_uint(x + 0.0f), key = b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);   // (-0 + 0 is 0)
+  return x != x ? 0xffffffffu : key;
+}
+__device__ __forceinline__ float weight_of(uint32_t key) {   // (a NaN, of many)
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
 // The kept positions of one sequence, layer and head.  The candidates are those before the newest; wave w has them from w S on,
@@ -883,11 +989,16 @@ __global__ __launch_bounds__(T) void paged_select(EvictArgs p) {
   const int read = min(old, p.weights_width);
   const float* w = p.weights + row * p.weights_width;
   const int its = tiles_of(old, T), first = wv * its * 64 + lane;
-  auto load = [&](int j) { return j < read ? order_of(w[j]) : j < old ? order_of(0.0f) : 0u; };
+  // (the loads without branches: one after the other they took 30 us of 30000 positions)
+  auto load = [&](int j) { return read > 0 ? w[min(j, read - 1)] : 0.0f; };
+  auto key_of = [&](int j, float x) { return j < old ? order_of(j < read ? x : 0.0f) : 0u; };
   uint32_t x[IT ? IT : 1];
   if constexpr (IT) {
+    float y[IT];
 #pragma unroll
-    for (int i = 0; i < IT; ++i) x[i] = i < its ? load(first + 64 * i) : 0;
+    for (int i = 0; i < IT; ++i) y[i] = load(first + 64 * i);
+#pragma unroll
+    for (int i = 0; i < IT; ++i) x[i] = i < its ? key_of(first + 64 * i, y[i]) : 0;
   }
   auto each = [&](auto f) {   // f(position, key)
     if constexpr (IT) {
@@ -895,7 +1006,7 @@ __global__ __launch_bounds__(T) void paged_select(EvictArgs p) {
       for (int i = 0; i < IT; ++i)
         if (i < its) f(first + 64 * i, x[i]);
     } else {
-      for (int i = 0; i < its; ++i) f(first + 64 * i, load(first + 64 * i));
+      for (int i = 0; i < its; ++i) f(first + 64 * i, key_of(first + 64 * i, load(first + 64 * i)));
     }
   };
   uint32_t key = heavy > 0 ? 0 : 0xffffffffu, need = 0;   // (all candidates, or none, stay)
@@ -957,14 +1068,7 @@ __global__ __launch_bounds__(T) void paged_select(EvictArgs p) {
     rank += sums[v][1];
   }
   at += min(rank, need);
-  const int32_t* table = p.tables + int64_t(s) * p.width;
   const uint64_t below = (uint64_t(1) << lane) - 1;
-  auto write = [&](uint32_t to, int j) {
-    const int page = table[j / kPage];
-    p.kept[row * p.keep + to] = j;
-    p.weights_out[row * p.keep + to] = j < p.weights_width ? w[j] : 0.0f;
-    p.source[row * p.keep + to] = uint32_t(page) < uint32_t(p.n_pages) ? page * kPage + j % kPage : -1;
-  };
   each([&](int j, uint32_t k) {
     const uint64_t e = __ballot(k == key);
     const bool stays = k > key || (k == key && rank + __popcll(e & below) < need);
@@ -972,13 +1076,15 @@ __global__ __launch_bounds__(T) void paged_select(EvictArgs p) {
     const uint64_t kept = __ballot(stays);
     const uint32_t to = at + __popcll(kept & below);
     at += __popcll(kept);
-    if (stays && to < uint32_t(p.keep)) write(to, j);
+    if (stays && to < uint32_t(p.keep)) {
+      p.kept[row * p.keep + to] = j;
+      p.weights_out[row * p.keep + to] = weight_of(k);
+    }
   });
-  for (int i = max(heavy, 0) + tid; i < held; i += T) write(i, len - held + i);   // the newest
-  for (int i = held + tid; i < p.keep; i += T) {
-    p.kept[row * p.keep + i] = -1;
-    p.weights_out[row * p.keep + i] = 0;
-    p.source[row * p.keep + i] = -1;
+  for (int i = max(heavy, 0) + tid; i < p.keep; i += T) {   // the newest, and what is behind them
+    const int j = len - held + i;
+    p.kept[row * p.keep + i] = i < held ? j : -1;
+    p.weights_out[row * p.keep + i] = i < held && j < p.weights_width ? w[j] : 0.0f;
   }
 }
 
@@ -989,29 +1095,34 @@ __global__ __launch_bounds__(256) void paged_move(EvictArgs p, int blocks) {
   const bool value = blockIdx.z;
   const int64_t row_stride = value ? p.v_row : p.k_row;
   uint16_t* base = value ? p.v + layer * p.v_layer + kvh * p.v_head : p.k + layer * p.k_layer + kvh * p.k_head;
-  const int32_t* source = p.source + ((int64_t(layer) * p.n_seqs + s) * p.KV + kvh) * p.keep;
-  const int64_t first = int64_t(blockIdx.x % blocks) * 256 * kMove;
-  u32x4 x[kMove];
-  uint16_t* to[kMove];
+  const int32_t *kept = p.kept + ((int64_t(layer) * p.n_seqs + s) * p.KV + kvh) * p.keep, *table = p.tables + int64_t(s) * p.width;
+  const int64_t first = int64_t(blockIdx.x % blocks) * 256 * kMove + threadIdx.x;
+  int from[kMove], page[kMove], to[kMove], row[kMove], piece[kMove];
 #pragma unroll
   for (int u = 0; u < kMove; ++u) {
-    const int64_t i = first + u * 256 + threadIdx.x;
-    const int j = int(i / p.pieces), c = int(i - int64_t(j) * p.pieces);
-    to[u] = nullptr;
-    if (j >= p.keep) continue;
-    const int from = source[j], page = p.to[int64_t(s) * p.to_width + j / kPage];
-    if (from < 0 || uint32_t(page) >= uint32_t(p.n_pages)) continue;
-    x[u] = *reinterpret_cast<const u32x4*>(base + int64_t(from) * row_stride + 8 * c);
-    to[u] = base + (int64_t(page) * kPage + j % kPage) * row_stride + 8 * c;
+    const int64_t i = first + u * 256;
+    row[u] = int(i / p.pieces);
+    piece[u] = int(i - int64_t(row[u]) * p.pieces);
+    from[u] = row[u] < p.keep ? kept[row[u]] : -1;
+    to[u] = row[u] < p.keep ? p.to[int64_t(s) * p.to_width + row[u] / kPage] : -1;
+  }
+#pragma unroll
+  for (int u = 0; u < kMove; ++u) page[u] = from[u] >= 0 ? table[from[u] / kPage] : -1;
+  u32x4 x[kMove];
+#pragma unroll
+  for (int u = 0; u < kMove; ++u) {
+    if (uint32_t(page[u]) >= uint32_t(p.n_pages) || uint32_t(to[u]) >= uint32_t(p.n_pages)) page[u] = -1;
+    if (page[u] >= 0) x[u] = *reinterpret_cast<const u32x4*>(base + (int64_t(page[u]) * kPage + from[u] % kPage) * row_stride + 8 * piece[u]);
   }
 #pragma unroll
   for (int u = 0; u < kMove; ++u)
-    if (to[u]) *reinterpret_cast<u32x4*>(to[u]) = x[u];
+    if (page[u] >= 0)
+      __builtin_nontemporal_store(x[u], reinterpret_cast<u32x4*>(base + (int64_t(to[u]) * kPage + row[u] % kPage) * row_stride + 8 * piece[u]));
 }
 
 // ---- host: the plan ----
 // Workgroups that a launch is shared out to, about, and tiles of a job at least.
-constexpr int kFewGroups = 1024, kManyGroups = 512;
+constexpr int kFewGroups = 2048, kManyGroups = 512;
 constexpr int kFewLeast = 4, kManyLeast = 8;
 
 struct Pieces {
@@ -1343,6 +1454,8 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
   p.n_pages = int(a->positions / kPage);
   p.plan = a->plan;
   p.tables = a->plan + h[AT_TABLES];
+  p.few = reinterpret_cast<const Job*>(a->plan + h[AT_FEW]);
+  p.many = reinterpret_cast<const Job*>(a->plan + h[AT_MANY]);
   p.n_few = h[N_FEW];
   p.n_many = h[N_MANY];
   p.out = static_cast<uint16_t*>(out);
@@ -1359,14 +1472,10 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
   const Job* manys = reinterpret_cast<const Job*>(a->plan + h[AT_MANYS]);
   with_head(a->d_head, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
-    if (h[N_FEW]) {
-      p.jobs = reinterpret_cast<const Job*>(a->plan + h[AT_FEW]);
-      hipLaunchKernelGGL((paged_few<DP>), dim3(unsigned(h[N_FEW] * KV)), dim3(64 * few_waves<DP>()), 0, s, p);
-    }
-    if (h[N_MANY]) {
-      p.jobs = reinterpret_cast<const Job*>(a->plan + h[AT_MANY]);
-      hipLaunchKernelGGL((paged_many<DP>), dim3(unsigned(h[N_MANY] * KV)), dim3(64 * kWaves), 0, s, p);
-    }
+    const unsigned few = unsigned(h[N_FEW] * KV), many = unsigned(h[N_MANY] * KV);
+    if (few && many) hipLaunchKernelGGL((paged_both<DP>), dim3(few + many), dim3(64 * kWaves), 0, s, p);
+    else if (few) hipLaunchKernelGGL((paged_few<DP>), dim3(few), dim3(64 * few_waves<DP>()), 0, s, p);
+    else if (many) hipLaunchKernelGGL((paged_many<DP>), dim3(many), dim3(64 * kWaves), 0, s, p);
   });
   if (finish)
     hipLaunchKernelGGL(paged_finish, dim3(unsigned(finish)), dim3(kFinish), 0, s, p, reinterpret_cast<const RowTile*>(a->plan + h[AT_TILES]),
@@ -1379,28 +1488,19 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
   return launched();
 }
 
-extern "C" int64_t msd_paged_evict_workspace_bytes(const msd_paged* a, int32_t n_layers, int32_t keep) {
+extern "C" int32_t msd_paged_evict(const msd_paged* a, int32_t n_layers, int64_t k_layer, int64_t v_layer, void* k, void* v,
+                                   const float* weights, int32_t weights_width, int32_t keep, int32_t recent, const int32_t* to,
+                                   int32_t to_width, float* weights_out, int32_t* kept, void* stream) {
   const int32_t rc = check(a);
   if (rc != MSD_OK) return rc;
   const int32_t* h = a->plan_host;
-  if (n_layers < 0 || keep < 0 || int64_t(n_layers) * h[MSD_PLAN_KV_HEADS] >= 65536 ||
-      int64_t(n_layers) * h[MSD_PLAN_KV_HEADS] * h[MSD_PLAN_SEQS] * std::max(keep, 1) >= int64_t(1) << 40)
-    return MSD_E_CONFIG;
-  return 4 * int64_t(n_layers) * h[MSD_PLAN_KV_HEADS] * h[MSD_PLAN_SEQS] * keep;
-}
-
-extern "C" int32_t msd_paged_evict(const msd_paged* a, int32_t n_layers, int64_t k_layer, int64_t v_layer, void* k, void* v,
-                                   const float* weights, int32_t weights_width, int32_t keep, int32_t recent, const int32_t* to,
-                                   int32_t to_width, float* weights_out, int32_t* kept, void* workspace, void* stream) {
-  const int64_t bytes = msd_paged_evict_workspace_bytes(a, n_layers, keep);
-  if (bytes < 0) return int32_t(bytes);
-  const int32_t* h = a->plan_host;
-  if (weights_width < 0 || recent < 0 || recent > keep || to_width < 0 || keep > int64_t(to_width) * kPage || k_layer % 8 || v_layer % 8 ||
+  const int64_t heads = int64_t(n_layers) * h[MSD_PLAN_KV_HEADS];
+  if (n_layers < 0 || keep < 0 || heads >= 65536 || heads * h[MSD_PLAN_SEQS] * std::max(keep, 1) >= int64_t(1) << 40 || weights_width < 0 || recent < 0 || recent > keep || to_width < 0 || keep > int64_t(to_width) * kPage || k_layer % 8 || v_layer % 8 ||
       k_layer < 0 || v_layer < 0 || k_layer > (int64_t(1) << 44) || v_layer > (int64_t(1) << 44))
     return MSD_E_CONFIG;
-  if (!bytes) return MSD_OK;
+  if (!heads || !h[MSD_PLAN_SEQS] || !keep) return MSD_OK;
   if (bad(k) || bad(v) || (weights_width && (!weights || reinterpret_cast<uintptr_t>(weights) % 4)) || !to || reinterpret_cast<uintptr_t>(to) % 4 ||
-      !weights_out || reinterpret_cast<uintptr_t>(weights_out) % 4 || !kept || reinterpret_cast<uintptr_t>(kept) % 4 || bad(workspace))
+      !weights_out || reinterpret_cast<uintptr_t>(weights_out) % 4 || !kept || reinterpret_cast<uintptr_t>(kept) % 4)
     return MSD_E_ARG;
   EvictArgs p{};
   p.k = static_cast<uint16_t*>(k);
@@ -1427,7 +1527,6 @@ extern "C" int32_t msd_paged_evict(const msd_paged* a, int32_t n_layers, int64_t
   p.pieces = a->d_head / 8;
   p.weights_out = weights_out;
   p.kept = kept;
-  p.source = static_cast<int32_t*>(workspace);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 rows(n_layers * p.KV, p.n_seqs);
   const int64_t blocks = cdiv(int64_t(keep) * p.pieces, 256 * kMove);

@@ -4,7 +4,7 @@
 // In C++ because a step's small calls are bound by the host: the backward of a call runs in a thread of the autograd engine, on
 // another core than the caller's, where a node in Python took 25 to 50 us.  The checks of arguments are the Python modules'
 // (attention.py, rotary.py, norm.py, swiglu.py): they make a plan per layout, which holds all that the C calls need, and hand
-// over operands that the kernels take as they lie.
+// over operands that the kernels take as they lie.  The paged cache's calls check theirs here.
 #include <torch/extension.h>
 
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -12,6 +12,8 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <algorithm>
+#include <cmath>
 #include <memory>
 #include <optional>
 #include <stdexcept>
@@ -404,18 +406,86 @@ Tensor swiglu(const Tensor& gate, const Tensor& up, const Glu& p) {
 }
 
 // ---- the paged cache ----
-struct PagedPlan : torch::CustomClassHolder {
-  msd_paged a;
-  int64_t k_new[2], v_new[2];   // strides of new rows (row, head)
-  Tensor table, host;           // of the sequences
-  uint64_t table_stream;        // that the table was made on
+// A step's sequences: the plan's words, on the device and on the host
+struct PagedSteps : torch::CustomClassHolder {
+  Tensor table, host;
+  uint64_t table_stream;   // that the table was made on
+  int32_t word(int i) const { return host.data_ptr<int32_t>()[i]; }
 };
-using Paged = c10::intrusive_ptr<PagedPlan>;
+using Paged = c10::intrusive_ptr<PagedSteps>;
 
 // keeps a table's memory until what is launched on stream s is done with it
 void use_table(const Tensor& table, uint64_t made_on, hipStream_t s) {
   if (reinterpret_cast<uint64_t>(s) != made_on)
     table.record_stream(c10::impl::VirtualGuardImpl(table.device().type()).getStream(table.device()));
+}
+
+// (The checks of arguments are here and not in paged_attention.py: a decode step makes these calls in every layer, on sequences that are new
+// in every step, and in Python they took longer than the launches.)
+template <class... X>
+void need(bool ok, const X&... x) {
+  if (!ok) throw std::invalid_argument(c10::str(x...));
+}
+
+// stride of an axis; 0 along one of one (or none)
+int64_t stride_of(const Tensor& x, int64_t axis) { return x.size(axis) > 1 ? x.stride(axis) : 0; }
+
+// Pages (.., n_kv_heads, positions, d_head) of keys and of values, as a call on them
+msd_paged paged_call(const Tensor& k, const Tensor& v, const PagedSteps& s, bool layers, bool written) {
+  for (const Tensor* x : {&k, &v}) need(x->scalar_type() == at::kBFloat16, "pages must be bfloat16");
+  const int64_t n = k.dim();
+  need((n == 3 || (layers && n == 4)) && k.sizes() == v.sizes() && k.size(n - 2) % MSD_PAGE == 0,
+       "pages of one shape (n_kv_heads, positions, d_head), positions a multiple of ", MSD_PAGE, ", expected, got ", k.sizes(), " and ", v.sizes());
+  const int64_t D = k.size(n - 1), positions = k.size(n - 2);
+  need(D % 8 == 0 && D > 0 && D <= 128, "d_head must be a multiple of 8 up to 128 (got ", D, ")");
+  need(k.size(n - 3) == s.word(MSD_PLAN_KV_HEADS), "pages of ", k.size(n - 3), " heads, sequences of ", s.word(MSD_PLAN_KV_HEADS));
+  need(k.is_cuda() && k.device() == v.device() && k.device() == s.table.device(), "pages and sequences must be on one GPU (got ", k.device(), ", ",
+       v.device(), " and ", s.table.device(), ")");
+  for (const Tensor* x : {&k, &v}) {
+    bool aligned = x->stride(n - 1) == 1 && reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0;
+    for (int64_t i = 0; i + 1 < n; ++i) aligned &= x->size(i) <= 1 || x->stride(i) % 8 == 0;
+    need(aligned, "pages must have contiguous heads on 16-byte boundaries");
+    bool near = x->stride(n - 2) < (int64_t(1) << 25);
+    for (int64_t i = 0; i + 2 < n; ++i) near &= x->size(i) <= 1 || x->stride(i) < (int64_t(1) << 40);
+    need(near, "pages: strides out of reach");
+    if (!written) continue;
+    std::vector<std::pair<int64_t, int64_t>> axes;   // no two places of the pages are one
+    for (int64_t i = 0; i + 1 < n; ++i)
+      if (x->size(i) > 1) axes.emplace_back(x->stride(i), x->size(i));
+    std::sort(axes.begin(), axes.end());
+    int64_t end = D;
+    for (const auto& [stride, size] : axes) {
+      need(stride >= end, "pages that are written must not overlap");
+      end = stride * size;
+    }
+  }
+  need(positions < (int64_t(1) << 31) && s.word(MSD_PLAN_PAGES) <= positions / MSD_PAGE, "tables reach page ", s.word(MSD_PLAN_PAGES) - 1,
+       ", the pages are ", positions / MSD_PAGE);
+  msd_paged a{};
+  a.d_head = int32_t(D);
+  a.scale = 1;
+  a.positions = positions;
+  a.k_stride[0] = stride_of(k, n - 3), a.k_stride[1] = stride_of(k, n - 2);
+  a.v_stride[0] = stride_of(v, n - 3), a.v_stride[1] = stride_of(v, n - 2);
+  a.plan = s.table.data_ptr<int32_t>();
+  a.plan_host = s.host.data_ptr<int32_t>();
+  return a;
+}
+
+// New rows (rows, heads, d_head) that can be read where they lie: x, or a copy of it
+Tensor paged_rows(const char* name, const Tensor& x, int64_t heads, const msd_paged& a, const PagedSteps& s, at::Device device) {
+  need(x.dim() == 3 && x.size(1) == heads && x.size(2) == a.d_head, name, " (rows, ", heads, ", ", a.d_head, ") expected, got ", x.sizes());
+  need(x.scalar_type() == at::kBFloat16, name, " must be bfloat16");
+  need(x.device() == device, name, " and the pages must be on one GPU");
+  need(s.word(MSD_PLAN_Q_END) <= x.size(0), "sequences reach row ", s.word(MSD_PLAN_Q_END), " of ", x.size(0), " rows of ", name);
+  need(x.size(0) < (int64_t(1) << 31) / s.word(MSD_PLAN_HEADS), name, ": rows times heads out of reach");
+  return attn_reads(x, heads) ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+void weights_fit(const Tensor& w, at::IntArrayRef sizes, at::Device device, const char* where) {
+  const int64_t n = int64_t(sizes.size());
+  need(w.dim() == n + 1 && w.sizes().slice(0, n) == sizes && w.scalar_type() == at::kFloat && w.device() == device && w.size(n) < (int64_t(1) << 31),
+       "weights must be float32 (", c10::Join(", ", sizes), ", width) on ", where, " GPU, got ", w.scalar_type(), " ", w.sizes(), " on ", w.device());
 }
 
 template <class... X>
@@ -424,58 +494,81 @@ void no_gradient(const char* what, const X&... x) {
     throw std::invalid_argument(std::string(what) + " has no gradient: call it under torch.no_grad(), or hand over detached tensors");
 }
 
-void paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Paged& p) {
-  only_run("paged_append", k, v, k_pages, v_pages);
-  no_gradient("paged_append", k, v, k_pages, v_pages);
+void paged_append(const Tensor& k_new, const Tensor& v_new, const Tensor& k_pages, const Tensor& v_pages, const Paged& steps) {
+  only_run("paged_append", k_new, v_new, k_pages, v_pages);
+  no_gradient("paged_append", k_new, v_new, k_pages, v_pages);
+  const PagedSteps& p = *steps;
+  msd_paged a = paged_call(k_pages, v_pages, p, false, true);
+  const int64_t heads = p.word(MSD_PLAN_KV_HEADS);
   Place on(k_pages);
-  use_table(p->table, p->table_stream, on.stream);
-  check(msd_paged_append(&p->a, at_(k), p->k_new, at_(v), p->v_new, at_(k_pages), at_(v_pages), on.stream), "msd_paged_append");
+  const Tensor k = paged_rows("k", k_new, heads, a, p, k_pages.device()), v = paged_rows("v", v_new, heads, a, p, k_pages.device());
+  need(k.size(0) == v.size(0), "k of ", k.size(0), " rows, v of ", v.size(0));
+  need(!p.word(MSD_PLAN_SHARED), "a page that takes new rows is in use elsewhere too");
+  a.q_rows = k.size(0);
+  const int64_t k_stride[2] = {stride_of(k, 0), stride_of(k, 1)}, v_stride[2] = {stride_of(v, 0), stride_of(v, 1)};
+  use_table(p.table, p.table_stream, on.stream);
+  check(msd_paged_append(&a, at_(k), k_stride, at_(v), v_stride, at_(k_pages), at_(v_pages), on.stream), "msd_paged_append");
   k_pages.unsafeGetTensorImpl()->bump_version();
   v_pages.unsafeGetTensorImpl()->bump_version();
 }
 
-variable_list paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const MaybeTensor& weights, const Paged& p) {
-  only_run("paged_attention", q, k_pages, v_pages, weights);
-  no_gradient("paged_attention", q, k_pages, v_pages);
+variable_list paged_attention(const Tensor& q_new, const Tensor& k_pages, const Tensor& v_pages, const Paged& steps, std::optional<double> scale,
+                              const MaybeTensor& weights) {
+  only_run("paged_attention", q_new, k_pages, v_pages, weights);
+  no_gradient("paged_attention", q_new, k_pages, v_pages);
   if (weights) no_gradient("paged_attention", *weights);
-  Place on(q);
-  const int32_t* h = p->host.data_ptr<int32_t>();
-  Tensor out = attn_output(q, h[MSD_PLAN_Q_COUNT] != q.size(0)), held, counted, ws;
+  const PagedSteps& p = *steps;
+  msd_paged a = paged_call(k_pages, v_pages, p, false, false);
+  const double c = scale.value_or(1 / std::sqrt(double(a.d_head)));
+  need(c >= 0x1p-60 && c <= 0x1p60, "scale must lie in [2 ** -60, 2 ** 60] (got ", c, ")");
+  a.scale = float(c);
+  const int64_t sizes[2] = {p.word(MSD_PLAN_SEQS), p.word(MSD_PLAN_KV_HEADS)};
+  if (weights) weights_fit(*weights, sizes, k_pages.device(), "the pages'");
+  Place on(k_pages);
+  const Tensor q = paged_rows("q", q_new, p.word(MSD_PLAN_HEADS), a, p, k_pages.device());
+  a.q_rows = q.size(0);
+  a.q_stride[0] = stride_of(q, 0), a.q_stride[1] = stride_of(q, 1);
+  Tensor out = attn_output(q, p.word(MSD_PLAN_Q_COUNT) != a.q_rows), held, counted, ws;
   if (weights) {
     held = weights->contiguous();
-    counted = at::empty({h[MSD_PLAN_SEQS], h[MSD_PLAN_KV_HEADS], h[MSD_PLAN_LONGEST]}, held.options());
+    counted = at::empty({sizes[0], sizes[1], p.word(MSD_PLAN_LONGEST)}, held.options());
   }
-  const int64_t n = msd_paged_attn_workspace_bytes(&p->a, counted.defined());
+  const int64_t n = msd_paged_attn_workspace_bytes(&a, counted.defined());
   if (n < 0) check(int32_t(n), "msd_paged_attn_workspace_bytes");
   if (n) ws = bytes(q, n);
-  use_table(p->table, p->table_stream, on.stream);
-  check(msd_paged_attn(&p->a, at_(q), at_(k_pages), at_(v_pages), at_(out), static_cast<const float*>(at_(held)),
+  use_table(p.table, p.table_stream, on.stream);
+  check(msd_paged_attn(&a, at_(q), at_(k_pages), at_(v_pages), at_(out), static_cast<const float*>(at_(held)),
                        held.defined() ? int32_t(held.size(2)) : 0, static_cast<float*>(at_(counted)), at_(ws), on.stream),
         "msd_paged_attn");
   if (!weights) return {out};
   return {out, counted};
 }
 
-variable_list paged_evict(const Tensor& k_pages, const Tensor& v_pages, const Tensor& weights, const Tensor& to, int32_t keep, int32_t recent,
-                          uint64_t to_stream, const Paged& p) {
+variable_list paged_evict(const Tensor& k_pages, const Tensor& v_pages, const Tensor& weights, const Paged& steps, const Tensor& to, uint64_t to_stream,
+                          int32_t pages, int32_t keep, int32_t recent) {
   only_run("paged_evict", k_pages, v_pages, weights);
   no_gradient("paged_evict", k_pages, v_pages, weights);
+  const PagedSteps& p = *steps;
+  msd_paged a = paged_call(k_pages, v_pages, p, true, true);
+  need(pages <= a.positions / MSD_PAGE, "tables reach page ", pages - 1, ", the pages are ", a.positions / MSD_PAGE);
+  a.q_rows = p.word(MSD_PLAN_Q_END);
+  const bool layers = k_pages.dim() == 4;
+  std::vector<int64_t> sizes;
+  if (layers) sizes.push_back(k_pages.size(0));
+  sizes.push_back(p.word(MSD_PLAN_SEQS));
+  sizes.push_back(p.word(MSD_PLAN_KV_HEADS));
+  need(!layers || k_pages.size(0) * k_pages.size(1) < 65536, "layers times heads must stay below 65536 (got ", k_pages.size(0), " and ", k_pages.size(1), ")");
+  weights_fit(weights, sizes, k_pages.device(), "the pages'");
   Place on(k_pages);
   const Tensor w = weights.contiguous();
-  auto sizes = w.sizes().vec();
-  sizes.back() = keep;
-  Tensor out = at::empty(sizes, w.options()), kept = at::empty(sizes, w.options().dtype(at::kInt)), ws;
-  const bool layers = k_pages.dim() == 4;
+  sizes.push_back(keep);
+  Tensor out = at::empty(sizes, w.options()), kept = at::empty(sizes, w.options().dtype(at::kInt));
   const int32_t n_layers = layers ? int32_t(k_pages.size(0)) : 1;
-  const int64_t n = msd_paged_evict_workspace_bytes(&p->a, n_layers, keep);
-  if (n < 0) check(int32_t(n), "msd_paged_evict_workspace_bytes");
-  if (n) ws = bytes(k_pages, n);
-  use_table(p->table, p->table_stream, on.stream);
+  use_table(p.table, p.table_stream, on.stream);
   use_table(to, to_stream, on.stream);
-  auto layer = [&](const Tensor& x) { return n_layers > 1 ? x.stride(0) : 0; };
-  check(msd_paged_evict(&p->a, n_layers, layer(k_pages), layer(v_pages), at_(k_pages), at_(v_pages), static_cast<const float*>(at_(w)),
-                        int32_t(w.size(-1)), keep, recent, static_cast<const int32_t*>(at_(to)), int32_t(to.size(1)),
-                        static_cast<float*>(at_(out)), static_cast<int32_t*>(at_(kept)), at_(ws), on.stream),
+  check(msd_paged_evict(&a, n_layers, layers ? stride_of(k_pages, 0) : 0, layers ? stride_of(v_pages, 0) : 0, at_(k_pages), at_(v_pages),
+                        static_cast<const float*>(at_(w)), int32_t(w.size(-1)), keep, recent, static_cast<const int32_t*>(at_(to)),
+                        int32_t(to.size(1)), static_cast<float*>(at_(out)), static_cast<int32_t*>(at_(kept)), on.stream),
         "msd_paged_evict");
   k_pages.unsafeGetTensorImpl()->bump_version();
   v_pages.unsafeGetTensorImpl()->bump_version();
@@ -541,18 +634,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         p->held = held;
         return p;
       }));
-  py::class_<PagedPlan, Paged>(m, "PagedPlan")
-      .def(py::init([](uintptr_t a, const Tensor& table, const Tensor& host, uint64_t table_stream, int64_t k_row, int64_t k_head,
-                       int64_t v_row, int64_t v_head) {
-        auto p = c10::make_intrusive<PagedPlan>();
-        p->a = *reinterpret_cast<const msd_paged*>(a);
-        p->table = table;
-        p->host = host;
-        p->table_stream = table_stream;
-        p->k_new[0] = k_row, p->k_new[1] = k_head;
-        p->v_new[0] = v_row, p->v_new[1] = v_head;
-        return p;
-      }));
+  py::class_<PagedSteps, Paged>(m, "PagedSteps").def(py::init([](const Tensor& table, const Tensor& host, uint64_t table_stream) {
+    auto p = c10::make_intrusive<PagedSteps>();
+    p->table = table;
+    p->host = host;
+    p->table_stream = table_stream;
+    return p;
+  }));
   m.def("attention", &attention, free_threads);
   m.def("rotary", &rotary, free_threads);
   m.def("rms_norm", &rms_norm, free_threads);

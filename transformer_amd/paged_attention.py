@@ -18,21 +18,20 @@ keys with the running maximum and sum of the softmax, on the matrix cores; f32 s
 probabilities are rounded to bf16 as operands of the product with the values (not in the weights), the output once to bf16.
 Deterministic.  No gradients.
 """
-import ctypes
-
 import numpy as np
 import torch
 
 from . import _lib
-from .attention import _fits, _ranges
+from .attention import _ranges
 from .paged import PAGE
 
 LONGEST = 2 ** 31 - 2 ** 16 - 1   # positions of a sequence
+PAGES = 2 ** 27 - 1               # of a pool
 
 
 def _words(q_lens, lengths, q_starts, tables, n_heads, n_kv_heads, longest):
     """The library's plan of a step as an int32 tensor on the host."""
-    seqs = np.ascontiguousarray(np.stack([np.asarray(x, dtype=np.int32) for x in (q_starts, q_lens, lengths)], 1)) if q_lens else np.zeros((0, 3), np.int32)
+    seqs = np.array([q_starts, q_lens, lengths], np.int32).reshape(3, -1).T.copy()
     n, width = tables.shape
     args = n, seqs.ctypes.data, tables.ctypes.data, width, n_heads, n_kv_heads, longest
     words = torch.empty(_lib.check(_lib.lib().msd_paged_plan(*args, None, 0), "msd_paged_plan"), dtype=torch.int32)
@@ -41,6 +40,7 @@ def _words(q_lens, lengths, q_starts, tables, n_heads, n_kv_heads, longest):
 
 
 def _integers(x, what):
+    x = x.tolist() if isinstance(x, (torch.Tensor, np.ndarray)) else x
     out = [int(n) for n in x]
     if any(a != b for a, b in zip(out, x)):
         raise ValueError(f"{what} must be whole numbers")
@@ -48,24 +48,30 @@ def _integers(x, what):
 
 
 def _tables(tables, needed, what):
-    """The tables of pages as one int32 array, each at least as long as `needed` says; what lies behind that is not looked at."""
+    """The tables of pages as one int32 array, each at least as long as `needed` says; what lies behind that is 0."""
     if isinstance(tables, torch.Tensor):
         tables = tables.cpu().numpy()
-    if isinstance(tables, np.ndarray) and (tables.ndim != 2 or tables.dtype.kind not in "iu"):
+    whole = isinstance(tables, np.ndarray)
+    if whole and (tables.ndim != 2 or tables.dtype.kind not in "iu"):
         raise ValueError(f"{what} must be a list of page numbers for each sequence, or a table of integers")
     if len(tables) != len(needed):
         raise ValueError(f"{len(tables)} {what} for {len(needed)} sequences")
-    out = np.zeros((len(needed), max(needed, default=0)), np.int32)
-    for row, pages, n in zip(out, tables, needed):
-        if len(pages) < n:
-            raise ValueError(f"{what}: {len(pages)} pages where {n} are needed")
-        pages = np.asarray(pages[:n])
-        if n and pages.dtype.kind not in "iu":
-            raise ValueError(f"{what} must be whole numbers")
-        if n and not (0 <= pages.min() and pages.max() < 2 ** 27 - 1):
-            raise ValueError(f"{what}: page numbers outside [0, 2**27 - 1)")
-        row[:n] = pages
-    return out
+    width = max(needed, default=0)
+    short = next(((len(pages), n) for pages, n in zip(tables, needed) if len(pages) < n), None)
+    if short:
+        raise ValueError("%s: %d pages where %d are needed" % (what, *short))
+    if whole:
+        out = np.where(np.arange(width) < np.asarray(needed, np.int64).reshape(-1, 1), tables[:, :width], 0)
+    else:
+        out = np.zeros((len(needed), width), np.int64)
+        for row, pages, n in zip(out, tables, needed):
+            pages = np.asarray(pages[:n])
+            if n and pages.dtype.kind not in "iu":
+                raise ValueError(f"{what} must be whole numbers")
+            row[:n] = pages
+    if out.size and not (0 <= out.min() and out.max() < PAGES):
+        raise ValueError(f"{what}: page numbers outside [0, {PAGES})")
+    return np.ascontiguousarray(out, np.int32)
 
 
 class PagedSequences:
@@ -93,7 +99,7 @@ class PagedSequences:
         self.host = self._plan(lengths, tables)
         self.table = self.host.to(device)
         self.stream = _lib.current_stream(self.table)
-        self._plans, self.version = {}, 0
+        self.native, self.version = _lib.ops().PagedSteps(self.table, self.host, self.stream or 0), 0
 
     def _plan(self, lengths, tables):
         lengths = _integers(lengths, "lengths")
@@ -121,7 +127,7 @@ class PagedSequences:
 
     def used(self):
         """The pages in use, in order, without repetitions."""
-        return np.unique(np.concatenate([np.zeros(0, np.int32)] + [p[:-(-n // PAGE)] for p, n in zip(self._pages, self.lengths)]))
+        return np.unique(self._pages[np.arange(self._pages.shape[1]) * PAGE < np.asarray(self.lengths, np.int64).reshape(-1, 1)])
 
 
 class PagedEviction:
@@ -137,126 +143,24 @@ class PagedEviction:
         self.lengths = [min(n, self.keep) for n in sequences.lengths]
         needed = [-(-n // PAGE) for n in self.lengths]
         pages = _tables(tables, needed, "tables")
-        flat = np.concatenate([np.zeros(0, np.int32)] + [p[:n] for p, n in zip(pages, needed)])
+        there = np.arange(pages.shape[1]) < np.asarray(needed, np.int64).reshape(-1, 1)
+        flat = pages[there]
         if len(np.unique(flat)) != len(flat):
             raise ValueError("tables: a page is named twice")
         if len(np.intersect1d(flat, sequences.used())):
             raise ValueError("tables: a page that the sequences use")
         self.pages = int(flat.max(initial=-1)) + 1
         host = np.full((sequences.n, -(-self.keep // PAGE)), -1, np.int32)   # (-1: not written)
-        for row, p, n in zip(host, pages, needed):
-            row[:n] = p[:n]
+        host[:, :pages.shape[1]][there] = flat
         self.table = torch.from_numpy(host).to(sequences.table.device)
         self.stream = _lib.current_stream(self.table)
-
-
-def _positions(x):
-    return x.shape[-2]
-
-
-def _check_pages(k_pages, v_pages, sequences, dims, written):
-    for x in (k_pages, v_pages):
-        if x.dtype != torch.bfloat16:
-            raise ValueError("pages must be bfloat16")
-    if k_pages.dim() not in dims or k_pages.shape != v_pages.shape or _positions(k_pages) % PAGE:
-        raise ValueError(f"pages of one shape (n_kv_heads, positions, d_head), positions a multiple of {PAGE}, expected, got "
-                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    D = k_pages.shape[-1]
-    if D % 8 or not 0 < D <= 128:
-        raise ValueError(f"d_head must be a multiple of 8 up to 128 (got {D})")
-    if k_pages.shape[-3] != sequences.n_kv_heads:
-        raise ValueError(f"pages of {k_pages.shape[-3]} heads, sequences of {sequences.n_kv_heads}")
-    if not k_pages.is_cuda or not k_pages.device == v_pages.device == sequences.table.device:
-        raise ValueError(f"pages and sequences must be on one GPU (got {k_pages.device}, {v_pages.device} and {sequences.table.device})")
-    for x in (k_pages, v_pages):
-        if x.stride(-1) != 1 or any(n > 1 and s % 8 for n, s in zip(x.shape, x.stride()[:-1])) or x.data_ptr() % 16:
-            raise ValueError("pages must have contiguous heads on 16-byte boundaries")
-        if x.stride(-2) >= 2 ** 25 or any(n > 1 and s >= 2 ** 40 for n, s in zip(x.shape, x.stride()[:-2])):
-            raise ValueError("pages: strides out of reach")
-        if written:   # no two places of the pages are one
-            end = D
-            for s, n in sorted((s, n) for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1):
-                if s < end:
-                    raise ValueError("pages that are written must not overlap")
-                end = s * n
-    if _positions(k_pages) >= 2 ** 31 or int(sequences.host[9]) > _positions(k_pages) // PAGE:
-        raise ValueError(f"tables reach page {int(sequences.host[9]) - 1}, the pages are {_positions(k_pages) // PAGE}")
-
-
-def _check_new(x, heads, k_pages, sequences, name):
-    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != k_pages.shape[-1]:
-        raise ValueError(f"{name} (rows, {heads}, {k_pages.shape[-1]}) expected, got {tuple(x.shape)}")
-    if x.dtype != torch.bfloat16:
-        raise ValueError(f"{name} must be bfloat16")
-    if x.device != k_pages.device:
-        raise ValueError(f"{name} and the pages must be on one GPU")
-    if sequences.q_end > x.shape[0]:
-        raise ValueError(f"sequences reach row {sequences.q_end} of {x.shape[0]} rows of {name}")
-    if x.shape[0] * sequences.n_heads >= 2 ** 31:
-        raise ValueError(f"{name}: rows times heads out of reach")
-
-
-def _stride(x, axis):
-    return x.stride(axis) if x.shape[axis] > 1 else 0
-
-
-class _Plan:
-    """How calls on operands of one layout go.  ``fits``: which new rows can be read where they lie; ``native``: the library's
-    arguments, where all can."""
-
-    def __init__(self, new, k_pages, v_pages, sequences, scale=1.0):
-        a = _lib.MsdPaged()
-        self.fits = tuple(_fits(x.shape, x.stride(), x.shape[1] // (sequences.n_kv_heads if len(new) == 1 else 1)) for x in new)
-        a.d_head, a.scale, a.positions = k_pages.shape[-1], scale, _positions(k_pages)
-        a.q_rows = new[0].shape[0] if new else sequences.q_end
-        if len(new) == 1:
-            a.q_stride[:] = _stride(new[0], 0), _stride(new[0], 1)
-        a.k_stride[:] = _stride(k_pages, -3), _stride(k_pages, -2)
-        a.v_stride[:] = _stride(v_pages, -3), _stride(v_pages, -2)
-        a.plan, a.plan_host = sequences.table.data_ptr(), sequences.host.data_ptr()
-        new_strides = [(_stride(x, 0), _stride(x, 1)) for x in new] if len(new) == 2 else [(0, 0)] * 2
-        self.native = _lib.ops().PagedPlan(ctypes.addressof(a), sequences.table, sequences.host, sequences.stream or 0, *new_strides[0],
-                                           *new_strides[1]) if all(self.fits) else None
-
-
-def _layout(x):
-    return x.shape, x.stride(), x.dtype, x.device
-
-
-def _plan(kind, check, new, k_pages, v_pages, sequences, scale=1.0):
-    key = (kind, scale, _layout(k_pages), _layout(v_pages), k_pages.data_ptr() % 16, v_pages.data_ptr() % 16, sequences.version, *map(_layout, new))
-    found = sequences._plans.get(key)
-    if found is None:
-        check()
-        found = _Plan(new, k_pages, v_pages, sequences, scale)
-        if len(sequences._plans) >= 64:
-            sequences._plans.clear()
-        sequences._plans[key] = found
-    return found
-
-
-def _operands(new, plan):
-    return [x if f and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format) for x, f in zip(new, plan.fits)]
 
 
 def paged_append(k, v, k_pages, v_pages, sequences):
     """Writes the new tokens' keys and values (rows, n_kv_heads, d_head; bf16, any strides) to their positions of the pages
     (n_kv_heads, positions, d_head; on 16-byte boundaries, strides that are multiples of 8).  Pages that take new rows must be
     in use by one sequence only."""
-    def check():
-        _check_pages(k_pages, v_pages, sequences, (3,), True)
-        for x, name in ((k, "k"), (v, "v")):
-            _check_new(x, sequences.n_kv_heads, k_pages, sequences, name)
-        if k.shape[0] != v.shape[0]:
-            raise ValueError(f"k of {k.shape[0]} rows, v of {v.shape[0]}")
-        if int(sequences.host[10]):
-            raise ValueError("a page that takes new rows is in use elsewhere too")
-
-    plan = _plan("append", check, (k, v), k_pages, v_pages, sequences)
-    if plan.native is None or (k.data_ptr() | v.data_ptr()) % 16:
-        k, v = _operands((k, v), plan)
-        plan = _plan("append", check, (k, v), k_pages, v_pages, sequences)
-    _lib.ops().paged_append(k, v, k_pages, v_pages, plan.native)
+    _lib.ops().paged_append(k, v, k_pages, v_pages, sequences.native)
 
 
 def paged_attention(q, k_pages, v_pages, sequences, scale=None, weights=None):
@@ -271,23 +175,7 @@ def paged_attention(q, k_pages, v_pages, sequences, scale=None, weights=None):
 
     What lies behind a sequence's length is not read.  Within it, a key or value row that is not finite reaches every query
     that sees it, and may reach those that do not."""
-    scale = q.shape[-1] ** -0.5 if scale is None and q.dim() and q.shape[-1] else float(scale or 0)
-
-    def check():
-        _check_pages(k_pages, v_pages, sequences, (3,), False)
-        _check_new(q, sequences.n_heads, k_pages, sequences, "q")
-        if not 2.0 ** -60 <= scale <= 2.0 ** 60:
-            raise ValueError(f"scale must lie in [2 ** -60, 2 ** 60] (got {scale})")
-
-    plan = _plan("attention", check, (q,), k_pages, v_pages, sequences, scale)
-    if weights is not None and (weights.dim() != 3 or weights.shape[:2] != (sequences.n, sequences.n_kv_heads) or weights.dtype != torch.float32
-                                or weights.device != q.device or weights.shape[2] >= 2 ** 31):
-        raise ValueError(f"weights must be float32 ({sequences.n}, {sequences.n_kv_heads}, width) on q's GPU, got {weights.dtype} "
-                         f"{tuple(weights.shape)} on {weights.device}")
-    if plan.native is None or q.data_ptr() % 16:
-        q, = _operands((q,), plan)
-        plan = _plan("attention", check, (q,), k_pages, v_pages, sequences, scale)
-    out = _lib.ops().paged_attention(q, k_pages, v_pages, weights, plan.native)
+    out = _lib.ops().paged_attention(q, k_pages, v_pages, sequences.native, scale, weights)
     return out[0] if weights is None else tuple(out)
 
 
@@ -302,17 +190,5 @@ def paged_evict(k_pages, v_pages, weights, eviction):
     sequences = eviction.sequences
     if sequences.version != eviction.version:
         raise ValueError("the sequences have been updated since the eviction was made")
-
-    def check():
-        _check_pages(k_pages, v_pages, sequences, (3, 4), True)
-        if eviction.pages > _positions(k_pages) // PAGE:
-            raise ValueError(f"tables reach page {eviction.pages - 1}, the pages are {_positions(k_pages) // PAGE}")
-        if k_pages.dim() == 4 and k_pages.shape[0] * k_pages.shape[1] >= 65536:
-            raise ValueError(f"layers times heads must stay below 65536 (got {k_pages.shape[0]} and {k_pages.shape[1]})")
-
-    plan = _plan(("evict", eviction.pages), check, (), k_pages, v_pages, sequences)
-    shape = (*k_pages.shape[:-3], sequences.n, sequences.n_kv_heads)
-    if weights.dim() != len(shape) + 1 or tuple(weights.shape[:-1]) != shape or weights.dtype != torch.float32 or weights.device != k_pages.device \
-            or weights.shape[-1] >= 2 ** 31:
-        raise ValueError(f"weights must be float32 {(*shape, 'width')} on the pages' GPU, got {weights.dtype} {tuple(weights.shape)} on {weights.device}")
-    return tuple(_lib.ops().paged_evict(k_pages, v_pages, weights, eviction.table, eviction.keep, eviction.recent, eviction.stream or 0, plan.native))
+    return tuple(_lib.ops().paged_evict(k_pages, v_pages, weights, sequences.native, eviction.table, eviction.stream or 0, eviction.pages,
+                                        eviction.keep, eviction.recent))
