@@ -692,7 +692,7 @@ __device__ __forceinline__ void join(const Args& p, float (*lds)[11], const floa
   if (keep && c == 0) p.lse[int64_t(q0) * p.H + int64_t(head) * n + pos] = l == 0 ? -INFINITY : -(m + __log2f(l)) / p.c;
 }
 
-__global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* tiles, int n_tiles, const Few* fews, int n_fews, int few_joins) {
+__global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* tiles, int n_tiles, const Few* fews, int n_fews, int few_joins, int join_rows) {
   __shared__ float lds[kFinish][11];
   __shared__ float row_lse[kFewRows];
   constexpr int kSubs = kManyRows / kJoinRows;
@@ -717,7 +717,7 @@ __global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* t
   if (!sound(p, f.q0, f.n, f.len, f.seq) || R > kFewRows || f.parts < 0 || f.slot < 0 || f.slot > p.n_few - f.parts) return;
   const int64_t at = (int64_t(f.slot) * p.KV + kvh) * kFewRows, stride = int64_t(p.KV) * kFewRows;
   if (!weigh) {
-    const int row0 = kJoinRows * nth, rows = min(R - row0, kJoinRows);
+    const int row0 = join_rows * nth, rows = min(R - row0, join_rows);
     if (f.parts > 1 && rows > 0)
       join(p, lds, p.few_part + (at + row0) * p.D, p.few_lse + at + row0, stride, f.parts, rows, f.q0, f.n, row0, kvh, false);
     return;
@@ -777,10 +777,10 @@ __global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* t
 // key's scores against 16 rows, so that its sum stays in the lane; a row's scores start as -L_i / c (what p.lse holds here).  Two
 // halves of four waves take the tiles of 64 rows in turn.  While the probabilities of 32 rows are formed, the matrix cores form the
 // next 32 rows' scores.
-constexpr int kHalves = 2;
+constexpr int kHalves = 4;
 template <int DP>
 __global__ __launch_bounds__(64 * kWaves * kHalves) void paged_weights(Args p, const Job* seqs, int n_seqs) {
-  constexpr int P = pitch<DP>(), R = 64, TILE = R * P, STAGE = TILE + 256 * kWaves, STAGES = 3, KS = DP / 16;
+  constexpr int P = pitch<DP>(), R = 64, TILE = R * P, STAGE = TILE + 256 * kWaves, STAGES = 2, KS = DP / 16;
   constexpr int LOADS = TILE / 1024 / kWaves + 1;   // of a wave and stage: rows, and their logsumexps, of which each wave has its own
   __shared__ __attribute__((aligned(16))) uint8_t lds[kHalves * STAGES * STAGE];
   __shared__ float other[kHalves][kWaves * 32];
@@ -883,13 +883,11 @@ __global__ __launch_bounds__(64 * kWaves * kHalves) void paged_weights(Args p, c
         pos += kHalves * R;
       }
     };
-    static_assert(STAGES == 3, "the stages in turn");
+    static_assert(STAGES == 2, "the stages in turn");
     for (int i = (all + kHalves - 1) / kHalves; i > 0;) {
-      tile(0, 2);
+      tile(0, 1);
       if (--i == 0) break;
       tile(1, 0);
-      if (--i == 0) break;
-      tile(2, 1);
       --i;
     }
 #pragma unroll
@@ -1426,7 +1424,8 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
   const int64_t KV = h[MSD_PLAN_KV_HEADS], longest = h[MSD_PLAN_LONGEST], most = (int64_t(1) << 32) / 256 - 1;
   const int64_t key_blocks = cdiv(longest, 128), weight_blocks = weighted ? cdiv(longest, kWeightKeys) : 0;
   const int n_tiles = h[MANY_PARTS] ? h[N_TILES] : 0, n_fews = h[FEW_PARTS] || weighted ? h[N_FEWS] : 0;
-  const int few_joins = h[FEW_PARTS] ? int(cdiv(h[FEW_ROWS], kJoinRows)) : 0;
+  // one row of few a workgroup as long as there are few of them (16 parts of 64 rows: 4.0 us, with four rows 5.6; 2048 rows: 6.7 and 5.0)
+  const int join_rows = int64_t(n_fews) * KV * h[FEW_ROWS] <= 1024 ? 1 : kJoinRows, few_joins = h[FEW_PARTS] ? int(cdiv(h[FEW_ROWS], join_rows)) : 0;
   const int64_t finish = int64_t(n_tiles) * KV * (kManyRows / kJoinRows) + int64_t(n_fews) * KV * (few_joins + weight_blocks);
   if (finish > most || key_blocks * KV * h[N_MANYS] > most) return MSD_E_CONFIG;
   if (h[MSD_PLAN_Q_COUNT] && (bad(q) || bad(k) || bad(v) || bad(out))) return MSD_E_ARG;
@@ -1479,7 +1478,7 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
   });
   if (finish)
     hipLaunchKernelGGL(paged_finish, dim3(unsigned(finish)), dim3(kFinish), 0, s, p, reinterpret_cast<const RowTile*>(a->plan + h[AT_TILES]),
-                       n_tiles, reinterpret_cast<const Few*>(a->plan + h[AT_FEWS]), n_fews, few_joins);
+                       n_tiles, reinterpret_cast<const Few*>(a->plan + h[AT_FEWS]), n_fews, few_joins, join_rows);
   if (weighted && h[N_MANYS] && key_blocks)
     with_head(a->d_head, [&](auto dp) {
       constexpr int DP = decltype(dp)::value;
