@@ -1191,11 +1191,12 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
       n_many += n;
       many_parts |= n > 1;
     }
-  if (longest) {   // as many as any lengths up to it give: at most one piece more than whole ones for each list
-    n_few = few_active ? few_active + cdiv(kFewGroups, KV) : 0;
-    n_many = row_tiles ? row_tiles + cdiv(kManyGroups, KV) : 0;
-    few_parts = few_active;
-    many_parts = row_tiles;
+  if (longest) {   // as many as any lengths up to it give: a piece more than whole ones for each list, none below the least
+    const int64_t most_few = cdiv(cdiv(longest, kFewKeys), kFewLeast), most_many = cdiv(cdiv(longest, kKeys), kManyLeast);
+    n_few = few_active ? std::min(few_active * most_few, few_active + cdiv(kFewGroups, KV)) : 0;
+    n_many = row_tiles ? std::min(row_tiles * most_many, row_tiles + cdiv(kManyGroups, KV)) : 0;
+    few_parts = few_active && most_few > 1;
+    many_parts = row_tiles && most_many > 1;
   }
   const int width = int(cdiv(table_width, 4) * 4);
   Writer w{words};

@@ -494,6 +494,11 @@ void no_gradient(const char* what, const X&... x) {
     throw std::invalid_argument(std::string(what) + " has no gradient: call it under torch.no_grad(), or hand over detached tensors");
 }
 
+// (first: an inference tensor outside inference mode raises here)
+void written(const Tensor& k, const Tensor& v) {
+  for (const Tensor* x : {&k, &v}) x->unsafeGetTensorImpl()->bump_version();
+}
+
 void paged_append(const Tensor& k_new, const Tensor& v_new, const Tensor& k_pages, const Tensor& v_pages, const Paged& steps) {
   only_run("paged_append", k_new, v_new, k_pages, v_pages);
   no_gradient("paged_append", k_new, v_new, k_pages, v_pages);
@@ -507,9 +512,8 @@ void paged_append(const Tensor& k_new, const Tensor& v_new, const Tensor& k_page
   a.q_rows = k.size(0);
   const int64_t k_stride[2] = {stride_of(k, 0), stride_of(k, 1)}, v_stride[2] = {stride_of(v, 0), stride_of(v, 1)};
   use_table(p.table, p.table_stream, on.stream);
+  written(k_pages, v_pages);
   check(msd_paged_append(&a, at_(k), k_stride, at_(v), v_stride, at_(k_pages), at_(v_pages), on.stream), "msd_paged_append");
-  k_pages.unsafeGetTensorImpl()->bump_version();
-  v_pages.unsafeGetTensorImpl()->bump_version();
 }
 
 variable_list paged_attention(const Tensor& q_new, const Tensor& k_pages, const Tensor& v_pages, const Paged& steps, std::optional<double> scale,
@@ -566,12 +570,11 @@ variable_list paged_evict(const Tensor& k_pages, const Tensor& v_pages, const Te
   const int32_t n_layers = layers ? int32_t(k_pages.size(0)) : 1;
   use_table(p.table, p.table_stream, on.stream);
   use_table(to, to_stream, on.stream);
+  written(k_pages, v_pages);
   check(msd_paged_evict(&a, n_layers, layers ? stride_of(k_pages, 0) : 0, layers ? stride_of(v_pages, 0) : 0, at_(k_pages), at_(v_pages),
                         static_cast<const float*>(at_(w)), int32_t(w.size(-1)), keep, recent, static_cast<const int32_t*>(at_(to)),
                         int32_t(to.size(1)), static_cast<float*>(at_(out)), static_cast<int32_t*>(at_(kept)), on.stream),
         "msd_paged_evict");
-  k_pages.unsafeGetTensorImpl()->bump_version();
-  v_pages.unsafeGetTensorImpl()->bump_version();
   return {out, kept};
 }
 
