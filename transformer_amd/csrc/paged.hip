@@ -204,12 +204,23 @@ struct Rows {
     }
     l += sum;
   }
+  // The probabilities as two bf16, of which the second is what the first's rounding has taken off: to 2^-17.  A few rows wait for
+  // memory, so the second product costs nothing; the output's own rounding is what is left (relative errors against 64 bits
+  // 0.0017, with one product 0.0023 to 0.0026).
   __device__ __forceinline__ void add(const f32x16& s, const uint8_t* V, int row0, int lane) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const bf16x8 pr = pack8(s, 8 * h);
+      f32x16 off;
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d) o[d] = mfma(cols_operand<pitch<DP>()>(V, row0 + 16 * h, d, lane), pr, o[d]);
+      for (int i = 0; i < 8; ++i) off[i] = s[8 * h + i] - float(pr[i]);
+      const bf16x8 rest = pack8(off, 0);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) {
+        const bf16x8 v = cols_operand<pitch<DP>()>(V, row0 + 16 * h, d, lane);
+        o[d] = mfma(v, pr, o[d]);
+        o[d] = mfma(v, rest, o[d]);
+      }
     }
   }
 };
