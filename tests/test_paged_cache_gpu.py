@@ -190,6 +190,14 @@ def test_evict_long(longest, kind):
     _evict([longest, longest // 2], 1, 64, longest // 3, 100, layers=1, kind=kind, seed=longest)
 
 
+@pytest.mark.parametrize("kind", ["ties", "any"])
+@pytest.mark.parametrize("D,keep,recent", [(64, 64, 8), (128, 100, 100), (72, 33, 0), (8, 1, 1)])
+def test_evict_all_layers(D, keep, recent, kind):
+    """Enough sequences, layers and heads for a workgroup each to choose and move."""
+    _evict([100, 33, 0, 1, 64, 257, 300], 2, D, keep, recent, layers=40, kind=kind, seed=keep)
+    _evict([700, 2048], 2, D, 3 * keep, recent, layers=128, kind=kind, seed=keep, width=500)
+
+
 @pytest.mark.parametrize("width", [0, 1, 100, 1000])
 def test_evict_with_weights_of_any_width(width):
     _evict([300, 120], 2, 64, 64, 8, width=width, seed=3)
