@@ -124,7 +124,7 @@ def test_an_eviction_of_pages_that_are_appended_to_afterwards():
     w = torch.rand((2, 2, 100), generator=torch.Generator().manual_seed(1)).cuda()
     left, kept = paged_evict(kp, vp, w, e)
     assert e.lengths == [32, 32]
-    tables, free = e.table.tolist(), int(max(e.table.max(), s.table[s.host[28]:].max()))
+    tables = e.table.tolist()
     spare = [p for p in range(kp.shape[1] // 16) if p not in {x for t in tables for x in t} | set(s.used().tolist())]
     t2 = [t + [spare[i]] for i, t in enumerate(tables)]
     step = PagedSequences([1, 2], [33, 34], t2, 4, 2)
@@ -134,4 +134,4 @@ def test_an_eviction_of_pages_that_are_appended_to_afterwards():
     ref, tol = reference(q[:3], kp, vp, [1, 2], [33, 34], t2, [0, 1], 0.125, left, 34)
     near(out, ref[0], tol[0], "out")
     near(counted, ref[1], tol[1], "weights")
-    assert all(torch.equal(rows_of(kp, t, 32), b) for t, b in zip(tables, before)) and free >= 0
+    assert all(torch.equal(rows_of(kp, t, 32), b) for t, b in zip(tables, before))

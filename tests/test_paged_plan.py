@@ -10,10 +10,11 @@ import torch
 from transformer_amd import _lib
 from transformer_amd.paged_attention import PagedEviction, PagedSequences, paged_append, paged_attention, paged_evict
 
-# words of a plan: the public ones, then the launches' sizes and where the lists lie
+# words of a plan: the public ones, then the launches' sizes and where the lists lie; those of few rows for calls without and with weights
 (MAGIC, WORDS, SEQS, HEADS, KV_HEADS, WIDTH, LONGEST, Q_END, Q_COUNT, PAGES, SHARED, RESERVED,
- N_FEW, N_MANY, N_FEWS, N_TILES, N_MANYS, N_APPENDS, FEW_PARTS, MANY_PARTS, FEW_ROWS, SCORES,
- AT_SEQS, AT_FEW, AT_MANY, AT_FEWS, AT_TILES, AT_MANYS, AT_APPENDS, AT_TABLES) = range(30)
+ N_MANY, N_FEWS, N_TILES, N_MANYS, N_APPENDS, MANY_PARTS, FEW_ROWS, SCORES,
+ AT_SEQS, AT_MANY, AT_TILES, AT_MANYS, AT_APPENDS, AT_TABLES, N_FEW) = range(27)
+FEW_PARTS, AT_FEW, AT_FEWS, END = N_FEW + 2, N_FEW + 4, N_FEW + 6, N_FEW + 8
 
 
 def tables_of(lengths, seed=0):
@@ -47,19 +48,21 @@ def check(q_lens, lengths, H, KV, longest=None, starts=None):
     assert [x[:3] for x in entries(w, w[AT_SEQS], n, 4)] == [[a, q, L] for a, q, L in zip(starts, q_lens, lengths)]
     assert w[PAGES] == max([p + 1 for t in tables for p in t], default=0) and not w[SHARED]
     # few rows
-    jobs = [j for j in entries(w, w[AT_FEW], w[N_FEW]) if j[3] >= 0]
-    fews = entries(w, w[AT_FEWS], w[N_FEWS])
-    slots, scores = 0, 0
-    assert [f[3] for f in fews] == [b for b in range(n) if q_lens[b] * g <= 32]
-    for q0, q, L, b, slot, parts, at, _ in fews:
-        assert [q0, q, L] == [starts[b], q_lens[b], lengths[b]] and slot == slots and at == scores
-        slots, scores = slots + parts, scores + q * g * -(-(longest or L) // 32)
-        mine = [j for j in jobs if j[3] == b]
-        assert all(j[:4] == [q0, q, L, b] and j[4] == 2 * at + (parts == 1) for j in mine) and (q > 0) == (parts > 0)
-        if parts:
-            covered(mine, parts, slot, -(-L // 32))
-            assert parts == 1 or w[FEW_PARTS]
-    assert slots == len(jobs) <= w[N_FEW] and scores == w[SCORES]
+    for c in (0, 1):
+        jobs = [j for j in entries(w, w[AT_FEW + c], w[N_FEW + c]) if j[3] >= 0]
+        fews = entries(w, w[AT_FEWS + c], w[N_FEWS])
+        slots, scores = 0, 0
+        assert [f[3] for f in fews] == [b for b in range(n) if q_lens[b] * g <= 32]
+        for q0, q, L, b, slot, parts, at, _ in fews:
+            assert [q0, q, L] == [starts[b], q_lens[b], lengths[b]] and slot == slots and at == scores
+            slots, scores = slots + parts, scores + q * g * -(-(longest or L) // 32)
+            mine = [j for j in jobs if j[3] == b]
+            assert all(j[:4] == [q0, q, L, b] and j[4] == 2 * at + (parts == 1) for j in mine) and (q > 0) == (parts > 0)
+            assert q * g <= w[FEW_ROWS]
+            if parts:
+                covered(mine, parts, slot, -(-L // 32))
+                assert parts == 1 or w[FEW_PARTS + c]
+        assert slots == len(jobs) <= w[N_FEW + c] and scores == w[SCORES]
     # many
     jobs = [j for j in entries(w, w[AT_MANY], w[N_MANY]) if j[3] >= 0]
     tiles = entries(w, w[AT_TILES], w[N_TILES])
@@ -102,7 +105,7 @@ def test_any_step(seed):
     plain = check(q_lens, lengths, H, KV, starts=starts)
     longest = max(max(lengths) + r.randint(0, 700), 1)
     roomy = check(q_lens, lengths, H, KV, longest=longest, starts=starts)
-    assert roomy[N_FEW] >= plain[N_FEW] and roomy[N_MANY] >= plain[N_MANY]
+    assert all(roomy[i] >= plain[i] for i in (N_FEW, N_FEW + 1, N_MANY))
 
 
 @pytest.mark.parametrize("seed", range(30))
@@ -112,7 +115,7 @@ def test_room_for_other_lengths(seed):
     KV = r.choice([1, 2, 4, 8])
     H, n, longest = KV * r.choice([1, 4, 7]), r.choice([1, 5, 33]), r.choice([40, 700, 20000])
     q_lens = [min(longest, r.choice([0, 1, 1, 5, r.randint(1, 400)])) for _ in range(n)]
-    same = (*range(WORDS, Q_COUNT + 1), *range(RESERVED, AT_TABLES + 1))
+    same = (*range(WORDS, Q_COUNT + 1), *range(RESERVED, END))
     plans = []
     for kind in range(4):
         lengths = [(q, longest, r.randint(q, longest), r.choice([q, longest]))[kind] for q in q_lens]

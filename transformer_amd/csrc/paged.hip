@@ -36,8 +36,9 @@ constexpr int32_t kMagic = 0x70616731;
 
 // Words of a plan behind the public ones: launches' sizes, then where the lists lie
 enum {
-  N_FEW = MSD_PLAN_RESERVED + 1, N_MANY, N_FEWS, N_TILES, N_MANYS, N_APPENDS, FEW_PARTS, MANY_PARTS, FEW_ROWS, SCORES,
-  AT_SEQS, AT_FEW, AT_MANY, AT_FEWS, AT_TILES, AT_MANYS, AT_APPENDS, AT_TABLES, END
+  N_MANY = MSD_PLAN_RESERVED + 1, N_FEWS, N_TILES, N_MANYS, N_APPENDS, MANY_PARTS, FEW_ROWS, SCORES,
+  AT_SEQS, AT_MANY, AT_TILES, AT_MANYS, AT_APPENDS, AT_TABLES,
+  N_FEW, FEW_PARTS = N_FEW + 2, AT_FEW = FEW_PARTS + 2, AT_FEWS = AT_FEW + 2, END = AT_FEWS + 2   // two each: without, with weights
 };
 static_assert(END <= MSD_PLAN_HEADER, "the header's words");
 
@@ -236,16 +237,13 @@ __device__ __forceinline__ f32x16 scores_of(const uint8_t* K, int row0, const bf
 // ---- few rows ----
 // The waves of a workgroup take a job's tiles in turn, each with LDS of its own that it fills itself, so that none waits for
 // another before the end, where they are joined.
-template <int DP>
-constexpr int few_waves() { return DP <= 64 ? 4 : 2; }
+template <int DP, int W>
+constexpr int few_lds() { return W * (4 * kFewKeys * pitch<DP>() + 256); }   // and two statistics of 32 rows a wave
 
-template <int DP>
-constexpr int few_lds() { return few_waves<DP>() * (4 * kFewKeys * pitch<DP>() + 256); }   // and two statistics of 32 rows a wave
-
-// Workgroup `group` of few rows
-template <int DP>
+// Workgroup `group` of few rows, W waves
+template <int DP, int W>
 __device__ __forceinline__ void few_rows(const Args& p, int group, uint8_t* lds) {
-  constexpr int P = pitch<DP>(), W = few_waves<DP>(), TILE = kFewKeys * P, OROW = DP + 4;
+  constexpr int P = pitch<DP>(), TILE = kFewKeys * P, OROW = DP + 4;
   float(*stats)[2][32] = reinterpret_cast<float(*)[2][32]>(lds + W * 4 * TILE);
   static_assert(4 * TILE >= 4 * 32 * OROW, "a wave's part of the output");
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -623,10 +621,12 @@ __device__ __forceinline__ void many_rows(const Args& p, int group, uint8_t* lds
   });
 }
 
+// Four waves at every head size (of heads above 64 one workgroup a CU; of two waves each and two a CU, 256 positions of 8 sequences took
+// 8.6 us in place of 7.4, 64 sequences of up to 16000 the same)
 template <int DP>
-__global__ __launch_bounds__(64 * few_waves<DP>(), 2) void paged_few(Args p) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds<DP>()];
-  few_rows<DP>(p, blockIdx.x, lds);
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_few(Args p) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds<DP, kWaves>()];
+  few_rows<DP, kWaves>(p, blockIdx.x, lds);
 }
 template <int DP>
 constexpr int many_lds() { return 8 * HalfTile<DP>::BYTES; }
@@ -635,13 +635,15 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void paged_many(Args
   __shared__ __attribute__((aligned(16))) uint8_t lds[many_lds<DP>()];
   many_rows<DP>(p, blockIdx.x, lds);
 }
-// A step of both: tokens' workgroups, which wait for memory, spread among the chunks', which wait for the matrix cores.
+// A step of both: tokens' workgroups, which wait for memory, spread among the chunks', which wait for the matrix cores; in no more LDS than
+// these take.
 template <int DP>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_both(Args p) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(few_lds<DP>(), many_lds<DP>())];
+  constexpr int W = DP <= 64 ? kWaves : 2;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(few_lds<DP, W>(), many_lds<DP>())];
   const uint32_t few = p.n_few * p.KV, b = blockIdx.x, before = uint32_t(uint64_t(b) * few / gridDim.x);
   if (uint32_t(uint64_t(b + 1) * few / gridDim.x) > before) {
-    if (threadIdx.x < 64 * few_waves<DP>()) few_rows<DP>(p, before, lds);   // (whole waves: the others end)
+    if (threadIdx.x < 64 * W) few_rows<DP, W>(p, before, lds);   // (whole waves: the others end)
   } else {
     many_rows<DP>(p, b - before, lds);
   }
@@ -1195,17 +1197,26 @@ __global__ __launch_bounds__(256) void paged_move(EvictArgs p, int blocks) {
 }
 
 // ---- host: the plan ----
-// Workgroups that a launch is shared out to, about, and tiles of a job at least.
+// Workgroups that a launch is shared out to, about, and tiles of a job at least.  Many rows: a job of 8 tiles split in two takes
+// 18.6 us with the join, whole 12.5 (8 x 128 rows of heads of 64).
 constexpr int kFewGroups = 2048, kManyGroups = 512;
 constexpr int kFewLeast = 4, kManyLeast = 8;
+// Few rows: pieces of four tiles, one a wave, as long as that is one round of the CUs; then longer ones, up to 16; and from 2048 pieces
+// on as many as make 2048 (64 sequences of up to 16000 positions: 425 us, with 1024 486, with 4096 447).
+constexpr int kFewRound = 256, kFewEnough = 16;
+// Without weights a sequence of up to this many tiles stays whole, as the join takes another launch: 512 positions of 8 sequences,
+// 4 K/V heads of 64: 6.7 us in place of 8.8, heads of 128 9.9 and 10.0; 1024: 9.7 and 8.9, 15.1 and 10.9.
+constexpr int kFewWhole = 16;
 
 struct Pieces {
-  int64_t each;
+  int64_t each, whole;
   // of a list of `tiles`: one until it has half as much again as the others' pieces
-  int of(int64_t tiles) const { return 2 * tiles <= 3 * each ? 1 : int(cdiv(tiles, each)); }
+  int of(int64_t tiles) const { return 2 * tiles <= 3 * each || tiles <= whole ? 1 : int(cdiv(tiles, each)); }
 };
-Pieces pieces(int64_t tiles, int n_kv, int groups, int least) {
-  return {std::max<int64_t>(least, cdiv(tiles * n_kv, groups))};
+Pieces many_pieces(int64_t tiles, int n_kv) { return {std::max<int64_t>(kManyLeast, cdiv(tiles * n_kv, kManyGroups)), 0}; }
+Pieces few_pieces(int64_t tiles, int n_kv, bool weighted) {
+  const int64_t round = std::min<int64_t>(std::max<int64_t>(kFewLeast, cdiv(tiles * n_kv, kFewRound)), kFewEnough);
+  return {std::max(round, cdiv(tiles * n_kv, kFewGroups)), weighted ? 0 : kFewWhole};
 }
 
 struct Writer {
@@ -1251,15 +1262,17 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
     else if (s[1]) appends += cdiv(s[2], kPage) - (s[2] - s[1]) / kPage;
   }
   if (longest > std::min<int64_t>(int64_t(table_width) * kPage, kLongest)) return MSD_E_CONFIG;
-  const Pieces fp = pieces(few_tiles, KV, kFewGroups, kFewLeast), mp = pieces(many_tiles, KV, kManyGroups, kManyLeast);
-  int64_t n_few = 0, n_many = 0, few_active = 0;
-  bool few_parts = false, many_parts = false;
+  const Pieces fp[2] = {few_pieces(few_tiles, KV, false), few_pieces(few_tiles, KV, true)}, mp = many_pieces(many_tiles, KV);
+  int64_t n_few[2] = {}, n_many = 0, few_active = 0;
+  bool few_parts[2] = {}, many_parts = false;
   for (int b : few) {
     if (!seqs[3 * b + 1]) continue;
-    const int n = fp.of(cdiv(seqs[3 * b + 2], kFewKeys));
     ++few_active;
-    n_few += n;
-    few_parts |= n > 1;
+    for (int c = 0; c < 2; ++c) {
+      const int n = fp[c].of(cdiv(seqs[3 * b + 2], kFewKeys));
+      n_few[c] += n;
+      few_parts[c] |= n > 1;
+    }
   }
   for (int b : many)
     for (int64_t r = 0, rows = seqs[3 * b + 1] * g; r < rows; r += kManyRows) {
@@ -1268,25 +1281,29 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
       many_parts |= n > 1;
     }
   if (longest) {   // as many as any lengths up to it give: a piece more than whole ones for each list, none below the least
-    const int64_t most_few = cdiv(cdiv(longest, kFewKeys), kFewLeast), most_many = cdiv(cdiv(longest, kKeys), kManyLeast);
-    n_few = few_active ? std::min(few_active * most_few, few_active + cdiv(kFewGroups, KV)) : 0;
+    const int64_t tiles = cdiv(longest, kFewKeys), most_many = cdiv(cdiv(longest, kKeys), kManyLeast);
+    for (int c = 0; c < 2; ++c) {
+      const int64_t most_few = tiles <= fp[c].whole ? 1 : cdiv(tiles, kFewLeast);
+      n_few[c] = few_active ? std::min(few_active * most_few, few_active + cdiv(kFewGroups, KV)) : 0;
+      few_parts[c] = few_active && most_few > 1;
+    }
     n_many = row_tiles ? std::min(row_tiles * most_many, row_tiles + cdiv(kManyGroups, KV)) : 0;
-    few_parts = few_active && most_few > 1;
     many_parts = row_tiles && most_many > 1;
   }
   const int width = int(cdiv(table_width, 4) * 4);
   Writer w{words};
-  const int64_t at_seqs = w.list(n_seqs, 4), at_few = w.list(n_few, 8), at_many = w.list(n_many, 8), at_fews = w.list(few.size(), 8),
-                at_tiles = w.list(row_tiles, 8), at_manys = w.list(many.size(), 8), at_appends = w.list(appends, 4),
-                at_tables = w.list(n_seqs, width);
-  if (w.at >= (int64_t(1) << 28) || scores >= (int64_t(1) << 30) || (n_few + int64_t(few.size())) * KV >= (1 << 24) ||
+  const int64_t at_seqs = w.list(n_seqs, 4), at_many = w.list(n_many, 8), at_tiles = w.list(row_tiles, 8), at_manys = w.list(many.size(), 8),
+                at_appends = w.list(appends, 4), at_few[2] = {w.list(n_few[0], 8), w.list(n_few[1], 8)},
+                at_fews[2] = {w.list(few.size(), 8), w.list(few.size(), 8)}, at_tables = w.list(n_seqs, width);
+  if (w.at >= (int64_t(1) << 28) || scores >= (int64_t(1) << 30) || (n_few[1] + int64_t(few.size())) * KV >= (1 << 24) ||
       (n_many + 4 * row_tiles) * KV >= (1 << 24))
     return MSD_E_CONFIG;
   if (!words) return w.at;
   if (room < w.at) return MSD_E_ARG;
   memset(words, 0, size_t(at_tables) * 4);
   // empty jobs, of a sequence that there is not
-  for (int64_t i = 0; i < n_few; ++i) words[at_few + 8 * i + 3] = -1;
+  for (int c = 0; c < 2; ++c)
+    for (int64_t i = 0; i < n_few[c]; ++i) words[at_few[c] + 8 * i + 3] = -1;
   for (int64_t i = 0; i < n_many; ++i) words[at_many + 8 * i + 3] = -1;
   words[MSD_PLAN_MAGIC] = kMagic;
   words[MSD_PLAN_WORDS] = int32_t(w.at);
@@ -1298,20 +1315,22 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
   words[MSD_PLAN_Q_END] = int32_t(q_end);
   words[MSD_PLAN_Q_COUNT] = int32_t(q_count);
   words[MSD_PLAN_RESERVED] = longest != 0;
-  words[N_FEW] = int32_t(n_few);
+  for (int c = 0; c < 2; ++c) {
+    words[N_FEW + c] = int32_t(n_few[c]);
+    words[FEW_PARTS + c] = few_parts[c];
+    words[AT_FEW + c] = int32_t(at_few[c]);
+    words[AT_FEWS + c] = int32_t(at_fews[c]);
+  }
   words[N_MANY] = int32_t(n_many);
   words[N_FEWS] = int32_t(few.size());
   words[N_TILES] = int32_t(row_tiles);
   words[N_MANYS] = int32_t(many.size());
   words[N_APPENDS] = int32_t(appends);
-  words[FEW_PARTS] = few_parts;
   words[MANY_PARTS] = many_parts;
   words[FEW_ROWS] = int32_t(few_rows);
   words[SCORES] = int32_t(scores);
   words[AT_SEQS] = int32_t(at_seqs);
-  words[AT_FEW] = int32_t(at_few);
   words[AT_MANY] = int32_t(at_many);
-  words[AT_FEWS] = int32_t(at_fews);
   words[AT_TILES] = int32_t(at_tiles);
   words[AT_MANYS] = int32_t(at_manys);
   words[AT_APPENDS] = int32_t(at_appends);
@@ -1354,32 +1373,34 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
   // jobs, the longest first
   struct List { int64_t each; int index; };
   std::vector<List> order;
-  Job* job = reinterpret_cast<Job*>(words + at_few);
-  Few* f = reinterpret_cast<Few*>(words + at_fews);
-  int slot = 0, score = 0;
-  for (size_t i = 0; i < few.size(); ++i) {
-    const int32_t* s = seqs + 3 * few[i];
-    const int64_t tiles = cdiv(s[2], kFewKeys);
-    const int n = s[1] ? fp.of(tiles) : 0;
-    f[i] = {s[0], s[1], s[2], few[i], slot, n, score, 0};
-    slot += n;
-    score += int(s[1] * g * cdiv(longest ? longest : s[2], kFewKeys));
-    if (n) order.push_back({cdiv(tiles, n), int(i)});
-  }
   auto longest_first = [](const List& a, const List& b) { return a.each > b.each; };
-  std::stable_sort(order.begin(), order.end(), longest_first);
-  for (const List& o : order) {
-    const Few& x = f[o.index];
-    const int64_t tiles = cdiv(x.len, kFewKeys);
-    for (int z = 0; z < x.parts; ++z)
-      *job++ = {x.q0, x.n, x.len, x.seq, 2 * x.scores + (x.parts == 1), int(tiles * z / x.parts), int(tiles * (z + 1) / x.parts), x.slot + z};
+  for (int c = 0; c < 2; ++c) {
+    Job* job = reinterpret_cast<Job*>(words + at_few[c]);
+    Few* f = reinterpret_cast<Few*>(words + at_fews[c]);
+    int slot = 0, score = 0;
+    order.clear();
+    for (size_t i = 0; i < few.size(); ++i) {
+      const int32_t* s = seqs + 3 * few[i];
+      const int64_t tiles = cdiv(s[2], kFewKeys);
+      const int n = s[1] ? fp[c].of(tiles) : 0;
+      f[i] = {s[0], s[1], s[2], few[i], slot, n, score, 0};
+      slot += n;
+      score += int(s[1] * g * cdiv(longest ? longest : s[2], kFewKeys));
+      if (n) order.push_back({cdiv(tiles, n), int(i)});
+    }
+    std::stable_sort(order.begin(), order.end(), longest_first);
+    for (const List& o : order) {
+      const Few& x = f[o.index];
+      const int64_t tiles = cdiv(x.len, kFewKeys);
+      for (int z = 0; z < x.parts; ++z)
+        *job++ = {x.q0, x.n, x.len, x.seq, 2 * x.scores + (x.parts == 1), int(tiles * z / x.parts), int(tiles * (z + 1) / x.parts), x.slot + z};
+    }
   }
   order.clear();
-  job = reinterpret_cast<Job*>(words + at_many);
+  Job* job = reinterpret_cast<Job*>(words + at_many);
   RowTile* t = reinterpret_cast<RowTile*>(words + at_tiles);
   Job* m = reinterpret_cast<Job*>(words + at_manys);
-  slot = 0;
-  int index = 0;
+  int slot = 0, index = 0;
   for (int b : many) {
     const int32_t* s = seqs + 3 * b;
     *m++ = {s[0], s[1], s[2], b, 0, 0, 0, 0};
@@ -1435,7 +1456,7 @@ struct Space {
 };
 Space space(const msd_paged& a, bool weighted) {
   const int32_t* h = a.plan_host;
-  const int64_t few = int64_t(h[N_FEW]) * h[MSD_PLAN_KV_HEADS] * kFewRows, many = int64_t(h[N_MANY]) * h[MSD_PLAN_KV_HEADS] * kManyRows;
+  const int64_t few = int64_t(h[N_FEW + weighted]) * h[MSD_PLAN_KV_HEADS] * kFewRows, many = int64_t(h[N_MANY]) * h[MSD_PLAN_KV_HEADS] * kManyRows;
   Space s{};
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -1443,8 +1464,8 @@ Space space(const msd_paged& a, bool weighted) {
     at += up(bytes);
     return from;
   };
-  s.few_part = take(h[FEW_PARTS] ? 4 * few * a.d_head : 0);
-  s.few_lse = take(h[FEW_PARTS] || weighted ? 4 * few : 0);
+  s.few_part = take(h[FEW_PARTS + weighted] ? 4 * few * a.d_head : 0);
+  s.few_lse = take(h[FEW_PARTS + weighted] || weighted ? 4 * few : 0);
   s.many_part = take(h[MANY_PARTS] ? 4 * many * a.d_head : 0);
   s.many_lse = take(h[MANY_PARTS] ? 4 * many : 0);
   s.lse = take(weighted && h[N_MANYS] ? 4 * a.q_rows * h[MSD_PLAN_HEADS] : 0);
@@ -1486,7 +1507,7 @@ extern "C" int32_t msd_paged_append(const msd_paged* a, const void* k_new, const
 
 extern "C" int64_t msd_paged_attn_workspace_bytes(const msd_paged* a, int32_t weighted) {
   const int32_t rc = check(a);
-  return rc != MSD_OK ? rc : space(*a, weighted).end;
+  return rc != MSD_OK ? rc : space(*a, weighted != 0).end;
 }
 
 extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void* k, const void* v, void* out, const float* weights,
@@ -1500,9 +1521,9 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
   if (reinterpret_cast<uintptr_t>(weights_out) % 4) return MSD_E_ARG;
   const int64_t KV = h[MSD_PLAN_KV_HEADS], longest = h[MSD_PLAN_LONGEST], most = (int64_t(1) << 32) / 256 - 1;
   const int64_t key_blocks = cdiv(longest, 128), weight_blocks = weighted ? cdiv(longest, kWeightKeys) : 0;
-  const int n_tiles = h[MANY_PARTS] ? h[N_TILES] : 0, n_fews = h[FEW_PARTS] || weighted ? h[N_FEWS] : 0;
+  const int n_tiles = h[MANY_PARTS] ? h[N_TILES] : 0, n_fews = h[FEW_PARTS + weighted] || weighted ? h[N_FEWS] : 0;
   // one row of few a workgroup as long as there are few of them (16 parts of 64 rows: 4.0 us, with four rows 5.6; 2048 rows: 6.7 and 5.0)
-  const int join_rows = int64_t(n_fews) * KV * h[FEW_ROWS] <= 1024 ? 1 : kJoinRows, few_joins = h[FEW_PARTS] ? int(cdiv(h[FEW_ROWS], join_rows)) : 0;
+  const int join_rows = int64_t(n_fews) * KV * h[FEW_ROWS] <= 1024 ? 1 : kJoinRows, few_joins = h[FEW_PARTS + weighted] ? int(cdiv(h[FEW_ROWS], join_rows)) : 0;
   const int64_t finish = int64_t(n_tiles) * KV * (kManyRows / kJoinRows) + int64_t(n_fews) * KV * (few_joins + weight_blocks);
   if (finish > most || key_blocks * KV * h[N_MANYS] > most) return MSD_E_CONFIG;
   if (h[MSD_PLAN_Q_COUNT] && (bad(q) || bad(k) || bad(v) || bad(out))) return MSD_E_ARG;
@@ -1530,12 +1551,12 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
   p.n_pages = int(a->positions / kPage);
   p.plan = a->plan;
   p.tables = a->plan + h[AT_TABLES];
-  p.few = reinterpret_cast<const Job*>(a->plan + h[AT_FEW]);
+  p.few = reinterpret_cast<const Job*>(a->plan + h[AT_FEW + weighted]);
   p.many = reinterpret_cast<const Job*>(a->plan + h[AT_MANY]);
-  p.n_few = h[N_FEW];
+  p.n_few = h[N_FEW + weighted];
   p.n_many = h[N_MANY];
   p.out = static_cast<uint16_t*>(out);
-  p.few_part = h[FEW_PARTS] ? floats(at.few_part) : nullptr;
+  p.few_part = h[FEW_PARTS + weighted] ? floats(at.few_part) : nullptr;
   p.few_lse = floats(at.few_lse);
   p.many_part = h[MANY_PARTS] ? floats(at.many_part) : nullptr;
   p.many_lse = floats(at.many_lse);
@@ -1548,14 +1569,14 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
   const Job* manys = reinterpret_cast<const Job*>(a->plan + h[AT_MANYS]);
   with_head(a->d_head, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
-    const unsigned few = unsigned(h[N_FEW] * KV), many = unsigned(h[N_MANY] * KV);
+    const unsigned few = unsigned(h[N_FEW + weighted] * KV), many = unsigned(h[N_MANY] * KV);
     if (few && many) hipLaunchKernelGGL((paged_both<DP>), dim3(few + many), dim3(64 * kWaves), 0, s, p);
-    else if (few) hipLaunchKernelGGL((paged_few<DP>), dim3(few), dim3(64 * few_waves<DP>()), 0, s, p);
+    else if (few) hipLaunchKernelGGL((paged_few<DP>), dim3(few), dim3(64 * kWaves), 0, s, p);
     else if (many) hipLaunchKernelGGL((paged_many<DP>), dim3(many), dim3(64 * kWaves), 0, s, p);
   });
   if (finish)
     hipLaunchKernelGGL(paged_finish, dim3(unsigned(finish)), dim3(kFinish), 0, s, p, reinterpret_cast<const RowTile*>(a->plan + h[AT_TILES]),
-                       n_tiles, reinterpret_cast<const Few*>(a->plan + h[AT_FEWS]), n_fews, few_joins, join_rows);
+                       n_tiles, reinterpret_cast<const Few*>(a->plan + h[AT_FEWS + weighted]), n_fews, few_joins, join_rows);
   if (weighted && h[N_MANYS] && key_blocks)
     with_head(a->d_head, [&](auto dp) {
       constexpr int DP = decltype(dp)::value;
