@@ -1197,10 +1197,13 @@ __global__ __launch_bounds__(256) void paged_move(EvictArgs p, int blocks) {
 }
 
 // ---- host: the plan ----
-// Workgroups that a launch is shared out to, about, and tiles of a job at least.  Many rows: a job of 8 tiles split in two takes
-// 18.6 us with the join, whole 12.5 (8 x 128 rows of heads of 64).
+// Workgroups that a launch is shared out to, about, and tiles of a job at least.
 constexpr int kFewGroups = 2048, kManyGroups = 512;
-constexpr int kFewLeast = 4, kManyLeast = 8;
+constexpr int kFewLeast = 4, kManyLeast = 6;
+// Many rows' lists of up to this many tiles stay whole: one of 8 tiles split in two takes 18.6 us with the join, whole 12.5 (8 x 128
+// rows of heads of 64).  Longer ones in pieces of 4, 6 and 8 tiles at least: 24.9, 24.6 and 26.7 (a step of tokens and chunks, up to
+// 46 tiles of heads of 96).
+constexpr int kManyWhole = 8;
 // Few rows: pieces of four tiles, one a wave, as long as that is one round of the CUs; then longer ones, up to 16; and from 2048 pieces
 // on as many as make 2048 (64 sequences of up to 16000 positions: 425 us, with 1024 486, with 4096 447).
 constexpr int kFewRound = 256, kFewEnough = 16;
@@ -1213,7 +1216,7 @@ struct Pieces {
   // of a list of `tiles`: one until it has half as much again as the others' pieces
   int of(int64_t tiles) const { return 2 * tiles <= 3 * each || tiles <= whole ? 1 : int(cdiv(tiles, each)); }
 };
-Pieces many_pieces(int64_t tiles, int n_kv) { return {std::max<int64_t>(kManyLeast, cdiv(tiles * n_kv, kManyGroups)), 0}; }
+Pieces many_pieces(int64_t tiles, int n_kv) { return {std::max<int64_t>(kManyLeast, cdiv(tiles * n_kv, kManyGroups)), kManyWhole}; }
 Pieces few_pieces(int64_t tiles, int n_kv, bool weighted) {
   const int64_t round = std::min<int64_t>(std::max<int64_t>(kFewLeast, cdiv(tiles * n_kv, kFewRound)), kFewEnough);
   return {std::max(round, cdiv(tiles * n_kv, kFewGroups)), weighted ? 0 : kFewWhole};
