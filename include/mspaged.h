@@ -9,8 +9,8 @@
  *
  * All calls but msd_paged_plan are asynchronous on `stream` (a hipStream_t of the current device), allocate nothing and return
  * MSD_OK or a negative MSD_E_* code (msdecode.h): MSD_E_ARG for a null or misaligned pointer or a plan that msd_paged_plan has
- * not made, MSD_E_CONFIG for a shape outside the limits below.  Every result is deterministic: sums are taken in a fixed
- * order, without atomics.
+ * not made, MSD_E_CONFIG for a shape outside the limits below.  Every result is deterministic: sums of floating-point numbers are
+ * taken in a fixed order.
  */
 #ifndef MSPAGED_H
 #define MSPAGED_H
@@ -43,8 +43,9 @@ enum {
  * words NULL: returns how many there are; otherwise writes them (`room` of them are there) and returns that.  Word MSD_PLAN_Q_END:
  * one past the last row; Q_COUNT: rows of all sequences; PAGES: one past the largest page in use; SHARED: whether a page
  * that takes new rows is in use elsewhere too.
- * Limits: 0 <= q_len <= length <= longest <= 16 table_width, below 2^31 - 2^16; n_heads a multiple of n_kv_heads, up to 4096; n_seqs up to 65535,
- * rows and pool positions below 2^31; q_len times the heads of a group below 2^30 - 256; the words below 2^28. */
+ * Limits: 0 <= q_len <= length <= longest <= 16 table_width, below 2^31 - 2^16; n_heads a multiple of n_kv_heads, up to 4096; n_seqs
+ * up to 65535, rows and pool positions below 2^31; q_len times the heads of a group below 2^30 - 256; the words below 2^28, the
+ * pages that take new rows and the pieces of work below 2^24. */
 int64_t msd_paged_plan(int32_t n_seqs, const int32_t* seqs, const int32_t* tables, int32_t table_width, int32_t n_heads,
                        int32_t n_kv_heads, int32_t longest, int32_t* words, int64_t room);
 
@@ -81,9 +82,9 @@ int32_t msd_paged_attn(const msd_paged* a, const void* q, const void* k, const v
                        int32_t weights_width, float* weights_out, void* workspace, void* stream);
 
 /* Of each sequence, layer and K/V head: the newest `recent` of its positions and, of the others, those with the largest weights
- * (of equal ones the lower position; a NaN counts as larger than any number and comes back as one of no particular bits), min(length, keep) in all, copied in their order to
- * positions 0, 1, .. of the pages that `to` (n_seqs rows of to_width page numbers, on the device) names, which are none
- * that the sequences use and different from one another.  Layers of k (v) are k_layer (v_layer) elements apart.  weights: f32
+ * (of equal ones the lower position; a NaN counts as larger than any number and comes back as one of no particular bits),
+ * min(length, keep) in all, copied in their order to positions 0, 1, .. of the pages that `to` (n_seqs rows of to_width page
+ * numbers, on the device) names, which are none that the sequences use and different from one another.  Layers of k (v) are k_layer (v_layer) elements apart.  weights: f32
  * (n_layers, n_seqs, n_kv_heads, weights_width), positions from weights_width on have weight 0; weights_out (.., keep) those of
  * the kept ones, kept (.., keep) int32 their positions; 0 and -1 behind the last.
  * Limits: 0 <= recent <= keep <= 16 to_width; n_layers times n_kv_heads below 65536, times n_seqs times keep below 2^40. */

@@ -102,6 +102,8 @@ def test_append_refusals():
                        ((k, k, rand((2, 16 * n, 68), 1)[..., :64], kp), "16-byte"), ((k, k, rand((2, 64, 16 * n), 1).transpose(1, 2), kp), "contiguous")):
         with pytest.raises(ValueError, match=match):
             paged_append(*bad, s)
+    with pytest.raises(ValueError, match="same memory"):
+        paged_append(k, k, kp, kp, s)
     with pytest.raises(ValueError, match="elsewhere"):
         paged_append(k, k, kp, kp.clone(), PagedSequences([1, 1], [20, 20], [tables[0]] * 2, 4, 2))
     leaf = k.clone().requires_grad_()

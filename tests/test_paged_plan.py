@@ -297,8 +297,8 @@ def test_c_calls_with_bad_pointers():
 
 def test_c_plans_outside_the_limits():
     L = _lib.lib()
-    plan = lambda seqs, pages, width, H=4, KV=2, longest=0, n=1, words=None, room=0: L.msd_paged_plan(  # noqa: E731
-        n, (ctypes.c_int32 * len(seqs))(*seqs), (ctypes.c_int32 * max(len(pages), 1))(*pages), width, H, KV, longest, words, room)
+    plan = lambda seqs, pages, width, H=4, KV=2, longest=0, n=1, words=None, room=0, pages_at=None: L.msd_paged_plan(  # noqa: E731
+        n, (ctypes.c_int32 * len(seqs))(*seqs), pages_at or (ctypes.c_int32 * max(len(pages), 1))(*pages), width, H, KV, longest, words, room)
     C, A = _lib.MSD_E_CONFIG, _lib.MSD_E_ARG
     n = plan((0, 1, 20), (0, 1), 2)
     assert n > 40 and plan((0, 1, 20), (0, 1), 2, words=(ctypes.c_int32 * n)(), room=n) == n
@@ -309,6 +309,12 @@ def test_c_plans_outside_the_limits():
                      ((0, 1, 20), dict(n=70000)), ((2 ** 31 - 1, 1, 20), {})):
         assert plan(seqs, (0, 1), 2, **kw) == C, (seqs, kw)
     assert plan((0, 2 ** 29, 2 ** 29), (0, 1), 2 ** 26) == C   # the rows of a group
+    # a launch's threads: pages that take new rows; few and many rows together (2^24 pieces and a little more, either alone fewer)
+    assert plan((0, 2 ** 28 - 16, 2 ** 28 - 16), (), 2 ** 24, H=1, KV=1, pages_at=256) > 0
+    assert plan((0, 2 ** 28, 2 ** 28), (), 2 ** 24, H=1, KV=1, pages_at=256) == C
+    few, many = [(i, 1, 16) for i in range(1800)], [(2000 + 40 * i, 40, 48) for i in range(600)]
+    for seqs, ok in ((few, True), (many, True), (few + many, False)):
+        assert (plan(sum(seqs, ()), (), 3, H=4096, KV=4096, n=len(seqs), pages_at=256) > 0) == ok
     assert L.msd_paged_plan(1, None, (ctypes.c_int32 * 2)(), 2, 4, 2, 0, None, 0) == A
     assert L.msd_paged_plan(1, (ctypes.c_int32 * 3)(0, 1, 20), None, 2, 4, 2, 0, None, 0) == A
     assert L.msd_paged_plan(0, None, None, 0, 4, 2, 0, None, 0) == 40

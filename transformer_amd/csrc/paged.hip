@@ -787,8 +787,8 @@ __global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* t
 
 // ---- the weights of many rows ----
 // 128 keys a workgroup, 32 a wave in registers, over the group's heads and the rows that see them: S = Q K^T, a lane holds one
-// key's scores against 16 rows, so that its sum stays in the lane; a row's scores start as -L_i / c (what p.lse holds here).  Two
-// halves of four waves take the tiles of 64 rows in turn.  While the probabilities of 32 rows are formed, the matrix cores form the
+// key's scores against 16 rows, so that its sum stays in the lane; a row's scores start as -L_i / c (what p.lse holds here).  Four
+// teams of four waves take the tiles of 64 rows in turn.  While the probabilities of 32 rows are formed, the matrix cores form the
 // next 32 rows' scores.
 constexpr int kHalves = 4;
 template <int DP>
@@ -1298,8 +1298,9 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
   const int64_t at_seqs = w.list(n_seqs, 4), at_many = w.list(n_many, 8), at_tiles = w.list(row_tiles, 8), at_manys = w.list(many.size(), 8),
                 at_appends = w.list(appends, 4), at_few[2] = {w.list(n_few[0], 8), w.list(n_few[1], 8)},
                 at_fews[2] = {w.list(few.size(), 8), w.list(few.size(), 8)}, at_tables = w.list(n_seqs, width);
-  if (w.at >= (int64_t(1) << 28) || scores >= (int64_t(1) << 30) || (n_few[1] + int64_t(few.size())) * KV >= (1 << 24) ||
-      (n_many + 4 * row_tiles) * KV >= (1 << 24))
+  // (a launch counts its threads in 32 bits)
+  if (w.at >= (int64_t(1) << 28) || scores >= (int64_t(1) << 30) || appends >= (1 << 24) ||
+      (n_few[1] + int64_t(few.size()) + n_many + 4 * row_tiles) * KV >= (1 << 24))
     return MSD_E_CONFIG;
   if (!words) return w.at;
   if (room < w.at) return MSD_E_ARG;
@@ -1308,7 +1309,6 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
   for (int c = 0; c < 2; ++c)
     for (int64_t i = 0; i < n_few[c]; ++i) words[at_few[c] + 8 * i + 3] = -1;
   for (int64_t i = 0; i < n_many; ++i) words[at_many + 8 * i + 3] = -1;
-  words[MSD_PLAN_MAGIC] = kMagic;
   words[MSD_PLAN_WORDS] = int32_t(w.at);
   words[MSD_PLAN_SEQS] = n_seqs;
   words[MSD_PLAN_HEADS] = H;
@@ -1423,6 +1423,7 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
     for (int z = 0; z < x.parts; ++z)
       *job++ = {x.q0, x.n, x.len, x.seq, x.parts == 1 ? -x.row0 - 1 : x.row0, int(tiles * z / x.parts), int(tiles * (z + 1) / x.parts), x.slot + z};
   }
+  words[MSD_PLAN_MAGIC] = kMagic;
   return w.at;
 }
 
@@ -1595,8 +1596,9 @@ extern "C" int32_t msd_paged_evict(const msd_paged* a, int32_t n_layers, int64_t
   if (rc != MSD_OK) return rc;
   const int32_t* h = a->plan_host;
   const int64_t heads = int64_t(n_layers) * h[MSD_PLAN_KV_HEADS];
-  if (n_layers < 0 || keep < 0 || heads >= 65536 || heads * h[MSD_PLAN_SEQS] * std::max(keep, 1) >= int64_t(1) << 40 || weights_width < 0 || recent < 0 || recent > keep || to_width < 0 || keep > int64_t(to_width) * kPage || k_layer % 8 || v_layer % 8 ||
-      k_layer < 0 || v_layer < 0 || k_layer > (int64_t(1) << 44) || v_layer > (int64_t(1) << 44))
+  if (n_layers < 0 || keep < 0 || heads >= 65536 || heads * h[MSD_PLAN_SEQS] * std::max(keep, 1) >= int64_t(1) << 40 || weights_width < 0 ||
+      recent < 0 || recent > keep || to_width < 0 || keep > int64_t(to_width) * kPage || k_layer % 8 || v_layer % 8 || k_layer < 0 || v_layer < 0 ||
+      k_layer > (int64_t(1) << 44) || v_layer > (int64_t(1) << 44))
     return MSD_E_CONFIG;
   if (!heads || !h[MSD_PLAN_SEQS] || !keep) return MSD_OK;
   if (bad(k) || bad(v) || (weights_width && (!weights || reinterpret_cast<uintptr_t>(weights) % 4)) || !to || reinterpret_cast<uintptr_t>(to) % 4 ||

@@ -496,6 +496,7 @@ void no_gradient(const char* what, const X&... x) {
 
 // (first: an inference tensor outside inference mode raises here)
 void written(const Tensor& k, const Tensor& v) {
+  need(k.numel() == 0 || k.data_ptr() != v.data_ptr(), "k_pages and v_pages are the same memory");
   for (const Tensor* x : {&k, &v}) x->unsafeGetTensorImpl()->bump_version();
 }
 

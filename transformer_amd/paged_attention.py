@@ -14,9 +14,9 @@ and ``[layer, 1]`` (values), each (n_kv_heads, positions, d_head) bf16, or any t
   weights, kept = paged_evict(k_pages, v_pages, weights, eviction)              # a layer's pages, or all layers'
 
 What runs (``msd_paged_append`` / ``msd_paged_attn`` / ``msd_paged_evict``, ``csrc/paged.hip``): attention in one pass over the
-keys with the running maximum and sum of the softmax, on the matrix cores; f32 scores, statistics and sums; the
-probabilities are rounded to bf16 as operands of the product with the values (not in the weights), the output once to bf16.
-Deterministic.  No gradients.
+keys with the running maximum and sum of the softmax, on the matrix cores; f32 scores, statistics and sums; as
+operands of the product with the values the probabilities are two bf16 (32 rows of a K/V head's group and fewer; 2^-17) or
+rounded to one; in the weights they are f32; the output is rounded to bf16 once.  Deterministic.  No gradients.
 """
 import numpy as np
 import torch
@@ -85,7 +85,9 @@ class PagedSequences:
 
     ``longest``: room for lengths up to it, and ``update``: the object, and a captured graph that reads it, then goes on with the
     lengths and pages of the next step (the launches are those of the longest lengths, what has no work ends at once).  A
-    captured graph's object has to be kept, and made before the capture."""
+    captured graph's object has to be kept, and made before the capture.  A replay checks nothing: pages that take new rows must
+    still be in use by one sequence only, pages outside the pool read as zeros and are not written, and a captured eviction
+    is of the lengths and pages that it was made for."""
 
     def __init__(self, q_lens, lengths, tables, n_heads, n_kv_heads, q_starts=None, longest=None, device="cuda"):
         self.q_lens = _integers(q_lens, "lengths")
