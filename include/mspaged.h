@@ -84,9 +84,9 @@ int32_t msd_paged_attn(const msd_paged* a, const void* q, const void* k, const v
 /* Of each sequence, layer and K/V head: the newest `recent` of its positions and, of the others, those with the largest weights
  * (of equal ones the lower position; a NaN counts as larger than any number and comes back as one of no particular bits),
  * min(length, keep) in all, copied in their order to positions 0, 1, .. of the pages that `to` (n_seqs rows of to_width page
- * numbers, on the device) names, which are none that the sequences use and different from one another.  Layers of k (v) are k_layer (v_layer) elements apart.  weights: f32
- * (n_layers, n_seqs, n_kv_heads, weights_width), positions from weights_width on have weight 0; weights_out (.., keep) those of
- * the kept ones, kept (.., keep) int32 their positions; 0 and -1 behind the last.
+ * numbers, on the device) names, which are none that the sequences use and different from one another.  Layers of k (v) are
+ * k_layer (v_layer) elements apart.  weights: f32 (n_layers, n_seqs, n_kv_heads, weights_width), positions from weights_width on
+ * have weight 0; weights_out (.., keep) those of the kept ones, kept (.., keep) int32 their positions; 0 and -1 behind the last.
  * Limits: 0 <= recent <= keep <= 16 to_width; n_layers times n_kv_heads below 65536, times n_seqs times keep below 2^40. */
 int32_t msd_paged_evict(const msd_paged* a, int32_t n_layers, int64_t k_layer, int64_t v_layer, void* k, void* v, const float* weights,
                         int32_t weights_width, int32_t keep, int32_t recent, const int32_t* to, int32_t to_width, float* weights_out,

@@ -11,7 +11,10 @@ Python surface (drop-in for the reference's decode path):
   * training, as torch calls with autograd: ``transformer_amd.xent`` (the output layer and its
     loss, reference model.py:279-379) and the operators of a layer (model.py:94-160):
     ``transformer_amd.attention``, ``transformer_amd.rotary``, ``transformer_amd.norm`` and
-    ``transformer_amd.swiglu``.
+    ``transformer_amd.swiglu``;
+  * serving over a paged cache, as torch calls: ``transformer_amd.paged`` (the pool, and the batched
+    decode of the whole model over it) and ``transformer_amd.paged_attention`` (a step's append,
+    attention and eviction for a model of the operators above).
 
 All compute runs in hand-written HIP kernels for gfx950 behind the C-ABI library
 ``libmsdecode.so`` (declared in ``include/msdecode.h``).

@@ -12,6 +12,16 @@
 // head r % g (see attn.hip, whose tiles these kernels use).
 //   few rows (up to 32 of a group: a token, a few drafts): paged_few, then paged_finish where the keys are split or weights counted
 //   more (a chunk of a prompt): paged_many, paged_finish where the keys are split, paged_weights where weights are counted
+//
+// Measured (us, kernels under a tracer):
+//   paged_few       memory.  64 tokens over up to 16000 positions, 8 K/V heads of 128: 418, 6.4 TB/s of reads (24 over up to 8000, 16 heads, with
+//                   weights: 187, 5.8 TB/s); 4 over up to 2000, 4 heads of 64: 4.9, a chain of plan, pages, rows
+//   paged_many      the matrix cores' power.  2048 rows at 16384, 32 / 8 heads of 128: 477-526 by card, 980-1080 TFLOP/s of the products under
+//                   the mask (a library's 8192^3 product: 1215-1242); 8 x 128 over up to 512, 16 / 4 heads of 64: 12, one round, a chain of tiles
+//   paged_finish    latency: 4.4-8
+//   paged_weights   LDS reads, and first loads where rows are few.  511 rows at 8191, 16 / 4 heads of 128: 27, 610 TFLOP/s
+//   paged_append    memory.  28665 tokens, 8 heads of 128: 46 with pages out of the caches, a copy's rate and above
+//   paged_select, paged_move   30000 positions of 64 heads: 25, latency of counts in LDS; 8000 rows each of 128: 93, a copy's rate
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -931,8 +941,8 @@ struct AppendArgs {
 };
 
 // The rows of one page and sequence, up to 256 16-byte pieces of a head: a thread has one piece of every head (of every second,
-// fourth, .. where there are fewer), K's heads, then V's.  Memory bound.  Stores that do not stay in the caches: 16383 tokens of 8
-// heads of 128 to pages that are not in them take 53 us in place of 58.
+// fourth, .. where there are fewer), K's heads, then V's.  Memory bound.  Stores that do not stay in the caches: 28665 tokens of 8
+// heads of 128 to pages that are not in them take 46 us, before that and the heads in flight together 58.
 __global__ __launch_bounds__(256) void paged_append(AppendArgs p) {
   const Append a = scalar_load(p.jobs + blockIdx.x);
   if (a.row < 0 || a.count <= 0 || a.count > kPage || a.row > p.q_rows - a.count || a.position < 0 || a.position > p.positions - a.count)
@@ -1246,8 +1256,8 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
   for (int b = 0; b < n_seqs; ++b) {
     const int32_t* s = seqs + 3 * b;
     const int64_t rows = s[1] * g;
-    if (s[0] < 0 || s[1] < 0 || s[2] < s[1] || s[2] > std::min<int64_t>(int64_t(table_width) * kPage, kLongest) || (longest && s[2] > longest) || s[0] > INT32_MAX - s[1] ||
-        rows >= (1 << 30) - 256)
+    if (s[0] < 0 || s[1] < 0 || s[2] < s[1] || s[2] > std::min<int64_t>(int64_t(table_width) * kPage, kLongest) || (longest && s[2] > longest) ||
+        s[0] > INT32_MAX - s[1] || rows >= (1 << 30) - 256)
       return MSD_E_CONFIG;
     most = std::max(most, s[2]);
     if (s[1]) q_end = std::max<int64_t>(q_end, int64_t(s[0]) + s[1]);
