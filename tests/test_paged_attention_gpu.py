@@ -151,6 +151,19 @@ def test_many_sequences():
     check([min(n, 1 + i % 2) for i, n in enumerate(lengths)], lengths, 2, 1, 64, seed=11)
 
 
+@pytest.mark.parametrize("q_lens,lengths,H,KV,D,longest", [
+    ([1] * 6, [511, 512, 513, 1, 32, 33], 8, 2, 64, None), ([1] * 4, [512, 480, 256, 257], 8, 2, 64, None), ([1, 1, 1], [1023, 1024, 700], 8, 2, 64, None),
+    ([1, 1], [1025, 1024], 8, 2, 64, None), ([1] * 32, [1024 - 29 * i for i in range(32)], 8, 2, 32, None), ([1] * 35, [900 - 25 * i for i in range(35)], 8, 2, 96, None),
+    ([1, 2, 4], [512, 100, 511], 8, 2, 128, None), ([4, 1], [1000, 3], 32, 4, 64, None), ([5, 1], [300, 3], 32, 4, 64, None), ([17, 1], [300, 20], 1, 1, 128, None),
+    ([16, 9], [16, 512], 2, 2, 128, None), ([0, 3, 0, 1], [40, 300, 0, 511], 6, 2, 80, None), ([32], [32], 1, 1, 8, None), ([1] * 128, [5 * i + 1 for i in range(128)], 4, 2, 72, None),
+    ([1] * 129, [3 * i + 1 for i in range(129)], 4, 2, 64, None), ([1, 0, 2], [50, 33, 260], 8, 2, 64, 512), ([1, 0, 2], [50, 33, 260], 8, 2, 64, 1000), ([2] * 40, [7 * i + 2 for i in range(40)], 4, 2, 128, 1024),
+])
+def test_few_short_sequences(q_lens, lengths, H, KV, D, longest):
+    """Around what a sequence by one workgroup takes: lengths, rows of a group, workgroups, sequences without new tokens."""
+    check(q_lens, lengths, H, KV, D, seed=9, longest=longest, width=200)
+    check(q_lens, lengths, H, KV, D, seed=10, longest=longest, weights=False)
+
+
 @pytest.mark.parametrize("width", [0, 1, 30, 63, 5000])
 def test_weights_of_any_width(width):
     check([1, 40, 2], [64, 300, 40], 4, 2, 64, seed=12, width=width)
@@ -255,14 +268,15 @@ def test_long_caches():
     check([70], [9000], 4, 1, 128, seed=22)
 
 
-def test_a_captured_step_goes_on():
+@pytest.mark.parametrize("last", [40, 4])
+def test_a_captured_step_goes_on(last):
     """A graph over sequences with room: lengths and pages of the next steps, replayed and beside eager calls on the same object;
     two graphs on two streams share it."""
-    q_lens, steps = [1, 2, 40], [[60, 700, 90], [61, 702, 130], [62, 1000, 400], [1, 2, 40], [1000, 1000, 1000]]
+    q_lens, steps = [1, 2, last], [[60, 700, 90], [61, 702, 130], [62, 1000, 400], [1, 2, 40], [1000, 1000, 1000]]
     n = 200
     order = torch.randperm(n, generator=torch.Generator().manual_seed(1)).tolist()
     tables = [order[i * 66:i * 66 + 66] for i in range(3)]
-    q, k, v = rand((43, 8, 64), 1, 1.5), rand((2, 16 * n, 64), 2), rand((2, 16 * n, 64), 3)
+    q, k, v = rand((3 + last, 8, 64), 1, 1.5), rand((2, 16 * n, 64), 2), rand((2, 16 * n, 64), 3)
     old = torch.rand((3, 2, 1000), generator=torch.Generator().manual_seed(3)).cuda()
     sequences = PagedSequences(q_lens, steps[0], tables, 8, 2, longest=1000)
     paged_attention(q, k, v, sequences, weights=old)
@@ -307,11 +321,11 @@ def test_two_streams():
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
-def test_device_words_that_have_been_overwritten():
+@pytest.mark.parametrize("q_lens,lengths", [([1, 60], [300, 200]), ([1, 3], [300, 200])])
+def test_device_words_that_have_been_overwritten(q_lens, lengths):
     """Page numbers outside the pool read as rows of zeros; jobs that leave their limits end."""
-    q_lens, lengths = [1, 60], [300, 200]
     tables, n = tables_of(lengths, 3)
-    q, k, v = rand((61, 4, 64), 1), rand((2, 16 * n, 64), 2), rand((2, 16 * n, 64), 3)
+    q, k, v = rand((sum(q_lens), 4, 64), 1), rand((2, 16 * n, 64), 2), rand((2, 16 * n, 64), 3)
     old = torch.rand((2, 2, 300)).cuda()
     s = PagedSequences(q_lens, lengths, tables, 4, 2)
     spare = next(p for p in range(n) if all(p not in t for t in tables))

@@ -11,6 +11,7 @@
 // job needs beside the pages, so that no workgroup is empty and none counts sequences.  Row r of a sequence's group is position r / g,
 // head r % g (see attn.hip, whose tiles these kernels use).
 //   few rows (up to 32 of a group: a token, a few drafts): paged_few, then paged_finish where the keys are split or weights counted
+//                                                   or, of few short sequences, paged_whole alone
 //   more (a chunk of a prompt): paged_many, paged_finish where the keys are split, paged_weights where weights are counted
 //
 // Measured (us, kernels under a tracer):
@@ -86,7 +87,7 @@ struct Args {
   float *few_part, *few_lse;      // [slot][kv head][32] rows of D, logsumexps
   float *many_part, *many_lse;    // [slot][kv head][128]
   float* lse;                     // -L_i / c of every row of many, sequence by sequence, head by head, or null
-  float* scores;                  // c q.k of few rows, [sequence][kv head][row][keys up to a multiple of 32], or null
+  float* scores;                  // c q.k of few rows, [sequence][kv head][tile of 32 keys][row][key], or null
   int64_t score_words;
   const float* weights;
   int weights_width;
@@ -270,26 +271,29 @@ __device__ __forceinline__ void few_rows(const Args& p, int group, uint8_t* lds)
   kt.init(p.k.row, p.D, lane, 0);
   vt.init(p.v.row, p.D, lane, 0);
   constexpr int HALF = decltype(kt)::N;
-  auto load = [&](int t, int stage) {
-    const int2 pages = scalar_load(reinterpret_cast<const int2*>(table) + t);
+  auto pages_of = [&](int t) { return scalar_load(reinterpret_cast<const int2*>(table) + min(t, j.t1 - 1)); };
+  auto load = [&](int2 pages, int t, int stage) {
     const int left = j.len - t * kFewKeys;
     auto page = [&](int i) { return pick(i, pages.x, pages.y, 0, 0); };
     kt.load(to + stage * 2 * TILE, left, 0, kb, p.k.row, p.n_pages, page);
     vt.load(to + stage * 2 * TILE + TILE, left, 0, vb, p.v.row, p.n_pages, page);
   };
   int t = j.t0 + wv;
-  if (t < j.t1) load(t, 0);
+  int2 pages{};   // of the next tile: asked for a tile ahead, as nothing can be fetched before they are there
+  if (t < j.t1) {
+    const int2 now = pages_of(t);
+    pages = pages_of(t + W);
+    load(now, t, 0);
+  }
   const int r = lane & 31, pos = div_g(p, min(r, R - 1));
   const bool ok = r < R;
   bf16x8 q[DP / 16];
   row_operands<DP>(q, p.q, row_at(p, j.q0, kvh, pos, ok ? r - pos * p.g : 0) - p.q, ok, p.D, lane);
   const int first = j.len - j.n + 1, seen = first + pos;   // keys that the first row sees, that this one sees
   const int padded = tiles_of(j.len, kFewKeys) * kFewKeys;
-  float* scores = nullptr;
-  if (p.scores) {
-    const int64_t at = int64_t(j.row0 >> 1) * kFewKeys * p.KV + int64_t(kvh) * R * padded;
-    if (at >= 0 && at + int64_t(R) * padded <= p.score_words) scores = p.scores + at + int64_t(r) * padded + 4 * (lane >> 5);
-  }
+  const int64_t scores_at = int64_t(j.row0 >> 1) * kFewKeys * p.KV + int64_t(kvh) * R * padded;
+  const bool keep = p.scores && scores_at >= 0 && scores_at + int64_t(R) * padded <= p.score_words;
+  float* scores = keep ? p.scores + scores_at + r * kFewKeys + 4 * (lane >> 5) : nullptr;
 
   Rows<DP> x;
   x.start();
@@ -299,7 +303,8 @@ __device__ __forceinline__ void few_rows(const Args& p, int group, uint8_t* lds)
     const bool more = t + W < j.t1;
     if (more) {
       reads_done();
-      load(t + W, stage ^ 1);
+      load(pages, t + W, stage ^ 1);
+      pages = pages_of(t + 2 * W);
       landed<3 * HALF>();
     } else {
       landed<HALF>();
@@ -313,13 +318,18 @@ __device__ __forceinline__ void few_rows(const Args& p, int group, uint8_t* lds)
         if (8 * (i >> 2) + (i & 3) >= left) s[i] = -INFINITY;
     }
     const float sub = x.new_maximum(s, p.c);
-    if (scores && ok)
+    if (keep && ok)
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        *reinterpret_cast<f32x4*>(scores + key0 + 8 * u) = f32x4{s[4 * u] * p.c, s[4 * u + 1] * p.c, s[4 * u + 2] * p.c, s[4 * u + 3] * p.c};
+        *reinterpret_cast<f32x4*>(scores + int64_t(t) * R * kFewKeys + 8 * u) = f32x4{s[4 * u] * p.c, s[4 * u + 1] * p.c, s[4 * u + 2] * p.c, s[4 * u + 3] * p.c};
     x.probabilities(s, p.c, sub);
-    if (more) landed<2 * HALF>();
-    else landed<0>();
+    if (keep) {   // (its four stores are behind the loads of V: waited for with them they took a quarter of the time)
+      if (more) landed<2 * HALF + 4>();
+      else landed<4>();
+    } else {
+      if (more) landed<2 * HALF>();
+      else landed<0>();
+    }
     x.add(s, V, 0, lane);
   }
   x.l += swap_halves(x.l);
@@ -634,7 +644,7 @@ __device__ __forceinline__ void many_rows(const Args& p, int group, uint8_t* lds
 // Four waves at every head size (of heads above 64 one workgroup a CU; of two waves each and two a CU, 256 positions of 8 sequences took
 // 8.6 us in place of 7.4, 64 sequences of up to 16000 the same)
 template <int DP>
-__global__ __launch_bounds__(64 * kWaves, 2) void paged_few(Args p) {
+__global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void paged_few(Args p) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds<DP, kWaves>()];
   few_rows<DP, kWaves>(p, blockIdx.x, lds);
 }
@@ -656,6 +666,166 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_both(Args p) {
     if (threadIdx.x < 64 * W) few_rows<DP, W>(p, before, lds);   // (whole waves: the others end)
   } else {
     many_rows<DP>(p, b - before, lds);
+  }
+}
+
+// ---- few rows of few short sequences ----
+// One workgroup of eight waves a sequence and K/V head, whose waves take up to four tiles each as in few_rows: no pieces to be joined by
+// another launch, and the weights at once, from scores that stay in registers.  Latency bound: the plan, the pages, the first tiles,
+// two joins in LDS.  (Keys straight into registers as operands, lanes by rows, took 11.5 us where this takes 6.9; 16 waves 11.)
+constexpr int kWholeWaves = 8, kWholeTiles = 4;   // tiles of a wave
+template <int DP>
+constexpr int whole_rows() { return DP <= 64 ? 32 : 16; }   // (by the LDS for their joining)
+
+template <int DP, bool WEIGHTED>
+__global__ __launch_bounds__(64 * kWholeWaves) void paged_whole(Args p, const Few* fews) {
+  constexpr int W = kWholeWaves, T = kWholeTiles, RS = whole_rows<DP>(), P = pitch<DP>(), TILE = kFewKeys * P, OROW = DP + 4, PROW = kFewKeys + 4;
+  constexpr int STAGES = DP <= 64 ? 2 : 1, MINE = 2 * STAGES * TILE;
+  static_assert(MINE >= RS * (OROW + PROW) * 4, "a wave's part of the output, and its probabilities");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[W * MINE];
+  __shared__ __attribute__((aligned(16))) float stats[2][RS][W + 4];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), kvh = blockIdx.x % p.KV;
+  const Few f = scalar_load(fews + blockIdx.x / p.KV);
+  const int R = f.n * p.g;
+  if (!sound(p, f.q0, f.n, f.len, f.seq) || R > RS || f.len > W * T * kFewKeys) return;
+  const int tiles = R ? tiles_of(f.len, kFewKeys) : 0, r = lane & 31;
+  uint8_t* mine = lds + wv * MINE;
+  const int64_t row = int64_t(f.seq) * p.KV + kvh;
+  float old[T] = {};
+  if constexpr (WEIGHTED)
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+      const int key = kFewKeys * (wv + W * i) + r;
+      if (key < f.len - f.n && key < p.weights_width) old[i] = p.weights[row * p.weights_width + key];
+    }
+  Rows<DP> x;
+  x.start();
+  f32x16 s[T];
+  const int pos = div_g(p, min(r, max(R - 1, 0)));
+  const bool ok = r < R;
+  if (wv < tiles) {
+    const uint16_t *kb = p.k.p + kvh * p.k.head, *vb = p.v.p + kvh * p.v.head;
+    const int32_t* table = p.tables + int64_t(f.seq) * p.width;
+    const uint32_t to = lds_address(mine);
+    PagedTile<DP, kFewKeys, 1> kt, vt;
+    kt.init(p.k.row, p.D, lane, 0);
+    vt.init(p.v.row, p.D, lane, 0);
+    constexpr int HALF = decltype(kt)::N;
+    int2 pages[T];
+#pragma unroll
+    for (int i = 0; i < T; ++i) pages[i] = scalar_load(reinterpret_cast<const int2*>(table) + min(wv + W * i, tiles - 1));
+    auto there = [&](int i) { return i < T && wv + W * i < tiles; };
+    auto load = [&](const PagedTile<DP, kFewKeys, 1>& tile, const uint16_t* head, int64_t stride, int i, int which) {
+      tile.load(to + (i % STAGES * 2 + which) * TILE, f.len - kFewKeys * (wv + W * i), 0, head, stride, p.n_pages,
+                [&](int h) { return pick(h, pages[i].x, pages[i].y, 0, 0); });
+    };
+    auto load_k = [&](int i) { load(kt, kb, p.k.row, i, 0); };
+    auto load_v = [&](int i) { load(vt, vb, p.v.row, i, 1); };
+    load_k(0);
+    load_v(0);
+    bf16x8 q[DP / 16];
+    row_operands<DP>(q, p.q, row_at(p, f.q0, kvh, pos, ok ? r - pos * p.g : 0) - p.q, ok, p.D, lane);
+    if (STAGES == 2 && there(1)) {
+      load_k(1);
+      load_v(1);
+    }
+    const int first = f.len - f.n + 1, seen = first + pos;
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+      if (!there(i)) break;
+      const uint8_t *K = mine + i % STAGES * 2 * TILE, *V = K + TILE;
+      const bool more = there(i + 1);
+      if (STAGES == 2 && more) landed<3 * HALF>();
+      else landed<HALF>();
+      f32x16 now = scores_of<DP>(K, 0, q, lane);
+      if (STAGES == 1 && more) {
+        reads_done();
+        load_k(i + 1);
+      }
+      const int key0 = (wv + W * i) * kFewKeys;
+      if (key0 + kFewKeys > first) {
+        const int left = seen - key0 - 4 * (lane >> 5);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (8 * (e >> 2) + (e & 3) >= left) now[e] = -INFINITY;
+      }
+      const float sub = x.new_maximum(now, p.c);
+      if constexpr (WEIGHTED) s[i] = now;
+      x.probabilities(now, p.c, sub);
+      if (more) landed<STAGES * HALF>();
+      else landed<0>();
+      x.add(now, V, 0, lane);
+      if (there(i + STAGES)) {
+        reads_done();
+        if (STAGES == 2) load_k(i + 2);
+        load_v(i + STAGES);
+      }
+    }
+    x.l += swap_halves(x.l);
+  }
+  if (lane < RS) {
+    stats[0][r][wv] = x.m;
+    stats[1][r][wv] = x.l;
+  }
+  __syncthreads();
+  // the row's statistics, from all waves'; what this wave's part counts
+  float m = -INFINITY, l = 0;
+  {
+    const int of = lane % RS;
+    float ms[W], ls[W];
+#pragma unroll
+    for (int w = 0; w < W; w += 4) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(&stats[0][of][w]), b = *reinterpret_cast<const f32x4*>(&stats[1][of][w]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ms[w + i] = a[i], ls[w + i] = b[i];
+    }
+#pragma unroll
+    for (int w = 0; w < W; ++w) m = fmaxf(m, ms[w]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) l = fmaf(ls[w] == 0 ? 0.0f : exp2_hw(ms[w] - m), ls[w], l);   // (a NaN sum stays one)
+  }
+  const float by = (x.l == 0 ? 0.0f : exp2_hw(x.m - m)) * (l == 0 ? 0.0f : 1.0f / l);
+  float* part = reinterpret_cast<float*>(mine);
+  if (ok)
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<f32x4*>(part + r * OROW + 32 * d + 8 * u + 4 * (lane >> 5)) =
+            f32x4{x.o[d][4 * u] * by, x.o[d][4 * u + 1] * by, x.o[d][4 * u + 2] * by, x.o[d][4 * u + 3] * by};
+  __syncthreads();
+  const int pieces = p.D / 4;
+  for (int i = tid; i < R * pieces; i += 64 * W) {
+    const int of = i / pieces, c = i - of * pieces;
+    f32x4 o = {};
+#pragma unroll
+    for (int w = 0; w < W; ++w) o += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * MINE) + of * OROW + 4 * c);
+    const int at = div_g(p, of);
+    *reinterpret_cast<u32x2*>(p.out + (int64_t(f.q0 + at) * p.H + kvh * p.g + of - at * p.g) * p.D + 4 * c) = u32x2{pack2(o[0], o[1]), pack2(o[2], o[3])};
+  }
+  if constexpr (WEIGHTED) {
+    const float lse = l == 0 ? INFINITY : m + __log2f(l);
+    float* here = part + RS * OROW;
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+      const int t = wv + W * i, key = kFewKeys * t + r;
+      float sum = 0;
+      if (t < tiles) {
+        if (ok)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            f32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = exp2_hw(fmaf(s[i][4 * u + e], p.c, -lse));
+            *reinterpret_cast<f32x4*>(here + r * PROW + 8 * u + 4 * (lane >> 5)) = w;
+          }
+        reads_done();
+#pragma unroll 4
+        for (int of = 0; of < R; ++of) sum += here[of * PROW + r];
+        reads_done();
+      }
+      if (lane < 32 && key < p.longest) p.weights_out[row * p.longest + key] = key < f.len ? old[i] + sum : 0.0f;
+    }
   }
 }
 
@@ -780,7 +950,7 @@ __global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* t
       f32x4 sum = {};
 #pragma unroll 4
       for (int r = 0; r < R; ++r) {
-        const f32x4 s = *reinterpret_cast<const f32x4*>(p.scores + base + int64_t(r) * padded + key);
+        const f32x4 s = *reinterpret_cast<const f32x4*>(p.scores + base + (int64_t(key / kFewKeys) * R + r) * kFewKeys + key % kFewKeys);
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] += exp2_hw(s[i] - row_lse[r]);
       }
@@ -1214,12 +1384,19 @@ constexpr int kFewLeast = 4, kManyLeast = 6;
 // rows of heads of 64).  Longer ones in pieces of 4, 6 and 8 tiles at least: 24.9, 24.6 and 26.7 (a step of tokens and chunks, up to
 // 46 tiles of heads of 96).
 constexpr int kManyWhole = 8;
-// Few rows: pieces of four tiles, one a wave, as long as that is one round of the CUs; then longer ones, up to 16; and from 2048 pieces
-// on as many as make 2048 (64 sequences of up to 16000 positions: 425 us, with 1024 486, with 4096 447).
+// Few rows: pieces of four tiles, one a wave, as long as that is one round of the CUs; then longer ones, up to 16, in as few whole rounds
+// as hold them (8 sequences of up to 2000, 8 K/V heads of 128: by 272 workgroups 18.9 us, by 256 14.0); and from eight rounds on as
+// many as make 2048 (64 sequences of up to 16000 positions: 425 us, with 1024 486, with 4096 447).
 constexpr int kFewRound = 256, kFewEnough = 16;
 // Without weights a sequence of up to this many tiles stays whole, as the join takes another launch: 512 positions of 8 sequences,
 // 4 K/V heads of 64: 6.7 us in place of 8.8, heads of 128 9.9 and 10.0; 1024: 9.7 and 8.9, 15.1 and 10.9.
 constexpr int kFewWhole = 16;
+
+// Few rows only, and not more workgroups than CUs: paged_whole, of up to 512 positions always, up to 1024 where the pieces would share
+// CUs or where there are no weights and heads are small.  In us, this and by pieces: 8 sequences of up to 512, 4 K/V heads of 64, weights
+// 6.9 and 9.4; 32 of up to 1000, 8 heads of 64 9.6 and 15.4, with weights 11.1 and 16.4; heads of 128 16.0 and 25.8; but 8 of up to 1000, 4
+// heads of 64, with weights 10.2 and 9.1; 64 of up to 500, 8 heads (512 workgroups) 12.9 and 8.3.
+constexpr int kWholeGroups = 256, kWholeShort = 512, kWholeSplit = 64;
 
 struct Pieces {
   int64_t each, whole;
@@ -1227,9 +1404,15 @@ struct Pieces {
   int of(int64_t tiles) const { return 2 * tiles <= 3 * each || tiles <= whole ? 1 : int(cdiv(tiles, each)); }
 };
 Pieces many_pieces(int64_t tiles, int n_kv) { return {std::max<int64_t>(kManyLeast, cdiv(tiles * n_kv, kManyGroups)), kManyWhole}; }
-Pieces few_pieces(int64_t tiles, int n_kv, bool weighted) {
-  const int64_t round = std::min<int64_t>(std::max<int64_t>(kFewLeast, cdiv(tiles * n_kv, kFewRound)), kFewEnough);
-  return {std::max(round, cdiv(tiles * n_kv, kFewGroups)), weighted ? 0 : kFewWhole};
+Pieces few_pieces(const std::vector<int64_t>& lists, int64_t tiles, int n_kv, bool weighted) {
+  const int64_t whole = weighted ? 0 : kFewWhole;
+  for (int64_t groups = kFewRound; groups <= kFewGroups && int64_t(lists.size()) * n_kv <= kFewGroups; groups += kFewRound)
+    for (Pieces x{std::max<int64_t>(kFewLeast, cdiv(tiles * n_kv, groups)), whole}; x.each <= kFewEnough; ++x.each) {
+      int64_t n = 0;
+      for (const int64_t t : lists) n += x.of(t);
+      if (n * n_kv <= groups) return x;
+    }
+  return {std::max<int64_t>(kFewEnough, cdiv(tiles * n_kv, kFewGroups)), whole};
 }
 
 struct Writer {
@@ -1251,6 +1434,7 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
   int most = 0;   // (lengths up to kLongest: the next tile's first position is a number too)
   int64_t q_end = 0, q_count = 0;
   std::vector<int> few, many;   // sequences
+  std::vector<int64_t> few_lists;
   int64_t few_tiles = 0, few_rows = 0, many_tiles = 0, row_tiles = 0, appends = 0, scores = 0;
   auto seen = [&](const int32_t* s, int64_t row) { return s[2] - s[1] + 1 + row / g; };   // positions that the row sees
   for (int b = 0; b < n_seqs; ++b) {
@@ -1264,7 +1448,10 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
     q_count += s[1];
     if (rows <= kFewRows) {
       few.push_back(b);
-      if (rows) few_tiles += cdiv(s[2], kFewKeys);
+      if (rows) {
+        few_lists.push_back(cdiv(s[2], kFewKeys));
+        few_tiles += few_lists.back();
+      }
       few_rows = std::max(few_rows, rows);
       scores += rows * cdiv(longest ? longest : s[2], kFewKeys);
     } else {
@@ -1275,7 +1462,7 @@ int64_t plan(int n_seqs, const int32_t* seqs, const int32_t* tables, int table_w
     else if (s[1]) appends += cdiv(s[2], kPage) - (s[2] - s[1]) / kPage;
   }
   if (longest > std::min<int64_t>(int64_t(table_width) * kPage, kLongest)) return MSD_E_CONFIG;
-  const Pieces fp[2] = {few_pieces(few_tiles, KV, false), few_pieces(few_tiles, KV, true)}, mp = many_pieces(many_tiles, KV);
+  const Pieces fp[2] = {few_pieces(few_lists, few_tiles, KV, false), few_pieces(few_lists, few_tiles, KV, true)}, mp = many_pieces(many_tiles, KV);
   int64_t n_few[2] = {}, n_many = 0, few_active = 0;
   bool few_parts[2] = {}, many_parts = false;
   for (int b : few) {
@@ -1580,6 +1767,18 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
   p.weights = weights;
   p.weights_width = weights_width;
   p.weights_out = weights_out;
+  const int64_t groups = h[N_FEWS] * KV;
+  bool whole = !h[N_MANYS] && groups && groups <= kWholeGroups && longest <= kWholeWaves * kWholeTiles * kFewKeys;
+  if (whole)
+    with_head(a->d_head, [&](auto dp) {
+      constexpr int DP = decltype(dp)::value;
+      whole = h[FEW_ROWS] <= whole_rows<DP>() && (longest <= kWholeShort || groups >= kWholeSplit || (DP <= 64 && !weighted));
+      if (!whole) return;
+      const Few* fews = reinterpret_cast<const Few*>(a->plan + h[AT_FEWS + weighted]);
+      if (weighted) hipLaunchKernelGGL((paged_whole<DP, true>), dim3(unsigned(groups)), dim3(64 * kWholeWaves), 0, s, p, fews);
+      else hipLaunchKernelGGL((paged_whole<DP, false>), dim3(unsigned(groups)), dim3(64 * kWholeWaves), 0, s, p, fews);
+    });
+  if (whole) return launched();
   const Job* manys = reinterpret_cast<const Job*>(a->plan + h[AT_MANYS]);
   with_head(a->d_head, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
