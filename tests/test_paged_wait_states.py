@@ -27,7 +27,9 @@ def test_a_tile_of_values_is_waited_for_past_the_scores_stores(assembly, DP, loa
     """A wave that stores scores waits for all but the next tile's loads and four stores: four there must be, before the wait."""
     body = re.search(rf"^_ZN3msp9paged_fewILi{DP}E.*?:\n(.*?)s_endpgm\n\s*\.section", assembly, re.S | re.M).group(1).split("\n")
     waits = [i for i, x in enumerate(body) if re.search(rf"s_waitcnt vmcnt\({2 * loads + 4}\)", x)]
-    assert waits
+    stores = []
     for i in waits:
         last = max(k for k in range(i) if re.search(r"buffer_load_dwordx4 .* lds", body[k]))
-        assert sum("global_store_dwordx4" in x for x in body[last:i]) == 4
+        stores.append(sum("global_store_dwordx4" in x for x in body[last:i]))
+    # (3 * 4 is 2 * 4 + 4: the wait for the keys, with no stores behind the loads yet)
+    assert stores == ([0, 4] if loads == 4 else [4])
