@@ -17,6 +17,8 @@
 // Measured (us, kernels under a tracer):
 //   paged_few       memory.  64 tokens over up to 16000 positions, 8 K/V heads of 128: 418, 6.4 TB/s of reads (24 over up to 8000, 16 heads, with
 //                   weights: 187, 5.8 TB/s); 4 over up to 2000, 4 heads of 64: 4.9, a chain of plan, pages, rows
+//   paged_whole     latency, then a CU's own rate of loads.  8 tokens over up to 512 positions, 4 K/V heads of 64, weights: 6.9 a pass; 32 over up
+//                   to 1000, 8 heads of 128: 16
 //   paged_many      the matrix cores' power.  2048 rows at 16384, 32 / 8 heads of 128: 477-526 by card, 980-1080 TFLOP/s of the products under
 //                   the mask (a library's 8192^3 product: 1215-1242); 8 x 128 over up to 512, 16 / 4 heads of 64: 12, one round, a chain of tiles
 //   paged_finish    latency: 4.4-8
