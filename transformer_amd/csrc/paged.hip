@@ -401,7 +401,7 @@ struct HalfTile {
   static constexpr int kLanes = P == 128 ? 4 : kPage;
   static constexpr int key_of(int i) { return P == 128 ? kPage * (i / 4) + i % 4 : kPage * 2 * (i / 4 % 2) + 4 * (i / 8) + i % 4; }
 };
-// Rows `rows` (0 .. 16) of a page's positions of a head, as a buffer
+// The rows (0 .. 16) of a page's positions of a head that exist, as a buffer
 struct PageRows {
   const uint16_t* p;
   uint32_t bytes;
@@ -447,8 +447,10 @@ __device__ __forceinline__ void many_rows(const Args& p, int group, uint8_t* lds
   auto rows_in = [&](int t, int page) {
     return t < j.t0 || t >= j.t1 || uint32_t(page) >= uint32_t(p.n_pages) ? 0 : min(max(j.len - t * kKeys - kPage * wv, 0), kPage);
   };
+  // (to the last row's end: rows may be nearer to each other than they are long.  What a row behind the last then reads lies within those
+  // that are there, its scores are masked)
   auto page_rows = [&](const uint16_t* head, uint32_t row, int page, int n) {
-    return PageRows{head + (uint64_t(uint32_t(n ? page : 0)) * (kPage * row) >> 1), n * row};
+    return PageRows{head + (uint64_t(uint32_t(n ? page : 0)) * (kPage * row) >> 1), n * row + min(n, 1) * (2 * p.D - row)};
   };
   auto k_page = [&](int t, int page) { return page_rows(kb, k_row, page, rows_in(t, page)); };
   auto v_page = [&](int t, int page) { return page_rows(vb, v_row, page, rows_in(t, page)); };
