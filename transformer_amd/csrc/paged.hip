@@ -263,7 +263,7 @@ __device__ __forceinline__ void few_rows(const Args& p, int group, uint8_t* lds)
   const int kvh = group % p.KV;
   const Job j = scalar_load(p.few + group / p.KV);
   const int R = j.n * p.g;
-  if (!sound(p, j.q0, j.n, j.len, j.seq) || R > kFewRows || j.t0 < 0 || j.t1 > tiles_of(j.len, kFewKeys) || j.slot < 0 || j.slot >= p.n_few)
+  if (!sound(p, j.q0, j.n, j.len, j.seq) || R > kFewRows || j.t0 < 0 || j.t1 < j.t0 || j.t1 > tiles_of(j.len, kFewKeys) || j.slot < 0 || j.slot >= p.n_few)
     return;
   uint8_t* mine = lds + wv * 4 * TILE;
   const uint32_t to = lds_address(mine);
@@ -899,7 +899,7 @@ __global__ __launch_bounds__(kFinish) void paged_finish(Args p, const RowTile* t
     const int kvh = id % p.KV, sub = id / p.KV % kSubs;
     const RowTile t = scalar_load(tiles + id / p.KV / kSubs);
     const int row0 = t.row0 + kJoinRows * sub, rows = min(t.n * p.g - row0, kJoinRows);
-    if (!sound(p, t.q0, t.n, t.len, t.seq) || t.row0 < 0 || rows <= 0 || t.parts < 2 || t.slot < 0 || t.slot > p.n_many - t.parts) return;
+    if (!sound(p, t.q0, t.n, t.len, t.seq) || t.row0 < 0 || t.row0 >= t.n * p.g || rows <= 0 || t.parts < 2 || t.slot < 0 || t.slot > p.n_many - t.parts) return;
     const int64_t at = (int64_t(t.slot) * p.KV + kvh) * kManyRows + kJoinRows * sub;
     join(p, lds, p.many_part + at * p.D, p.many_lse + at, int64_t(p.KV) * kManyRows, t.parts, rows, t.q0, t.n, row0, kvh, p.lse);
     return;
@@ -984,7 +984,7 @@ __global__ __launch_bounds__(64 * kWaves * kHalves) void paged_weights(Args p, c
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wv = wave % kWaves, half = wave / kWaves;
   const int kvh = blockIdx.x % p.KV, kb = blockIdx.x / p.KV / n_seqs;
   const Job j = scalar_load(seqs + blockIdx.x / p.KV % n_seqs);
-  if (!sound(p, j.q0, j.n, j.len, j.seq)) return;
+  if (!sound(p, j.q0, j.n, j.len, j.seq) || !j.n) return;   // (without new tokens there is no way through the tiles below)
   const int k0 = 128 * kb + 32 * wv, key = k0 + (lane & 31);
   float sum = 0;
   if (128 * kb < j.len) {
