@@ -1,4 +1,5 @@
-"""Attention over pages whose positions share memory.  Tolerances as in test_paged_attention_gpu.py."""
+"""Attention in layouts outside the ordinary: pages whose positions share memory, sequences without new tokens that start anywhere.
+Tolerances as in test_paged_attention_gpu.py."""
 import pytest
 import torch
 
@@ -40,3 +41,21 @@ def test_one_row_for_all_positions():
     want = row[:, 0].repeat_interleave(2, 0).expand(201, -1, -1)
     # (sums of up to 219 probabilities, each rounded to bf16 as an operand, and the output)
     assert ((out.double() - want.double()).abs() <= (2.0 ** -7 + 2.0 ** -12) * want.double().abs()).all()
+
+
+@pytest.mark.parametrize("q_lens,lengths", [([1, 0], [30, 40]), ([0, 2, 0], [500, 300, 16]), ([1, 0], [3000, 2000]), ([50, 0], [300, 40]), ([0, 0], [30, 700]),
+                                            ([0, 0, 1, 70], [5, 900, 60, 700])])
+@pytest.mark.parametrize("longest", [None, 3100])
+def test_weights_of_a_sequence_that_starts_behind_the_rows(q_lens, lengths, longest):
+    """A sequence without new tokens keeps its weights, wherever its start lies: in one launch, in pieces, beside chunks."""
+    rows, H, KV = sum(q_lens), 4, 2
+    tables, n = tables_of(lengths, 1)
+    starts = [sum(q_lens[:s]) if q else rows + 7 + 2 ** 30 * (s % 2) for s, q in enumerate(q_lens)]
+    q, k, v = rand((rows, H, 64), 2, 1.5), rand((KV, 16 * n, 64), 3), rand((KV, 16 * n, 64), 4)
+    old = 1 + torch.rand((len(q_lens), KV, max(lengths)), generator=torch.Generator().manual_seed(5)).cuda()
+    sequences = PagedSequences(q_lens, lengths, tables, H, KV, q_starts=starts, longest=longest)
+    torch.full((4096, 1024), float("nan"), device="cuda")   # (freed: what a call leaves unwritten is not a number)
+    ref, tol = reference(q, k, v, q_lens, lengths, tables, starts, 0.125, old, sequences.longest)
+    out, weights = paged_attention(q, k, v, sequences, weights=old)
+    near(out, ref[0], tol[0], "out")
+    near(weights, ref[1], tol[1], "weights")

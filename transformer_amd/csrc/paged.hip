@@ -118,9 +118,10 @@ __device__ __forceinline__ int pick(int i, int a, int b, int c, int d) {   // (o
   return i & 2 ? high : low;
 }
 
-// The host has checked its own numbers; device words that have been overwritten since must not lead out of anything.
+// The host has checked its own numbers; device words that have been overwritten since must not lead out of anything.  (A sequence without
+// new tokens has no rows and may start anywhere, behind the last row too.)
 __device__ __forceinline__ bool sound(const Args& p, int q0, int n, int len, int seq) {
-  return q0 >= 0 && n >= 0 && q0 <= p.q_rows - n && len >= n && len <= p.longest && seq >= 0 && seq < p.n_seqs;
+  return n >= 0 && (n == 0 || (q0 >= 0 && q0 <= p.q_rows - n)) && len >= n && len <= p.longest && seq >= 0 && seq < p.n_seqs;
 }
 
 __device__ __forceinline__ int tiles_of(int len, int keys) { return len / keys + (len % keys != 0); }
