@@ -77,7 +77,10 @@ int64_t msd_paged_attn_workspace_bytes(const msd_paged* a, int32_t weighted);
  * weights_out: NULL, or f32 (n_seqs, n_kv_heads, longest): per position the sum, over the sequence's new tokens and the heads of
  * the group, of the probabilities that it has in the softmax, plus what `weights` (n_seqs, n_kv_heads, weights_width; NULL
  * with a width of 0) has for it, if it is not a new token's and lies inside weights_width; zeros behind the length.  It may be
- * `weights` itself where weights_width is longest. */
+ * `weights` itself where weights_width is longest.
+ * Limits of a call with weights: the sequences of more than 32 rows of a group, times the K/V heads, times longest / 128 rounded up, below 2^22;
+ * the others times the K/V heads times longest / 1024 rounded up, and with them what joins pieces, below 2^24.  Nothing has been launched
+ * where a call is refused. */
 int32_t msd_paged_attn(const msd_paged* a, const void* q, const void* k, const void* v, void* out, const float* weights,
                        int32_t weights_width, float* weights_out, void* workspace, void* stream);
 

@@ -1725,13 +1725,15 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
   if (weights_width < 0) return MSD_E_CONFIG;
   if (weighted && weights_width && (!weights || reinterpret_cast<uintptr_t>(weights) % 4)) return MSD_E_ARG;
   if (reinterpret_cast<uintptr_t>(weights_out) % 4) return MSD_E_ARG;
-  const int64_t KV = h[MSD_PLAN_KV_HEADS], longest = h[MSD_PLAN_LONGEST], most = (int64_t(1) << 32) / 256 - 1;
+  const int64_t KV = h[MSD_PLAN_KV_HEADS], longest = h[MSD_PLAN_LONGEST];
   const int64_t key_blocks = cdiv(longest, 128), weight_blocks = weighted ? cdiv(longest, kWeightKeys) : 0;
   const int n_tiles = h[MANY_PARTS] ? h[N_TILES] : 0, n_fews = h[FEW_PARTS + weighted] || weighted ? h[N_FEWS] : 0;
   // one row of few a workgroup as long as there are few of them (16 parts of 64 rows: 4.0 us, with four rows 5.6; 2048 rows: 6.7 and 5.0)
   const int join_rows = int64_t(n_fews) * KV * h[FEW_ROWS] <= 1024 ? 1 : kJoinRows, few_joins = h[FEW_PARTS + weighted] ? int(cdiv(h[FEW_ROWS], join_rows)) : 0;
   const int64_t finish = int64_t(n_tiles) * KV * (kManyRows / kJoinRows) + int64_t(n_fews) * KV * (few_joins + weight_blocks);
-  if (finish > most || key_blocks * KV * h[N_MANYS] > most) return MSD_E_CONFIG;
+  // (a launch counts its threads in 32 bits)
+  constexpr int64_t threads = int64_t(1) << 32;
+  if (finish >= threads / kFinish || (weighted && key_blocks * KV * h[N_MANYS] >= threads / (64 * kWaves * kHalves))) return MSD_E_CONFIG;
   if (h[MSD_PLAN_Q_COUNT] && (bad(q) || bad(k) || bad(v) || bad(out))) return MSD_E_ARG;
   const Space at = space(*a, weighted);
   if (at.end && bad(workspace)) return MSD_E_ARG;
