@@ -22,6 +22,7 @@
 
 #include "../../include/mslayers.h"
 #include "../../include/mspaged.h"
+#include "overlap.h"
 
 namespace {
 
@@ -494,9 +495,17 @@ void no_gradient(const char* what, const X&... x) {
     throw std::invalid_argument(std::string(what) + " has no gradient: call it under torch.no_grad(), or hand over detached tensors");
 }
 
+// k's and v's axes with the strides of both, and how far behind k v starts
+bool share_memory(const Tensor& k, const Tensor& v) {
+  std::vector<msd_overlap::Axis> axes;
+  const int64_t n = k.dim();
+  for (int64_t i = 0; i + 1 < n; ++i) axes.push_back({k.size(i), k.stride(i), v.stride(i)});
+  return msd_overlap::share(std::move(axes), k.size(n - 1), static_cast<const uint16_t*>(v.data_ptr()) - static_cast<const uint16_t*>(k.data_ptr()));
+}
+
 // (first: an inference tensor outside inference mode raises here)
 void written(const Tensor& k, const Tensor& v) {
-  need(k.numel() == 0 || k.data_ptr() != v.data_ptr(), "k_pages and v_pages are the same memory");
+  need(!share_memory(k, v), "k_pages and v_pages are the same memory, or share some of it");
   for (const Tensor* x : {&k, &v}) x->unsafeGetTensorImpl()->bump_version();
 }
 
