@@ -64,7 +64,8 @@ typedef struct msd_paged {
   const int32_t *plan, *plan_host;
 } msd_paged;
 
-/* k_new, v_new (q_rows, n_kv_heads, d_head by (row, head) strides) to the positions of their rows.  No two places of k and v are one. */
+/* k_new, v_new (q_rows, n_kv_heads, d_head by (row, head) strides) to the positions of their rows.  No two places of k and v are one, and
+ * none that is written is one of the new rows'. */
 int32_t msd_paged_append(const msd_paged* a, const void* k_new, const int64_t* k_new_stride, const void* v_new,
                          const int64_t* v_new_stride, void* k, void* v, void* stream);
 

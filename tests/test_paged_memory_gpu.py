@@ -1,4 +1,4 @@
-"""Pages of keys and values that share memory: refused where they are written."""
+"""Pages and rows that share memory: what is refused, and what is as if the rows had been read before any page is written."""
 import pytest
 import torch
 
@@ -72,3 +72,21 @@ def test_layers_of_keys_and_values_in_one_memory():
     with pytest.raises(ValueError, match="same memory"):
         paged_evict(flat[::2], flat[2:6:1], torch.rand(4, 2, 2, 40).cuda(), e)   # (other strides, which may meet)
     paged_evict(pool[:, 0], pool[:, 1], torch.rand(4, 2, 2, 40).cuda(), e)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_new_rows_that_lie_in_the_pages(D):
+    """A page's rows as another sequence's, and rows that each move on by one position or one page."""
+    n = 40
+    for count, first, length in ((16, 0, 32), (13, 3, 20), (200, 0, 217), (600, 0, 616), (600, 5, 606)):
+        k_pages, v_pages = rand((2, 16 * n, D), 1), rand((2, 16 * n, D), 2)
+        k, v = (x[:, first:first + count].transpose(0, 1) for x in (k_pages, v_pages))
+        s = PagedSequences([count], [length], [range(-(-length // 16))], 4, 2)
+        want = [appended(x.clone(), pages, [count], [length], [range(n)], [0]) for x, pages in ((k, k_pages), (v, v_pages))]
+        paged_append(k, v, k_pages, v_pages, s)
+        assert same(k_pages, want[0]) and same(v_pages, want[1]), (count, first, length)
+        k_pages, v_pages = rand((2, 16 * n, D), 1), rand((2, 16 * n, D), 2)
+        k, v = (x[:, first:first + count].transpose(0, 1) for x in (v_pages, k_pages))   # each from the other's
+        want = [appended(x.clone(), pages, [count], [length], [range(n)], [0]) for x, pages in ((k, k_pages), (v, v_pages))]
+        paged_append(k, v, k_pages, v_pages, s)
+        assert same(k_pages, want[0]) and same(v_pages, want[1]), (count, first, length)

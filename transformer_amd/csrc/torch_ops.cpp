@@ -509,6 +509,22 @@ void written(const Tensor& k, const Tensor& v) {
   for (const Tensor* x : {&k, &v}) x->unsafeGetTensorImpl()->bump_version();
 }
 
+// x, or a copy of it where it lies among pages that are about to be written: the rows are those from before the call
+Tensor apart(const Tensor& x, const Tensor& k_pages, const Tensor& v_pages) {
+  auto ends = [](const Tensor& t) {
+    uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr()), end = at;
+    if (t.numel()) end += t.element_size();
+    for (int64_t i = 0; t.numel() && i < t.dim(); ++i) end += (t.size(i) - 1) * t.stride(i) * t.element_size();
+    return std::make_pair(at, end);
+  };
+  const auto mine = ends(x);
+  for (const Tensor* pages : {&k_pages, &v_pages}) {
+    const auto theirs = ends(*pages);
+    if (mine.first < theirs.second && theirs.first < mine.second) return x.clone(at::MemoryFormat::Contiguous);
+  }
+  return x;
+}
+
 void paged_append(const Tensor& k_new, const Tensor& v_new, const Tensor& k_pages, const Tensor& v_pages, const Paged& steps) {
   only_run("paged_append", k_new, v_new, k_pages, v_pages);
   no_gradient("paged_append", k_new, v_new, k_pages, v_pages);
@@ -516,7 +532,8 @@ void paged_append(const Tensor& k_new, const Tensor& v_new, const Tensor& k_page
   msd_paged a = paged_call(k_pages, v_pages, p, false, true);
   const int64_t heads = p.word(MSD_PLAN_KV_HEADS);
   Place on(k_pages);
-  const Tensor k = paged_rows("k", k_new, heads, a, p, k_pages.device()), v = paged_rows("v", v_new, heads, a, p, k_pages.device());
+  const Tensor k = apart(paged_rows("k", k_new, heads, a, p, k_pages.device()), k_pages, v_pages);
+  const Tensor v = apart(paged_rows("v", v_new, heads, a, p, k_pages.device()), k_pages, v_pages);
   need(k.size(0) == v.size(0), "k of ", k.size(0), " rows, v of ", v.size(0));
   need(!p.word(MSD_PLAN_SHARED), "a page that takes new rows is in use elsewhere too");
   a.q_rows = k.size(0);

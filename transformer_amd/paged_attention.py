@@ -161,7 +161,8 @@ class PagedEviction:
 def paged_append(k, v, k_pages, v_pages, sequences):
     """Writes the new tokens' keys and values (rows, n_kv_heads, d_head; bf16, any strides) to their positions of the pages
     (n_kv_heads, positions, d_head; on 16-byte boundaries, strides that are multiples of 8; no two places of the keys and the values in
-    one memory).  Pages that take new rows must be in use by one sequence only."""
+    one memory).  Pages that take new rows must be in use by one sequence only.  k and v may lie in the pages themselves: they are
+    read before any page is written."""
     _lib.ops().paged_append(k, v, k_pages, v_pages, sequences.native)
 
 
