@@ -254,8 +254,8 @@ __device__ __forceinline__ f32x16 scores_of(const uint8_t* K, int row0, const bf
 template <int DP, int W>
 constexpr int few_lds() { return W * (4 * kFewKeys * pitch<DP>() + 256); }   // and two statistics of 32 rows a wave
 
-// Workgroup `group` of few rows, W waves
-template <int DP, int W>
+// Workgroup `group` of few rows by W of its NW waves; the others take no tiles and meet them at the barrier
+template <int DP, int W, int NW = W>
 __device__ __forceinline__ void few_rows(const Args& p, int group, uint8_t* lds) {
   constexpr int P = pitch<DP>(), TILE = kFewKeys * P, OROW = DP + 4;
   float(*stats)[2][32] = reinterpret_cast<float(*)[2][32]>(lds + W * 4 * TILE);
@@ -266,7 +266,8 @@ __device__ __forceinline__ void few_rows(const Args& p, int group, uint8_t* lds)
   const int R = j.n * p.g;
   if (!sound(p, j.q0, j.n, j.len, j.seq) || R > kFewRows || j.t0 < 0 || j.t1 < j.t0 || j.t1 > tiles_of(j.len, kFewKeys) || j.slot < 0 || j.slot >= p.n_few)
     return;
-  uint8_t* mine = lds + wv * 4 * TILE;
+  const bool works = W == NW || wv < W;
+  uint8_t* mine = lds + (works ? wv : 0) * 4 * TILE;
   const uint32_t to = lds_address(mine);
   const uint16_t *kb = p.k.p + kvh * p.k.head, *vb = p.v.p + kvh * p.v.head;
   const int32_t* table = p.tables + int64_t(j.seq) * p.width;
@@ -281,7 +282,7 @@ __device__ __forceinline__ void few_rows(const Args& p, int group, uint8_t* lds)
     kt.load(to + stage * 2 * TILE, left, 0, kb, p.k.row, p.n_pages, page);
     vt.load(to + stage * 2 * TILE + TILE, left, 0, vb, p.v.row, p.n_pages, page);
   };
-  int t = j.t0 + wv;
+  int t = works ? j.t0 + wv : j.t1;
   int2 pages{};   // of the next tile: asked for a tile ahead, as nothing can be fetched before they are there
   if (t < j.t1) {
     const int2 now = pages_of(t);
@@ -289,7 +290,7 @@ __device__ __forceinline__ void few_rows(const Args& p, int group, uint8_t* lds)
     load(now, t, 0);
   }
   const int r = lane & 31, pos = div_g(p, min(r, R - 1));
-  const bool ok = r < R;
+  const bool ok = works && r < R;
   bf16x8 q[DP / 16];
   row_operands<DP>(q, p.q, row_at(p, j.q0, kvh, pos, ok ? r - pos * p.g : 0) - p.q, ok, p.D, lane);
   const int first = j.len - j.n + 1, seen = first + pos;   // keys that the first row sees, that this one sees
@@ -337,24 +338,26 @@ __device__ __forceinline__ void few_rows(const Args& p, int group, uint8_t* lds)
   }
   x.l += swap_halves(x.l);
   // the waves' parts, joined
-  reads_done();
-  float* part = reinterpret_cast<float*>(mine);
+  if (works) {
+    reads_done();
+    float* part = reinterpret_cast<float*>(mine);
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      *reinterpret_cast<f32x4*>(part + r * OROW + 32 * d + 8 * u + 4 * (lane >> 5)) =
-          f32x4{x.o[d][4 * u], x.o[d][4 * u + 1], x.o[d][4 * u + 2], x.o[d][4 * u + 3]};
-  if (lane < 32) {
-    stats[wv][0][r] = x.m;
-    stats[wv][1][r] = x.l;
+      for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<f32x4*>(part + r * OROW + 32 * d + 8 * u + 4 * (lane >> 5)) =
+            f32x4{x.o[d][4 * u], x.o[d][4 * u + 1], x.o[d][4 * u + 2], x.o[d][4 * u + 3]};
+    if (lane < 32) {
+      stats[wv][0][r] = x.m;
+      stats[wv][1][r] = x.l;
+    }
   }
   __syncthreads();
   const bool only = j.row0 & 1;
   if (!only && !p.few_part) return;   // (overwritten device words)
   const int64_t slot = (int64_t(j.slot) * p.KV + kvh) * kFewRows;
   const int pieces = p.D / 4;
-  for (int i = tid; i < R * pieces; i += 64 * W) {
+  for (int i = tid; i < R * pieces; i += 64 * NW) {
     const int row = i / pieces, c = i - row * pieces;
     float m = -INFINITY;
 #pragma unroll
@@ -668,7 +671,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_both(Args p) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(few_lds<DP, W>(), many_lds<DP>())];
   const uint32_t few = p.n_few * p.KV, b = blockIdx.x, before = uint32_t(uint64_t(b) * few / gridDim.x);
   if (uint32_t(uint64_t(b + 1) * few / gridDim.x) > before) {
-    if (threadIdx.x < 64 * W) few_rows<DP, W>(p, before, lds);   // (whole waves: the others end)
+    few_rows<DP, W, kWaves>(p, before, lds);
   } else {
     many_rows<DP>(p, b - before, lds);
   }
