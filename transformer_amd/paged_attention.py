@@ -98,12 +98,13 @@ class PagedSequences:
         if longest is not None and not 1 <= longest <= LONGEST:
             raise ValueError(f"longest must lie in [1, {LONGEST}] (got {longest})")
         self._reserved = 0 if longest is None else int(longest)
-        self.host = self._plan(lengths, tables)
+        self.host, self.lengths, self.longest, self._pages = self._plan(lengths, tables)
         self.table = self.host.to(device)
         self.stream = _lib.current_stream(self.table)
         self.native, self.version = _lib.ops().PagedSteps(self.table, self.host, self.stream or 0), 0
 
     def _plan(self, lengths, tables):
+        """(the library's words, lengths, longest, pages) of a step."""
         lengths = _integers(lengths, "lengths")
         if len(lengths) != self.n:
             raise ValueError(f"{self.n} lengths of new tokens, {len(lengths)} lengths")
@@ -115,16 +116,17 @@ class PagedSequences:
         if self._reserved:
             pages = np.pad(pages, ((0, 0), (0, -(-self._reserved // PAGE) - pages.shape[1])))
         words = _words(self.q_lens, lengths, self.q_starts, np.ascontiguousarray(pages), self.n_heads, self.n_kv_heads, self._reserved)
-        self.lengths, self.longest, self._pages = lengths, self._reserved or max(lengths, default=0), pages
-        return words
+        return words, lengths, self._reserved or max(lengths, default=0), pages
 
     def update(self, lengths, tables):
         """The same sequences' next step: new lengths and pages, as many new tokens in the same rows.  Ordered on the current stream, on
         which the calls have to be."""
         if not self._reserved:
             raise ValueError("update needs room: give the sequences a longest length")
-        self.host.copy_(self._plan(lengths, tables))
-        self.table.copy_(self.host)
+        words, *state = self._plan(lengths, tables)
+        self.table.copy_(words)   # (first: where this fails, as in a capture, nothing has changed)
+        self.host.copy_(words)
+        self.lengths, self.longest, self._pages = state
         self.version += 1
 
     def used(self):
