@@ -8,7 +8,8 @@
 //   P_ij = 2^(c q_i.k_j - L_i), L_i = log2 sum_j 2^(c q_i.k_j);   O_i = sum_j P_ij v_j;   W'_j = W_j + sum_i P_ij
 //
 // Work is shared out on the host (msd_paged_plan), which has the lengths: lists of jobs that the device reads, with all that a
-// job needs beside the pages, so that no workgroup is empty and none counts sequences.  Row r of a sequence's group is position r / g,
+// job needs beside the pages, so that none of the attention's workgroups is empty or counts sequences.  (What follows it, joins and the
+// weights of pieces and of chunks, is launched for the most rows, parts and positions that a sequence has, and ends where one has less.)  Row r of a sequence's group is position r / g,
 // head r % g (see attn.hip, whose tiles these kernels use).
 //   few rows (up to 32 of a group: a token, a few drafts): paged_few, then paged_finish where the keys are split or weights counted
 //                                                   or, of few short sequences, paged_whole alone
@@ -81,7 +82,6 @@ struct Args {
   float c;
   int64_t q_rows;
   int n_seqs, width, longest, n_pages;
-  const int32_t* plan;
   const int32_t* tables;
   const Job *few, *many;
   int n_few, n_many;
@@ -509,7 +509,10 @@ __device__ __forceinline__ void many_rows(const Args& p, int group, uint8_t* lds
 #endif
   f32x16 o[DB] = {};
   float m = -INFINITY, l = 0;   // running maximum of c s, up to 2^8 too small; sum of 2^(c s - m) over this lane's keys
-  bf16x8 pr[2] = {};            // the half before, as operands
+  // The half before, as operands: one bf16 of each probability, off by up to 2^-8 of it (outputs 0.0023 from 64 bits where their own rounding
+  // leaves 0.0017), as in attn.hip.  A second one, as few rows have it, would be half as many matrix products again, which are what
+  // bounds these.  The sums and the weights are of the f32 values.
+  bf16x8 pr[2] = {};
   // operand n of a half: K's for the scores, then V's for the product
   auto operand = [&](int n, int k, int v) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -663,8 +666,10 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 3 : 2) void paged_many(Args
   __shared__ __attribute__((aligned(16))) uint8_t lds[many_lds<DP>()];
   many_rows<DP>(p, blockIdx.x, lds);
 }
-// A step of both: tokens' workgroups, which wait for memory, spread among the chunks', which wait for the matrix cores; in no more LDS than
-// these take.
+// A step of both: tokens' workgroups, which wait for memory, spread among the chunks', which wait for the matrix cores.  The tokens' LDS is the
+// larger: 66,560 bytes where heads are up to 64, of which two workgroups share a CU in place of three of the chunks' 32,768; 66,048 (65,536)
+// above.  It pays all the same: chunks of 333 and 248 and six tokens over up to 2900 positions take 33.0 us, in calls of their own 27.2 and 9.9
+// (16 / 4 heads of 64); 24.2, 20.4 and 10.5 (6 / 2 heads of 96).
 template <int DP>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_both(Args p) {
   constexpr int W = DP <= 64 ? kWaves : 2;
@@ -1760,7 +1765,6 @@ extern "C" int32_t msd_paged_attn(const msd_paged* a, const void* q, const void*
   p.width = h[MSD_PLAN_WIDTH];
   p.longest = int(longest);
   p.n_pages = int(a->positions / kPage);
-  p.plan = a->plan;
   p.tables = a->plan + h[AT_TABLES];
   p.few = reinterpret_cast<const Job*>(a->plan + h[AT_FEW + weighted]);
   p.many = reinterpret_cast<const Job*>(a->plan + h[AT_MANY]);
