@@ -51,8 +51,8 @@ int64_t msd_paged_plan(int32_t n_seqs, const int32_t* seqs, const int32_t* table
 
 /* One call on a plan (on the device, 16-byte aligned, and on the host, read during the call).  q_rows: rows of the flat tensors;
  * positions: of the pool, a multiple of 16; strides in elements, multiples of 8 and not negative, the d_head values of a head
- * contiguous; every pointer 16-byte aligned.  Heads and positions of pages that are only read may lie over one another (stride 0: one for all).  A page number outside the pool that only the device's words hold reads as rows of
- * zeros and is not written.
+ * contiguous; every pointer 16-byte aligned.  Heads and positions of pages that are only read may lie over one another (stride 0: one
+ * for all).  A page number outside the pool that only the device's words hold reads as rows of zeros and is not written.
  * Limits: d_head a multiple of 8 up to 128; scale in [2^-60, 2^60]; 128 consecutive rows of one head and the heads of one group
  * together span less than 2^30 elements, as do 16 positions of a page; q_rows times n_heads below 2^31. */
 typedef struct msd_paged {

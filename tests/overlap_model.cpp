@@ -1,5 +1,6 @@
-// Compares transformer_amd/csrc/overlap.h with lists of places, over small arrays of all kinds: those of one stride have to agree,
-// those of several must not be called apart where they meet.  Prints how many were compared of each kind and answer.
+// Compares transformer_amd/csrc/overlap.h with lists of places, over small arrays of all kinds: they have to agree, and where the strides
+// differ and no places are tried one by one, arrays must not be called apart where they meet.  Prints how many were compared of each kind
+// and answer.
 #include <cstdio>
 #include <random>
 #include <set>
@@ -43,7 +44,8 @@ int main() {
     const auto p = places(false), q = places(true);
     bool meet = false;
     for (const int64_t x : p) meet |= q.count(x) > 0;
-    const bool said = msd_overlap::share(axes, row, distance);
+    if (meet != msd_overlap::share(axes, row, distance)) return std::printf("not exact\n"), 1;
+    const bool said = msd_overlap::share(axes, row, distance, 0);
     if (meet && !said) return std::printf("missed\n"), 1;
     if (equal && meet != said) return std::printf("not exact\n"), 1;
     ++(equal ? same : other)[meet];

@@ -30,10 +30,12 @@ def _views(n):
         (z[:2], z[2:], False),
         (z[::2], z[1::2], False),
         (z[:2], y[:, :, 0], False),                          # other strides in other memory
+        (z[::3], z[1:3], False),                             # heads 0 and 3, heads 1 and 2
+        (z[::3], z[2:], True),
     ]
 
 
-@pytest.mark.parametrize("which", range(14))
+@pytest.mark.parametrize("which", range(16))
 def test_keys_and_values_in_one_memory(which):
     lengths = [40, 20]
     tables, n = tables_of(lengths + [16, 16], 1)
@@ -70,7 +72,7 @@ def test_layers_of_keys_and_values_in_one_memory():
     with pytest.raises(ValueError, match="same memory"):
         paged_evict(flat[:4], flat[1:5], torch.rand(4, 2, 2, 40).cuda(), e)
     with pytest.raises(ValueError, match="same memory"):
-        paged_evict(flat[::2], flat[2:6:1], torch.rand(4, 2, 2, 40).cuda(), e)   # (other strides, which may meet)
+        paged_evict(flat[::2], flat[2:6:1], torch.rand(4, 2, 2, 40).cuda(), e)   # (other strides; two of four are the same)
     paged_evict(pool[:, 0], pool[:, 1], torch.rand(4, 2, 2, 40).cuda(), e)
 
 
