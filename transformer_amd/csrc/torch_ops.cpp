@@ -457,7 +457,7 @@ msd_paged paged_call(const Tensor& k, const Tensor& v, const PagedSteps& s, bool
     int64_t end = D;
     for (const auto& [stride, size] : axes) {
       need(stride >= end, "pages that are written must not overlap");
-      end = stride * size;
+      end += (size - 1) * stride;
     }
   }
   need(positions < (int64_t(1) << 31) && s.word(MSD_PLAN_PAGES) <= positions / MSD_PAGE, "tables reach page ", s.word(MSD_PLAN_PAGES) - 1,
