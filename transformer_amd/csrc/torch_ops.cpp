@@ -495,7 +495,19 @@ void no_gradient(const char* what, const X&... x) {
     throw std::invalid_argument(std::string(what) + " has no gradient: call it under torch.no_grad(), or hand over detached tensors");
 }
 
-// k's and v's axes with the strides of both, and how far behind k v starts
+// x's memory, from its first place to behind its last
+struct Ends {
+  uintptr_t first, last;
+  explicit Ends(const Tensor& x) : first(reinterpret_cast<uintptr_t>(x.data_ptr())) {
+    const auto sizes = x.sizes(), strides = x.strides();
+    int64_t n = x.numel() ? 1 : 0;
+    for (size_t i = 0; n && i < sizes.size(); ++i) n += (sizes[i] - 1) * strides[i];
+    last = first + n * x.element_size();
+  }
+  bool meet(const Ends& other) const { return first < other.last && other.first < last; }
+};
+
+// Of pages of one shape, none of which overlaps with itself
 bool share_memory(const Tensor& k, const Tensor& v) {
   std::vector<msd_overlap::Axis> axes;
   const int64_t n = k.dim();
@@ -503,27 +515,22 @@ bool share_memory(const Tensor& k, const Tensor& v) {
   return msd_overlap::share(std::move(axes), k.size(n - 1), static_cast<const uint16_t*>(v.data_ptr()) - static_cast<const uint16_t*>(k.data_ptr()));
 }
 
-// (first: an inference tensor outside inference mode raises here)
-void written(const Tensor& k, const Tensor& v) {
-  need(!share_memory(k, v), "k_pages and v_pages are the same memory, or share some of it");
-  for (const Tensor* x : {&k, &v}) x->unsafeGetTensorImpl()->bump_version();
-}
-
-// x, or a copy of it where it lies among pages that are about to be written: the rows are those from before the call
-Tensor apart(const Tensor& x, const Tensor& k_pages, const Tensor& v_pages) {
-  auto ends = [](const Tensor& t) {
-    uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr()), end = at;
-    if (t.numel()) end += t.element_size();
-    for (int64_t i = 0; t.numel() && i < t.dim(); ++i) end += (t.size(i) - 1) * t.stride(i) * t.element_size();
-    return std::make_pair(at, end);
-  };
-  const auto mine = ends(x);
-  for (const Tensor* pages : {&k_pages, &v_pages}) {
-    const auto theirs = ends(*pages);
-    if (mine.first < theirs.second && theirs.first < mine.second) return x.clone(at::MemoryFormat::Contiguous);
+// Pages that a call is about to write
+struct Written {
+  const Tensor &k, &v;
+  Ends k_ends, v_ends;
+  Written(const Tensor& k_pages, const Tensor& v_pages) : k(k_pages), v(v_pages), k_ends(k), v_ends(v) {}
+  // (before anything is launched: an inference tensor outside inference mode raises here)
+  void mark() const {
+    need(!k_ends.meet(v_ends) || !share_memory(k, v), "k_pages and v_pages are the same memory, or share some of it");
+    for (const Tensor* x : {&k, &v}) x->unsafeGetTensorImpl()->bump_version();
   }
-  return x;
-}
+  // x, or a copy of it where it lies among the pages: new rows are those from before the call
+  Tensor apart(const Tensor& x) const {
+    const Ends e(x);
+    return e.meet(k_ends) || e.meet(v_ends) ? x.clone(at::MemoryFormat::Contiguous) : x;
+  }
+};
 
 void paged_append(const Tensor& k_new, const Tensor& v_new, const Tensor& k_pages, const Tensor& v_pages, const Paged& steps) {
   only_run("paged_append", k_new, v_new, k_pages, v_pages);
@@ -532,14 +539,15 @@ void paged_append(const Tensor& k_new, const Tensor& v_new, const Tensor& k_page
   msd_paged a = paged_call(k_pages, v_pages, p, false, true);
   const int64_t heads = p.word(MSD_PLAN_KV_HEADS);
   Place on(k_pages);
-  const Tensor k = apart(paged_rows("k", k_new, heads, a, p, k_pages.device()), k_pages, v_pages);
-  const Tensor v = apart(paged_rows("v", v_new, heads, a, p, k_pages.device()), k_pages, v_pages);
+  const Written pages(k_pages, v_pages);
+  const Tensor k = pages.apart(paged_rows("k", k_new, heads, a, p, k_pages.device()));
+  const Tensor v = pages.apart(paged_rows("v", v_new, heads, a, p, k_pages.device()));
   need(k.size(0) == v.size(0), "k of ", k.size(0), " rows, v of ", v.size(0));
   need(!p.word(MSD_PLAN_SHARED), "a page that takes new rows is in use elsewhere too");
   a.q_rows = k.size(0);
   const int64_t k_stride[2] = {stride_of(k, 0), stride_of(k, 1)}, v_stride[2] = {stride_of(v, 0), stride_of(v, 1)};
   use_table(p.table, p.table_stream, on.stream);
-  written(k_pages, v_pages);
+  pages.mark();
   check(msd_paged_append(&a, at_(k), k_stride, at_(v), v_stride, at_(k_pages), at_(v_pages), on.stream), "msd_paged_append");
 }
 
@@ -590,6 +598,7 @@ variable_list paged_evict(const Tensor& k_pages, const Tensor& v_pages, const Te
   sizes.push_back(p.word(MSD_PLAN_KV_HEADS));
   need(!layers || k_pages.size(0) * k_pages.size(1) < 65536, "layers times heads must stay below 65536 (got ", k_pages.size(0), " and ", k_pages.size(1), ")");
   weights_fit(weights, sizes, k_pages.device(), "the pages'");
+  const Written memory(k_pages, v_pages);
   Place on(k_pages);
   const Tensor w = weights.contiguous();
   sizes.push_back(keep);
@@ -597,7 +606,7 @@ variable_list paged_evict(const Tensor& k_pages, const Tensor& v_pages, const Te
   const int32_t n_layers = layers ? int32_t(k_pages.size(0)) : 1;
   use_table(p.table, p.table_stream, on.stream);
   use_table(to, to_stream, on.stream);
-  written(k_pages, v_pages);
+  memory.mark();
   check(msd_paged_evict(&a, n_layers, layers ? stride_of(k_pages, 0) : 0, layers ? stride_of(v_pages, 0) : 0, at_(k_pages), at_(v_pages),
                         static_cast<const float*>(at_(w)), int32_t(w.size(-1)), keep, recent, static_cast<const int32_t*>(at_(to)),
                         int32_t(to.size(1)), static_cast<float*>(at_(out)), static_cast<int32_t*>(at_(kept)), on.stream),
