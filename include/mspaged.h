@@ -35,11 +35,11 @@ enum {
 
 /* The plan of a step: how `n_seqs` sequences' work is shared out, in int32 words that the calls below read on the host and, from
  * a copy of the caller's, on the device.  seqs: (q_start, q_len, length) of each: its new tokens are rows q_start ..
- * q_start + q_len of flat tensors (the ranges do not overlap; one without new tokens has none and starts anywhere), the last q_len of its `length` positions.  tables: n_seqs rows
- * of table_width page numbers (those behind a sequence's length are not read).  longest 0: for these lengths, launches as large as
- * they need.  Otherwise lengths up to `longest`: plans of the same n_seqs, q_starts, q_lens, heads, width and longest have
- * the same words but for the numbers that the device reads, and the same launches, so that a captured graph goes on with a new
- * plan in the same memory.
+ * q_start + q_len of flat tensors (the ranges do not overlap; one without new tokens has none and starts anywhere), the last q_len of
+ * its `length` positions.  tables: n_seqs rows of table_width page numbers (those behind a sequence's length are not read).  longest 0:
+ * for these lengths, launches as large as they need.  Otherwise lengths up to `longest`: plans of the same n_seqs, q_starts, q_lens,
+ * heads, width and longest have the same words but for the numbers that the device reads, and the same launches, so that a captured
+ * graph goes on with a new plan in the same memory.
  * words NULL: returns how many there are; otherwise writes them (`room` of them are there) and returns that.  Word MSD_PLAN_Q_END:
  * one past the last row; Q_COUNT: rows of all sequences; PAGES: one past the largest page in use; SHARED: whether a page
  * that takes new rows is in use elsewhere too.
